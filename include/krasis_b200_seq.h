@@ -321,6 +321,42 @@ KB2SEQ_API int kb2_seq_depth_mix(float* stack, long long stride, int n, const fl
 KB2SEQ_API int kb2_seq_stream_mix(float* xs, int n, const float* x0, const float* y, const float* mix, const float* out, const float* read,
                                   const float* w, float w_shift, void* h, int dt_h, int T, int W, float eps, void* stream);
 
+/* ---- A paged cache of keys and values in 8 bits, and what reads it.
+ * Pools k [layers][pages][G][page_size][d] and v [...][dv] of codes, and k_scale, v_scale [layers][pages][G][page_size] fp32, all on 16 bytes; a number is code * scale.
+ * A row is one token's key or value of one kv head, with a = max |x|.  fmt 0: e4m3 codes, scale 2^k, the least k >= -126 with a <= 448 2^k; fmt 1: int8 codes within
+ * +-127, scale a times fp32(1 / 127) in fp32; codes are the nearest ones to x / scale, ties to even.  a = 0: scale 0, codes 0.  A row with a number that is not finite: scale NaN,
+ * codes 0.  d and dv multiples of 16 up to 256; page_size a power of two from 16 to 1024. */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int layers, pages, page_size, G, d, dv, fmt;
+} kb2_seq_kv_cache;
+/* The tables of a step (see above; layout and replayed as in kb2_seq_attention_step).  For drafted tokens rows [T] says where a token's key and value lie, behind
+ * the committed rows of its sequence in the order of the tokens, positions holds first row + depth, and bits [T][words] which tokens of its sequence a token sees: bit i
+ * is set for token i if that is the token itself or one of its ancestors, which come before it.  rows and bits null: positions and order of a portion.
+ * Tokens behind cu[S] are left alone by every call below.  Pages that are not in the pool hold nothing: no row is written there or seen. */
+typedef struct {
+  const int *positions, *seq_of, *cu, *pages, *rows;
+  const unsigned* bits;
+  const int* layout;
+  int words, T, S, max_pages, replayed, device;
+} kb2_seq_kv_step;
+/* The step's keys k [T][G][d] and values v [T][G][dv] (dt; numbers of a head side by side, ld* and h* numbers from token to token and head to head) into the pages. */
+KB2SEQ_API int kb2_seq_kv_write(const kb2_seq_kv_cache* cache, int layer, const kb2_seq_kv_step* step, const void* k, long long ldk, long long hk, const void* v,
+                                long long ldv, long long hv, int dt, void* stream);
+/* Rows first .. first + count - 1 of sequence s: k [count][G][d] and v [count][G][dv] in dt, on 16 bytes. */
+KB2SEQ_API int kb2_seq_kv_read(const kb2_seq_kv_cache* cache, int layer, const kb2_seq_kv_step* step, int s, int first, int count, void* k, void* v, int dt,
+                               void* stream);
+/* out [T][H][dv] in dt_out: softmax(scale q k^T) v over the rows j <= pos of a token's sequence with pos - j < window (0: no window) or j < first; a drafted token sees
+ * the committed rows by that rule and of the drafted ones its ancestors and itself, whose place in the rule is their position.  Nothing to see: zeros.
+ * sinks [H] (may be null): the softmax denominator of head h also holds exp(sinks[h]).  The step's own rows have been written before.  q [T][H][d] in dt_q as k above. */
+KB2SEQ_API size_t kb2_seq_kv_attn_workspace(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first);
+KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const kb2_seq_kv_step* step, const void* q, int dt_q, long long ldq, long long hq, int H,
+                               float scale, int window, int first, const float* sinks, void* out, int dt_out, void* work, size_t work_bytes, void* stream);
+/* Drafted tokens that were accepted: row base + path[s][i] of sequence s becomes row base + i, in every layer; base is the first drafted row.  path [S][P] (P <= 512) holds
+ * rising token numbers and ends at the first one that does not rise or that the sequence does not have. */
+KB2SEQ_API int kb2_seq_kv_keep(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, const int* path, int P, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -470,6 +470,42 @@ class HeadKVCache(PagedKVCache):
         return (self.kp[layer_offset], self.vp[layer_offset]) if self.kp[layer_offset] is not None else None
 
 
+class CompactKVCache(PagedKVCache):
+    """Paged cache of per-head keys and values in 8 bits for several live sequences: codes k [num_layers, max_pages, kv_heads, page_size, dim] and v [..., vdim], and
+    one fp32 scale per row (token and head) beside each, k_scale and v_scale [num_layers, max_pages, kv_heads, page_size].  A number is its code times its row's scale.
+
+    fmt "e4m3": scale 2^k, the least with the row's largest magnitude <= 448 2^k; "int8": that magnitude / 127 (times fp32(1 / 127)).  int8 keeps rows of numbers of one size to 1/254 of the
+    largest, e4m3 every number to 1/16 of itself.  A row with a number that is not finite is held as NaN.  All layers are alike and share one page numbering; the free
+    list is that of `PagedKVCache`.  `seqops.kv_write` fills it, `kv_attn`, `kv_tree_attn` and `kv_read` read it, `kv_keep` moves rows: codes are always finite there."""
+
+    FORMATS = {"e4m3": (0, torch.float8_e4m3fn), "int8": (1, torch.int8)}
+
+    def __init__(self, num_layers: int, num_kv_heads: int, dim: int, vdim: int, device, max_pages: int, fmt: str = "int8", page_size: int = 64):
+        from . import seqops
+        if fmt not in self.FORMATS:
+            raise ValueError(f"cache format {fmt!r}: e4m3 or int8")
+        if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
+            raise ValueError("page_size: a power of two from 16 to 1024")
+        if any(not 16 <= n <= 256 or n % 16 for n in (dim, vdim)):
+            raise ValueError(f"head sizes {dim} / {vdim}: multiples of 16 up to 256")
+        if num_layers < 1 or num_kv_heads < 1 or max_pages < 1:
+            raise ValueError("at least one layer, head and page")
+        if max_pages * num_kv_heads * (page_size // 16) > 0x7FFFFFFF:
+            raise ValueError("too many rows in a layer")
+        code, dtype = self.FORMATS[fmt]
+        self.num_layers, self.num_kv_heads, self.dim, self.vdim = num_layers, num_kv_heads, dim, vdim
+        self.fmt, self.kv_dtype, self.page_size, self.max_pages, self.device = fmt, dtype, page_size, max_pages, torch.device(device)
+        shape = (num_layers, max_pages, num_kv_heads, page_size)
+        self.k, self.v = (torch.zeros(shape + (n,), dtype=dtype, device=self.device) for n in (dim, vdim))
+        self.k_scale, self.v_scale = (torch.zeros(shape, dtype=torch.float32, device=self.device) for _ in range(2))
+        self._free = list(range(max_pages - 1, -1, -1))
+        self.args = seqops.KvCacheArgs(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), num_layers, max_pages, page_size,
+                                       num_kv_heads, dim, vdim, code)
+
+    def get_layer_caches(self, layer_offset: int):
+        return self.k[layer_offset], self.v[layer_offset]
+
+
 class RecurrentStatePool:
     """State slots of recurrent mixers for several live sequences.  A slot is one index into every registered tensor
     ([slots, ...] fp32, one per recurrent layer run); `alloc()` hands out a zeroed slot, `free()` returns it for reuse."""

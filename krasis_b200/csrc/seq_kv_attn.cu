@@ -1,0 +1,581 @@
+// Attention over the 8-bit cache (seq_kv.cu) for few query rows per key / value head: decoded tokens, short portions, small trees.
+//
+//   o = sum_j w_j v_j / (sum_j w_j + exp(sink)),  w_j = exp(scale q . k_j - max),  over the rows j that a token sees
+//
+// The H / G query heads of a kv head read the same rows, so a tile is 8 or 16 (token, head) pairs of one sequence and kv head, and a warp takes 16 keys at a time
+// through mma.m16n8k16 in fp16, in which every code of both formats is exact: S = Q K^T with the queries as rows, then O^T = V^T P^T with the value columns as rows,
+// so that S's accumulators are P's fragments where they stand, without a shuffle.  Dimensions and keys may be summed in any order, so a lane takes 16 neighbouring
+// bytes of a key row and 8 or 16 of a value row for its fragments: everything a lane multiplies it has copied itself (cp.async into its own slots), no warp waits for
+// another, and no byte is read from shared memory twice.
+// What bounds it: the cache's bytes.  16 keys of 128 + 128 dimensions are 4.2 KB a warp and iteration; 3 stages x 16 warps an SM keep 200 KB on the way.
+//
+// Rounding.  q: a row is scaled by a power of two to the top of fp16's range, bf16 numbers keep their 8 bits, fp32 ones are rounded to 11 (PARTS 1) or split into two
+// fp16 numbers with 22 together (PARTS 2, for fp32 results).  Scores, maxima and sums are fp32; the key's scale multiplies the fp32 score.  The weight times the value's
+// scale is rounded to fp16, relative to a reference R of its own that follows the largest such product (2^6 to 2^15 of it), so that small scales or weights do not
+// fall out of fp16's range: 11 bits, or 22 with PARTS 2, down to 2^-30 of the largest.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "ptx.cuh"
+#include "seq_kv.cuh"
+
+namespace kb2seq {
+namespace {
+
+constexpr int kSWarps = 8, kSStages = 3, kSMostGroups = 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// bytes 0, 1 and bytes 2, 3 of a word of codes as pairs of fp16
+template <int FMT>
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == KV_E4M3) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u;                      // 0 .. 255 for -128 .. 127: 0x6400 + u is the fp16 number 1024 + u
+    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 f16_get(uint32_t p) { return __half22float2(*reinterpret_cast<const __half2*>(&p)); }
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts4(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+__device__ __forceinline__ void cp_async8(uint32_t to, const void* from, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(in ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+struct KvAttn {                              // what a call says beside the cache and the tables
+  const void* q;
+  long long ldq, hq;
+  int dtq, H, window, first;
+  float scale;
+  const float* sinks;
+  void* out;
+  int dt_out, per_seq;                       // per_seq: tiles of every sequence where all bring as many tokens, else 0
+  int piece, pieces;                         // groups of 16 keys a piece; the most pieces of a tile
+  float *part_o, *part_ml;                   // [T H][pieces][dv] and [T H][pieces][2]
+};
+
+// DU, VU: units of 64 of d and dv.
+template <int DU, int VU, int NQ, int PARTS>
+struct StreamShape {
+  static constexpr int MT = 8 * NQ;
+  static constexpr int VB = VU % 2 ? 8 : 16, VC = VU * 8 / VB;            // a lane's bytes of a value row: VC times VB
+  static constexpr int kK = 2 * DU * 512, kV = 4 * VU * 256, kStage = kK + kV + 128;
+  static constexpr bool kQShared = DU * 8 * NQ * PARTS > 32;              // registers of the queries
+  static constexpr int kQ = kQShared ? DU * 4 * PARTS * 2 * NQ * 128 : 0;
+  static constexpr int kRing = kSWarps * kSStages * kStage, kRed = kSWarps * MT * VU * 64 * 4;
+  static constexpr int kOffRow = kRing > kRed ? kRing : kRed, kOffStat = kOffRow + kSMostGroups * 4, kOffQ = kOffStat + kSWarps * MT * 4 * 4;
+  static constexpr int kTotal = kOffQ + kQ;
+  static constexpr int kBlocks = 2 * (kTotal + 1024) <= 227 * 1024 ? 2 : 1;
+  static_assert(kTotal <= 227 * 1024 && kOffQ % 16 == 0 && kStage % 16 == 0, "shared memory");
+};
+
+template <int FMT, int DU, int VU, int NQ, int PARTS>
+__global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>::kBlocks)) kv_stream_kernel(KvLayer c, KvStep t, KvAttn a) {
+  using L = StreamShape<DU, VU, NQ, PARTS>;
+  constexpr int MT = L::MT, VB = L::VB, VC = L::VC, MV = VU * 4;         // MV: 16-row tiles of O^T
+  extern __shared__ __align__(16) uint8_t smem[];
+  kb2::pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+  const int per = a.H / c.G, head = blockIdx.y;
+  int s, tile;
+  if (a.per_seq) {
+    s = blockIdx.x / a.per_seq;
+    tile = blockIdx.x - s * a.per_seq;
+  } else if (!kv_find_tile(t, per, MT, blockIdx.x, &s, &tile)) {
+    return;
+  }
+  const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * MT, nr = (int)min((long long)n * per - r0, (long long)MT);
+  if (nr <= 0) return;
+  const int t0 = c0 + r0 / per, t1 = c0 + (r0 + nr - 1) / per;
+  const KvSpan span = kv_span(c, t, s, t0, t1, a.window, a.first);
+  const int total = span.groups(), np = min((total + a.piece - 1) / a.piece, a.pieces), z = blockIdx.z;
+  if (z > 0 && z >= np) return;
+  const int u0 = z * a.piece, u1 = min(total, u0 + a.piece);   // z = 0 of nothing to see: no group
+
+  // where the piece's groups lie: a row of this head in units of 16, or -1
+  int* rows = reinterpret_cast<int*>(smem + L::kOffRow);
+  for (int i = threadIdx.x; i < u1 - u0; i += kSWarps * 32) {
+    const long long r = kv_row(c, t, s, span.group(u0 + i) * kKvGroup);
+    rows[i] = r < 0 ? -1 : (int)((r + ((long long)head << c.lps)) / kKvGroup);
+  }
+  __syncthreads();
+
+  const uint32_t ring = kb2::smem_u32(smem) + warp * (kSStages * L::kStage);
+  const auto issue = [&](int u, int st) {
+    if (u < u1) {
+      const int r16 = rows[u - u0];
+      if (r16 >= 0) {
+        const long long row = (long long)r16 * kKvGroup;
+        const uint32_t to = ring + st * L::kStage;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint8_t* from = c.k + (row + 4 * (g8 >> 1) + 2 * j + (g8 & 1)) * c.d + 16 * t4;
+#pragma unroll
+          for (int i = 0; i < DU; ++i) cp_async16_stream(to + ((j * DU + i) * 32 + lane) * 16, from + (64 * i + 16 * t4 < c.d ? 64 * i : -16 * t4), 64 * i + 16 * t4 < c.d);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint8_t* from = c.v + (row + 4 * t4 + k) * c.dv;
+#pragma unroll
+          for (int i = 0; i < VC; ++i) {
+            const int e = (8 * i + g8) * VB;
+            const uint32_t at = to + L::kK + ((k * VC + i) * 32 + lane) * VB;
+            if constexpr (VB == 16) cp_async16_stream(at, from + (e < c.dv ? e : 0), e < c.dv);
+            else cp_async8(at, from + (e < c.dv ? e : 0), e < c.dv);
+          }
+        }
+        if (lane < 8) cp_async16_stream(to + L::kK + L::kV + lane * 16, (lane < 4 ? c.ks : c.vs) + row + 4 * (lane & 3), true);
+      }
+    }
+    kb2::cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kSStages; ++i) issue(u0 + warp + i * kSWarps, i);
+
+  // queries: row r of the tile is head `r0 + r` mod per of a token.  A lane's 16 numbers of a unit are its fragments of four products.
+  constexpr int QR = L::kQShared ? 1 : DU * 4;
+  uint32_t qf[QR][PARTS][2 * NQ];
+  float rf[NQ];
+  int pos[NQ], tok[NQ];
+  float m[NQ], l[NQ], ref[NQ];
+  int pmin = 0x7FFFFFFF, pmax = -1;
+#pragma unroll
+  for (int h = 0; h < NQ; ++h) {
+    const int r = g8 + 8 * h;
+    const bool in = r < nr;
+    const int rr = r0 + (in ? r : 0), tk = c0 + rr / per, hd = head * per + rr % per;
+    tok[h] = tk;
+    pos[h] = in ? t.positions[tk] : -1;
+    m[h] = -INFINITY;
+    l[h] = ref[h] = 0.f;
+    const long long from = tk * a.ldq + hd * a.hq;
+    float x[DU][16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < DU; ++i) {
+      const int e = 64 * i + 16 * t4;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        x[i][j] = in && e < c.d ? (a.dtq ? __bfloat162float(((const bf16*)a.q)[from + e + j]) : ((const float*)a.q)[from + e + j]) : 0.f;
+        top = max(top, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+      }
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^e brings the largest below 2^15; of a row of smallest or no numbers, or of one that is not finite, it stays within fp32
+    const int e = min(max(141 - (int)(top >> 23), -113), 100);
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+    rf[h] = a.scale * kLog2e * __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < DU; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {        // dimensions 4 k + 2 b, + 1 of the lane's 16
+          const float y0 = x[i][4 * k + 2 * b] * up, y1 = x[i][4 * k + 2 * b + 1] * up;
+          uint32_t p[PARTS];
+          p[0] = f16_pair(y0, y1);
+          if constexpr (PARTS == 2) {
+            const float2 f = f16_get(p[0]);
+            p[1] = f16_pair(y0 - f.x, y1 - f.y);
+          }
+#pragma unroll
+          for (int o = 0; o < PARTS; ++o) {
+            if constexpr (L::kQShared) {
+              if (warp == (i * 4 + k) % kSWarps) sts4(kb2::smem_u32(smem) + L::kOffQ + ((((i * 4 + k) * PARTS + o) * 32 + lane) * 2 * NQ + b * NQ + h) * 4, p[o]);
+            } else {
+              qf[i * 4 + k][o][b * NQ + h] = p[o];
+            }
+          }
+        }
+  }
+  {
+    const int p0 = t.positions[t0], p1 = t.positions[t1];    // of a portion: the first and the last; of a tree: anything from base on
+    pmin = span.base < kKvNoWindow ? span.base : p0;
+    pmax = p1;
+    if (span.base < kKvNoWindow) {
+      for (int x = t0; x <= t1; ++x) pmax = max(pmax, t.positions[x]);
+    }
+  }
+  if constexpr (L::kQShared) __syncthreads();
+
+  float o[MV][NQ][4];
+#pragma unroll
+  for (int i = 0; i < MV; ++i)
+#pragma unroll
+    for (int h = 0; h < NQ; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][h][e] = 0.f;
+
+  const auto sees = [&](int j, int h) {      // row h of the lane, position j
+    if (r0 + g8 + 8 * h >= r0 + nr) return false;
+    int spot = j;
+    if (j >= span.base) {
+      const int i = j - span.base;
+      if (i >= n || !(t.bits[(long long)tok[h] * t.words + (i >> 5)] >> (i & 31) & 1u)) return false;
+      spot = t.positions[c0 + i];
+    }
+    return spot <= pos[h] && (pos[h] - spot < a.window || spot < a.first);
+  };
+
+  int st = 0;
+  for (int u = u0 + warp; u < u1; u += kSWarps) {
+    kb2::cp_async_wait<kSStages - 1>();
+    __syncwarp();
+    const uint32_t at = ring + st * L::kStage;
+    if (rows[u - u0] >= 0) {
+      const int key0 = span.group(u) * kKvGroup;
+      float sc[2][4] = {};
+#pragma unroll
+      for (int i = 0; i < DU; ++i) {
+        const uint4 k0 = lds16(at + (i * 32 + lane) * 16), k1 = lds16(at + ((DU + i) * 32 + lane) * 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t b[2][2];
+          codes_f16<FMT>(word(k0, k), b[0][0], b[0][1]);
+          codes_f16<FMT>(word(k1, k), b[1][0], b[1][1]);
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) {
+            uint32_t x[2 * NQ];              // [dimensions 0, 1 | 8, 9 of the product][row]
+            if constexpr (L::kQShared) {
+              const uint32_t qa = kb2::smem_u32(smem) + L::kOffQ + (((i * 4 + k) * PARTS + p) * 32 + lane) * 8 * NQ;
+              if constexpr (NQ == 2) {
+                const uint4 v = lds16(qa);
+                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+              } else {
+                const uint2 v = lds8(qa);
+                x[0] = v.x; x[1] = v.y;
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2 * NQ; ++e) x[e] = qf[i * 4 + k][p][e];
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) mma_f16(sc[j], x[0], NQ == 2 ? x[1] : 0u, x[NQ], NQ == 2 ? x[NQ + 1] : 0u, b[j][0], b[j][1]);
+          }
+        }
+      }
+      const uint4 kq = lds16(at + L::kK + L::kV + t4 * 16), vq = lds16(at + L::kK + L::kV + 64 + t4 * 16);
+      // all rows of the tile see all 16 keys
+      const bool all = key0 + kKvGroup <= span.base && key0 + kKvGroup - 1 <= pmin && (pmax - key0 < a.window || key0 + kKvGroup <= a.first);
+      uint32_t w[NQ][PARTS][2];
+      bool again = false;
+      float grow[NQ];
+#pragma unroll
+      for (int h = 0; h < NQ; ++h) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = sc[e >> 1][2 * h + (e & 1)] * __uint_as_float(word(kq, e)) * rf[h];
+          if (!all && !sees(key0 + 4 * t4 + e, h)) y[e] = -INFINITY;
+        }
+        float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m[h], top), from = mn == -INFINITY ? 0.f : mn, back = ex2(m[h] - from);
+        m[h] = mn;
+        float sum = 0.f, big = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = ex2(y[e] - from);
+          sum += p;
+          y[e] = y[e] == -INFINITY ? 0.f : p * __uint_as_float(word(vq, e));      // a row that nobody sees may hold anything
+          big = fmaxf(big, y[e]);
+        }
+        l[h] = l[h] * back + sum;
+        ref[h] *= back;
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        grow[h] = 1.f;
+        if (big > ref[h] * 32768.f && big > 1e-37f) {
+          const float r = fmaxf(big * 0.015625f, 1e-37f);
+          grow[h] = ref[h] / r;
+          ref[h] = r;
+          again = true;
+        }
+        const float inv = ref[h] >= 1e-37f ? __frcp_rn(ref[h]) : 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float f0 = y[2 * b] * inv, f1 = y[2 * b + 1] * inv;
+          w[h][0][b] = f16_pair(f0, f1);
+          if constexpr (PARTS == 2) {
+            const float2 f = f16_get(w[h][0][b]);
+            w[h][PARTS - 1][b] = f16_pair(f0 - f.x, f1 - f.y);
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, again)) {
+#pragma unroll
+        for (int h = 0; h < NQ; ++h) {       // the columns of O^T that a lane holds are the rows 2 t4, 2 t4 + 1 of the queries
+          const float f0 = __shfl_sync(0xffffffffu, grow[h], 8 * t4), f1 = __shfl_sync(0xffffffffu, grow[h], 8 * t4 + 4);
+#pragma unroll
+          for (int i = 0; i < MV; ++i) {
+            o[i][h][0] *= f0;
+            o[i][h][1] *= f1;
+            o[i][h][2] *= f0;
+            o[i][h][3] *= f1;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VC; ++i) {
+        uint32_t v[4][VB / 4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t va = at + L::kK + ((k * VC + i) * 32 + lane) * VB;
+          if constexpr (VB == 16) {
+            const uint4 q = lds16(va);
+            v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][VB / 4 - 1] = q.w;
+          } else {
+            const uint2 q = lds8(va);
+            v[k][0] = q.x; v[k][1] = q.y;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < VB / 4; ++x)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {      // bytes 2 b, 2 b + 1 of the word: rows g8 and g8 + 8 of a tile of O^T
+            uint32_t a0, a1, a2, a3;
+            codes_f16<FMT>(__byte_perm(v[0][x], v[1][x], b ? 0x7362 : 0x5140), a0, a1);
+            codes_f16<FMT>(__byte_perm(v[2][x], v[3][x], b ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+            for (int h = 0; h < NQ; ++h)
+#pragma unroll
+              for (int p = 0; p < PARTS; ++p) mma_f16(o[i * (VB / 2) + 2 * x + b][h], a0, a1, a2, a3, w[h][p][0], w[h][p][1]);
+          }
+      }
+    }
+    __syncwarp();
+    issue(u + kSStages * kSWarps, st);
+    st = st + 1 == kSStages ? 0 : st + 1;
+  }
+  kb2::cp_async_wait<0>();
+
+  // the warps' shares, joined in their order
+  float4* stat = reinterpret_cast<float4*>(smem + L::kOffStat);            // [warp][row]: maximum, sum, reference
+#pragma unroll
+  for (int h = 0; h < NQ; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    if (t4 == 0) stat[warp * MT + g8 + 8 * h] = make_float4(m[h], l[h], ref[h], 0.f);
+  }
+  __syncthreads();                           // the rings are free from here on
+  float* red = reinterpret_cast<float*>(smem);                             // [warp][row][VU 64]
+#pragma unroll
+  for (int h = 0; h < NQ; ++h)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int q = 8 * h + 2 * t4 + e;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kSWarps; ++w) top = fmaxf(top, stat[w * MT + q].x);
+      const float4 x = stat[warp * MT + q];
+      const float f = x.x == -INFINITY ? 0.f : x.z * ex2(x.x - top);
+#pragma unroll
+      for (int i = 0; i < MV; ++i) {
+        const int dim = (i / (VB / 2)) * 8 * VB + VB * g8 + 2 * (i % (VB / 2));
+        *reinterpret_cast<float2*>(red + (warp * MT + q) * (VU * 64) + dim) = make_float2(o[i][h][e] * f, o[i][h][2 + e] * f);
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nr * c.dv; i += kSWarps * 32) {
+    const int q = i / c.dv, dim = i - q * c.dv;
+    float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSWarps; ++w) top = fmaxf(top, stat[w * MT + q].x);
+#pragma unroll
+    for (int w = 0; w < kSWarps; ++w) {
+      const float4 x = stat[w * MT + q];
+      sum += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top);                // a sum without a maximum is 0, or NaN from a row that holds one
+      acc += red[(w * MT + q) * (VU * 64) + dim];
+    }
+    const int rr = r0 + q, hd = head * per + rr % per;
+    const long long row = (long long)(c0 + rr / per) * a.H + hd;
+    if (np <= 1) {
+      if (a.sinks != nullptr && top != -INFINITY) sum += ex2(fmaf(a.sinks[hd], kLog2e, -top));
+      st_dt(a.out, a.dt_out, row * c.dv + dim, sum == 0.f ? 0.f : acc / sum);
+    } else {
+      const long long p = row * a.pieces + z;
+      a.part_o[p * c.dv + dim] = acc;
+      if (dim == 0) {
+        a.part_ml[2 * p] = top;
+        a.part_ml[2 * p + 1] = sum;
+      }
+    }
+  }
+}
+
+// The pieces of a row, joined in their order.  One warp a row (token, head); rows that one piece finished are left alone.
+__global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAttn a, int tile_rows) {
+  kb2::pdl_wait();
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, tok = (int)(row / a.H), hd = (int)(row - (long long)tok * a.H);
+  if (tok >= t.T || tok >= t.cu[t.S]) return;
+  const int per = a.H / c.G, s = t.seq_of[tok], c0 = t.cu[s], n = t.cu[s + 1] - c0;
+  const int r0 = ((tok - c0) * per + hd % per) / tile_rows * tile_rows, nr = (int)min((long long)n * per - r0, (long long)tile_rows);
+  const KvSpan span = kv_span(c, t, s, c0 + r0 / per, c0 + (r0 + nr - 1) / per, a.window, a.first);
+  const int np = min((span.groups() + a.piece - 1) / a.piece, a.pieces);
+  if (np <= 1) return;
+  const long long p0 = row * a.pieces;
+  float top = -INFINITY, sum = 0.f;
+  for (int i = lane; i < np; i += 32) top = fmaxf(top, a.part_ml[2 * (p0 + i)]);
+  top = warp_max(top);
+  for (int i = lane; i < np; i += 32) {
+    const float x = a.part_ml[2 * (p0 + i)], y = a.part_ml[2 * (p0 + i) + 1];
+    sum += x == -INFINITY ? y : y * ex2(x - top);
+  }
+  sum = warp_sum(sum);
+  if (a.sinks != nullptr && top != -INFINITY) sum += ex2(fmaf(a.sinks[hd], kLog2e, -top));
+  float acc[8] = {};
+  for (int i = 0; i < np; ++i) {
+    const float x = a.part_ml[2 * (p0 + i)], f = x == -INFINITY ? 1.f : ex2(x - top);      // a piece without a maximum holds zeros, or NaN
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e * 32 + lane < c.dv) acc[e] = fmaf(a.part_o[(p0 + i) * c.dv + e * 32 + lane], f, acc[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e * 32 + lane < c.dv) st_dt(a.out, a.dt_out, row * c.dv + e * 32 + lane, sum == 0.f ? 0.f : acc[e] / sum);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+// How a call's keys are cut.  groups: the most groups of 16 keys that a sequence's tokens see.
+struct StreamPlan {
+  int tile_rows, tiles, per_seq, piece, pieces;
+};
+inline long long groups_seen(long long start, long long n, int window, int first) {
+  const long long lo = window < kKvNoWindow ? std::max(0ll, start - window + 1) : 0;
+  return (start + n - lo + 30) / 16 + (std::min<long long>(first, lo) + 15) / 16;
+}
+StreamPlan stream_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first) {
+  StreamPlan p{};
+  const int per = H / cache->G;
+  long long most = 0, work = 0, rows = 0;
+  bool same = true;
+  for (int s = 0; s < step->S; ++s) rows = std::max(rows, (long long)step->layout[4 * s + 1] * per);
+  p.tile_rows = rows <= 8 ? 8 : 16;
+  for (int s = 0; s < step->S; ++s) {
+    const int* l = step->layout + 4 * s;
+    const int tiles = (int)(((long long)l[1] * per + p.tile_rows - 1) / p.tile_rows);
+    // captured launches are run again with later positions: what the page lists hold
+    const long long end = step->replayed ? (long long)step->max_pages * cache->page_size : (long long)l[2] + l[1];
+    const long long g = l[1] ? groups_seen(end - l[1], l[1], window, first) : 0;
+    p.tiles += tiles;
+    most = std::max(most, g);
+    work += g * tiles;
+    same = same && l[1] == step->layout[1];
+  }
+  p.per_seq = same && p.tiles ? p.tiles / step->S : 0;
+  const long long want = 4ll * 2 * kb2::current_sms();                     // blocks
+  long long piece = std::max((work * cache->G + want - 1) / want, (most + 63) / 64);
+  piece = std::min<long long>((piece + kSWarps - 1) / kSWarps * kSWarps, kSMostGroups);
+  p.piece = (int)std::max<long long>(piece, kSWarps);
+  p.pieces = (int)std::max(1ll, (most + p.piece - 1) / p.piece);
+  return p;
+}
+inline size_t stream_bytes(const StreamPlan& p, const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H) {
+  return p.pieces > 1 ? (size_t)step->T * H * p.pieces * (cache->dv + 2) * 4 : 0;
+}
+
+template <int FMT, int DU, int VU, int NQ, int PARTS>
+int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const StreamPlan& p, cudaStream_t st) {
+  using L = StreamShape<DU, VU, NQ, PARTS>;
+  SEQ_CUDA((kb2::allow_smem<kv_stream_kernel<FMT, DU, VU, NQ, PARTS>>(L::kTotal)));
+  auto kern = kv_stream_kernel<FMT, DU, VU, NQ, PARTS>;
+  kb2::launch_pdl(kern, dim3(p.tiles, c.G, p.pieces), kSWarps * 32, L::kTotal, st, c, t, a);
+  SEQ_LAUNCHED();
+  return KB2SEQ_OK;
+}
+template <int FMT, int DU, int VU>
+int stream_rows(const KvLayer& c, const KvStep& t, const KvAttn& a, const StreamPlan& p, cudaStream_t st) {
+  if (p.tile_rows == 8) return a.dt_out ? stream_launch<FMT, DU, VU, 1, 1>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 1, 2>(c, t, a, p, st);
+  return a.dt_out ? stream_launch<FMT, DU, VU, 2, 1>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 2, 2>(c, t, a, p, st);
+}
+template <int FMT>
+int stream_sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, const StreamPlan& p, cudaStream_t st) {
+  if (c.d <= 64 && c.dv <= 64) return stream_rows<FMT, 1, 1>(c, t, a, p, st);
+  if (c.d <= 128 && c.dv <= 128) return stream_rows<FMT, 2, 2>(c, t, a, p, st);
+  if (c.d <= 192 && c.dv <= 128) return stream_rows<FMT, 3, 2>(c, t, a, p, st);
+  if (c.d <= 128) return stream_rows<FMT, 2, 4>(c, t, a, p, st);
+  return stream_rows<FMT, 4, 4>(c, t, a, p, st);
+}
+}  // namespace
+}  // namespace kb2seq
+
+using namespace kb2seq;
+
+extern "C" {
+
+KB2SEQ_API size_t kb2_seq_kv_attn_workspace(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first) {
+  if (!cache || !step || !step->layout || cache->G < 1 || H < cache->G) return 0;
+  return stream_bytes(stream_plan(cache, step, H, window > 0 ? window : kKvNoWindow, first), cache, step, H);
+}
+
+KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const kb2_seq_kv_step* step, const void* q, int dt_q, long long ldq, long long hq, int H,
+                               float scale, int window, int first, const float* sinks, void* out, int dt_out, void* work, size_t work_bytes, void* stream) {
+  KvLayer c;
+  KvStep t;
+  if (int e = kv_args("kv_attn", cache, layer, step, &c, &t)) return e;
+  if (!q || !out || bad_dt(dt_q) || bad_dt(dt_out) || H < c.G || H % c.G || window < 0 || first < 0) return failf(KB2SEQ_ERR_VALUE, "kv_attn: bad argument");
+  if (c.G > 65535) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many heads");
+  if (t.T == 0) return KB2SEQ_OK;
+  OnDevice on(step->device);
+  SEQ_CUDA(on.err);
+  const int win = window > 0 ? std::min(window, kKvNoWindow) : kKvNoWindow;
+  const StreamPlan p = stream_plan(cache, step, H, win, first);
+  if (p.tiles == 0) return KB2SEQ_OK;
+  if (work_bytes < stream_bytes(p, cache, step, H) || (p.pieces > 1 && (!work || ((uintptr_t)work & 15))))
+    return failf(KB2SEQ_ERR_VALUE, "kv_attn: workspace of %zu bytes, %zu needed", work_bytes, stream_bytes(p, cache, step, H));
+  KvAttn a{};
+  a.q = q;
+  a.ldq = ldq;
+  a.hq = hq;
+  a.dtq = dt_q;
+  a.H = H;
+  a.window = win;
+  a.first = first;
+  a.scale = scale;
+  a.sinks = sinks;
+  a.out = out;
+  a.dt_out = dt_out;
+  a.per_seq = p.per_seq;
+  a.piece = p.piece;
+  a.pieces = p.pieces;
+  a.part_o = (float*)work;
+  a.part_ml = a.part_o + (size_t)t.T * H * p.pieces * c.dv;
+  const int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, a, p, (cudaStream_t)stream) : stream_sizes<KV_INT8>(c, t, a, p, (cudaStream_t)stream);
+  if (e || p.pieces == 1) return e;
+  kb2::launch_pdl(kv_join_kernel, (unsigned)(((long long)t.T * H + 3) / 4), 128, 0, (cudaStream_t)stream, c, t, a, p.tile_rows);
+  SEQ_LAUNCHED();
+  return KB2SEQ_OK;
+}
+
+}  // extern "C"

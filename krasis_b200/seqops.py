@@ -65,6 +65,11 @@ SIGNATURES = {
     "kb2_seq_rms_rows": (_I, [_P, _L, _I, _P, _F, _P, _I, _L, _I, _P]),
     "kb2_seq_branch_merge": (_I, [_P, _P, _P, _P, _F, _F, _P, _I, _I, _P]),
     "kb2_seq_depth_mix": (_I, [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _P]),
+    "kb2_seq_kv_write": (_I, [_P, _I, _P, _P, _L, _L, _P, _L, _L, _I, _P]),
+    "kb2_seq_kv_read": (_I, [_P, _I, _P, _I, _I, _I, _P, _P, _I, _P]),
+    "kb2_seq_kv_attn_workspace": (C.c_size_t, [_P, _P, _I, _I, _I]),
+    "kb2_seq_kv_attn": (_I, [_P, _I, _P, _P, _I, _L, _L, _I, _F, _I, _I, _P, _P, _I, _P, C.c_size_t, _P]),
+    "kb2_seq_kv_keep": (_I, [_P, _P, _P, _I, _P]),
     "kb2_seq_stream_mix": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _I, _F, _P]),
 }
 
@@ -445,3 +450,163 @@ def stream_mix(xs: torch.Tensor, x0=None, y=None, mix=None, out=None, read=None,
     check(load().kb2_seq_stream_mix(xs.data_ptr(), n, _ptr(x0), _ptr(y), _ptr(mix), _ptr(out), _ptr(read), _ptr(norm), float(w_shift), _ptr(h),
                                     dt_code(out_dtype), T, W, float(eps), _s(xs)))
     return h
+
+
+# ------------------------------------------------------------------------------------------------ the 8-bit cache and what reads it
+
+class KvCacheArgs(C.Structure):
+    """kb2_seq_kv_cache."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P)] + [(n, _I) for n in ("layers", "pages", "page_size", "G", "d", "dv", "fmt")]
+
+
+class KvStepArgs(C.Structure):
+    """kb2_seq_kv_step."""
+    _fields_ = [(n, _P) for n in ("positions", "seq_of", "cu", "pages", "rows", "bits", "layout")] + [(n, _I) for n in ("words", "T", "S", "max_pages", "replayed", "device")]
+
+
+class DraftTables(StepTables):
+    """The tables of a step whose sequences bring drafted tokens: a tree each, which the model checks in one pass.
+
+    entries: [(tokens, start, state_slot, page_list, parents)]; parents[i] is the number of token i's parent among the tokens of its entry, a smaller one, or -1 where the
+    parent is the last committed token.  Token i's key and value lie in row start + i (`rows`); its position is start + its depth (`positions`, which rotations go by);
+    `bits` [T, words] int32 says which tokens of its entry it sees: itself and its ancestors.  device_buf and draft_buf, if given, receive the tables (a captured graph
+    reads them from fixed buffers): the first as in StepTables, the second int32 with `draft_numel` numbers."""
+
+    def __init__(self, entries, device, pad_pages_to: int = 1, device_buf=None, draft_buf=None):
+        import numpy as np
+        for tokens, _, _, _, parents in entries:
+            if len(parents) != len(tokens):
+                raise ValueError("one parent per drafted token")
+            if any(not -1 <= p < i for i, p in enumerate(parents)):
+                raise ValueError("a drafted token's parent comes before it, or is -1")
+        if (device_buf is None) != (draft_buf is None):
+            raise ValueError("device_buf and draft_buf go together")
+        super().__init__([e[:4] for e in entries], device, pad_pages_to, device_buf)
+        T = self.T
+        self.words = max(1, (self.max_portion + 31) // 32)
+        self.draft_numel = T * (1 + self.words)
+        host = torch.zeros(self.draft_numel, dtype=torch.int32, pin_memory=torch.cuda.is_available())
+        a = host.numpy()
+        positions, bits, row = a[:T], a[T:].reshape(T, self.words).view(np.uint32), 0
+        for _, start, _, _, parents in entries:
+            for i, p in enumerate(parents):
+                positions[row + i] = start if p < 0 else positions[row + p] + 1
+                if p >= 0:
+                    bits[row + i] = bits[row + p]
+                bits[row + i, i // 32] |= np.uint32(1 << i % 32)
+            row += len(parents)
+        if draft_buf is not None:
+            if draft_buf.numel() != self.draft_numel:
+                raise ValueError("draft_buf does not fit this step's tables")
+            draft_buf.copy_(host, non_blocking=True)
+            self.draft_buf = draft_buf
+        else:
+            self.draft_buf = host.to(device, non_blocking=True)
+        self._draft_host = host
+        self.rows, self.positions, self.bits = self.positions, self.draft_buf[:T], self.draft_buf[T:].view(T, self.words)
+        self.h2d_bytes += 4 * self.draft_numel
+
+
+def _kv_step(tb: StepTables):
+    """The tables as the C interface takes them; made once per step, and again if the step's layout is set anew."""
+    kept = getattr(tb, "_kv_step", None)
+    if kept is not None and kept[1] is tb._layout_host:
+        return kept[0]
+    rows, bits = getattr(tb, "rows", None), getattr(tb, "bits", None)
+    a = KvStepArgs(tb.positions.data_ptr(), tb.seq_of.data_ptr(), tb.cu.data_ptr(), tb.pages.data_ptr(), _ptr(rows), _ptr(bits), tb.layout_ptr,
+                   tb.words if bits is not None else 0, tb.T, tb.S, tb.max_pages, int(tb.replayed), tb.buf.get_device())
+    tb._kv_step, tb._kv_sizes = (a, tb._layout_host), {}
+    return a
+
+
+def _kv_call(name, tb, cache, *tensors):
+    """(cache, tables) for the C interface; everything on one GPU."""
+    dev = tb.buf.get_device()
+    if dev < 0 or cache.k.get_device() != dev or any(t.get_device() != dev for t in tensors):
+        raise ValueError(f"{name}: the tables, the cache and the tensors belong on one CUDA device (krasis_b200 has no CPU path)")
+    return C.byref(cache.args), C.byref(_kv_step(tb))
+
+
+def _kv_rows(name, what, t, T, heads, width):
+    if t.dim() != 3 or t.shape[0] != T or t.shape[1] != heads or t.shape[2] != width:
+        raise ValueError(f"{name}: {what} has shape {tuple(t.shape)}, expected {(T, heads, width)}")
+    if t.stride(2) != 1 and width > 1:
+        raise ValueError(f"{name}: the numbers of a head of {what} lie side by side")
+
+
+def kv_write(k: torch.Tensor, v: torch.Tensor, tb: StepTables, cache, layer: int):
+    """Quantises the step's keys k [T, G, d] and values v [T, G, dv] (fp32 or bfloat16, any strides with a unit last one) into the pages of a CompactKVCache."""
+    p, q = _kv_call("kv_write", tb, cache, k, v)
+    _kv_rows("kv_write", "k", k, tb.T, cache.num_kv_heads, cache.dim)
+    _kv_rows("kv_write", "v", v, tb.T, cache.num_kv_heads, cache.vdim)
+    if k.dtype != v.dtype:
+        raise ValueError(f"kv_write: k is {k.dtype}, v {v.dtype}")
+    dt = dt_code(k.dtype)
+    check(load().kb2_seq_kv_write(p, layer, q, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dt, _s(k)))
+
+
+def kv_read(tb: StepTables, s: int, first: int, count: int, cache, layer: int, dtype=torch.bfloat16):
+    """Rows first .. first + count - 1 of the step's sequence s: (keys [count, G, d], values [count, G, dv]) in float32 or bfloat16."""
+    p, q = _kv_call("kv_read", tb, cache)
+    if not 0 <= s < tb.S or first < 0 or count < 0:
+        raise ValueError(f"kv_read: {count} rows from {first} of sequence {s} of {tb.S}")
+    dt, G = dt_code(dtype), cache.num_kv_heads
+    k = torch.empty((count, G, cache.dim), dtype=dtype, device=cache.k.device)
+    v = torch.empty((count, G, cache.vdim), dtype=dtype, device=cache.k.device)
+    check(load().kb2_seq_kv_read(p, layer, q, s, first, count, k.data_ptr(), v.data_ptr(), dt, _s(cache.k)))
+    return k, v
+
+
+def _kv_attend(name, q, tb, cache, layer, scale, window, first, sinks, dtype, out):
+    p, st = _kv_call(name, tb, cache, q)
+    H, G, T = q.shape[1] if q.dim() == 3 else 0, cache.num_kv_heads, tb.T
+    _kv_rows(name, "q", q, T, H, cache.dim)
+    if H == 0 or H % G:
+        raise ValueError(f"{name}: {H} heads on {G} key / value heads")
+    if (window is not None and window < 1) or first < 0:
+        raise ValueError(f"{name}: a window of {window} with {first} first tokens")
+    window = 0 if window is None else min(int(window), 1 << 30)
+    first = min(int(first), 1 << 30)
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != H or not sinks.is_contiguous() or sinks.get_device() != q.get_device()):
+        raise ValueError(f"{name}: one fp32 sink per head")
+    if out is None:
+        out = torch.empty((T, H, cache.vdim), dtype=q.dtype if dtype is None else dtype, device=q.device)
+    elif out.shape != (T, H, cache.vdim) or not out.is_contiguous() or out.get_device() != q.get_device() or (dtype is not None and out.dtype != dtype):
+        raise ValueError(f"{name}: out is a contiguous {(T, H, cache.vdim)}")
+    dq, do = dt_code(q.dtype), dt_code(out.dtype)
+    lib, key = load(), (G, cache.vdim, cache.page_size, H, window, first)
+    size = tb._kv_sizes.get(key)
+    if size is None:
+        size = tb._kv_sizes[key] = lib.kb2_seq_kv_attn_workspace(p, st, H, window, first)
+    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    check(lib.kb2_seq_kv_attn(p, layer, st, q.data_ptr(), dq, q.stride(0), q.stride(1), H, float(scale), window, first, _ptr(sinks), out.data_ptr(), do,
+                              _ptr(work), size, _s(q)))
+    return out
+
+
+def kv_attn(q: torch.Tensor, tb: StepTables, cache, layer: int, scale: float, window=None, first: int = 0, sinks=None, dtype=None, out=None) -> torch.Tensor:
+    """Softmax attention of q [T, H, d] (fp32 or bfloat16) over a CompactKVCache that holds the step's own rows already (kv_write): [T, H, dv] in `dtype` (q's own).
+    A token at position p sees row j <= p if p - j < window (None: no window) or j < first: the sequence's first tokens stay visible.  sinks [H] fp32: exp(sinks[h])
+    joins head h's softmax denominator.  float32 results carry 22 bits of queries and weights, bfloat16 ones 11."""
+    if isinstance(tb, DraftTables):
+        raise ValueError("kv_attn: drafted tokens see a tree: kv_tree_attn")
+    return _kv_attend("kv_attn", q, tb, cache, layer, scale, window, first, sinks, dtype, out)
+
+
+def kv_tree_attn(q: torch.Tensor, tb: DraftTables, cache, layer: int, scale: float, window=None, first: int = 0, sinks=None, dtype=None, out=None) -> torch.Tensor:
+    """kv_attn for drafted tokens: each sees the committed rows of its sequence by the rule of kv_attn, with its own position start + depth, and of the drafted ones itself
+    and its ancestors as far as the rule reaches."""
+    if not isinstance(tb, DraftTables):
+        raise ValueError("kv_tree_attn: the step's tables are DraftTables")
+    return _kv_attend("kv_tree_attn", q, tb, cache, layer, scale, window, first, sinks, dtype, out)
+
+
+def kv_keep(tb: DraftTables, path: torch.Tensor, cache):
+    """Moves the rows of accepted drafted tokens to the front, in all layers: row start + path[s, i] becomes row start + i.  path [S, P] int32: rising token numbers per
+    sequence, ended by -1 (or by any number that does not rise or is no token of the sequence).  The sequence then has start + (its path's length) rows."""
+    if not isinstance(tb, DraftTables):
+        raise ValueError("kv_keep: the step's tables are DraftTables")
+    p, q = _kv_call("kv_keep", tb, cache, path)
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != tb.S or not path.is_contiguous():
+        raise ValueError(f"kv_keep: path is a contiguous int32 [{tb.S}, P]")
+    check(load().kb2_seq_kv_keep(p, q, path.data_ptr(), path.shape[1], _s(path)))
