@@ -32,6 +32,7 @@ __device__ __forceinline__ long long kv_row(const KvLayer& c, const KvStep& t, i
 // What the tokens t0 .. t1 of sequence s see at all, in groups of 16 positions: the groups 0 .. na - 1 of the first tokens, then nb groups from b0 on.
 struct KvSpan {
   int na, b0, nb, base;                      // base: the first drafted row, or past every position
+  int lo, hi;                                // seen are the positions below `first` and lo .. hi - 1
   __device__ __forceinline__ int groups() const { return na + nb; }
   __device__ __forceinline__ int group(int i) const { return i < na ? i : b0 + i - na; }
 };
@@ -45,7 +46,7 @@ __device__ __forceinline__ KvSpan kv_span(const KvLayer& c, const KvStep& t, int
     lo = r.base;
     hi = r.base + (t1 - c0) + 1;
   } else {
-    r.base = kKvNoWindow * 2 - 1;
+    r.base = 0x7FFFFFFF;
     lo = t.positions[t0];
     hi = t.positions[t1] + 1;
   }
@@ -53,18 +54,23 @@ __device__ __forceinline__ KvSpan kv_span(const KvLayer& c, const KvStep& t, int
   lo = window < kKvNoWindow ? max(0, lo - window + 1) : 0;
   r.na = (min(min(first, lo), max(hi, 0)) + kKvGroup - 1) / kKvGroup;
   r.b0 = max(lo / kKvGroup, r.na);
+  r.lo = lo;
+  r.hi = hi;
   r.nb = max(0, (hi + kKvGroup - 1) / kKvGroup - r.b0);
   return r;
 }
 
-// The next (sequence, tile) of `rows` rows a tile, `per` rows a token: tile number `at` of the step.  One warp; false behind the last tile.
-__device__ __forceinline__ bool kv_find_tile(const KvStep& t, int per, int rows, int at, int* seq, int* tile) {
+// Tile number `at` of the sequences that have least .. most rows, `per` a token and `rows` a tile.  One warp; false behind the last tile.
+__device__ __forceinline__ bool kv_find_tile(const KvStep& t, int per, int rows, int least, int most, int at, int* seq, int* tile) {
   const int lane = threadIdx.x & 31;
   int before = 0;
   for (int s0 = 0; s0 < t.S; s0 += 32) {
     const int s = s0 + lane;
     int n = 0;
-    if (s < t.S) n = (int)(((long long)(t.cu[s + 1] - t.cu[s]) * per + rows - 1) / rows);
+    if (s < t.S) {
+      const int have = (t.cu[s + 1] - t.cu[s]) * per;
+      n = have >= least && have <= most ? (have + rows - 1) / rows : 0;
+    }
     int upto = n;                            // tiles up to and with sequence s
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

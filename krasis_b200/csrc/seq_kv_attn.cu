@@ -13,47 +13,17 @@
 // fp16 numbers with 22 together (PARTS 2, for fp32 results).  Scores, maxima and sums are fp32; the key's scale multiplies the fp32 score.  The weight times the value's
 // scale is rounded to fp16, relative to a reference R of its own that follows the largest such product (2^6 to 2^15 of it), so that small scales or weights do not
 // fall out of fp16's range: 11 bits, or 22 with PARTS 2, down to 2^-30 of the largest.
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
-#include "ptx.cuh"
-#include "seq_kv.cuh"
+#include "seq_kv_attn.cuh"
 
 namespace kb2seq {
 namespace {
 
 constexpr int kSWarps = 8, kSStages = 3, kSMostGroups = 1024;
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// bytes 0, 1 and bytes 2, 3 of a word of codes as pairs of fp16
-template <int FMT>
-__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (FMT == KV_E4M3) {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-  } else {
-    const uint32_t u = w ^ 0x80808080u;                      // 0 .. 255 for -128 .. 127: 0x6400 + u is the fp16 number 1024 + u
-    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  }
-}
-__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 f16_get(uint32_t p) { return __half22float2(*reinterpret_cast<const __half2*>(&p)); }
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -68,20 +38,6 @@ __device__ __forceinline__ void sts4(uint32_t a, uint32_t v) { asm volatile("st.
 __device__ __forceinline__ void cp_async8(uint32_t to, const void* from, bool in) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(in ? 8 : 0) : "memory");
 }
-__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-struct KvAttn {                              // what a call says beside the cache and the tables
-  const void* q;
-  long long ldq, hq;
-  int dtq, H, window, first;
-  float scale;
-  const float* sinks;
-  void* out;
-  int dt_out, per_seq;                       // per_seq: tiles of every sequence where all bring as many tokens, else 0
-  int piece, pieces;                         // groups of 16 keys a piece; the most pieces of a tile
-  float *part_o, *part_ml;                   // [T H][pieces][dv] and [T H][pieces][2]
-};
-
 // DU, VU: units of 64 of d and dv.
 template <int DU, int VU, int NQ, int PARTS>
 struct StreamShape {
@@ -109,7 +65,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   if (a.per_seq) {
     s = blockIdx.x / a.per_seq;
     tile = blockIdx.x - s * a.per_seq;
-  } else if (!kv_find_tile(t, per, MT, blockIdx.x, &s, &tile)) {
+  } else if (!kv_find_tile(t, per, MT, a.least, a.most, blockIdx.x, &s, &tile)) {
     return;
   }
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * MT, nr = (int)min((long long)n * per - r0, (long long)MT);
@@ -166,7 +122,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   float rf[NQ];
   int pos[NQ], tok[NQ];
   float m[NQ], l[NQ], ref[NQ];
-  int pmin = 0x7FFFFFFF, pmax = -1;
+  int pmin, pmax;
 #pragma unroll
   for (int h = 0; h < NQ; ++h) {
     const int r = g8 + 8 * h;
@@ -190,10 +146,9 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^e brings the largest below 2^15; of a row of smallest or no numbers, or of one that is not finite, it stays within fp32
-    const int e = min(max(141 - (int)(top >> 23), -113), 100);
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    rf[h] = a.scale * kLog2e * __uint_as_float((uint32_t)(127 - e) << 23);
+    float up, down;
+    kv_row_scale(top, &up, &down);
+    rf[h] = a.scale * kLog2e * down;
 #pragma unroll
     for (int i = 0; i < DU; ++i)
 #pragma unroll
@@ -217,14 +172,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
           }
         }
   }
-  {
-    const int p0 = t.positions[t0], p1 = t.positions[t1];    // of a portion: the first and the last; of a tree: anything from base on
-    pmin = span.base < kKvNoWindow ? span.base : p0;
-    pmax = p1;
-    if (span.base < kKvNoWindow) {
-      for (int x = t0; x <= t1; ++x) pmax = max(pmax, t.positions[x]);
-    }
-  }
+  kv_reach(t, span, t0, t1, &pmin, &pmax);
   if constexpr (L::kQShared) __syncthreads();
 
   float o[MV][NQ][4];
@@ -235,16 +183,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][h][e] = 0.f;
 
-  const auto sees = [&](int j, int h) {      // row h of the lane, position j
-    if (r0 + g8 + 8 * h >= r0 + nr) return false;
-    int spot = j;
-    if (j >= span.base) {
-      const int i = j - span.base;
-      if (i >= n || !(t.bits[(long long)tok[h] * t.words + (i >> 5)] >> (i & 31) & 1u)) return false;
-      spot = t.positions[c0 + i];
-    }
-    return spot <= pos[h] && (pos[h] - spot < a.window || spot < a.first);
-  };
+  const auto sees = [&](int j, int h) { return g8 + 8 * h < nr && kv_sees(t, a, span, c0, n, tok[h], pos[h], j); };      // row h of the lane, position j
 
   int st = 0;
   for (int u = u0 + warp; u < u1; u += kSWarps) {
@@ -433,14 +372,16 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   }
 }
 
-// The pieces of a row, joined in their order.  One warp a row (token, head); rows that one piece finished are left alone.
-__global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAttn a, int tile_rows) {
+// The pieces of a row, joined in their order.  One warp a row (token, head); rows that one piece finished are left alone.  x, y: the two kinds of sequences.
+__global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAttn x, KvAttn y) {
   kb2::pdl_wait();
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, tok = (int)(row / a.H), hd = (int)(row - (long long)tok * a.H);
+  const int lane = threadIdx.x & 31, tok = (int)(row / x.H), hd = (int)(row - (long long)tok * x.H);
   if (tok >= t.T || tok >= t.cu[t.S]) return;
-  const int per = a.H / c.G, s = t.seq_of[tok], c0 = t.cu[s], n = t.cu[s + 1] - c0;
-  const int r0 = ((tok - c0) * per + hd % per) / tile_rows * tile_rows, nr = (int)min((long long)n * per - r0, (long long)tile_rows);
+  const int per = x.H / c.G, s = t.seq_of[tok], c0 = t.cu[s], n = t.cu[s + 1] - c0;
+  const KvAttn& a = n * per <= x.most ? x : y;
+  if (a.pieces <= 1) return;
+  const int r0 = ((tok - c0) * per + hd % per) / a.rows * a.rows, nr = (int)min((long long)n * per - r0, (long long)a.rows);
   const KvSpan span = kv_span(c, t, s, c0 + r0 / per, c0 + (r0 + nr - 1) / per, a.window, a.first);
   const int np = min((span.groups() + a.piece - 1) / a.piece, a.pieces);
   if (np <= 1) return;
@@ -467,46 +408,87 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// How a call's keys are cut.  groups: the most groups of 16 keys that a sequence's tokens see.
-struct StreamPlan {
-  int tile_rows, tiles, per_seq, piece, pieces;
+// Rows per kv head (a sequence's tokens times the heads that share one) from which a sequence runs on the tensor cores' tiles of 128.
+constexpr int kTileFrom = 17;
+// How the sequences of one kind are cut: into tiles of rows, and the keys that a tile sees (in groups of 16) into pieces.
+struct KvPlan {
+  int least, most, rows, tiles, per_seq, piece, pieces;
+  size_t floats;                             // workspace
 };
+// The most groups of 16 that the tokens start .. start + n - 1 see.
 inline long long groups_seen(long long start, long long n, int window, int first) {
   const long long lo = window < kKvNoWindow ? std::max(0ll, start - window + 1) : 0;
   return (start + n - lo + 30) / 16 + (std::min<long long>(first, lo) + 15) / 16;
 }
-StreamPlan stream_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first) {
-  StreamPlan p{};
+KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int least, int most, bool wide) {
+  KvPlan p{};
   const int per = H / cache->G;
-  long long most = 0, work = 0, rows = 0;
+  long long top = 0, work = 0, rows = 0;
   bool same = true;
-  for (int s = 0; s < step->S; ++s) rows = std::max(rows, (long long)step->layout[4 * s + 1] * per);
-  p.tile_rows = rows <= 8 ? 8 : 16;
+  for (int s = 0; s < step->S; ++s) {
+    const long long r = (long long)step->layout[4 * s + 1] * per;
+    if (r >= least && r <= most) rows = std::max(rows, r);
+  }
+  p.least = least;
+  p.most = most;
+  p.rows = wide ? kTileRows : rows <= 8 ? 8 : 16;
   for (int s = 0; s < step->S; ++s) {
     const int* l = step->layout + 4 * s;
-    const int tiles = (int)(((long long)l[1] * per + p.tile_rows - 1) / p.tile_rows);
+    const long long r = (long long)l[1] * per;
+    same = same && l[1] == step->layout[1];
+    if (r < least || r > most || r == 0) continue;
+    const int tiles = (int)((r + p.rows - 1) / p.rows);
     // captured launches are run again with later positions: what the page lists hold
     const long long end = step->replayed ? (long long)step->max_pages * cache->page_size : (long long)l[2] + l[1];
-    const long long g = l[1] ? groups_seen(end - l[1], l[1], window, first) : 0;
+    const long long g = groups_seen(end - l[1], l[1], window, first);
     p.tiles += tiles;
-    most = std::max(most, g);
+    top = std::max(top, g);
     work += g * tiles;
-    same = same && l[1] == step->layout[1];
   }
-  p.per_seq = same && p.tiles ? p.tiles / step->S : 0;
-  const long long want = 4ll * 2 * kb2::current_sms();                     // blocks
-  long long piece = std::max((work * cache->G + want - 1) / want, (most + 63) / 64);
-  piece = std::min<long long>((piece + kSWarps - 1) / kSWarps * kSWarps, kSMostGroups);
-  p.piece = (int)std::max<long long>(piece, kSWarps);
-  p.pieces = (int)std::max(1ll, (most + p.piece - 1) / p.piece);
+  if (p.tiles == 0) return p;
+  p.per_seq = same ? p.tiles / step->S : 0;
+  long long piece;
+  if (wide) {                                // one block an SM, two to four tiles of keys a piece at least
+    const long long want = 2ll * kb2::current_sms();
+    piece = std::max((work * cache->G + want - 1) / want, std::max(16ll, (top + 63) / 64));
+    piece = (piece + 7) / 8 * 8;
+    if ((long long)p.tiles * cache->G >= want) piece = (top + 7) / 8 * 8;
+  } else {
+    const long long want = 4ll * 2 * kb2::current_sms();
+    piece = std::max((work * cache->G + want - 1) / want, (top + 63) / 64);
+    piece = std::min<long long>((piece + kSWarps - 1) / kSWarps * kSWarps, kSMostGroups);
+    piece = std::max<long long>(piece, kSWarps);
+  }
+  p.piece = (int)std::max(piece, 8ll);
+  p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
+  p.floats = p.pieces > 1 ? (size_t)step->T * H * p.pieces * (cache->dv + 2) : 0;
   return p;
 }
-inline size_t stream_bytes(const StreamPlan& p, const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H) {
-  return p.pieces > 1 ? (size_t)step->T * H * p.pieces * (cache->dv + 2) * 4 : 0;
+struct KvPlans {
+  KvPlan few, many;
+  size_t bytes() const { return (few.floats + many.floats) * 4; }
+};
+KvPlans kv_plans(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int dt_out) {
+  const int split = dt_out ? kTileFrom - 1 : 0x7FFFFFFF;                   // fp32 results carry 22 bits: the tiles have 11
+  KvPlans p{};
+  p.few = kv_plan(cache, step, H, window, first, 1, split, false);
+  if (dt_out) p.many = kv_plan(cache, step, H, window, first, split + 1, 0x7FFFFFFF, true);
+  return p;
+}
+inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, int dv) {
+  a.least = p.least;
+  a.most = p.most;
+  a.rows = p.rows;
+  a.per_seq = p.per_seq;
+  a.piece = p.piece;
+  a.pieces = p.pieces;
+  a.part_o = work;
+  a.part_ml = work + (size_t)rows_total * p.pieces * dv;
+  return a;
 }
 
 template <int FMT, int DU, int VU, int NQ, int PARTS>
-int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const StreamPlan& p, cudaStream_t st) {
+int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
   using L = StreamShape<DU, VU, NQ, PARTS>;
   SEQ_CUDA((kb2::allow_smem<kv_stream_kernel<FMT, DU, VU, NQ, PARTS>>(L::kTotal)));
   auto kern = kv_stream_kernel<FMT, DU, VU, NQ, PARTS>;
@@ -515,12 +497,12 @@ int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const Stre
   return KB2SEQ_OK;
 }
 template <int FMT, int DU, int VU>
-int stream_rows(const KvLayer& c, const KvStep& t, const KvAttn& a, const StreamPlan& p, cudaStream_t st) {
-  if (p.tile_rows == 8) return a.dt_out ? stream_launch<FMT, DU, VU, 1, 1>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 1, 2>(c, t, a, p, st);
+int stream_rows(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
+  if (p.rows == 8) return a.dt_out ? stream_launch<FMT, DU, VU, 1, 1>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 1, 2>(c, t, a, p, st);
   return a.dt_out ? stream_launch<FMT, DU, VU, 2, 1>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 2, 2>(c, t, a, p, st);
 }
 template <int FMT>
-int stream_sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, const StreamPlan& p, cudaStream_t st) {
+int stream_sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
   if (c.d <= 64 && c.dv <= 64) return stream_rows<FMT, 1, 1>(c, t, a, p, st);
   if (c.d <= 128 && c.dv <= 128) return stream_rows<FMT, 2, 2>(c, t, a, p, st);
   if (c.d <= 192 && c.dv <= 128) return stream_rows<FMT, 3, 2>(c, t, a, p, st);
@@ -534,9 +516,9 @@ using namespace kb2seq;
 
 extern "C" {
 
-KB2SEQ_API size_t kb2_seq_kv_attn_workspace(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first) {
-  if (!cache || !step || !step->layout || cache->G < 1 || H < cache->G) return 0;
-  return stream_bytes(stream_plan(cache, step, H, window > 0 ? window : kKvNoWindow, first), cache, step, H);
+KB2SEQ_API size_t kb2_seq_kv_attn_workspace(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int dt_out) {
+  if (!cache || !step || !step->layout || cache->G < 1 || H < cache->G || bad_dt(dt_out)) return 0;
+  return kv_plans(cache, step, H, window > 0 ? std::min(window, kKvNoWindow) : kKvNoWindow, first, dt_out).bytes();
 }
 
 KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const kb2_seq_kv_step* step, const void* q, int dt_q, long long ldq, long long hq, int H,
@@ -544,16 +526,16 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   KvLayer c;
   KvStep t;
   if (int e = kv_args("kv_attn", cache, layer, step, &c, &t)) return e;
-  if (!q || !out || bad_dt(dt_q) || bad_dt(dt_out) || H < c.G || H % c.G || window < 0 || first < 0) return failf(KB2SEQ_ERR_VALUE, "kv_attn: bad argument");
-  if (c.G > 65535) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many heads");
+  if (!q || !out || ((uintptr_t)out & 15) || bad_dt(dt_q) || bad_dt(dt_out) || H < c.G || H % c.G || window < 0 || first < 0)
+    return failf(KB2SEQ_ERR_VALUE, "kv_attn: bad argument");
+  if (c.G > 65535 || (long long)t.T * (H / c.G) > 0x7FFFFFFFll / 2) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many heads or tokens");
   if (t.T == 0) return KB2SEQ_OK;
   OnDevice on(step->device);
   SEQ_CUDA(on.err);
   const int win = window > 0 ? std::min(window, kKvNoWindow) : kKvNoWindow;
-  const StreamPlan p = stream_plan(cache, step, H, win, first);
-  if (p.tiles == 0) return KB2SEQ_OK;
-  if (work_bytes < stream_bytes(p, cache, step, H) || (p.pieces > 1 && (!work || ((uintptr_t)work & 15))))
-    return failf(KB2SEQ_ERR_VALUE, "kv_attn: workspace of %zu bytes, %zu needed", work_bytes, stream_bytes(p, cache, step, H));
+  const KvPlans p = kv_plans(cache, step, H, win, first, dt_out);
+  if (work_bytes < p.bytes() || (p.bytes() && (!work || ((uintptr_t)work & 15))))
+    return failf(KB2SEQ_ERR_VALUE, "kv_attn: workspace of %zu bytes, %zu needed", work_bytes, p.bytes());
   KvAttn a{};
   a.q = q;
   a.ldq = ldq;
@@ -566,14 +548,16 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   a.sinks = sinks;
   a.out = out;
   a.dt_out = dt_out;
-  a.per_seq = p.per_seq;
-  a.piece = p.piece;
-  a.pieces = p.pieces;
-  a.part_o = (float*)work;
-  a.part_ml = a.part_o + (size_t)t.T * H * p.pieces * c.dv;
-  const int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, a, p, (cudaStream_t)stream) : stream_sizes<KV_INT8>(c, t, a, p, (cudaStream_t)stream);
-  if (e || p.pieces == 1) return e;
-  kb2::launch_pdl(kv_join_kernel, (unsigned)(((long long)t.T * H + 3) / 4), 128, 0, (cudaStream_t)stream, c, t, a, p.tile_rows);
+  const KvAttn few = with_plan(a, p.few, (float*)work, t.T * H, c.dv), many = with_plan(a, p.many, (float*)work + p.few.floats, t.T * H, c.dv);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (p.many.tiles) {
+    if (int e = kv_tile_attend(cache->fmt, c, t, many, p.many.tiles, st)) return e;
+  }
+  if (p.few.tiles) {
+    if (int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, few, p.few, st) : stream_sizes<KV_INT8>(c, t, few, p.few, st)) return e;
+  }
+  if (p.few.pieces <= 1 && p.many.pieces <= 1) return KB2SEQ_OK;
+  kb2::launch_pdl(kv_join_kernel, (unsigned)(((long long)t.T * H + 3) / 4), 128, 0, st, c, t, few, many);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }

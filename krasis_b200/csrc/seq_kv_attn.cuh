@@ -1,0 +1,84 @@
+// Attention over the 8-bit cache: what its two kernels and their join share.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "ptx.cuh"
+#include "seq_kv.cuh"
+
+namespace kb2seq {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct KvAttn {                              // what a call says beside the cache and the tables
+  const void* q;
+  long long ldq, hq;
+  int dtq, H, window, first;
+  float scale;
+  const float* sinks;
+  void* out;
+  int dt_out;
+  int least, most, rows, per_seq;            // the sequences that have least .. most rows (tokens times heads per kv head), in tiles of `rows`; per_seq: the tiles of
+                                             // each where the step's sequences bring as many tokens each, else 0
+  int piece, pieces;                         // groups of 16 keys a piece; the most pieces of a tile
+  float *part_o, *part_ml;                   // [T H][pieces][dv] and [T H][pieces][2]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// bytes 0, 1 and bytes 2, 3 of a word of codes as pairs of fp16
+template <int FMT>
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == KV_E4M3) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u;                      // 0 .. 255 for -128 .. 127: 0x6400 + u is the fp16 number 1024 + u
+    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 f16_get(uint32_t p) { return __half22float2(*reinterpret_cast<const __half2*>(&p)); }
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// Whether token `tok` at position `pos` of a sequence (first token c0, n of them) sees its row j.
+__device__ __forceinline__ bool kv_sees(const KvStep& t, const KvAttn& a, const KvSpan& span, int c0, int n, int tok, int pos, int j) {
+  int spot = j;
+  if (j >= span.base) {
+    const int i = j - span.base;
+    if (i >= n || !(t.bits[(long long)tok * t.words + (i >> 5)] >> (i & 31) & 1u)) return false;
+    spot = t.positions[c0 + i];
+  }
+  return spot <= pos && (pos - spot < a.window || spot < a.first);
+}
+// The least and the most position of the tokens t0 .. t1: the first and the last of a portion; of a tree the least is any that is no more.
+__device__ __forceinline__ void kv_reach(const KvStep& t, const KvSpan& span, int t0, int t1, int* least, int* most) {
+  *least = t.positions[t0];
+  *most = t.positions[t1];
+  if (span.base < kKvNoWindow) {
+    *least = span.base;
+    for (int x = t0; x < t1; ++x) *most = max(*most, t.positions[x]);
+  }
+}
+
+// 2^e that brings a row's largest magnitude (its bits: top) below 2^15, and 2^-e.  Of a row of smallest numbers or one that is not finite both stay within fp32.
+__device__ __forceinline__ void kv_row_scale(uint32_t top, float* up, float* down) {
+  const int e = min(max(141 - (int)(top >> 23), -113), 100);
+  *up = __uint_as_float((uint32_t)(127 + e) << 23);
+  *down = __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+// Tiles of 128 rows on the tensor cores (seq_kv_tile.cu).
+int kv_tile_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t stream);
+constexpr int kTileRows = 128;
+
+}  // namespace kb2seq

@@ -1,0 +1,537 @@
+// Attention over the 8-bit cache for many query rows per key / value head (portions of prompts, trees of drafted tokens) on tcgen05.
+//
+// A tile is 128 (token, head) rows of one sequence and kv head: the H / G heads that share keys fill it together, so a key tile is decoded once for all of them.  Roles of
+// a CTA of 16 warps:
+//   warps 12-15  decode: codes from the pages into registers a job ahead, as fp16 into the swizzled operand tiles.  A row's scale over a power of two
+//                near the tile's largest one is multiplied in there (one packed product for two codes; exact for scales that are powers of two), the power joins the
+//                softmax's factor
+//   warp  0      tcgen05.mma: S = Q K^T, O += P V (P from tensor memory)
+//   warps 4-11   softmax, two threads a row
+// S and P have two buffers each.  FK = 128 keys a tile, 64 where d or dv is above 128 (tensor memory: 3 FK + dv columns).
+//
+// Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value scale are fp16 (11 bits).  Weights are rounded relative to a reference R per row
+// that follows the largest weight times scale (2^6 to 2^15 of it), as in the kernel for few rows; maxima, weights and their sum are fp32.
+// A row whose scale is NaN gets NaN keys and zero values: scores that nobody sees are replaced, and those that see it carry the NaN into the sum.
+#include "seq_kv_attn.cuh"
+
+namespace kb2seq {
+namespace {
+using namespace kb2;
+
+constexpr int kThreads = 512;
+
+template <int NC, int NV>                    // chunks of 64 of d and dv
+struct TileShape {
+  static constexpr int FK = NC > 2 || NV > 2 ? 64 : 128;
+  static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128;
+  static constexpr int kOffQ = 0, kOffK = kQ, kOffV = kOffK + 2 * kK, kOffBar = kOffV + 2 * kV, kOffRef = kOffBar + 128, kOffTmem = kOffRef + 32, kOffX = kOffTmem + 16, kOffRow = kOffX + 2 * 2 * 128 * 4;
+  static constexpr int kTotal = kOffRow + 128 * 4;
+  static_assert(kTotal <= 227 * 1024 && 3 * FK + 64 * NV <= 512, "memory");
+};
+
+__device__ __forceinline__ uint32_t idesc_f16(uint32_t n, bool mn) {       // A and B fp16, accumulator fp32, 128 rows; mn: B lies with its columns side by side
+  return (1u << 4) | ((uint32_t)mn << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// rows of 64 numbers (128 bytes) one key apart, chunks of 64 columns `chunk` bytes apart
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t chunk) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(chunk >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ float2 pair_get(uint64_t p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
+  return p;
+}
+__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+  uint64_t p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+  return p;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
+  uint64_t p;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+  return p;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+      "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// 2^-7 of the least power of two above a scale (its bits), and one over it: codes of 448 times 2^7 stay within fp16, and a scale keeps its bits down to 2^-21 of the
+// tile's largest.
+__device__ __forceinline__ void scale_unit(uint32_t bits, float* p, float* inv) {
+  const uint32_t e = min(max(bits >> 23, 8u), 252u) - 6;
+  *p = __uint_as_float(e << 23);
+  *inv = __uint_as_float((254 - e) << 23);
+}
+
+// What a decoding thread knows of a tile: it has the rows row0 + 32 i, and 16 bytes of each chunk of 64 of those.
+template <int NR>
+struct Where {
+  int r16[NR];                               // the rows' groups in the pools, -1: none
+  float ks[NR], vs[NR];
+  bool see[NR];
+  uint4 ks4, vs4;                            // scales of rows 4 lane .. 4 lane + 3 of the tile, zeros where nobody sees them
+};
+template <int NR, int CH>
+__device__ __forceinline__ void decode_load(const uint8_t* pool, int width, int ct, const Where<NR>& w, uint4 (&x)[NR * CH]) {
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+#pragma unroll
+    for (int h = 0; h < CH; ++h) {
+      const int e = h * 64 + (ct & 3) * 16, row = (ct >> 2) + 32 * i;
+      x[i * CH + h] = w.see[i] && e < width ? ld_stream16(pool + ((long long)w.r16[i] * kKvGroup + (row & 15)) * width + e) : make_uint4(0, 0, 0, 0);
+    }
+}
+// A warp's store of 16 bytes a lane meets 8 rows' swizzles, two of them in eight lanes: no bank twice.
+template <int FMT, int NR, int CH>
+__device__ __forceinline__ void decode_store(uint8_t* to, int ct, const float (&f)[NR], const uint4 (&x)[NR * CH]) {
+  const int q = ct & 3;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int row = (ct >> 2) + 32 * i;
+    const uint32_t m = f16_pair(f[i], f[i]);
+#pragma unroll
+    for (int h = 0; h < CH; ++h) {
+      const uint4 v = x[i * CH + h];
+      uint32_t y[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        codes_f16<FMT>(word(v, e), y[2 * e], y[2 * e + 1]);
+        y[2 * e] = hmul2(y[2 * e], m);
+        y[2 * e + 1] = hmul2(y[2 * e + 1], m);
+      }
+      uint8_t* p = to + h * (2048 * NR * 2) + row * 128;                   // chunks of 32 NR rows
+      *reinterpret_cast<uint4*>(p + (((2 * q) ^ (row & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(p + (((2 * q + 1) ^ (row & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+template <int FMT, int NC, int NV>
+__global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep t, KvAttn a) {
+  using L = TileShape<NC, NV>;
+  constexpr int FK = L::FK, GT = FK / kKvGroup;                            // groups a tile
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *s_cons = bars + 10, *p_full = bars + 12, *pv_done = bars + 14;
+  float2* refs = reinterpret_cast<float2*>(smem + L::kOffRef);             // [4] tile's powers of two: keys, values
+  float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [128] what the queries' own scaling is undone with
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&pv_done[i], 1);
+      mbar_init(&s_cons[i], 8);
+      mbar_init(&p_full[i], 8);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 2) tmem_alloc(tmem_at, 512);
+  pdl_wait();
+
+  // which tile, and what its rows see: the same in every warp
+  const int per = a.H / c.G, head = blockIdx.y;
+  int s = 0, tile = 0;
+  bool in = true;
+  if (a.per_seq) {
+    s = blockIdx.x / a.per_seq;
+    tile = blockIdx.x - s * a.per_seq;
+  } else {
+    in = kv_find_tile(t, per, kTileRows, a.least, a.most, blockIdx.x, &s, &tile);
+  }
+  const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * kTileRows, nr = in ? (int)min((long long)n * per - r0, (long long)kTileRows) : 0;
+  int u0 = 0, u1 = 0, np = 0, t0 = c0, t1 = c0;
+  KvSpan span{};
+  if (nr > 0) {
+    t0 = c0 + r0 / per;
+    t1 = c0 + (r0 + nr - 1) / per;
+    span = kv_span(c, t, s, t0, t1, a.window, a.first);
+    np = min((span.groups() + a.piece - 1) / a.piece, a.pieces);
+    u0 = blockIdx.z * a.piece;
+    u1 = min(span.groups(), u0 + a.piece);
+  }
+  const bool work = nr > 0 && (blockIdx.z == 0 || (int)blockIdx.z < np);   // piece 0 of a tile that sees nothing writes its zeros
+  const int n_tiles = work ? max(0, (u1 - u0 + GT - 1) / GT) : 0;
+
+  // queries, 8 rows a warp: scaled by a power of two, rounded to fp16, in the operand's layout (rows of 64 numbers, 16-byte pieces swizzled by the row)
+  if (work) {
+    const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;  // factors on scores are positive: a row's maximum is its largest raw score's
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+      const int r = warp * 8 + i, rr = r0 + r;
+      const bool row = r < nr;
+      const long long from = row ? (c0 + rr / per) * a.ldq + (head * per + rr % per) * a.hq : 0;
+      float x[2][4];
+      uint32_t top = 0;
+#pragma unroll
+      for (int b = 0; b < (NC + 1) / 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = b * 128 + lane * 4 + j;
+          x[b][j] = row && e < c.d ? (a.dtq ? __bfloat162float(((const bf16*)a.q)[from + e]) : ((const float*)a.q)[from + e]) : 0.f;
+          top = max(top, __float_as_uint(x[b][j]) & 0x7FFFFFFFu);
+        }
+      top = __reduce_max_sync(0xffffffffu, top);
+      float up, down;
+      kv_row_scale(top, &up, &down);
+      up *= sign;
+#pragma unroll
+      for (int b = 0; b < (NC + 1) / 2; ++b) {
+        const int e = b * 128 + lane * 4;
+        if (e < NC * 64)
+          *reinterpret_cast<uint2*>(smem + L::kOffQ + (e >> 6) * (128 * 128) + r * 128 + ((((e & 63) >> 3) ^ (r & 7)) << 4) + (e & 4) * 2) =
+              make_uint2(f16_pair(x[b][0] * up, x[b][1] * up), f16_pair(x[b][2] * up, x[b][3] * up));
+      }
+      if (lane == 0) rows_down[r] = sign == 0.f ? 1.f : fabsf(a.scale) * kLog2e * down;
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_at;
+  constexpr uint32_t kColS = 0, kColP = 2 * FK, kColO = 3 * FK;
+
+  if (n_tiles == 0) {
+    if (work && warp >= 4 && warp < 12) {                                  // nothing to see (no piece shares this tile): zeros
+      for (int i = (warp - 4) * 32 + lane; i < nr * c.dv; i += 256) {
+        const int r = i / c.dv, rr = r0 + r;
+        st_dt(a.out, a.dt_out, ((long long)(c0 + rr / per) * a.H + head * per + rr % per) * c.dv + i - r * c.dv, 0.f);
+      }
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------ decode
+    const int ct = threadIdx.x - 384, row0 = ct >> 2;
+    constexpr int NR = FK / 32;
+    const auto at_row = [&](int u, int* r16) {
+      const long long r = u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
+      *r16 = r < 0 ? -1 : (int)((r + ((long long)head << c.lps)) / kKvGroup);
+    };
+    const auto seen = [&](int u, int row) {  // by any row of the tile
+      const int j = span.group(u) * kKvGroup + (row & 15);
+      return j < span.hi && (j >= span.lo || j < a.first);
+    };
+    const auto where = [&](int it, Where<NR>& w) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int row = row0 + 32 * i, u = u0 + it * GT + row / 16;
+        at_row(u, &w.r16[i]);
+        w.see[i] = w.r16[i] >= 0 && seen(u, row);
+        w.ks[i] = w.vs[i] = 0.f;
+        if (w.see[i]) {
+          const long long r = (long long)w.r16[i] * kKvGroup + (row & 15);
+          w.ks[i] = c.ks[r];
+          w.vs[i] = c.vs[r];
+        }
+      }
+      w.ks4 = w.vs4 = make_uint4(0, 0, 0, 0);
+      if (lane * 4 < FK) {
+        const int u = u0 + it * GT + lane / 4;
+        int r16;
+        at_row(u, &r16);
+        if (r16 >= 0) {
+          const long long r = (long long)r16 * kKvGroup + (lane & 3) * 4;
+          w.ks4 = *reinterpret_cast<const uint4*>(c.ks + r);
+          w.vs4 = *reinterpret_cast<const uint4*>(c.vs + r);
+          uint32_t* k = reinterpret_cast<uint32_t*>(&w.ks4);
+          uint32_t* v = reinterpret_cast<uint32_t*>(&w.vs4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool no = !seen(u, (lane & 3) * 4 + e);
+            if (no || k[e] >= 0x7F800000u) k[e] = 0;
+            if (no || v[e] >= 0x7F800000u) v[e] = 0;
+          }
+        }
+      }
+    };
+    Where<NR> w, next;
+    uint4 xk[NR * NC], xv[NR * NV];
+    where(0, w);
+    decode_load<NR, NC>(c.k, c.d, ct, w, xk);
+    decode_load<NR, NV>(c.v, c.dv, ct, w, xv);
+    for (int it = 0; it < n_tiles; ++it) {
+      const int b = it & 1;
+      if (it + 1 < n_tiles) where(it + 1, next);
+      // the tile's largest scales
+      const uint32_t kt = __reduce_max_sync(0xffffffffu, max(max(w.ks4.x, w.ks4.y), max(w.ks4.z, w.ks4.w)));
+      const uint32_t vt = __reduce_max_sync(0xffffffffu, max(max(w.vs4.x, w.vs4.y), max(w.vs4.z, w.vs4.w)));
+      float kp, ki, vp, vi, fk[NR], fv[NR];
+      scale_unit(kt, &kp, &ki);
+      scale_unit(vt, &vp, &vi);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const bool nan_v = w.vs[i] != w.vs[i];
+        fk[i] = nan_v ? w.vs[i] : w.ks[i] * ki;
+        fv[i] = nan_v ? 0.f : w.vs[i] * vi;
+      }
+      mbar_wait(&k_empty[b], (it >> 1 & 1) ^ 1);
+      decode_store<FMT, NR, NC>(smem + L::kOffK + b * L::kK, ct, fk, xk);
+      if (ct == 0) refs[it & 3] = make_float2(kp, vt ? vp : 0.f);
+      if (lane == 0) mbar_arrive(&k_full[b]);
+      if (it + 1 < n_tiles) decode_load<NR, NC>(c.k, c.d, ct, next, xk);
+      mbar_wait(&v_empty[b], (it >> 1 & 1) ^ 1);
+      decode_store<FMT, NR, NV>(smem + L::kOffV + b * L::kV, ct, fv, xv);
+      if (lane == 0) mbar_arrive(&v_full[b]);
+      if (it + 1 < n_tiles) decode_load<NR, NV>(c.v, c.dv, ct, next, xv);
+      w = next;
+    }
+  } else if (warp == 0) {
+    // ------------------------------------------------------------ tensor cores
+    const uint32_t id_s = idesc_f16(FK, false), id_o = idesc_f16(64 * NV, true);
+    const uint32_t q_at = smem_u32(smem + L::kOffQ);
+    const auto scores = [&](int it) {
+      const int b = it & 1;
+      mbar_wait(&k_full[b], it >> 1 & 1);
+      if (it >= 2) mbar_wait(&s_cons[b], (it >> 1 & 1) ^ 1);
+      tc_fence_after_sync();
+      const uint32_t k_at = smem_u32(smem + L::kOffK + b * L::kK);
+      if (elect_one()) {
+#pragma unroll
+        for (int h = 0; h < NC; ++h) {
+          const uint64_t ad = umma_desc_k_sw128(q_at + h * (128 * 128)), bd = umma_desc_k_sw128(k_at + h * (FK * 128));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16(tmem + kColS + b * FK, ad + 2 * k, bd + 2 * k, id_s, h > 0 || k > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[b]);
+        umma_commit(&k_empty[b]);
+      }
+      __syncwarp();
+    };
+    scores(0);
+    if (n_tiles > 1) scores(1);
+    for (int it = 0; it < n_tiles; ++it) {
+      const int b = it & 1;
+      if (it + 2 < n_tiles) scores(it + 2);
+      mbar_wait(&v_full[b], it >> 1 & 1);
+      mbar_wait(&p_full[b], it >> 1 & 1);
+      tc_fence_after_sync();
+      const uint32_t v_at = smem_u32(smem + L::kOffV + b * L::kV);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < FK / 16; ++k)
+          umma_bf16_ts(tmem + kColO, tmem + kColP + b * (FK / 2) + 8 * k, desc_mn(v_at + k * 2048, FK * 128), id_o, it > 0 || k > 0 ? 1u : 0u);
+        umma_commit(&pv_done[b]);
+        umma_commit(&v_empty[b]);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax: warp w has the rows of quarter w & 3; warps 4-7 the first 32 of every 64 keys and half of the
+    // output columns, warps 8-11 the others.  The two threads of a row exchange their maxima through shared memory.
+    const int quarter = warp & 3, hf = (warp - 4) >> 2, row = quarter * 32 + lane, rr = r0 + row;
+    const bool live = row < nr;
+    const int tok = live ? c0 + rr / per : t0, pos = live ? t.positions[tok] : -1;
+    int least, most;
+    {                                        // of the warp's rows
+      const int ra = min(r0 + quarter * 32, r0 + nr - 1), rb = min(r0 + quarter * 32 + 31, r0 + nr - 1);
+      kv_reach(t, span, c0 + ra / per, c0 + rb / per, &least, &most);
+    }
+    const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
+    float* xchg = reinterpret_cast<float*>(smem + L::kOffX);
+    const float down = rows_down[row];
+    constexpr int NB = FK / 64, OH = 32 * NV;
+    float m = -INFINITY, l = 0.f, ref = 0.f;
+    const auto tell = [&](uint64_t* bar) {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    const auto pv_wait = [&](int it) {
+      mbar_wait(&pv_done[it & 1], it >> 1 & 1);
+      tc_fence_after_sync();
+    };
+    for (int it = 0; it < n_tiles; ++it) {
+      const int b = it & 1;
+      mbar_wait(&s_full[b], it >> 1 & 1);
+      tc_fence_after_sync();
+      const float2 p2 = refs[it & 3];        // written ahead of the keys; the tile after next writes none before this one's scores are taken
+      float x[NB][32];
+      {
+        uint32_t r[NB][2][16];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          tmem_ld16(lane_at + kColS + b * FK + i * 64 + hf * 32, r[i][0]);
+          tmem_ld16(lane_at + kColS + b * FK + i * 64 + hf * 32 + 16, r[i][1]);
+        }
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[i][j] = __uint_as_float(r[i][j / 16][j % 16]);
+      }
+      tell(&s_cons[b]);
+      const int ua = u0 + it * GT, ub = min(ua + GT, u1) - 1;              // groups of the tile
+      const int pa = span.group(ua) * kKvGroup, pb = span.group(ub) * kKvGroup + kKvGroup - 1;
+      const bool all = ub == ua + GT - 1 && pb < span.base && pb <= least && (pb < a.first || (ua >= span.na && most - pa < a.window));
+      if (!all) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int u = ua + i * 4 + hf * 2 + g, j0 = span.group(u) * kKvGroup;
+            uint32_t see = 0;
+            if (u < u1 && live) {
+#pragma unroll 1
+              for (int j = 0; j < 16; ++j) see |= (uint32_t)kv_sees(t, a, span, c0, n, tok, pos, j0 + j) << j;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (!(see >> j & 1u)) x[i][16 * g + j] = -INFINITY;
+          }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], x[i][j], x[i][j + 1]);
+      float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+      float* xb = xchg + b * 256;
+      xb[hf * 128 + row] = mt;
+      __syncwarp();
+      named_bar_sync(1 + quarter, 64);
+      const float fac = fminf(fmaxf(down * p2.x, 1e-37f), 1e37f);
+      mt = fmaxf(mt, xb[(hf ^ 1) * 128 + row]) * fac;
+      const float mn = fmaxf(m, mt), from = mn == -INFINITY ? 0.f : mn, back = ex2(m - from);
+      m = mn;
+      l *= back;
+      ref *= back;
+      const float big = ex2(mt - from) * p2.y;                             // the tile's largest weight times scale
+      float grow = 1.f;
+      bool again = false;
+      if (big > ref * 32768.f && big > 1e-37f) {
+        const float r = fmaxf(big * 0.015625f, 1e-37f);
+        grow = ref / r;
+        again = it > 0;                      // a reference that has shrunk to nothing as well: what O holds is then far below
+        ref = r;
+      }
+      const float f = ref >= 1e-37f ? p2.y * __frcp_rn(ref) : 0.f;
+      const uint64_t fac2 = pair_of(fac, fac), neg2 = pair_of(-from, -from), f2 = pair_of(f, f);
+      uint64_t sum[2] = {0, 0};
+      uint32_t pk[NB][16];
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 e = pair_get(pair_fma(pair_of(x[i][j], x[i][j + 1]), fac2, neg2));
+          const uint64_t p = pair_of(ex2(e.x), ex2(e.y));
+          sum[j >> 1 & 1] = pair_add(sum[j >> 1 & 1], p);
+          const float2 y = pair_get(pair_mul(p, f2));
+          pk[i][j / 2] = f16_pair(y.x, y.y);
+        }
+      const float2 s2 = pair_get(pair_add(sum[0], sum[1]));
+      l += s2.x + s2.y;
+      if (it >= 2) pv_wait(it - 2);          // PV(it - 2) has read this P buffer
+      if (__any_sync(0xffffffffu, again)) {
+        pv_wait(it - 1);                     // O holds every product so far 
+        const float sc = again ? grow : 1.f;
+#pragma unroll 2
+        for (int o = hf * OH; o < (hf + 1) * OH; o += 16) {
+          uint32_t r[16];
+          tmem_ld16(lane_at + kColO + o, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * sc);
+          tmem_st16(lane_at + kColO + o, r);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) tmem_st16(lane_at + kColP + b * (FK / 2) + i * 32 + hf * 16, pk[i]);
+      tmem_st_wait();
+      tell(&p_full[b]);
+    }
+    float* xb = xchg + (n_tiles & 1) * 256;  // the buffer that the last tile did not use
+    xb[hf * 128 + row] = l;
+    __syncwarp();
+    named_bar_sync(1 + quarter, 64);
+    l += xb[(hf ^ 1) * 128 + row];
+    if (n_tiles >= 2) pv_wait(n_tiles - 2);
+    pv_wait(n_tiles - 1);
+    const int hd = head * per + rr % per;
+    const long long orow = (long long)tok * a.H + hd, part = orow * a.pieces + blockIdx.z;
+    const bool whole = np <= 1;
+    if (whole && live && a.sinks != nullptr && m != -INFINITY) l += ex2(fmaf(a.sinks[hd], kLog2e, -m));
+    const float by = whole ? (l == 0.f ? 0.f : ref / l) : ref;
+    if (!whole && live && hf == 0) {
+      a.part_ml[2 * part] = m;
+      a.part_ml[2 * part + 1] = l;
+    }
+#pragma unroll 2
+    for (int o = hf * OH; o < (hf + 1) * OH; o += 16) {
+      uint32_t r[16];
+      tmem_ld16(lane_at + kColO + o, r);
+      tmem_ld_wait();
+      if (!live || o >= c.dv) continue;
+      float y[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]) * by + (l != l ? l : 0.f);         // a sum that is NaN has a zero for its reference, maybe
+      if (whole && a.dt_out) {
+        uint4* to = reinterpret_cast<uint4*>((bf16*)a.out + orow * c.dv + o);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          to[j] = make_uint4(bf16x2_bits_rn(y[8 * j + 1], y[8 * j]), bf16x2_bits_rn(y[8 * j + 3], y[8 * j + 2]), bf16x2_bits_rn(y[8 * j + 5], y[8 * j + 4]),
+                             bf16x2_bits_rn(y[8 * j + 7], y[8 * j + 6]));
+      } else {
+        float4* to = reinterpret_cast<float4*>(whole ? (float*)a.out + orow * c.dv + o : a.part_o + part * c.dv + o);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+template <int FMT, int NC, int NV>
+int launch(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t st) {
+  using L = TileShape<NC, NV>;
+  SEQ_CUDA((kb2::allow_smem<kv_tile_kernel<FMT, NC, NV>>(L::kTotal)));
+  auto kern = kv_tile_kernel<FMT, NC, NV>;
+  kb2::launch_pdl(kern, dim3(tiles, c.G, a.pieces), kThreads, L::kTotal, st, c, t, a);
+  SEQ_LAUNCHED();
+  return KB2SEQ_OK;
+}
+template <int FMT>
+int sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t st) {
+  if (c.d <= 64 && c.dv <= 64) return launch<FMT, 1, 1>(c, t, a, tiles, st);
+  if (c.d <= 128 && c.dv <= 128) return launch<FMT, 2, 2>(c, t, a, tiles, st);
+  if (c.d <= 192 && c.dv <= 128) return launch<FMT, 3, 2>(c, t, a, tiles, st);
+  if (c.d <= 128) return launch<FMT, 2, 4>(c, t, a, tiles, st);
+  return launch<FMT, 4, 4>(c, t, a, tiles, st);
+}
+}  // namespace
+
+int kv_tile_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t stream) {
+  return fmt == KV_E4M3 ? sizes<KV_E4M3>(c, t, a, tiles, stream) : sizes<KV_INT8>(c, t, a, tiles, stream);
+}
+
+}  // namespace kb2seq

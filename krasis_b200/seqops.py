@@ -67,7 +67,7 @@ SIGNATURES = {
     "kb2_seq_depth_mix": (_I, [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _P]),
     "kb2_seq_kv_write": (_I, [_P, _I, _P, _P, _L, _L, _P, _L, _L, _I, _P]),
     "kb2_seq_kv_read": (_I, [_P, _I, _P, _I, _I, _I, _P, _P, _I, _P]),
-    "kb2_seq_kv_attn_workspace": (C.c_size_t, [_P, _P, _I, _I, _I]),
+    "kb2_seq_kv_attn_workspace": (C.c_size_t, [_P, _P, _I, _I, _I, _I]),
     "kb2_seq_kv_attn": (_I, [_P, _I, _P, _P, _I, _L, _L, _I, _F, _I, _I, _P, _P, _I, _P, C.c_size_t, _P]),
     "kb2_seq_kv_keep": (_I, [_P, _P, _P, _I, _P]),
     "kb2_seq_stream_mix": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _I, _F, _P]),
@@ -574,10 +574,10 @@ def _kv_attend(name, q, tb, cache, layer, scale, window, first, sinks, dtype, ou
     elif out.shape != (T, H, cache.vdim) or not out.is_contiguous() or out.get_device() != q.get_device() or (dtype is not None and out.dtype != dtype):
         raise ValueError(f"{name}: out is a contiguous {(T, H, cache.vdim)}")
     dq, do = dt_code(q.dtype), dt_code(out.dtype)
-    lib, key = load(), (G, cache.vdim, cache.page_size, H, window, first)
+    lib, key = load(), (G, cache.vdim, cache.page_size, H, window, first, do)
     size = tb._kv_sizes.get(key)
     if size is None:
-        size = tb._kv_sizes[key] = lib.kb2_seq_kv_attn_workspace(p, st, H, window, first)
+        size = tb._kv_sizes[key] = lib.kb2_seq_kv_attn_workspace(p, st, H, window, first, do)
     work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     check(lib.kb2_seq_kv_attn(p, layer, st, q.data_ptr(), dq, q.stride(0), q.stride(1), H, float(scale), window, first, _ptr(sinks), out.data_ptr(), do,
                               _ptr(work), size, _s(q)))

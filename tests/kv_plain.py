@@ -101,14 +101,17 @@ def attention(q, cache, layer, seqs, scale, window=None, first=0, sinks=None):
     return out, mag, top, small
 
 
-def off_by(q_dtype, out_dtype, keys, d, want, mag, top, small):
+def off_by(q_dtype, out_dtype, keys, d, want, mag, top, small, decoded=False):
     """How far a result may be from `want`: one rounding of the result; weights that are rounded to 11 bits (22 for fp32 results) beside their fp32 sums; and the scores'
     error, which a weight and the sum that divides it both see.  Queries: bf16 numbers are held whole (22 bits of the largest), fp32 ones to 11 bits (22 for fp32 results).
     A sum of n fp32 terms is off by at most n 2^-23 of the terms' magnitudes (the tensor cores may cut instead of round).
     A weight times its value row's scale is held in fp16 over a reference R, and the largest such product so far is at least 2^6 R: it was when R was set, and both shrink by
     the same factor when the maximum grows.  fp16's least step is 2^-24, so each product is off by at most half of that times R, 2^-31 of the largest product, whatever its own
     size, and the result by that times the sum of the codes' magnitudes: `small`."""
+    # decoded (bf16 results of sequences with more than 16 rows per kv head): keys and values reach the tensor cores as fp16(code * fp16(scale / unit)), two roundings of
+    # 2^-11 on each number of a score's sum and of the result's, where scales are no further apart than 2^21
     wide = out_dtype == torch.float32
+    decode = 2.0 ** -10 * 1.001 if decoded and not wide else 0.0
     part = 2.0 ** -21 if wide else 2.0 ** -11
-    score = top * ((2.0 ** -21 if wide or q_dtype == torch.bfloat16 else 2.0 ** -11) + (d + 4) * 2.0 ** -23)
-    return want.abs() * torch.finfo(out_dtype).eps / 2 + mag * (2 * torch.expm1(score) + part + (keys / 16 + 8) * 2.0 ** -23 + 2.0 ** -20) + small * 2.0 ** -31 + 1e-30
+    score = top * (decode + (2.0 ** -21 if wide or q_dtype == torch.bfloat16 else 2.0 ** -11) + (d + 4) * 2.0 ** -23)
+    return want.abs() * torch.finfo(out_dtype).eps / 2 + mag * (2 * torch.expm1(score) + part + decode + (keys / 16 + 8) * 2.0 ** -23 + 2.0 ** -20) + small * 2.0 ** -31 + 1e-30

@@ -9,6 +9,13 @@ pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True)
+def waits():
+    yield
+    from krasis_b200 import seqops as ops
+    ops.check_waits()
+
+
 def _gen(seed):
     return torch.Generator().manual_seed(seed)
 
@@ -37,7 +44,7 @@ def _step(lens, page_size, seed=0, spare=2, parents=None):
 def _check(got, q, cache, seqs, layer=0, known=None, **kw):
     want, *sizes = known = known or kv_plain.attention(q, cache, layer, seqs, **kw)
     keys = max(n + s for n, s, _, _ in seqs)
-    off = kv_plain.off_by(q.dtype, got.dtype, keys, cache.dim, want, *sizes)
+    off = kv_plain.off_by(q.dtype, got.dtype, keys, cache.dim, want, *sizes, decoded=max(n for n, _, _, _ in seqs) * q.shape[1] // cache.num_kv_heads > 16)
     err = (got.double().cpu() - want).abs()
     assert bool(torch.isfinite(got).all())
     assert bool((err <= off).all()), (float((err / off).max()), float(err.max()))

@@ -136,7 +136,7 @@ def test_interface_refuses_arguments():
     assert lib.kb2_seq_kv_keep(p, q, 4096, 513, None) == 2 and lib.kb2_seq_kv_keep(p, q, 4096, -1, None) == 2 and lib.kb2_seq_kv_keep(p, q, None, 1, None) == 2
     big, layout = 200000, [[0, 1, 199999, 12500]]
     c, s, keep = _structs(pages=12500, max_pages=12500, layout=layout, T=1)
-    size = lib.kb2_seq_kv_attn_workspace(C.byref(c), C.byref(s), 4, 0, 0)
+    size = lib.kb2_seq_kv_attn_workspace(C.byref(c), C.byref(s), 4, 0, 0, 0)
     assert size > 0 and lib.kb2_seq_kv_attn(C.byref(c), 0, C.byref(s), 4096, 0, 256, 64, 4, 1.0, 0, 0, None, 4096, 0, 4096, size - 1, None) in (2, 3)
     assert big == layout[0][2] + 1
 
