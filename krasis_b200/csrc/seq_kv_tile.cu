@@ -2,7 +2,8 @@
 //
 // A tile is 128 (token, head) rows of one sequence and kv head: the H / G heads that share keys fill it together, so a key tile is decoded once for all of them.  Roles of
 // a CTA of 16 warps:
-//   warps 12-15  decode: codes from the pages into registers a job ahead, as fp16 into the swizzled operand tiles.  A row's scale over a power of two
+//   warp  1      brings codes and scales from the pages into a ring of three half tiles (bulk copies of 16 rows)
+//   warps 12-15  decode: codes as fp16 into the swizzled operand tiles.  A row's scale over a power of two
 //                near the tile's largest one is multiplied in there (one packed product for two codes; exact for scales that are powers of two), the power joins the
 //                softmax's factor
 //   warp  0      tcgen05.mma: S = Q K^T, O += P V (P from tensor memory)
@@ -23,10 +24,13 @@ constexpr int kThreads = 512;
 template <int NC, int NV>                    // chunks of 64 of d and dv
 struct TileShape {
   static constexpr int FK = NC > 2 || NV > 2 ? 64 : 128;
+  static constexpr int VS = NC + NV > 6 ? 1 : 2;                           // buffers of values
   static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128;
-  static constexpr int kOffQ = 0, kOffK = kQ, kOffV = kOffK + 2 * kK, kOffBar = kOffV + 2 * kV, kOffRef = kOffBar + 128, kOffTmem = kOffRef + 32, kOffX = kOffTmem + 16, kOffRow = kOffX + 2 * 2 * 128 * 4;
+  static constexpr int kSlots = 3, kCodes = FK * 64 * (NC > NV ? NC : NV), kSlot = kCodes + FK * 8;       // codes as they come | scales of keys | of values
+  static constexpr int kOffQ = 0, kOffK = kQ, kOffV = kOffK + 2 * kK, kOffSlot = kOffV + VS * kV, kOffBar = kOffSlot + kSlots * kSlot, kOffRef = kOffBar + 192,
+                       kOffX = kOffRef + 64, kOffRow = kOffX + 2 * 2 * 128 * 4;
   static constexpr int kTotal = kOffRow + 128 * 4;
-  static_assert(kTotal <= 227 * 1024 && 3 * FK + 64 * NV <= 512, "memory");
+  static_assert(kTotal <= 227 * 1024 && 3 * FK + 64 * NV <= 512 && kSlot % 128 == 0, "memory");
 };
 
 __device__ __forceinline__ uint32_t idesc_f16(uint32_t n, bool mn) {       // A and B fp16, accumulator fp32, 128 rows; mn: B lies with its columns side by side
@@ -85,35 +89,20 @@ __device__ __forceinline__ void scale_unit(uint32_t bits, float* p, float* inv) 
   *inv = __uint_as_float((254 - e) << 23);
 }
 
-// What a decoding thread knows of a tile: it has the rows row0 + 32 i, and 16 bytes of each chunk of 64 of those.
-template <int NR>
-struct Where {
-  int r16[NR];                               // the rows' groups in the pools, -1: none
-  float ks[NR], vs[NR];
-  bool see[NR];
-  uint4 ks4, vs4;                            // scales of rows 4 lane .. 4 lane + 3 of the tile, zeros where nobody sees them
-};
-template <int NR, int CH>
-__device__ __forceinline__ void decode_load(const uint8_t* pool, int width, int ct, const Where<NR>& w, uint4 (&x)[NR * CH]) {
-#pragma unroll
-  for (int i = 0; i < NR; ++i)
-#pragma unroll
-    for (int h = 0; h < CH; ++h) {
-      const int e = h * 64 + (ct & 3) * 16, row = (ct >> 2) + 32 * i;
-      x[i * CH + h] = w.see[i] && e < width ? ld_stream16(pool + ((long long)w.r16[i] * kKvGroup + (row & 15)) * width + e) : make_uint4(0, 0, 0, 0);
-    }
-}
-// A warp's store of 16 bytes a lane meets 8 rows' swizzles, two of them in eight lanes: no bank twice.
+// Codes of a tile from `from` (rows of `width` bytes) into the operand at `to`.  A thread has the rows ct / 4 + 32 i and 16 bytes of each chunk of 64 of those, f times the
+// codes where see.  Odd rows take their chunks in another order: eight lanes that are served together then read 128 neighbouring bytes or two rows' halves, and the stores
+// of 16 bytes meet 8 rows' swizzles, two of them in eight lanes: no bank twice either way.
 template <int FMT, int NR, int CH>
-__device__ __forceinline__ void decode_store(uint8_t* to, int ct, const float (&f)[NR], const uint4 (&x)[NR * CH]) {
+__device__ __forceinline__ void decode(uint8_t* to, const uint8_t* from, int width, int ct, const float (&f)[NR], const bool (&see)[NR]) {
   const int q = ct & 3;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const int row = (ct >> 2) + 32 * i;
     const uint32_t m = f16_pair(f[i], f[i]);
 #pragma unroll
-    for (int h = 0; h < CH; ++h) {
-      const uint4 v = x[i * CH + h];
+    for (int h0 = 0; h0 < CH; ++h0) {
+      const int h = CH % 2 ? h0 : h0 ^ (row & 1), e0 = h * 64 + q * 16;
+      const uint4 v = see[i] && e0 < width ? *reinterpret_cast<const uint4*>(from + row * width + e0) : make_uint4(0, 0, 0, 0);
       uint32_t y[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -121,7 +110,7 @@ __device__ __forceinline__ void decode_store(uint8_t* to, int ct, const float (&
         y[2 * e] = hmul2(y[2 * e], m);
         y[2 * e + 1] = hmul2(y[2 * e + 1], m);
       }
-      uint8_t* p = to + h * (2048 * NR * 2) + row * 128;                   // chunks of 32 NR rows
+      uint8_t* p = to + h * (32 * NR * 128) + row * 128;
       *reinterpret_cast<uint4*>(p + (((2 * q) ^ (row & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
       *reinterpret_cast<uint4*>(p + (((2 * q + 1) ^ (row & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
     }
@@ -136,10 +125,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
   constexpr int FK = L::FK, GT = FK / kKvGroup;                            // groups a tile
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
-  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *s_cons = bars + 10, *p_full = bars + 12, *pv_done = bars + 14;
-  float2* refs = reinterpret_cast<float2*>(smem + L::kOffRef);             // [4] tile's powers of two: keys, values
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *s_cons = bars + 10, *p_full = bars + 12, *pv_done = bars + 14,
+           *c_full = bars + 16, *c_empty = bars + 19;
+  float2* refs = reinterpret_cast<float2*>(smem + L::kOffRef);             // [4] tile's units: keys, values
+  uint32_t* have = reinterpret_cast<uint32_t*>(refs + 4);                  // [3] a slot's groups that are there, a bit each
+  uint32_t* tmem_at = have + 3;
   float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [128] what the queries' own scaling is undone with
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -151,6 +142,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       mbar_init(&pv_done[i], 1);
       mbar_init(&s_cons[i], 8);
       mbar_init(&p_full[i], 8);
+    }
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&c_full[i], 1);
+      mbar_init(&c_empty[i], 4);
     }
     fence_mbar_init();
   }
@@ -228,80 +223,110 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       }
     }
   } else if (warp >= 12) {
-    // ------------------------------------------------------------ decode
-    const int ct = threadIdx.x - 384, row0 = ct >> 2;
+    // ------------------------------------------------------------ decode: K(0), then K(it + 1) and V(it) in turn
+    const int ct = threadIdx.x - 384;
     constexpr int NR = FK / 32;
-    const auto at_row = [&](int u, int* r16) {
-      const long long r = u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
-      *r16 = r < 0 ? -1 : (int)((r + ((long long)head << c.lps)) / kKvGroup);
-    };
-    const auto seen = [&](int u, int row) {  // by any row of the tile
-      const int j = span.group(u) * kKvGroup + (row & 15);
-      return j < span.hi && (j >= span.lo || j < a.first);
-    };
-    const auto where = [&](int it, Where<NR>& w) {
+    bool see[NR], see_v[NR];
+    float fk[NR], fv[NR], fv_next[NR];
+    int job = 0;
+    const auto keys = [&](int it) {
+      const int b = it & 1, slot = job % L::kSlots;
+      const uint8_t* from = smem + L::kOffSlot + slot * L::kSlot;
+      const float *ks = reinterpret_cast<const float*>(from + L::kCodes), *vs = ks + FK;
+      mbar_wait(&c_full[slot], job / L::kSlots & 1);
+      const uint32_t groups = have[slot];
+      const auto seen = [&](int row) {       // by any row of the tile
+        const int j = span.group(u0 + it * GT + row / 16) * kKvGroup + (row & 15);
+        return (groups >> (row / 16) & 1u) && j < span.hi && (j >= span.lo || j < a.first);
+      };
+      uint32_t kt = 0, vt = 0;               // the tile's largest scales
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        const int row = row0 + 32 * i, u = u0 + it * GT + row / 16;
-        at_row(u, &w.r16[i]);
-        w.see[i] = w.r16[i] >= 0 && seen(u, row);
-        w.ks[i] = w.vs[i] = 0.f;
-        if (w.see[i]) {
-          const long long r = (long long)w.r16[i] * kKvGroup + (row & 15);
-          w.ks[i] = c.ks[r];
-          w.vs[i] = c.vs[r];
+      for (int i = 0; i < FK / 32; ++i) {
+        const int row = i * 32 + lane;
+        if (seen(row)) {
+          const uint32_t x = __float_as_uint(ks[row]), y = __float_as_uint(vs[row]);
+          if (x < 0x7F800000u) kt = max(kt, x);
+          if (y < 0x7F800000u) vt = max(vt, y);
         }
       }
-      w.ks4 = w.vs4 = make_uint4(0, 0, 0, 0);
-      if (lane * 4 < FK) {
-        const int u = u0 + it * GT + lane / 4;
-        int r16;
-        at_row(u, &r16);
-        if (r16 >= 0) {
-          const long long r = (long long)r16 * kKvGroup + (lane & 3) * 4;
-          w.ks4 = *reinterpret_cast<const uint4*>(c.ks + r);
-          w.vs4 = *reinterpret_cast<const uint4*>(c.vs + r);
-          uint32_t* k = reinterpret_cast<uint32_t*>(&w.ks4);
-          uint32_t* v = reinterpret_cast<uint32_t*>(&w.vs4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool no = !seen(u, (lane & 3) * 4 + e);
-            if (no || k[e] >= 0x7F800000u) k[e] = 0;
-            if (no || v[e] >= 0x7F800000u) v[e] = 0;
-          }
-        }
-      }
-    };
-    Where<NR> w, next;
-    uint4 xk[NR * NC], xv[NR * NV];
-    where(0, w);
-    decode_load<NR, NC>(c.k, c.d, ct, w, xk);
-    decode_load<NR, NV>(c.v, c.dv, ct, w, xv);
-    for (int it = 0; it < n_tiles; ++it) {
-      const int b = it & 1;
-      if (it + 1 < n_tiles) where(it + 1, next);
-      // the tile's largest scales
-      const uint32_t kt = __reduce_max_sync(0xffffffffu, max(max(w.ks4.x, w.ks4.y), max(w.ks4.z, w.ks4.w)));
-      const uint32_t vt = __reduce_max_sync(0xffffffffu, max(max(w.vs4.x, w.vs4.y), max(w.vs4.z, w.vs4.w)));
-      float kp, ki, vp, vi, fk[NR], fv[NR];
-      scale_unit(kt, &kp, &ki);
+      float kp, ki, vp, vi;
+      scale_unit(__reduce_max_sync(0xffffffffu, kt), &kp, &ki);
+      vt = __reduce_max_sync(0xffffffffu, vt);
       scale_unit(vt, &vp, &vi);
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        const bool nan_v = w.vs[i] != w.vs[i];
-        fk[i] = nan_v ? w.vs[i] : w.ks[i] * ki;
-        fv[i] = nan_v ? 0.f : w.vs[i] * vi;
+        const int row = (ct >> 2) + 32 * i;
+        see[i] = seen(row);
+        const float x = see[i] ? ks[row] : 0.f, y = see[i] ? vs[row] : 0.f;
+        fk[i] = y != y ? y : x * ki;         // a row that is no number: its keys say so
+        fv_next[i] = y != y ? 0.f : y * vi;
       }
       mbar_wait(&k_empty[b], (it >> 1 & 1) ^ 1);
-      decode_store<FMT, NR, NC>(smem + L::kOffK + b * L::kK, ct, fk, xk);
+      decode<FMT, NR, NC>(smem + L::kOffK + b * L::kK, from, c.d, ct, fk, see);
       if (ct == 0) refs[it & 3] = make_float2(kp, vt ? vp : 0.f);
-      if (lane == 0) mbar_arrive(&k_full[b]);
-      if (it + 1 < n_tiles) decode_load<NR, NC>(c.k, c.d, ct, next, xk);
-      mbar_wait(&v_empty[b], (it >> 1 & 1) ^ 1);
-      decode_store<FMT, NR, NV>(smem + L::kOffV + b * L::kV, ct, fv, xv);
-      if (lane == 0) mbar_arrive(&v_full[b]);
-      if (it + 1 < n_tiles) decode_load<NR, NV>(c.v, c.dv, ct, next, xv);
-      w = next;
+      if (lane == 0) {
+        mbar_arrive(&k_full[b]);
+        mbar_arrive(&c_empty[slot]);
+      }
+      ++job;
+    };
+    keys(0);
+    for (int it = 0; it < n_tiles; ++it) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        fv[i] = fv_next[i];
+        see_v[i] = see[i];
+      }
+      if (it + 1 < n_tiles) keys(it + 1);
+      const int b = it % L::VS, slot = job % L::kSlots;
+      mbar_wait(&c_full[slot], job / L::kSlots & 1);
+      mbar_wait(&v_empty[b], (it / L::VS & 1) ^ 1);
+      decode<FMT, NR, NV>(smem + L::kOffV + b * L::kV, smem + L::kOffSlot + slot * L::kSlot, c.dv, ct, fv, see_v);
+      if (lane == 0) {
+        mbar_arrive(&v_full[b]);
+        mbar_arrive(&c_empty[slot]);
+      }
+      ++job;
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ codes and scales from the pages, in the decoders' order.  A group of 16 rows is one run of bytes in each pool.
+    const auto at_row = [&](int it) {        // lane's group of a tile
+      const int u = u0 + it * GT + lane % GT;
+      const long long r = it < n_tiles && u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
+      return r < 0 ? -1ll : r + ((long long)head << c.lps);
+    };
+    int job = 0;
+    const auto fetch = [&](long long r, bool val) {
+      const int slot = job % L::kSlots, kind = lane / GT;                  // codes, scales of keys, of values
+      uint8_t* to = smem + L::kOffSlot + slot * L::kSlot;
+      mbar_wait(&c_empty[slot], (job / L::kSlots & 1) ^ 1);
+      const uint32_t there = __ballot_sync(0xffffffffu, r >= 0) & ((1u << GT) - 1);
+      const uint32_t bytes = __popc(there) * (kKvGroup * (val ? c.dv : c.d + 8));
+      if (lane == 0) {
+        have[slot] = there;
+        if (bytes) mbar_arrive_expect_tx(&c_full[slot], bytes);
+        else mbar_arrive(&c_full[slot]);
+      }
+      __syncwarp();
+      if (r >= 0) {
+        const int g = lane % GT;
+        if (kind == 0) {
+          const int n = kKvGroup * (val ? c.dv : c.d);
+          bulk_g2s(to + g * n, (val ? c.v + r * c.dv : c.k + r * c.d), n, &c_full[slot]);
+        } else if (!val && kind <= 2) {
+          bulk_g2s(to + L::kCodes + ((kind - 1) * FK + g * kKvGroup) * 4, (kind == 1 ? c.ks : c.vs) + r, kKvGroup * 4, &c_full[slot]);
+        }
+      }
+      ++job;
+    };
+    long long cur = at_row(0), next = at_row(1);
+    fetch(cur, false);
+    for (int it = 0; it < n_tiles; ++it) {
+      const long long later = at_row(it + 2);
+      if (it + 1 < n_tiles) fetch(next, false);
+      fetch(cur, true);
+      cur = next;
+      next = later;
     }
   } else if (warp == 0) {
     // ------------------------------------------------------------ tensor cores
@@ -330,16 +355,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     for (int it = 0; it < n_tiles; ++it) {
       const int b = it & 1;
       if (it + 2 < n_tiles) scores(it + 2);
-      mbar_wait(&v_full[b], it >> 1 & 1);
+      const int vb = it % L::VS;
+      mbar_wait(&v_full[vb], it / L::VS & 1);
       mbar_wait(&p_full[b], it >> 1 & 1);
       tc_fence_after_sync();
-      const uint32_t v_at = smem_u32(smem + L::kOffV + b * L::kV);
+      const uint32_t v_at = smem_u32(smem + L::kOffV + vb * L::kV);
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < FK / 16; ++k)
           umma_bf16_ts(tmem + kColO, tmem + kColP + b * (FK / 2) + 8 * k, desc_mn(v_at + k * 2048, FK * 128), id_o, it > 0 || k > 0 ? 1u : 0u);
         umma_commit(&pv_done[b]);
-        umma_commit(&v_empty[b]);
+        umma_commit(&v_empty[vb]);
       }
       __syncwarp();
     }
