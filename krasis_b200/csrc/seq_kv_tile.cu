@@ -119,6 +119,11 @@ __device__ __forceinline__ void decode(uint8_t* to, const uint8_t* from, int wid
   __syncwarp();
 }
 
+// This thread's arrival once its copies so far (cp.async) are there.
+__device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 template <int FMT, int NC, int NV>
 __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep t, KvAttn a) {
   using L = TileShape<NC, NV>;
@@ -144,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       mbar_init(&p_full[i], 8);
     }
     for (int i = 0; i < 3; ++i) {
-      mbar_init(&c_full[i], 1);
+      mbar_init(&c_full[i], 33);                // the bytes of the bulk copies, and the lanes that copy scales
       mbar_init(&c_empty[i], 4);
     }
     fence_mbar_init();
@@ -289,34 +294,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       ++job;
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ codes and scales from the pages, in the decoders' order.  A group of 16 rows is one run of bytes in each pool.
+    // ------------------------------------------------------------ codes and scales from the pages, in the decoders' order.  A run of groups that one page holds is one run of
+    // bytes in each pool, and one bulk copy (one a group: 1083 us for a portion of 4096 tokens); scales go 16 bytes a lane.
     const auto at_row = [&](int it) {        // lane's group of a tile
-      const int u = u0 + it * GT + lane % GT;
-      const long long r = it < n_tiles && u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
+      const int u = u0 + it * GT + lane;
+      const long long r = lane < GT && it < n_tiles && u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
       return r < 0 ? -1ll : r + ((long long)head << c.lps);
     };
     int job = 0;
     const auto fetch = [&](long long r, bool val) {
-      const int slot = job % L::kSlots, kind = lane / GT;                  // codes, scales of keys, of values
+      const int slot = job % L::kSlots;
       uint8_t* to = smem + L::kOffSlot + slot * L::kSlot;
+      const long long before = __shfl_up_sync(0xffffffffu, r, 1), mine = __shfl_sync(0xffffffffu, r, lane / 4);      // the lane's scales are its group's: row 4 lane of the tile
+      const uint32_t there = __ballot_sync(0xffffffffu, r >= 0);
+      const uint32_t lead = __ballot_sync(0xffffffffu, r >= 0 && !(lane && before >= 0 && r == before + kKvGroup)) | ~there;      // a run ends where another or a gap begins
+      const int run = lane < 31 ? __ffs(lead >> (lane + 1)) : 0;           // lanes behind the last group are gaps
       mbar_wait(&c_empty[slot], (job / L::kSlots & 1) ^ 1);
-      const uint32_t there = __ballot_sync(0xffffffffu, r >= 0) & ((1u << GT) - 1);
-      const uint32_t bytes = __popc(there) * (kKvGroup * (val ? c.dv : c.d + 8));
       if (lane == 0) {
         have[slot] = there;
-        if (bytes) mbar_arrive_expect_tx(&c_full[slot], bytes);
-        else mbar_arrive(&c_full[slot]);
+        mbar_arrive_expect_tx(&c_full[slot], __popc(there) * kKvGroup * (val ? c.dv : c.d));
       }
       __syncwarp();
-      if (r >= 0) {
-        const int g = lane % GT;
-        if (kind == 0) {
-          const int n = kKvGroup * (val ? c.dv : c.d);
-          bulk_g2s(to + g * n, (val ? c.v + r * c.dv : c.k + r * c.d), n, &c_full[slot]);
-        } else if (!val && kind <= 2) {
-          bulk_g2s(to + L::kCodes + ((kind - 1) * FK + g * kKvGroup) * 4, (kind == 1 ? c.ks : c.vs) + r, kKvGroup * 4, &c_full[slot]);
-        }
+      if (r >= 0 && (lead >> lane & 1u)) {
+        const int n = kKvGroup * (val ? c.dv : c.d);
+        bulk_g2s(to + lane * n, val ? c.v + r * c.dv : c.k + r * c.d, run * n, &c_full[slot]);
       }
+      if (!val && lane * 4 < FK && mine >= 0) {
+        cp_async16_stream(smem_u32(to + L::kCodes) + lane * 16, c.ks + mine + (lane & 3) * 4, true);
+        cp_async16_stream(smem_u32(to + L::kCodes) + FK * 4 + lane * 16, c.vs + mine + (lane & 3) * 4, true);
+      }
+      arrive_behind_copies(&c_full[slot]);
       ++job;
     };
     long long cur = at_row(0), next = at_row(1);
