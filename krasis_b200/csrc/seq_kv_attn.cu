@@ -431,7 +431,7 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
   }
   p.least = least;
   p.most = most;
-  p.rows = wide ? kTileRows : rows <= 8 ? 8 : 16;
+  p.rows = wide ? (kv_pairs(cache->d, cache->dv) ? 256 : 128) : rows <= 8 ? 8 : 16;
   for (int s = 0; s < step->S; ++s) {
     const int* l = step->layout + 4 * s;
     const long long r = (long long)l[1] * per;
@@ -551,7 +551,7 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   const KvAttn few = with_plan(a, p.few, (float*)work, t.T * H, c.dv), many = with_plan(a, p.many, (float*)work + p.few.floats, t.T * H, c.dv);
   const cudaStream_t st = (cudaStream_t)stream;
   if (p.many.tiles) {
-    if (int e = kv_tile_attend(cache->fmt, c, t, many, p.many.tiles, st)) return e;
+    if (int e = (kv_pairs(c.d, c.dv) ? kv_pair_attend : kv_tile_attend)(cache->fmt, c, t, many, p.many.tiles, st)) return e;
   }
   if (p.few.tiles) {
     if (int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, few, p.few, st) : stream_sizes<KV_INT8>(c, t, few, p.few, st)) return e;

@@ -77,8 +77,9 @@ __device__ __forceinline__ void kv_row_scale(uint32_t top, float* up, float* dow
   *down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
 
-// Tiles of 128 rows on the tensor cores (seq_kv_tile.cu).
+// Tiles on the tensor cores: 256 rows (seq_kv_pair.cu), 128 where tensor memory has no room for two outputs (seq_kv_tile.cu).
+int kv_pair_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t stream);
 int kv_tile_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t stream);
-constexpr int kTileRows = 128;
+inline bool kv_pairs(int d, int dv) { return d <= 192 && dv <= 128; }
 
 }  // namespace kb2seq

@@ -1,0 +1,542 @@
+// Attention over the 8-bit cache for many query rows per key / value head on tcgen05, heads of up to 192 (keys) and 128 (values): two tiles of 128 (token, head) rows of one
+// sequence and kv head share every key tile that is decoded.  The H / G heads that share keys fill the rows together.  Roles of a CTA of 16 warps:
+//   warp  1      plans: looks up the key tiles' groups in the page list, reads their scales, and leaves for each row the factors that its codes are multiplied with
+//   warps 12-15  decode: codes from the pages into registers, a tile ahead, as fp16 (code times factor, one packed product for two) into the swizzled operand tiles
+//   warp  0      tcgen05.mma: S = Q K^T and O += P V for both row tiles as their inputs come (P from tensor memory, in S's place)
+//   warps 4-7, 8-11  softmax of the first and of the second row tile, a thread a row: while one works the tensor cores make the other's scores
+// Where a sequence has no more than 128 rows left both softmax groups have the same rows and take the key tiles in turn; they are joined at the end.
+// FK = 128 keys a tile (64 for keys of 192).  Tensor memory: S 2 FK | O 2 x 64 NV.
+//
+// What bounds it: for a tile of 128 keys and 256 rows 32768 exponentials take 2048 cycles (16 a cycle), and shared memory's 128 bytes a cycle are taken for 2048 as well
+// (both products read Q, K and V: 192 KB; decoding writes 64 KB).
+//
+// Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value unit are fp16 (11 bits).  A row's factor is its scale over a unit, a power of two
+// near the tile's largest scale (exact for scales that are powers of two); the units join the softmax's factors.  Weights are rounded relative to a reference R per row that
+// follows the largest weight times unit (2^6 to 2^15 of it), as in the kernel for few rows; maxima, weights and their sum are fp32.
+// A row whose scale is NaN gets NaN keys and zero values: scores that nobody sees are replaced, and those that see it carry the NaN into the sum.
+#include "seq_kv_tc.cuh"
+
+namespace kb2seq {
+namespace {
+
+constexpr int kThreads = 512;
+// Registers a thread of each warpgroup: planning and tensor cores, softmax (twice), decoding: 4 x 128 at launch.
+constexpr int kRegMma = 56, kRegSoftmax = 176, kRegDecode = 104;
+static_assert(kRegMma + 2 * kRegSoftmax + kRegDecode <= 4 * 128, "registers of the launch");
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+constexpr int kPlans = 4, kUnits = 8;        // tiles that are planned ahead; units are read later than the rest
+
+template <int NC, int NV>                    // chunks of 64 of d and dv
+struct PairShape {
+  static constexpr int FK = NC > 2 ? 64 : 128;
+  static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128;
+  static constexpr int kOffQ = 0, kOffK = 2 * kQ, kOffV = kOffK + 2 * kK, kOffFac = kOffV + 2 * kV, kOffGroup = kOffFac + kPlans * FK * 4, kOffBar = kOffGroup + kPlans * 32,
+                       kOffUnit = kOffBar + 192, kOffTmem = kOffUnit + kUnits * 8, kOffRow = kOffTmem + 16, kTotal = kOffRow + 256 * 4;
+  static_assert(kTotal <= 227 * 1024 && 2 * FK + 128 * NV <= 512, "memory");
+  static_assert(128 * (64 * NV + 1) * 4 + 128 * 12 <= 2 * kQ + 2 * kK + 2 * kV, "the second group's share at the end");
+};
+
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+
+// A thread's 16 bytes of each chunk of 64 of the rows ct / 4 + 32 i.
+template <int NR, int CH>
+__device__ __forceinline__ void pair_load(const uint8_t* pool, int width, int ct, const int* groups, uint4 (&x)[NR * CH]) {
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int row = (ct >> 2) + 32 * i, r16 = groups[row >> 4];
+    const uint8_t* from = pool + ((long long)r16 * kKvGroup + (row & 15)) * width + (ct & 3) * 16;
+#pragma unroll
+    for (int h = 0; h < CH; ++h) x[i * CH + h] = r16 >= 0 && h * 64 + (ct & 3) * 16 < width ? ld_stream16(from + h * 64) : make_uint4(0, 0, 0, 0);
+  }
+}
+// The same as fp16 in the operand at `to`, times the rows' factors.  The stores of 16 bytes a lane meet 8 rows' swizzles, two of them in eight lanes: no bank twice.
+template <int FMT, int NR, int CH>
+__device__ __forceinline__ void pair_store(uint8_t* to, int ct, const uint32_t (&f)[NR], const uint4 (&x)[NR * CH]) {
+  const int q = ct & 3;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int row = (ct >> 2) + 32 * i;
+#pragma unroll
+    for (int h = 0; h < CH; ++h) {
+      uint32_t y[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        codes_f16<FMT>(word(x[i * CH + h], e), y[2 * e], y[2 * e + 1]);
+        y[2 * e] = hmul2(y[2 * e], f[i]);
+        y[2 * e + 1] = hmul2(y[2 * e + 1], f[i]);
+      }
+      uint8_t* p = to + h * (32 * NR * 128) + row * 128;
+      *reinterpret_cast<uint4*>(p + (((2 * q) ^ (row & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(p + (((2 * q + 1) ^ (row & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+template <int FMT, int NC, int NV>
+__global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep t, KvAttn a) {
+  using L = PairShape<NC, NV>;
+  constexpr int FK = L::FK, GT = FK / kKvGroup;                            // groups a tile
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  // by buffer: k_full .. v_empty; by row tile: s_full, p_full, pv_done; by plan: plan_full, plan_empty
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10, *pv_done = bars + 12, *plan_full = bars + 14,
+           *plan_empty = bars + 14 + kPlans;
+  uint32_t* factors = reinterpret_cast<uint32_t*>(smem + L::kOffFac);      // [kPlans][FK] fp16: of the row's key codes, of its value codes
+  int* groups = reinterpret_cast<int*>(smem + L::kOffGroup);               // [kPlans][8] where the groups lie (rows / 16), -1: nowhere
+  float2* units = reinterpret_cast<float2*>(smem + L::kOffUnit);           // [kUnits] of keys, of values
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
+  float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [256] what the queries' own scaling is undone with
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  if (warp == 2) tmem_alloc(tmem_at, 512);
+  pdl_wait();
+
+  // which tile, and what its rows see: the same in every warp
+  const int per = a.H / c.G, head = blockIdx.y;
+  int s = 0, tile = 0;
+  bool in = true;
+  if (a.per_seq) {
+    s = blockIdx.x / a.per_seq;
+    tile = blockIdx.x - s * a.per_seq;
+  } else {
+    in = kv_find_tile(t, per, 256, a.least, a.most, blockIdx.x, &s, &tile);
+  }
+  const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * 256, nr = in ? (int)min((long long)n * per - r0, 256ll) : 0;
+  int u0 = 0, u1 = 0, np = 0, t0 = c0;
+  KvSpan span{};
+  if (nr > 0) {
+    t0 = c0 + r0 / per;
+    span = kv_span(c, t, s, t0, c0 + (r0 + nr - 1) / per, a.window, a.first);
+    np = min((span.groups() + a.piece - 1) / a.piece, a.pieces);
+    u0 = blockIdx.z * a.piece;
+    u1 = min(span.groups(), u0 + a.piece);
+  }
+  const bool work = nr > 0 && (blockIdx.z == 0 || (int)blockIdx.z < np);   // piece 0 of a tile that sees nothing writes its zeros
+  const int n_tiles = work ? max(0, (u1 - u0 + GT - 1) / GT) : 0;
+  const bool two = nr > 128;                 // two row tiles; else one whose key tiles go to both groups in turn
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&k_empty[i], two ? 2 : 1);
+      mbar_init(&v_empty[i], two ? 2 : 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < kPlans; ++i) {
+      mbar_init(&plan_full[i], 1);
+      mbar_init(&plan_empty[i], 4);
+    }
+    fence_mbar_init();
+  }
+
+  // queries, a warp a row: scaled by a power of two, rounded to fp16, in the operand's layout (rows of 64 numbers, 16-byte pieces swizzled by the row)
+  if (work) {
+    const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;  // factors on scores are positive: a row's maximum is its largest raw score's
+    const int rows = two ? 16 : 8;
+#pragma unroll 4
+    for (int i = 0; i < rows; ++i) {
+      const int r = warp * rows + i, rr = r0 + r;
+      const bool row = r < nr;
+      const long long from = row ? (c0 + rr / per) * a.ldq + (head * per + rr % per) * a.hq : 0;
+      float x[2][4];
+      uint32_t top = 0;
+#pragma unroll
+      for (int b = 0; b < (NC + 1) / 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = b * 128 + lane * 4 + j;
+          x[b][j] = row && e < c.d ? (a.dtq ? __bfloat162float(((const bf16*)a.q)[from + e]) : ((const float*)a.q)[from + e]) : 0.f;
+          top = max(top, __float_as_uint(x[b][j]) & 0x7FFFFFFFu);
+        }
+      top = __reduce_max_sync(0xffffffffu, top);
+      float up, down;
+      kv_row_scale(top, &up, &down);
+      up *= sign;
+#pragma unroll
+      for (int b = 0; b < (NC + 1) / 2; ++b) {
+        const int e = b * 128 + lane * 4;
+        if (e < NC * 64)
+          *reinterpret_cast<uint2*>(smem + L::kOffQ + (r >> 7) * L::kQ + (e >> 6) * (128 * 128) + (r & 127) * 128 + ((((e & 63) >> 3) ^ (r & 7)) << 4) + (e & 4) * 2) =
+              make_uint2(f16_pair(x[b][0] * up, x[b][1] * up), f16_pair(x[b][2] * up, x[b][3] * up));
+      }
+      if (lane == 0) rows_down[r] = sign == 0.f ? 1.f : fabsf(a.scale) * kLog2e * down;
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_at;
+  constexpr uint32_t kColO = 2 * FK;
+
+  if (n_tiles == 0) {
+    if (work && warp >= 4 && warp < 12) {                                  // nothing to see (no piece shares this tile): zeros
+      for (int i = (warp - 4) * 32 + lane; i < nr * c.dv; i += 256) {
+        const int r = i / c.dv, rr = r0 + r;
+        st_dt(a.out, a.dt_out, ((long long)(c0 + rr / per) * a.H + head * per + rr % per) * c.dv + i - r * c.dv, 0.f);
+      }
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------ decode: K(0), then K(it + 1) and V(it) in turn; each tile's codes are on their way a tile ahead
+    regs_down<kRegDecode>();
+    const int ct = threadIdx.x - 384;
+    constexpr int NR = FK / 32;
+    uint4 xk[NR * NC], xv[NR * NV];
+    uint32_t f[NR], fk[NR], fv[NR];
+    const auto plan = [&](int it) { mbar_wait(&plan_full[it % kPlans], it / kPlans & 1); };
+    const auto factor = [&](int it) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) f[i] = factors[it % kPlans * FK + (ct >> 2) + 32 * i];
+    };
+    const auto keys = [&](int it) {
+      const int b = it & 1;
+      factor(it);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) fk[i] = __byte_perm(f[i], 0, 0x1010);
+      mbar_wait(&k_empty[b], (it >> 1 & 1) ^ 1);
+      pair_store<FMT, NR, NC>(smem + L::kOffK + b * L::kK, ct, fk, xk);
+      if (lane == 0) mbar_arrive(&k_full[b]);
+    };
+    plan(0);
+    pair_load<NR, NC>(c.k, c.d, ct, groups, xk);
+    pair_load<NR, NV>(c.v, c.dv, ct, groups, xv);
+    keys(0);
+    if (n_tiles > 1) {
+      plan(1);
+      pair_load<NR, NC>(c.k, c.d, ct, groups + 8, xk);
+    }
+    for (int it = 0; it < n_tiles; ++it) {
+      if (it + 1 < n_tiles) keys(it + 1);
+      if (it + 2 < n_tiles) {
+        plan(it + 2);
+        pair_load<NR, NC>(c.k, c.d, ct, groups + (it + 2) % kPlans * 8, xk);
+      }
+      const int b = it & 1;
+      factor(it);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) fv[i] = __byte_perm(f[i], 0, 0x3232);
+      mbar_wait(&v_empty[b], (it >> 1 & 1) ^ 1);
+      pair_store<FMT, NR, NV>(smem + L::kOffV + b * L::kV, ct, fv, xv);
+      if (lane == 0) {
+        mbar_arrive(&v_full[b]);
+        mbar_arrive(&plan_empty[it % kPlans]);
+      }
+      if (it + 1 < n_tiles) pair_load<NR, NV>(c.v, c.dv, ct, groups + (it + 1) % kPlans * 8, xv);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax: group w has row tile w (or the key tiles w, w + 2 ... of the one there is), a thread a row
+    regs_up<kRegSoftmax>();
+    const int grp = (warp - 4) >> 2, quarter = warp & 3, row = (two ? grp * 128 : 0) + quarter * 32 + lane, rr = r0 + row;
+    const bool live = row < nr;
+    const int tok = live ? c0 + rr / per : t0, pos = live ? t.positions[tok] : -1;
+    int least, most;
+    {                                        // of the warp's rows
+      const int w0 = row - lane, ra = min(r0 + w0, r0 + nr - 1), rb = min(r0 + w0 + 31, r0 + nr - 1);
+      kv_reach(t, span, c0 + ra / per, c0 + rb / per, &least, &most);
+    }
+    const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lane_at + grp * FK, o_at = lane_at + kColO + grp * (64 * NV);
+    const float down = rows_down[row];
+    float m = -INFINITY, l = 0.f, ref = 0.f;
+    int k = 0;                               // tiles of this group so far
+    for (int it = two ? 0 : grp; it < n_tiles; it += two ? 1 : 2, ++k) {
+      mbar_wait(&s_full[grp], k & 1);
+      tc_fence_after_sync();
+      const float2 unit = units[it % kUnits];
+      float x[FK];
+      {
+        uint32_t r[FK / 16][16];
+#pragma unroll
+        for (int i = 0; i < FK / 16; ++i) tmem_ld16(s_at + 16 * i, r[i]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < FK; ++j) x[j] = __uint_as_float(r[j / 16][j % 16]);
+      }
+      const int ua = u0 + it * GT, ub = min(ua + GT, u1) - 1;              // groups of the tile
+      const int pa = span.group(ua) * kKvGroup, pb = span.group(ub) * kKvGroup + kKvGroup - 1;
+      const bool all = ub == ua + GT - 1 && pb < span.base && pb <= least && (pb < a.first || (ua >= span.na && most - pa < a.window));
+      if (!all) {
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+          const int u = ua + g, j0 = span.group(u) * kKvGroup;
+          uint32_t see = 0;
+          if (u < u1 && live) {
+            if (j0 + kKvGroup <= span.base) {                              // the positions of a group that are no further than the row's, and near enough or among the first
+              see = pos < j0 ? 0u : pos - j0 >= 15 ? 0xFFFFu : (2u << (pos - j0)) - 1;
+              const int far = pos - a.window - j0 + 1;                     // these of the group lie ahead of the window
+              if (far > 0) see &= (far >= 16 ? 0u : 0xFFFFu << far) | (a.first <= j0 ? 0u : a.first - j0 >= 16 ? 0xFFFFu : (1u << (a.first - j0)) - 1);
+            } else {
+#pragma unroll 1
+              for (int j = 0; j < 16; ++j) see |= (uint32_t)kv_sees(t, a, span, c0, n, tok, pos, j0 + j) << j;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (!(see >> j & 1u)) x[16 * g + j] = -INFINITY;
+        }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < FK; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], x[j], x[j + 1]);
+      const float fac = fminf(fmaxf(down * unit.x, 1e-37f), 1e37f);
+      const float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * fac;
+      const float mn = fmaxf(m, mt), from = mn == -INFINITY ? 0.f : mn, back = ex2(m - from);
+      m = mn;
+      l *= back;
+      ref *= back;
+      const float big = ex2(mt - from) * unit.y;                           // the tile's largest weight times unit
+      float grow = 1.f;
+      if (big > ref * 32768.f && big > 1e-37f) {
+        const float r = fmaxf(big * 0.015625f, 1e-37f);
+        grow = ref / r;
+        ref = r;
+      }
+      if (k > 0 && __any_sync(0xffffffffu, grow != 1.f)) {                 // the products so far are in O: this tile's scores came behind them
+#pragma unroll 2
+        for (int o = 0; o < 64 * NV; o += 16) {
+          uint32_t r[16];
+          tmem_ld16(o_at + o, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * grow);
+          tmem_st16(o_at + o, r);
+        }
+      }
+      const float f = ref >= 1e-37f ? unit.y * __frcp_rn(ref) : 0.f;
+      const uint64_t fac2 = pair_of(fac, fac), neg2 = pair_of(-from, -from), f2 = pair_of(f, f);
+      uint64_t sum[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < FK / 32; ++i) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 e = pair_get(pair_fma(pair_of(x[32 * i + j], x[32 * i + j + 1]), fac2, neg2));
+          const uint64_t p = pair_of(ex2(e.x), ex2(e.y));
+          sum[j >> 1 & 1] = pair_add(sum[j >> 1 & 1], p);
+          const float2 y = pair_get(pair_mul(p, f2));
+          pk[j / 2] = f16_pair(y.x, y.y);
+        }
+        tmem_st16(s_at + 16 * i, pk);
+      }
+      const float2 s2 = pair_get(pair_add(sum[0], sum[1]));
+      l += s2.x + s2.y;
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[grp]);
+    }
+    if (k > 0) {
+      mbar_wait(&pv_done[grp], (k - 1) & 1);
+      tc_fence_after_sync();
+    }
+    const int hd = head * per + rr % per;
+    const long long orow = (long long)tok * a.H + hd, part = orow * a.pieces + blockIdx.z;
+    const bool whole = np <= 1;
+    float ref1 = 0.f;
+    constexpr int kPad = 64 * NV + 1;        // numbers a row, an odd number: a row a thread meets every bank once
+    float* share = reinterpret_cast<float*>(smem + L::kOffQ) + (quarter * 32 + lane) * kPad;
+    float* stat = reinterpret_cast<float*>(smem + L::kOffQ) + 128 * kPad + (quarter * 32 + lane) * 3;
+    if (!two) {                              // the second group's share goes through the operands' memory, which no product reads any more once both groups are here
+      named_bar_sync(1, 256);
+      if (grp == 1) {
+        for (int o = 0; o < 64 * NV; o += 16) {
+          uint32_t r[16];
+          if (k > 0) {
+            tmem_ld16(o_at + o, r);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) share[o + j] = k > 0 ? __uint_as_float(r[j]) : 0.f;
+        }
+        stat[0] = m;
+        stat[1] = l;
+        stat[2] = ref;
+      }
+      named_bar_sync(1, 256);
+      if (grp == 0) {
+        const float m1 = stat[0], mn = fmaxf(m, m1), from = mn == -INFINITY ? 0.f : mn, back = ex2(m - from), back1 = ex2(m1 - from);
+        l = l * back + stat[1] * back1 + (stat[1] != stat[1] ? stat[1] : 0.f);
+        ref *= back;
+        ref1 = stat[2] * back1;
+        m = mn;
+      }
+    }
+    if (two || grp == 0) {
+      if (whole && live && a.sinks != nullptr && m != -INFINITY) l += ex2(fmaf(a.sinks[hd], kLog2e, -m));
+      const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f, by = ref * inv, by1 = ref1 * inv, none = l != l ? l : 0.f;      // a NaN may have a reference of 0
+      if (!whole && live) {
+        a.part_ml[2 * part] = m;
+        a.part_ml[2 * part + 1] = l;
+      }
+#pragma unroll 2
+      for (int o = 0; o < 64 * NV; o += 16) {
+        uint32_t r[16];
+        __syncwarp();                          // the warp reads tensor memory together
+        tmem_ld16(o_at + o, r);
+        tmem_ld_wait();
+        if (!live || o >= c.dv) continue;
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]) * by + none;
+        if (!two) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) y[j] = fmaf(share[o + j], by1, y[j]);
+        }
+        if (whole && a.dt_out) {
+          uint4* to = reinterpret_cast<uint4*>((bf16*)a.out + orow * c.dv + o);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            to[j] = make_uint4(bf16x2_bits_rn(y[8 * j + 1], y[8 * j]), bf16x2_bits_rn(y[8 * j + 3], y[8 * j + 2]), bf16x2_bits_rn(y[8 * j + 5], y[8 * j + 4]),
+                               bf16x2_bits_rn(y[8 * j + 7], y[8 * j + 6]));
+        } else {
+          float4* to = reinterpret_cast<float4*>(whole ? (float*)a.out + orow * c.dv + o : a.part_o + part * c.dv + o);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+        }
+      }
+    }
+  } else {
+    regs_down<kRegMma>();
+    if (warp == 1) {
+      // ---------------------------------------------------------- plans: lane l has the rows 4 l .. 4 l + 3 of a tile
+      const auto at_row = [&](int it) {
+        const int u = u0 + it * GT + lane / 4;
+        const long long r = lane * 4 < FK && it < n_tiles && u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
+        return r < 0 ? -1ll : r + ((long long)head << c.lps);
+      };
+      long long r = at_row(0);
+      for (int it = 0; it < n_tiles; ++it) {
+        float ks[4] = {}, vs[4] = {};
+        if (r >= 0) {
+          const float4 x = *reinterpret_cast<const float4*>(c.ks + r + (lane & 3) * 4), y = *reinterpret_cast<const float4*>(c.vs + r + (lane & 3) * 4);
+          ks[0] = x.x; ks[1] = x.y; ks[2] = x.z; ks[3] = x.w;
+          vs[0] = y.x; vs[1] = y.y; vs[2] = y.z; vs[3] = y.w;
+        }
+        const long long next = at_row(it + 1);
+        uint32_t kt = 0, vt = 0;             // the largest scales of rows that any row of the tile sees
+        const int j0 = span.group(u0 + it * GT + lane / 4) * kKvGroup + (lane & 3) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!(j0 + e < span.hi && (j0 + e >= span.lo || j0 + e < a.first))) ks[e] = vs[e] = 0.f;
+          const uint32_t x = __float_as_uint(ks[e]), y = __float_as_uint(vs[e]);
+          if (x < 0x7F800000u) kt = max(kt, x);
+          if (y < 0x7F800000u) vt = max(vt, y);
+        }
+        float kp, ki, vp, vi;
+        scale_unit(__reduce_max_sync(0xffffffffu, kt), &kp, &ki);
+        vt = __reduce_max_sync(0xffffffffu, vt);
+        scale_unit(vt, &vp, &vi);
+        uint32_t f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool none = vs[e] != vs[e];  // a row that is no number: its keys say so
+          f[e] = f16_pair(none ? vs[e] : ks[e] * ki, none ? 0.f : vs[e] * vi);
+        }
+        const int slot = it % kPlans;
+        mbar_wait(&plan_empty[slot], (it / kPlans & 1) ^ 1);
+        if (lane * 4 < FK) {
+          *reinterpret_cast<uint4*>(factors + slot * FK + lane * 4) = make_uint4(f[0], f[1], f[2], f[3]);
+          if ((lane & 3) == 0) groups[slot * 8 + lane / 4] = r < 0 ? -1 : (int)(r / kKvGroup);
+        }
+        if (lane == 0) units[it % kUnits] = make_float2(kp, vt ? vp : 0.f);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&plan_full[slot]);
+        r = next;
+      }
+    } else if (warp == 0) {
+      // ---------------------------------------------------------- tensor cores: whichever row tile's inputs are there
+      const uint32_t id_s = idesc_f16(FK, false), id_o = idesc_f16(64 * NV, true);
+      const uint32_t q_at = smem_u32(smem + L::kOffQ), k_at = smem_u32(smem + L::kOffK), v_at = smem_u32(smem + L::kOffV);
+      int it[2] = {0, two ? 0 : 1}, k[2] = {0, 0};
+      bool scored[2] = {false, false};
+      uint32_t idle = 0;
+      long long since = 0;
+      while (it[0] < n_tiles || it[1] < n_tiles) {
+        bool did = false;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (it[g] >= n_tiles) continue;
+          const int b = it[g] & 1;
+          if (!scored[g]) {
+            // S(k) lies where P(k - 1) did
+            if ((k[g] > 0 && !mbar_test(&pv_done[g], (k[g] - 1) & 1)) || !mbar_test(&k_full[b], it[g] >> 1 & 1)) continue;
+            tc_fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int h = 0; h < NC; ++h) {
+                const uint64_t ad = umma_desc_k_sw128(q_at + (two ? g : 0) * L::kQ + h * (128 * 128)), bd = umma_desc_k_sw128(k_at + b * L::kK + h * (FK * 128));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) umma_bf16(tmem + g * FK, ad + 2 * i, bd + 2 * i, id_s, h > 0 || i > 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[g]);
+              umma_commit(&k_empty[b]);
+            }
+            __syncwarp();
+            scored[g] = did = true;
+          } else {
+            if (!mbar_test(&p_full[g], k[g] & 1) || !mbar_test(&v_full[b], it[g] >> 1 & 1)) continue;
+            tc_fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int i = 0; i < FK / 16; ++i)
+                umma_bf16_ts(tmem + kColO + g * (64 * NV), tmem + g * FK + 8 * i, desc_mn(v_at + b * L::kV + i * 2048, FK * 128), id_o, k[g] > 0 || i > 0 ? 1u : 0u);
+              umma_commit(&pv_done[g]);
+              umma_commit(&v_empty[b]);
+            }
+            __syncwarp();
+            scored[g] = false;
+            did = true;
+            ++k[g];
+            it[g] += two ? 1 : 2;
+          }
+        }
+        if (did) {
+          idle = 0;
+          since = 0;
+        } else if ((++idle & 0xFFFu) == 0) {                               // bounded as every wait is: what comes then is wrong, and flagged
+          if (*reinterpret_cast<volatile int*>(&g_mbar_timed_out)) break;
+          const long long now = clock64();
+          if (since == 0) since = now;
+          else if (now - since > 4000000000ll) {
+            *reinterpret_cast<volatile int*>(&g_mbar_timed_out) = 1;
+            break;
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+template <int FMT, int NC, int NV>
+int launch(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t st) {
+  using L = PairShape<NC, NV>;
+  SEQ_CUDA((kb2::allow_smem<kv_pair_kernel<FMT, NC, NV>>(L::kTotal)));
+  auto kern = kv_pair_kernel<FMT, NC, NV>;
+  kb2::launch_pdl(kern, dim3(tiles, c.G, a.pieces), kThreads, L::kTotal, st, c, t, a);
+  SEQ_LAUNCHED();
+  return KB2SEQ_OK;
+}
+template <int FMT>
+int sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t st) {
+  if (c.d <= 64 && c.dv <= 64) return launch<FMT, 1, 1>(c, t, a, tiles, st);
+  return c.d <= 128 ? launch<FMT, 2, 2>(c, t, a, tiles, st) : launch<FMT, 3, 2>(c, t, a, tiles, st);
+}
+}  // namespace
+
+int kv_pair_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t stream) {
+  return fmt == KV_E4M3 ? sizes<KV_E4M3>(c, t, a, tiles, stream) : sizes<KV_INT8>(c, t, a, tiles, stream);
+}
+
+}  // namespace kb2seq

@@ -13,13 +13,13 @@
 // Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value scale are fp16 (11 bits).  Weights are rounded relative to a reference R per row
 // that follows the largest weight times scale (2^6 to 2^15 of it), as in the kernel for few rows; maxima, weights and their sum are fp32.
 // A row whose scale is NaN gets NaN keys and zero values: scores that nobody sees are replaced, and those that see it carry the NaN into the sum.
-#include "seq_kv_attn.cuh"
+#include "seq_kv_tc.cuh"
 
 namespace kb2seq {
 namespace {
 using namespace kb2;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512, kRows = 128;
 
 template <int NC, int NV>                    // chunks of 64 of d and dv
 struct TileShape {
@@ -32,62 +32,6 @@ struct TileShape {
   static constexpr int kTotal = kOffRow + 128 * 4;
   static_assert(kTotal <= 227 * 1024 && 3 * FK + 64 * NV <= 512 && kSlot % 128 == 0, "memory");
 };
-
-__device__ __forceinline__ uint32_t idesc_f16(uint32_t n, bool mn) {       // A and B fp16, accumulator fp32, 128 rows; mn: B lies with its columns side by side
-  return (1u << 4) | ((uint32_t)mn << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
-}
-// rows of 64 numbers (128 bytes) one key apart, chunks of 64 columns `chunk` bytes apart
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t chunk) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(chunk >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float m;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
-  return m;
-}
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
-  return p;
-}
-__device__ __forceinline__ float2 pair_get(uint64_t p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-  return f;
-}
-__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t p;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
-  return p;
-}
-__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
-  uint64_t p;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
-  return p;
-}
-__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
-  uint64_t p;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
-  return p;
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-      "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-// 2^-7 of the least power of two above a scale (its bits), and one over it: codes of 448 times 2^7 stay within fp16, and a scale keeps its bits down to 2^-21 of the
-// tile's largest.
-__device__ __forceinline__ void scale_unit(uint32_t bits, float* p, float* inv) {
-  const uint32_t e = min(max(bits >> 23, 8u), 252u) - 6;
-  *p = __uint_as_float(e << 23);
-  *inv = __uint_as_float((254 - e) << 23);
-}
 
 // Codes of a tile from `from` (rows of `width` bytes) into the operand at `to`.  A thread has the rows ct / 4 + 32 i and 16 bytes of each chunk of 64 of those, f times the
 // codes where see.  Odd rows take their chunks in another order: eight lanes that are served together then read 128 neighbouring bytes or two rows' halves, and the stores
@@ -165,9 +109,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     s = blockIdx.x / a.per_seq;
     tile = blockIdx.x - s * a.per_seq;
   } else {
-    in = kv_find_tile(t, per, kTileRows, a.least, a.most, blockIdx.x, &s, &tile);
+    in = kv_find_tile(t, per, kRows, a.least, a.most, blockIdx.x, &s, &tile);
   }
-  const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * kTileRows, nr = in ? (int)min((long long)n * per - r0, (long long)kTileRows) : 0;
+  const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * kRows, nr = in ? (int)min((long long)n * per - r0, (long long)kRows) : 0;
   int u0 = 0, u1 = 0, np = 0, t0 = c0, t1 = c0;
   KvSpan span{};
   if (nr > 0) {
@@ -519,6 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
 #pragma unroll 2
     for (int o = hf * OH; o < (hf + 1) * OH; o += 16) {
       uint32_t r[16];
+      __syncwarp();                          // the warp reads tensor memory together
       tmem_ld16(lane_at + kColO + o, r);
       tmem_ld_wait();
       if (!live || o >= c.dv) continue;
@@ -555,11 +500,7 @@ int launch(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaSt
 }
 template <int FMT>
 int sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t st) {
-  if (c.d <= 64 && c.dv <= 64) return launch<FMT, 1, 1>(c, t, a, tiles, st);
-  if (c.d <= 128 && c.dv <= 128) return launch<FMT, 2, 2>(c, t, a, tiles, st);
-  if (c.d <= 192 && c.dv <= 128) return launch<FMT, 3, 2>(c, t, a, tiles, st);
-  if (c.d <= 128) return launch<FMT, 2, 4>(c, t, a, tiles, st);
-  return launch<FMT, 4, 4>(c, t, a, tiles, st);
+  return c.d <= 128 ? launch<FMT, 2, 4>(c, t, a, tiles, st) : launch<FMT, 4, 4>(c, t, a, tiles, st);
 }
 }  // namespace
 
