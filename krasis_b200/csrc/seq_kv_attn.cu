@@ -541,6 +541,7 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   a.ldq = ldq;
   a.hq = hq;
   a.dtq = dt_q;
+  a.vec = ((uintptr_t)q & (dt_q ? 7 : 15)) == 0 && ldq % 4 == 0 && hq % 4 == 0;
   a.H = H;
   a.window = win;
   a.first = first;

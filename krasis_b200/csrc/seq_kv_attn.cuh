@@ -14,6 +14,7 @@ struct KvAttn {                              // what a call says beside the cach
   const void* q;
   long long ldq, hq;
   int dtq, H, window, first;
+  bool vec;                                  // four numbers of a query at a time lie on whole addresses
   float scale;
   const float* sinks;
   void* out;
@@ -75,6 +76,38 @@ __device__ __forceinline__ void kv_row_scale(uint32_t top, float* up, float* dow
   const int e = min(max(141 - (int)(top >> 23), -113), 100);
   *up = __uint_as_float((uint32_t)(127 + e) << 23);
   *down = __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+// Four numbers of the queries from `from` on, of which `left` are the row's (none or all four).  vec: addresses are whole in them.
+__device__ __forceinline__ void query4(const KvAttn& a, long long from, int left, float (&x)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = 0.f;
+  if (left <= 0) return;
+  if (a.dtq) {
+    const bf16* p = (const bf16*)a.q + from;
+    if (a.vec) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      x[0] = __uint_as_float(v.x << 16);
+      x[1] = __uint_as_float(v.x & 0xFFFF0000u);
+      x[2] = __uint_as_float(v.y << 16);
+      x[3] = __uint_as_float(v.y & 0xFFFF0000u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = __bfloat162float(p[j]);
+    }
+  } else {
+    const float* p = (const float*)a.q + from;
+    if (a.vec) {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      x[0] = v.x;
+      x[1] = v.y;
+      x[2] = v.z;
+      x[3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = p[j];
+    }
+  }
 }
 
 // Tiles on the tensor cores: 256 rows (seq_kv_pair.cu), 128 where tensor memory has no room for two outputs (seq_kv_tile.cu).

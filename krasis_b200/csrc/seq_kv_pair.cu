@@ -26,6 +26,9 @@ static_assert(kRegMma + 2 * kRegSoftmax + kRegDecode <= 4 * 128, "registers of t
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+constexpr int kBarShare = 1, kBarTurn = 2;   // named barriers: both groups; the first group's turn, the second's
+__device__ __forceinline__ void named_bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
 constexpr int kPlans = 4, kUnits = 8;        // tiles that are planned ahead; units are read later than the rest
 
 template <int NC, int NV>                    // chunks of 64 of d and dv
@@ -88,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   // by buffer: k_full .. v_empty; by row tile: s_full, p_full, pv_done; by plan: plan_full, plan_empty
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10, *pv_done = bars + 12, *plan_full = bars + 14,
-           *plan_empty = bars + 14 + kPlans;
+           *plan_empty = bars + 14 + kPlans, *q_full = bars + 14 + 2 * kPlans;
   uint32_t* factors = reinterpret_cast<uint32_t*>(smem + L::kOffFac);      // [kPlans][FK] fp16: of the row's key codes, of its value codes
   int* groups = reinterpret_cast<int*>(smem + L::kOffGroup);               // [kPlans][8] where the groups lie (rows / 16), -1: nowhere
   float2* units = reinterpret_cast<float2*>(smem + L::kOffUnit);           // [kUnits] of keys, of values
@@ -135,43 +138,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       mbar_init(&plan_full[i], 1);
       mbar_init(&plan_empty[i], 4);
     }
+    mbar_init(q_full, 8);
     fence_mbar_init();
   }
-
-  // queries, a warp a row: scaled by a power of two, rounded to fp16, in the operand's layout (rows of 64 numbers, 16-byte pieces swizzled by the row)
-  if (work) {
-    const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;  // factors on scores are positive: a row's maximum is its largest raw score's
-    const int rows = two ? 16 : 8;
-#pragma unroll 4
-    for (int i = 0; i < rows; ++i) {
-      const int r = warp * rows + i, rr = r0 + r;
-      const bool row = r < nr;
-      const long long from = row ? (c0 + rr / per) * a.ldq + (head * per + rr % per) * a.hq : 0;
-      float x[2][4];
-      uint32_t top = 0;
-#pragma unroll
-      for (int b = 0; b < (NC + 1) / 2; ++b)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = b * 128 + lane * 4 + j;
-          x[b][j] = row && e < c.d ? (a.dtq ? __bfloat162float(((const bf16*)a.q)[from + e]) : ((const float*)a.q)[from + e]) : 0.f;
-          top = max(top, __float_as_uint(x[b][j]) & 0x7FFFFFFFu);
-        }
-      top = __reduce_max_sync(0xffffffffu, top);
-      float up, down;
-      kv_row_scale(top, &up, &down);
-      up *= sign;
-#pragma unroll
-      for (int b = 0; b < (NC + 1) / 2; ++b) {
-        const int e = b * 128 + lane * 4;
-        if (e < NC * 64)
-          *reinterpret_cast<uint2*>(smem + L::kOffQ + (r >> 7) * L::kQ + (e >> 6) * (128 * 128) + (r & 127) * 128 + ((((e & 63) >> 3) ^ (r & 7)) << 4) + (e & 4) * 2) =
-              make_uint2(f16_pair(x[b][0] * up, x[b][1] * up), f16_pair(x[b][2] * up, x[b][3] * up));
-      }
-      if (lane == 0) rows_down[r] = sign == 0.f ? 1.f : fabsf(a.scale) * kLog2e * down;
-    }
-  }
-  fence_proxy_async_smem();
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -244,10 +213,57 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       kv_reach(t, span, c0 + ra / per, c0 + rb / per, &least, &most);
     }
     const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lane_at + grp * FK, o_at = lane_at + kColO + grp * (64 * NV);
+    // queries, a warp a row: scaled by a power of two, rounded to fp16, in the operand's layout (rows of 64 numbers, 16-byte pieces swizzled by the row).  A warp brings
+    // its own rows; where both groups have the same, the first half of its group's 32.
+    const int own = two ? 32 : 16, first_row = (two ? grp * 128 : 0) + quarter * 32 + (two ? 0 : grp * 16);
+    const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;  // factors on scores are positive: a row's maximum is its largest raw score's
+    for (int i0 = 0; i0 < own; i0 += 16) {
+      float x[16][(NC + 1) / 2][4];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = first_row + i0 + i, q = r0 + r, e = lane * 4;
+        const long long from = r < nr ? (c0 + q / per) * a.ldq + (head * per + q % per) * a.hq : 0;
+#pragma unroll
+        for (int b = 0; b < (NC + 1) / 2; ++b) query4(a, from + b * 128 + e, r < nr ? c.d - b * 128 - e : 0, x[i][b]);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = first_row + i0 + i;
+        uint32_t top = 0;
+#pragma unroll
+        for (int b = 0; b < (NC + 1) / 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[i][b][j]) & 0x7FFFFFFFu);
+        top = __reduce_max_sync(0xffffffffu, top);
+        float up, undo;
+        kv_row_scale(top, &up, &undo);
+        up *= sign;
+#pragma unroll
+        for (int b = 0; b < (NC + 1) / 2; ++b) {
+          const int e = b * 128 + lane * 4;
+          if (e < NC * 64)
+            *reinterpret_cast<uint2*>(smem + L::kOffQ + (r >> 7) * L::kQ + (e >> 6) * (128 * 128) + (r & 127) * 128 + ((((e & 63) >> 3) ^ (r & 7)) << 4) + (e & 4) * 2) =
+                make_uint2(f16_pair(x[i][b][0] * up, x[i][b][1] * up), f16_pair(x[i][b][2] * up, x[i][b][3] * up));
+        }
+        if (lane == 0) rows_down[r] = sign == 0.f ? 1.f : fabsf(a.scale) * kLog2e * undo;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+    if (!two) named_bar_sync(kBarShare, 256);
     const float down = rows_down[row];
     float m = -INFINITY, l = 0.f, ref = 0.f;
+    // The groups take turns at the exponentials, so that the tensor cores have one's products to do meanwhile: both at once they wait for the other's unit at once too.
+    if (grp == 1) named_bar_arrive(kBarTurn, 256);
     int k = 0;                               // tiles of this group so far
-    for (int it = two ? 0 : grp; it < n_tiles; it += two ? 1 : 2, ++k) {
+    const int turns = two ? n_tiles : (n_tiles + 1) / 2;
+    for (; k < turns; ++k) {
+      const int it = two ? k : 2 * k + grp;
+      if (it >= n_tiles) {                   // one tile fewer: the turn is passed on
+        named_bar_sync(kBarTurn + grp, 256);
+        break;
+      }
       mbar_wait(&s_full[grp], k & 1);
       tc_fence_after_sync();
       const float2 unit = units[it % kUnits];
@@ -313,6 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       const float f = ref >= 1e-37f ? unit.y * __frcp_rn(ref) : 0.f;
       const uint64_t fac2 = pair_of(fac, fac), neg2 = pair_of(-from, -from), f2 = pair_of(f, f);
       uint64_t sum[2] = {0, 0};
+      named_bar_sync(kBarTurn + grp, 256);
 #pragma unroll
       for (int i = 0; i < FK / 32; ++i) {
         uint32_t pk[16];
@@ -326,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
         }
         tmem_st16(s_at + 16 * i, pk);
       }
+      if (grp == 0 || k + 1 < turns) named_bar_arrive(kBarTurn + (grp ^ 1), 256);
       const float2 s2 = pair_get(pair_add(sum[0], sum[1]));
       l += s2.x + s2.y;
       tmem_st_wait();
@@ -345,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     float* share = reinterpret_cast<float*>(smem + L::kOffQ) + (quarter * 32 + lane) * kPad;
     float* stat = reinterpret_cast<float*>(smem + L::kOffQ) + 128 * kPad + (quarter * 32 + lane) * 3;
     if (!two) {                              // the second group's share goes through the operands' memory, which no product reads any more once both groups are here
-      named_bar_sync(1, 256);
+      named_bar_sync(kBarShare, 256);
       if (grp == 1) {
         for (int o = 0; o < 64 * NV; o += 16) {
           uint32_t r[16];
@@ -360,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
         stat[1] = l;
         stat[2] = ref;
       }
-      named_bar_sync(1, 256);
+      named_bar_sync(kBarShare, 256);
       if (grp == 0) {
         const float m1 = stat[0], mn = fmaxf(m, m1), from = mn == -INFINITY ? 0.f : mn, back = ex2(m - from), back1 = ex2(m1 - from);
         l = l * back + stat[1] * back1 + (stat[1] != stat[1] ? stat[1] : 0.f);
@@ -459,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       bool scored[2] = {false, false};
       uint32_t idle = 0;
       long long since = 0;
+      mbar_wait(q_full, 0);
       while (it[0] < n_tiles || it[1] < n_tiles) {
         bool did = false;
 #pragma unroll
