@@ -1,14 +1,15 @@
 // Attention over the 8-bit cache for many query rows per key / value head on tcgen05, heads of up to 192 (keys) and 128 (values): two tiles of 128 (token, head) rows of one
 // sequence and kv head share every key tile that is decoded.  The H / G heads that share keys fill the rows together.  Roles of a CTA of 16 warps:
-//   warp  1      plans: looks up the key tiles' groups in the page list, reads their scales, and leaves for each row the factors that its codes are multiplied with
-//   warps 12-15  decode: codes from the pages into registers, a tile ahead, as fp16 (code times factor, one packed product for two) into the swizzled operand tiles
-//   warp  0      tcgen05.mma: S = Q K^T and O += P V for both row tiles as their inputs come (P from tensor memory, in S's place)
-//   warps 4-7, 8-11  softmax of the first and of the second row tile, a thread a row: while one works the tensor cores make the other's scores
+//   warp  1      plans 128 keys at a time: looks up their groups in the page list, reads their scales, and leaves for each row the factors that its codes are multiplied with
+//   warps 12-15  decode 64 keys at a time: codes from the pages into registers, two tiles ahead, as fp16 (code times factor, one packed product for two) into the operands
+//   warps 0, 3   tcgen05.mma for a row tile each: S = Q K^T and O += P V (P from tensor memory, in S's place)
+//   warps 4-7, 8-11  softmax of the first and of the second row tile, a thread a row
 // Where a sequence has no more than 128 rows left both softmax groups have the same rows and take the key tiles in turn; they are joined at the end.
-// FK = 128 keys a tile (64 for keys of 192).  Tensor memory: S 2 FK | O 2 x 64 NV.
+// Key tiles of 64 with two buffers of scores per row tile, so that the next scores are made while a tile's are worked on; four buffers of keys and of values.
+// Tensor memory: S 2 x 2 x 64 | O 2 x 64 NV.
 //
-// What bounds it: for a tile of 128 keys and 256 rows 32768 exponentials take 2048 cycles (16 a cycle), and shared memory's 128 bytes a cycle are taken for 2048 as well
-// (both products read Q, K and V: 192 KB; decoding writes 64 KB).
+// What bounds it: for 128 keys and 256 rows 32768 exponentials take 2048 cycles (16 a cycle), and shared memory's 128 bytes a cycle are taken for 2560 (the first product
+// reads Q again for every 64 keys: 192 KB, the second V: 64 KB, decoding writes 64 KB).
 //
 // Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value unit are fp16 (11 bits).  A row's factor is its scale over a unit, a power of two
 // near the tile's largest scale (exact for scales that are powers of two); the units join the softmax's factors.  Weights are rounded relative to a reference R per row that
@@ -19,33 +20,18 @@
 namespace kb2seq {
 namespace {
 
-constexpr int kThreads = 512;
-// Registers a thread of each warpgroup: planning and tensor cores, softmax (twice), decoding: 4 x 128 at launch.
-constexpr int kRegMma = 56, kRegSoftmax = 176, kRegDecode = 104;
-static_assert(kRegMma + 2 * kRegSoftmax + kRegDecode <= 4 * 128, "registers of the launch");
-template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
-constexpr int kBarShare = 1, kBarTurn = 2;   // named barriers: both groups; the first group's turn, the second's
-__device__ __forceinline__ void named_bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-
-constexpr int kPlans = 4, kUnits = 8;        // tiles that are planned ahead; units are read later than the rest
+constexpr int kThreads = 512, FK = 64, GT = FK / kKvGroup, kBufs = 4;      // keys of a tile, their groups; operand buffers
+constexpr int kBarShare = 1;                 // named barrier of both softmax groups
+constexpr int kPlans = 4, kUnits = 8;        // pairs of tiles that are planned ahead; units are read later than the rest
 
 template <int NC, int NV>                    // chunks of 64 of d and dv
 struct PairShape {
-  static constexpr int FK = NC > 2 ? 64 : 128;
-  static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128;
-  static constexpr int kOffQ = 0, kOffK = 2 * kQ, kOffV = kOffK + 2 * kK, kOffFac = kOffV + 2 * kV, kOffGroup = kOffFac + kPlans * FK * 4, kOffBar = kOffGroup + kPlans * 32,
-                       kOffUnit = kOffBar + 192, kOffTmem = kOffUnit + kUnits * 8, kOffRow = kOffTmem + 16, kTotal = kOffRow + 256 * 4;
-  static_assert(kTotal <= 227 * 1024 && 2 * FK + 128 * NV <= 512, "memory");
-  static_assert(128 * (64 * NV + 1) * 4 + 128 * 12 <= 2 * kQ + 2 * kK + 2 * kV, "the second group's share at the end");
+  static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128, kKeys = NC > 2 ? 2 : kBufs;      // kKeys: buffers of keys
+  static constexpr int kOffQ = 0, kOffK = 2 * kQ, kOffV = kOffK + kKeys * kK, kOffFac = kOffV + kBufs * kV, kOffGroup = kOffFac + kPlans * 512,
+                       kOffBar = kOffGroup + kPlans * 32, kOffUnit = kOffBar + 320, kOffTmem = kOffUnit + kUnits * 8, kOffRow = kOffTmem + 16, kTotal = kOffRow + 256 * 4;
+  static_assert(kTotal <= 227 * 1024 && 4 * FK + 128 * NV <= 512, "memory");
+  static_assert(128 * (64 * NV + 1) * 4 + 128 * 12 <= 2 * kQ + kKeys * kK + kBufs * kV, "the second group's share at the end");
 };
-
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return ok != 0;
-}
 
 // A thread's 16 bytes of each chunk of 64 of the rows ct / 4 + 32 i.
 template <int NR, int CH>
@@ -86,13 +72,12 @@ __device__ __forceinline__ void pair_store(uint8_t* to, int ct, const uint32_t (
 template <int FMT, int NC, int NV>
 __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep t, KvAttn a) {
   using L = PairShape<NC, NV>;
-  constexpr int FK = L::FK, GT = FK / kKvGroup;                            // groups a tile
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
-  // by buffer: k_full .. v_empty; by row tile: s_full, p_full, pv_done; by plan: plan_full, plan_empty
-  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10, *pv_done = bars + 12, *plan_full = bars + 14,
-           *plan_empty = bars + 14 + kPlans, *q_full = bars + 14 + 2 * kPlans;
-  uint32_t* factors = reinterpret_cast<uint32_t*>(smem + L::kOffFac);      // [kPlans][FK] fp16: of the row's key codes, of its value codes
+  // by buffer: k_full .. v_empty; by row tile and buffer of scores: s_full, p_full, pv_done; by plan: plan_full, plan_empty
+  uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 12, *s_full = bars + 16, *p_full = bars + 20, *pv_done = bars + 24, *plan_full = bars + 28,
+           *plan_empty = bars + 28 + kPlans, *q_full = bars + 28 + 2 * kPlans;
+  uint32_t* factors = reinterpret_cast<uint32_t*>(smem + L::kOffFac);      // [kPlans][128] fp16: of the row's key codes, of its value codes
   int* groups = reinterpret_cast<int*>(smem + L::kOffGroup);               // [kPlans][8] where the groups lie (rows / 16), -1: nowhere
   float2* units = reinterpret_cast<float2*>(smem + L::kOffUnit);           // [kUnits] of keys, of values
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
@@ -125,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
   const int n_tiles = work ? max(0, (u1 - u0 + GT - 1) / GT) : 0;
   const bool two = nr > 128;                 // two row tiles; else one whose key tiles go to both groups in turn
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&k_full[i], 4);
       mbar_init(&v_full[i], 4);
       mbar_init(&k_empty[i], two ? 2 : 1);
@@ -145,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_at;
-  constexpr uint32_t kColO = 2 * FK;
+  constexpr uint32_t kColO = 4 * FK;
 
   if (n_tiles == 0) {
     if (work && warp >= 4 && warp < 12) {                                  // nothing to see (no piece shares this tile): zeros
@@ -155,55 +140,48 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       }
     }
   } else if (warp >= 12) {
-    // ------------------------------------------------------------ decode: K(0), then K(it + 1) and V(it) in turn; each tile's codes are on their way a tile ahead
-    regs_down<kRegDecode>();
+    // ------------------------------------------------------------ decode
     const int ct = threadIdx.x - 384;
     constexpr int NR = FK / 32;
-    uint4 xk[NR * NC], xv[NR * NV];
-    uint32_t f[NR], fk[NR], fv[NR];
-    const auto plan = [&](int it) { mbar_wait(&plan_full[it % kPlans], it / kPlans & 1); };
-    const auto factor = [&](int it) {
-#pragma unroll
-      for (int i = 0; i < NR; ++i) f[i] = factors[it % kPlans * FK + (ct >> 2) + 32 * i];
+    uint4 xk[2][NR * NC], xv[2][NR * NV];
+    const auto fetch = [&](int it, auto& k, auto& v) {
+      if (it >= n_tiles) return;
+      const int p = it >> 1, slot = p % kPlans;
+      mbar_wait(&plan_full[slot], p / kPlans & 1);
+      const int* g = groups + slot * 8 + (it & 1) * GT;
+      pair_load<NR, NC>(c.k, c.d, ct, g, k);
+      pair_load<NR, NV>(c.v, c.dv, ct, g, v);
     };
-    const auto keys = [&](int it) {
-      const int b = it & 1;
-      factor(it);
+    const auto work_on = [&](int it, auto& k, auto& v) {
+      if (it >= n_tiles) return;
+      const int kb = it % L::kKeys, vb = it % kBufs, slot = (it >> 1) % kPlans;
+      uint32_t f[NR], fk[NR], fv[NR];
 #pragma unroll
-      for (int i = 0; i < NR; ++i) fk[i] = __byte_perm(f[i], 0, 0x1010);
-      mbar_wait(&k_empty[b], (it >> 1 & 1) ^ 1);
-      pair_store<FMT, NR, NC>(smem + L::kOffK + b * L::kK, ct, fk, xk);
-      if (lane == 0) mbar_arrive(&k_full[b]);
-    };
-    plan(0);
-    pair_load<NR, NC>(c.k, c.d, ct, groups, xk);
-    pair_load<NR, NV>(c.v, c.dv, ct, groups, xv);
-    keys(0);
-    if (n_tiles > 1) {
-      plan(1);
-      pair_load<NR, NC>(c.k, c.d, ct, groups + 8, xk);
-    }
-    for (int it = 0; it < n_tiles; ++it) {
-      if (it + 1 < n_tiles) keys(it + 1);
-      if (it + 2 < n_tiles) {
-        plan(it + 2);
-        pair_load<NR, NC>(c.k, c.d, ct, groups + (it + 2) % kPlans * 8, xk);
+      for (int i = 0; i < NR; ++i) {
+        f[i] = factors[slot * 128 + (it & 1) * FK + (ct >> 2) + 32 * i];
+        fk[i] = __byte_perm(f[i], 0, 0x1010);
+        fv[i] = __byte_perm(f[i], 0, 0x3232);
       }
-      const int b = it & 1;
-      factor(it);
-#pragma unroll
-      for (int i = 0; i < NR; ++i) fv[i] = __byte_perm(f[i], 0, 0x3232);
-      mbar_wait(&v_empty[b], (it >> 1 & 1) ^ 1);
-      pair_store<FMT, NR, NV>(smem + L::kOffV + b * L::kV, ct, fv, xv);
+      mbar_wait(&k_empty[kb], (it / L::kKeys & 1) ^ 1);
+      pair_store<FMT, NR, NC>(smem + L::kOffK + kb * L::kK, ct, fk, k);
+      if (lane == 0) mbar_arrive(&k_full[kb]);
+      mbar_wait(&v_empty[vb], (it / kBufs & 1) ^ 1);
+      pair_store<FMT, NR, NV>(smem + L::kOffV + vb * L::kV, ct, fv, v);
       if (lane == 0) {
-        mbar_arrive(&v_full[b]);
-        mbar_arrive(&plan_empty[it % kPlans]);
+        mbar_arrive(&v_full[vb]);
+        if ((it & 1) || it + 1 == n_tiles) mbar_arrive(&plan_empty[slot]);
       }
-      if (it + 1 < n_tiles) pair_load<NR, NV>(c.v, c.dv, ct, groups + (it + 1) % kPlans * 8, xv);
+    };
+    fetch(0, xk[0], xv[0]);
+    fetch(1, xk[1], xv[1]);
+    for (int it = 0; it < n_tiles; it += 2) {
+      work_on(it, xk[0], xv[0]);
+      fetch(it + 2, xk[0], xv[0]);
+      work_on(it + 1, xk[1], xv[1]);
+      fetch(it + 3, xk[1], xv[1]);
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax: group w has row tile w (or the key tiles w, w + 2 ... of the one there is), a thread a row
-    regs_up<kRegSoftmax>();
     const int grp = (warp - 4) >> 2, quarter = warp & 3, row = (two ? grp * 128 : 0) + quarter * 32 + lane, rr = r0 + row;
     const bool live = row < nr;
     const int tok = live ? c0 + rr / per : t0, pos = live ? t.positions[tok] : -1;
@@ -212,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       const int w0 = row - lane, ra = min(r0 + w0, r0 + nr - 1), rb = min(r0 + w0 + 31, r0 + nr - 1);
       kv_reach(t, span, c0 + ra / per, c0 + rb / per, &least, &most);
     }
-    const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lane_at + grp * FK, o_at = lane_at + kColO + grp * (64 * NV);
+    const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lane_at + grp * (2 * FK), o_at = lane_at + kColO + grp * (64 * NV);
     // queries, a warp a row: scaled by a power of two, rounded to fp16, in the operand's layout (rows of 64 numbers, 16-byte pieces swizzled by the row).  A warp brings
     // its own rows; where both groups have the same, the first half of its group's 32.
     const int own = two ? 32 : 16, first_row = (two ? grp * 128 : 0) + quarter * 32 + (two ? 0 : grp * 16);
@@ -253,25 +231,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     if (lane == 0) mbar_arrive(q_full);
     if (!two) named_bar_sync(kBarShare, 256);
     const float down = rows_down[row];
-    float m = -INFINITY, l = 0.f, ref = 0.f;
-    // The groups take turns at the exponentials, so that the tensor cores have one's products to do meanwhile: both at once they wait for the other's unit at once too.
-    if (grp == 1) named_bar_arrive(kBarTurn, 256);
+    float m = -INFINITY, l = 0.f, ref = 0.f, inv_ref = 0.f;
     int k = 0;                               // tiles of this group so far
-    const int turns = two ? n_tiles : (n_tiles + 1) / 2;
-    for (; k < turns; ++k) {
-      const int it = two ? k : 2 * k + grp;
-      if (it >= n_tiles) {                   // one tile fewer: the turn is passed on
-        named_bar_sync(kBarTurn + grp, 256);
-        break;
-      }
-      mbar_wait(&s_full[grp], k & 1);
+    for (int it = two ? 0 : grp; it < n_tiles; it += two ? 1 : 2, ++k) {
+      const int b = grp * 2 + (k & 1), turn = k >> 1 & 1;
+      const uint32_t x_at = s_at + (k & 1) * FK;
+      mbar_wait(&s_full[b], turn);
       tc_fence_after_sync();
-      const float2 unit = units[it % kUnits];
+      const float2 unit = units[(it >> 1) % kUnits];
       float x[FK];
       {
         uint32_t r[FK / 16][16];
 #pragma unroll
-        for (int i = 0; i < FK / 16; ++i) tmem_ld16(s_at + 16 * i, r[i]);
+        for (int i = 0; i < FK / 16; ++i) tmem_ld16(x_at + 16 * i, r[i]);
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < FK; ++j) x[j] = __uint_as_float(r[j / 16][j % 16]);
@@ -304,32 +276,37 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       for (int j = 0; j < FK; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], x[j], x[j + 1]);
       const float fac = fminf(fmaxf(down * unit.x, 1e-37f), 1e37f);
       const float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * fac;
-      const float mn = fmaxf(m, mt), from = mn == -INFINITY ? 0.f : mn, back = ex2(m - from);
-      m = mn;
-      l *= back;
-      ref *= back;
-      const float big = ex2(mt - from) * unit.y;                           // the tile's largest weight times unit
-      float grow = 1.f;
-      if (big > ref * 32768.f && big > 1e-37f) {
-        const float r = fmaxf(big * 0.015625f, 1e-37f);
-        grow = ref / r;
-        ref = r;
-      }
-      if (k > 0 && __any_sync(0xffffffffu, grow != 1.f)) {                 // the products so far are in O: this tile's scores came behind them
+      // a new maximum, or values whose unit may take a weight beyond fp16: seldom after the first tiles
+      if (__any_sync(0xffffffffu, mt > m || unit.y > ref * 32768.f)) {
+        const float mn = fmaxf(m, mt), from = mn == -INFINITY ? 0.f : mn, back = ex2(m - from);
+        m = mn;
+        l *= back;
+        ref *= back;
+        const float big = ex2(mt - from) * unit.y;                         // the tile's largest weight times unit
+        float grow = 1.f;
+        if (big > ref * 32768.f && big > 1e-37f) {
+          const float r = fmaxf(big * 0.015625f, 1e-37f);
+          grow = ref / r;
+          ref = r;
+        }
+        inv_ref = ref >= 1e-37f ? 1.f / ref : 0.f;
+        if (k > 0 && __any_sync(0xffffffffu, grow != 1.f)) {
+          mbar_wait(&pv_done[grp * 2 + ((k - 1) & 1)], (k - 1) >> 1 & 1);  // O holds every product so far
+          tc_fence_after_sync();
 #pragma unroll 2
-        for (int o = 0; o < 64 * NV; o += 16) {
-          uint32_t r[16];
-          tmem_ld16(o_at + o, r);
-          tmem_ld_wait();
+          for (int o = 0; o < 64 * NV; o += 16) {
+            uint32_t r[16];
+            tmem_ld16(o_at + o, r);
+            tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * grow);
-          tmem_st16(o_at + o, r);
+            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * grow);
+            tmem_st16(o_at + o, r);
+          }
         }
       }
-      const float f = ref >= 1e-37f ? unit.y * __frcp_rn(ref) : 0.f;
+      const float from = m == -INFINITY ? 0.f : m, f = unit.y * inv_ref;
       const uint64_t fac2 = pair_of(fac, fac), neg2 = pair_of(-from, -from), f2 = pair_of(f, f);
       uint64_t sum[2] = {0, 0};
-      named_bar_sync(kBarTurn + grp, 256);
 #pragma unroll
       for (int i = 0; i < FK / 32; ++i) {
         uint32_t pk[16];
@@ -341,18 +318,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
           const float2 y = pair_get(pair_mul(p, f2));
           pk[j / 2] = f16_pair(y.x, y.y);
         }
-        tmem_st16(s_at + 16 * i, pk);
+        tmem_st16(x_at + 16 * i, pk);
       }
-      if (grp == 0 || k + 1 < turns) named_bar_arrive(kBarTurn + (grp ^ 1), 256);
       const float2 s2 = pair_get(pair_add(sum[0], sum[1]));
       l += s2.x + s2.y;
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[grp]);
+      if (lane == 0) mbar_arrive(&p_full[b]);
     }
     if (k > 0) {
-      mbar_wait(&pv_done[grp], (k - 1) & 1);
+      mbar_wait(&pv_done[grp * 2 + ((k - 1) & 1)], (k - 1) >> 1 & 1);      // products end in their order
       tc_fence_after_sync();
     }
     const int hd = head * per + rr % per;
@@ -422,25 +398,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       }
     }
   } else {
-    regs_down<kRegMma>();
     if (warp == 1) {
-      // ---------------------------------------------------------- plans: lane l has the rows 4 l .. 4 l + 3 of a tile
-      const auto at_row = [&](int it) {
-        const int u = u0 + it * GT + lane / 4;
-        const long long r = lane * 4 < FK && it < n_tiles && u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
+      // ---------------------------------------------------------- plans: lane l has the rows 4 l .. 4 l + 3 of two tiles
+      const auto at_row = [&](int p) {
+        const int u = u0 + p * (2 * GT) + lane / 4;
+        const long long r = u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
         return r < 0 ? -1ll : r + ((long long)head << c.lps);
       };
       long long r = at_row(0);
-      for (int it = 0; it < n_tiles; ++it) {
+      for (int p = 0; p < (n_tiles + 1) / 2; ++p) {
         float ks[4] = {}, vs[4] = {};
         if (r >= 0) {
           const float4 x = *reinterpret_cast<const float4*>(c.ks + r + (lane & 3) * 4), y = *reinterpret_cast<const float4*>(c.vs + r + (lane & 3) * 4);
           ks[0] = x.x; ks[1] = x.y; ks[2] = x.z; ks[3] = x.w;
           vs[0] = y.x; vs[1] = y.y; vs[2] = y.z; vs[3] = y.w;
         }
-        const long long next = at_row(it + 1);
+        const long long next = at_row(p + 1);
         uint32_t kt = 0, vt = 0;             // the largest scales of rows that any row of the tile sees
-        const int j0 = span.group(u0 + it * GT + lane / 4) * kKvGroup + (lane & 3) * 4;
+        const int j0 = span.group(u0 + p * (2 * GT) + lane / 4) * kKvGroup + (lane & 3) * 4;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (!(j0 + e < span.hi && (j0 + e >= span.lo || j0 + e < a.first))) ks[e] = vs[e] = 0.f;
@@ -458,77 +433,60 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
           const bool none = vs[e] != vs[e];  // a row that is no number: its keys say so
           f[e] = f16_pair(none ? vs[e] : ks[e] * ki, none ? 0.f : vs[e] * vi);
         }
-        const int slot = it % kPlans;
-        mbar_wait(&plan_empty[slot], (it / kPlans & 1) ^ 1);
-        if (lane * 4 < FK) {
-          *reinterpret_cast<uint4*>(factors + slot * FK + lane * 4) = make_uint4(f[0], f[1], f[2], f[3]);
-          if ((lane & 3) == 0) groups[slot * 8 + lane / 4] = r < 0 ? -1 : (int)(r / kKvGroup);
-        }
-        if (lane == 0) units[it % kUnits] = make_float2(kp, vt ? vp : 0.f);
+        const int slot = p % kPlans;
+        mbar_wait(&plan_empty[slot], (p / kPlans & 1) ^ 1);
+        *reinterpret_cast<uint4*>(factors + slot * 128 + lane * 4) = make_uint4(f[0], f[1], f[2], f[3]);
+        if ((lane & 3) == 0) groups[slot * 8 + lane / 4] = r < 0 ? -1 : (int)(r / kKvGroup);
+        if (lane == 0) units[p % kUnits] = make_float2(kp, vt ? vp : 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&plan_full[slot]);
         r = next;
       }
-    } else if (warp == 0) {
-      // ---------------------------------------------------------- tensor cores: whichever row tile's inputs are there
+    } else if (warp == 0 || warp == 3) {
+      // ---------------------------------------------------------- tensor cores.  A warp for each row tile: the tensor cores take few products ahead (two or so), so what a warp does
+      // between its batches (waits, commits: some 300 cycles) is hidden by the other's.  S(k + 2) lies where P(k) did and waits for the second product of k.
+      const int g = warp == 3;
       const uint32_t id_s = idesc_f16(FK, false), id_o = idesc_f16(64 * NV, true);
       const uint32_t q_at = smem_u32(smem + L::kOffQ), k_at = smem_u32(smem + L::kOffK), v_at = smem_u32(smem + L::kOffV);
-      int it[2] = {0, two ? 0 : 1}, k[2] = {0, 0};
-      bool scored[2] = {false, false};
-      uint32_t idle = 0;
-      long long since = 0;
+      const auto scores = [&](int k) {                              // S = Q K^T of the group's tile k
+        const int it = two ? k : 2 * k + g, b = it % L::kKeys, x = g * 2 + (k & 1);
+        if (it >= n_tiles) return;
+        mbar_wait(&k_full[b], it / L::kKeys & 1);
+        if (k >= 2) mbar_wait(&pv_done[x], ((k - 2) >> 1) & 1);
+        tc_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int h = 0; h < NC; ++h) {
+            const uint64_t ad = umma_desc_k_sw128(q_at + (two ? g : 0) * L::kQ + h * (128 * 128)), bd = umma_desc_k_sw128(k_at + b * L::kK + h * (FK * 128));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) umma_bf16(tmem + x * FK, ad + 2 * i, bd + 2 * i, id_s, h > 0 || i > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[x]);
+          umma_commit(&k_empty[b]);
+        }
+        __syncwarp();
+      };
+      const auto output = [&](int k) {                              // O += P V
+        const int it = two ? k : 2 * k + g, b = it % kBufs, x = g * 2 + (k & 1);
+        if (it >= n_tiles) return;
+        mbar_wait(&v_full[b], it / kBufs & 1);
+        mbar_wait(&p_full[x], k >> 1 & 1);
+        tc_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < FK / 16; ++i)
+            umma_bf16_ts(tmem + kColO + g * (64 * NV), tmem + x * FK + 8 * i, desc_mn(v_at + b * L::kV + i * 2048, FK * 128), id_o, k > 0 || i > 0 ? 1u : 0u);
+          umma_commit(&pv_done[x]);
+          umma_commit(&v_empty[b]);
+        }
+        __syncwarp();
+      };
       mbar_wait(q_full, 0);
-      while (it[0] < n_tiles || it[1] < n_tiles) {
-        bool did = false;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (it[g] >= n_tiles) continue;
-          const int b = it[g] & 1;
-          if (!scored[g]) {
-            // S(k) lies where P(k - 1) did
-            if ((k[g] > 0 && !mbar_test(&pv_done[g], (k[g] - 1) & 1)) || !mbar_test(&k_full[b], it[g] >> 1 & 1)) continue;
-            tc_fence_after_sync();
-            if (elect_one()) {
-#pragma unroll
-              for (int h = 0; h < NC; ++h) {
-                const uint64_t ad = umma_desc_k_sw128(q_at + (two ? g : 0) * L::kQ + h * (128 * 128)), bd = umma_desc_k_sw128(k_at + b * L::kK + h * (FK * 128));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) umma_bf16(tmem + g * FK, ad + 2 * i, bd + 2 * i, id_s, h > 0 || i > 0 ? 1u : 0u);
-              }
-              umma_commit(&s_full[g]);
-              umma_commit(&k_empty[b]);
-            }
-            __syncwarp();
-            scored[g] = did = true;
-          } else {
-            if (!mbar_test(&p_full[g], k[g] & 1) || !mbar_test(&v_full[b], it[g] >> 1 & 1)) continue;
-            tc_fence_after_sync();
-            if (elect_one()) {
-#pragma unroll
-              for (int i = 0; i < FK / 16; ++i)
-                umma_bf16_ts(tmem + kColO + g * (64 * NV), tmem + g * FK + 8 * i, desc_mn(v_at + b * L::kV + i * 2048, FK * 128), id_o, k[g] > 0 || i > 0 ? 1u : 0u);
-              umma_commit(&pv_done[g]);
-              umma_commit(&v_empty[b]);
-            }
-            __syncwarp();
-            scored[g] = false;
-            did = true;
-            ++k[g];
-            it[g] += two ? 1 : 2;
-          }
-        }
-        if (did) {
-          idle = 0;
-          since = 0;
-        } else if ((++idle & 0xFFFu) == 0) {                               // bounded as every wait is: what comes then is wrong, and flagged
-          if (*reinterpret_cast<volatile int*>(&g_mbar_timed_out)) break;
-          const long long now = clock64();
-          if (since == 0) since = now;
-          else if (now - since > 4000000000ll) {
-            *reinterpret_cast<volatile int*>(&g_mbar_timed_out) = 1;
-            break;
-          }
-        }
+      scores(0);
+      scores(1);
+      for (int k = 0; (two ? k : 2 * k + g) < n_tiles; ++k) {
+        output(k);
+        scores(k + 2);
       }
     }
   }
