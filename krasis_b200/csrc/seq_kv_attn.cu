@@ -139,9 +139,14 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     for (int i = 0; i < DU; ++i) {
       const int e = 64 * i + 16 * t4;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        x[i][j] = in && e < c.d ? (a.dtq ? __bfloat162float(((const bf16*)a.q)[from + e + j]) : ((const float*)a.q)[from + e + j]) : 0.f;
-        top = max(top, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+      for (int b = 0; b < 4; ++b) {
+        float y[4];
+        query4(a, from + e + 4 * b, in ? c.d - e : 0, y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[i][4 * b + j] = y[j];
+          top = max(top, __float_as_uint(y[j]) & 0x7FFFFFFFu);
+        }
       }
     }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -345,29 +350,41 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
       }
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < nr * c.dv; i += kSWarps * 32) {
-    const int q = i / c.dv, dim = i - q * c.dv;
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
+  // a thread takes eight columns of a row
+  constexpr int kCols = VU * 8;
+  for (int i = threadIdx.x; i < MT * kCols; i += kSWarps * 32) {
+    const int q = i / kCols, dim = (i - q * kCols) * 8;
+    if (q >= nr || dim >= c.dv) continue;
+    float top = -INFINITY, sum = 0.f, acc[8] = {};
 #pragma unroll
     for (int w = 0; w < kSWarps; ++w) top = fmaxf(top, stat[w * MT + q].x);
 #pragma unroll
     for (int w = 0; w < kSWarps; ++w) {
       const float4 x = stat[w * MT + q];
       sum += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top);                // a sum without a maximum is 0, or NaN from a row that holds one
-      acc += red[(w * MT + q) * (VU * 64) + dim];
+      const float4* r = reinterpret_cast<const float4*>(red + (w * MT + q) * (VU * 64) + dim);
+      const float4 lo = r[0], hi = r[1];
+      acc[0] += lo.x; acc[1] += lo.y; acc[2] += lo.z; acc[3] += lo.w;
+      acc[4] += hi.x; acc[5] += hi.y; acc[6] += hi.z; acc[7] += hi.w;
     }
     const int rr = r0 + q, hd = head * per + rr % per;
     const long long row = (long long)(c0 + rr / per) * a.H + hd;
     if (np <= 1) {
       if (a.sinks != nullptr && top != -INFINITY) sum += ex2(fmaf(a.sinks[hd], kLog2e, -top));
-      st_dt(a.out, a.dt_out, row * c.dv + dim, sum == 0.f ? 0.f : acc / sum);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= inv;
+    } else if (dim == 0) {
+      a.part_ml[2 * (row * a.pieces + z)] = top;
+      a.part_ml[2 * (row * a.pieces + z) + 1] = sum;
+    }
+    if (np <= 1 && a.dt_out) {
+      *reinterpret_cast<uint4*>((bf16*)a.out + row * c.dv + dim) =
+          make_uint4(kb2::bf16x2_bits_rn(acc[1], acc[0]), kb2::bf16x2_bits_rn(acc[3], acc[2]), kb2::bf16x2_bits_rn(acc[5], acc[4]), kb2::bf16x2_bits_rn(acc[7], acc[6]));
     } else {
-      const long long p = row * a.pieces + z;
-      a.part_o[p * c.dv + dim] = acc;
-      if (dim == 0) {
-        a.part_ml[2 * p] = top;
-        a.part_ml[2 * p + 1] = sum;
-      }
+      float4* to = reinterpret_cast<float4*>(np <= 1 ? (float*)a.out + row * c.dv + dim : a.part_o + (row * a.pieces + z) * c.dv + dim);
+      to[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
     }
   }
 }
