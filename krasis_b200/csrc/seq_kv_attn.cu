@@ -53,7 +53,8 @@ struct StreamShape {
   static_assert(kTotal <= 227 * 1024 && kOffQ % 16 == 0 && kStage % 16 == 0, "shared memory");
 };
 
-template <int FMT, int DU, int VU, int NQ, int PARTS>
+// FULL: d and dv are whole units, and every copy's address is one of two a lane has plus a constant.
+template <int FMT, int DU, int VU, int NQ, int PARTS, bool FULL>
 __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>::kBlocks)) kv_stream_kernel(KvLayer c, KvStep t, KvAttn a) {
   using L = StreamShape<DU, VU, NQ, PARTS>;
   constexpr int MT = L::MT, VB = L::VB, VC = L::VC, MV = VU * 4;         // MV: 16-row tiles of O^T
@@ -85,30 +86,33 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   __syncthreads();
 
   const uint32_t ring = kb2::smem_u32(smem) + warp * (kSStages * L::kStage);
+  const int d = FULL ? 64 * DU : c.d, dv = FULL ? 64 * VU : c.dv;
+  const uint8_t *k_lane = c.k + (4 * (g8 >> 1) + (g8 & 1)) * d + 16 * t4, *v_lane = c.v + 4 * t4 * dv + VB * g8;
+  const float* s_lane = (lane < 4 ? c.ks : c.vs) + 4 * (lane & 3);
   const auto issue = [&](int u, int st) {
     if (u < u1) {
       const int r16 = rows[u - u0];
       if (r16 >= 0) {
-        const long long row = (long long)r16 * kKvGroup;
         const uint32_t to = ring + st * L::kStage;
+        const uint8_t *k = k_lane + (long long)r16 * (kKvGroup * d), *v = v_lane + (long long)r16 * (kKvGroup * dv);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint8_t* from = c.k + (row + 4 * (g8 >> 1) + 2 * j + (g8 & 1)) * c.d + 16 * t4;
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int i = 0; i < DU; ++i) cp_async16_stream(to + ((j * DU + i) * 32 + lane) * 16, from + (64 * i + 16 * t4 < c.d ? 64 * i : -16 * t4), 64 * i + 16 * t4 < c.d);
-        }
+          for (int i = 0; i < DU; ++i) {
+            const bool in = FULL || 64 * i + 16 * t4 < d;
+            cp_async16_stream(to + ((j * DU + i) * 32 + lane) * 16, k + 2 * j * d + (in ? 64 * i : -16 * t4), in);
+          }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint8_t* from = c.v + (row + 4 * t4 + k) * c.dv;
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
           for (int i = 0; i < VC; ++i) {
-            const int e = (8 * i + g8) * VB;
-            const uint32_t at = to + L::kK + ((k * VC + i) * 32 + lane) * VB;
-            if constexpr (VB == 16) cp_async16_stream(at, from + (e < c.dv ? e : 0), e < c.dv);
-            else cp_async8(at, from + (e < c.dv ? e : 0), e < c.dv);
+            const bool in = FULL || (8 * i + g8) * VB < dv;
+            const uint32_t at = to + L::kK + ((x * VC + i) * 32 + lane) * VB;
+            const uint8_t* from = v + x * dv + (in ? 8 * i * VB : -VB * g8);
+            if constexpr (VB == 16) cp_async16_stream(at, from, in);
+            else cp_async8(at, from, in);
           }
-        }
-        if (lane < 8) cp_async16_stream(to + L::kK + L::kV + lane * 16, (lane < 4 ? c.ks : c.vs) + row + 4 * (lane & 3), true);
+        if (lane < 8) cp_async16_stream(to + L::kK + L::kV + lane * 16, s_lane + (long long)r16 * kKvGroup, true);
       }
     }
     kb2::cp_async_commit();
@@ -121,7 +125,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   uint32_t qf[QR][PARTS][2 * NQ];
   float rf[NQ];
   int pos[NQ], tok[NQ];
-  float m[NQ], l[NQ], ref[NQ];
+  float m[NQ], l[NQ], ref[NQ], inv[NQ];
   int pmin, pmax;
 #pragma unroll
   for (int h = 0; h < NQ; ++h) {
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     tok[h] = tk;
     pos[h] = in ? t.positions[tk] : -1;
     m[h] = -INFINITY;
-    l[h] = ref[h] = 0.f;
+    l[h] = ref[h] = inv[h] = 0.f;
     const long long from = tk * a.ldq + hd * a.hq;
     float x[DU][16];
     uint32_t top = 0;
@@ -230,53 +234,74 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
       const uint4 kq = lds16(at + L::kK + L::kV + t4 * 16), vq = lds16(at + L::kK + L::kV + 64 + t4 * 16);
       // all rows of the tile see all 16 keys
       const bool all = key0 + kKvGroup <= span.base && key0 + kKvGroup - 1 <= pmin && (pmax - key0 < a.window || key0 + kKvGroup <= a.first);
+      float y[NQ][4], p[NQ][4];              // scores in powers of two, weights
       uint32_t w[NQ][PARTS][2];
-      bool again = false;
-      float grow[NQ];
 #pragma unroll
-      for (int h = 0; h < NQ; ++h) {
-        float y[4];
+      for (int h = 0; h < NQ; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[e] = sc[e >> 1][2 * h + (e & 1)] * __uint_as_float(word(kq, e)) * rf[h];
-          if (!all && !sees(key0 + 4 * t4 + e, h)) y[e] = -INFINITY;
-        }
-        float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float mn = fmaxf(m[h], top), from = mn == -INFINITY ? 0.f : mn, back = ex2(m[h] - from);
-        m[h] = mn;
-        float sum = 0.f, big = 0.f;
+        for (int e = 0; e < 4; ++e) y[h][e] = sc[e >> 1][2 * h + (e & 1)] * (__uint_as_float(word(kq, e)) * rf[h]);
+      if (!all) {
+#pragma unroll
+        for (int h = 0; h < NQ; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!sees(key0 + 4 * t4 + e, h)) y[h][e] = -INFINITY;
+      }
+      const auto weigh = [&](int h) {        // against the row's maximum and reference: the largest of the lane's scores and products over them
+        float top = -INFINITY, big = 0.f;
+        const float from = m[h] == -INFINITY ? 0.f : m[h];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = ex2(y[e] - from);
-          sum += p;
-          y[e] = y[e] == -INFINITY ? 0.f : p * __uint_as_float(word(vq, e));      // a row that nobody sees may hold anything
-          big = fmaxf(big, y[e]);
+          const float z = y[h][e] - from;
+          p[h][e] = ex2(z);
+          top = fmaxf(top, z);
         }
-        l[h] = l[h] * back + sum;
-        ref[h] *= back;
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        grow[h] = 1.f;
-        if (big > ref[h] * 32768.f && big > 1e-37f) {
-          const float r = fmaxf(big * 0.015625f, 1e-37f);
-          grow[h] = ref[h] / r;
-          ref[h] = r;
-          again = true;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = p[h][e] * (__uint_as_float(word(vq, e)) * inv[h]);
+          if (!all && y[h][e] == -INFINITY) x[e] = 0.f;                    // a row that nobody sees may hold anything
+          big = fmaxf(big, x[e]);
         }
-        const float inv = ref[h] >= 1e-37f ? __frcp_rn(ref[h]) : 0.f;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const float f0 = y[2 * b] * inv, f1 = y[2 * b + 1] * inv;
-          w[h][0][b] = f16_pair(f0, f1);
+          w[h][0][b] = f16_pair(x[2 * b], x[2 * b + 1]);
           if constexpr (PARTS == 2) {
             const float2 f = f16_get(w[h][0][b]);
-            w[h][PARTS - 1][b] = f16_pair(f0 - f.x, f1 - f.y);
+            w[h][PARTS - 1][b] = f16_pair(x[2 * b] - f.x, x[2 * b + 1] - f.y);
           }
         }
-      }
-      if (__any_sync(0xffffffffu, again)) {
+        return top > 8.f || big > 32768.f;   // a weight above 2^8, a product above fp16's range
+      };
+      bool again = false;
+#pragma unroll
+      for (int h = 0; h < NQ; ++h) again |= weigh(h) || m[h] == -INFINITY;
+      if (__any_sync(0xffffffffu, again)) {  // seldom after the first keys: maxima and references anew
+        float grow[NQ];
+#pragma unroll
+        for (int h = 0; h < NQ; ++h) {
+          float top = fmaxf(fmaxf(y[h][0], y[h][1]), fmaxf(y[h][2], y[h][3]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float mn = fmaxf(m[h], top), from = mn == -INFINITY ? 0.f : mn, back = ex2(m[h] - from);
+          m[h] = mn;
+          l[h] *= back;
+          ref[h] *= back;
+          float big = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (y[h][e] != -INFINITY) big = fmaxf(big, ex2(y[h][e] - from) * __uint_as_float(word(vq, e)));
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+          grow[h] = 1.f;
+          if (big > ref[h] * 32768.f && big > 1e-37f) {
+            const float r = fmaxf(big * 0.015625f, 1e-37f);
+            grow[h] = ref[h] / r;
+            ref[h] = r;
+          }
+          inv[h] = ref[h] >= 1e-37f ? 1.f / ref[h] : 0.f;
+          weigh(h);
+        }
 #pragma unroll
         for (int h = 0; h < NQ; ++h) {       // the columns of O^T that a lane holds are the rows 2 t4, 2 t4 + 1 of the queries
           const float f0 = __shfl_sync(0xffffffffu, grow[h], 8 * t4), f1 = __shfl_sync(0xffffffffu, grow[h], 8 * t4 + 4);
@@ -289,6 +314,8 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
           }
         }
       }
+#pragma unroll
+      for (int h = 0; h < NQ; ++h) l[h] += (p[h][0] + p[h][1]) + (p[h][2] + p[h][3]);
 #pragma unroll
       for (int i = 0; i < VC; ++i) {
         uint32_t v[4][VB / 4];
@@ -471,7 +498,7 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
     piece = (piece + 7) / 8 * 8;
     if ((long long)p.tiles * cache->G >= want) piece = (top + 7) / 8 * 8;
   } else {
-    const long long want = 4ll * 2 * kb2::current_sms();
+    const long long want = 2ll * 2 * kb2::current_sms();
     piece = std::max((work * cache->G + want - 1) / want, (top + 63) / 64);
     piece = std::min<long long>((piece + kSWarps - 1) / kSWarps * kSWarps, kSMostGroups);
     piece = std::max<long long>(piece, kSWarps);
@@ -504,27 +531,29 @@ inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, 
   return a;
 }
 
-template <int FMT, int DU, int VU, int NQ, int PARTS>
+template <int FMT, int DU, int VU, int NQ, int PARTS, bool FULL>
 int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
   using L = StreamShape<DU, VU, NQ, PARTS>;
-  SEQ_CUDA((kb2::allow_smem<kv_stream_kernel<FMT, DU, VU, NQ, PARTS>>(L::kTotal)));
-  auto kern = kv_stream_kernel<FMT, DU, VU, NQ, PARTS>;
+  SEQ_CUDA((kb2::allow_smem<kv_stream_kernel<FMT, DU, VU, NQ, PARTS, FULL>>(L::kTotal)));
+  auto kern = kv_stream_kernel<FMT, DU, VU, NQ, PARTS, FULL>;
   kb2::launch_pdl(kern, dim3(p.tiles, c.G, p.pieces), kSWarps * 32, L::kTotal, st, c, t, a);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }
-template <int FMT, int DU, int VU>
+template <int FMT, int DU, int VU, bool FULL>
 int stream_rows(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
-  if (p.rows == 8) return a.dt_out ? stream_launch<FMT, DU, VU, 1, 1>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 1, 2>(c, t, a, p, st);
-  return a.dt_out ? stream_launch<FMT, DU, VU, 2, 1>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 2, 2>(c, t, a, p, st);
+  if (p.rows == 8) return a.dt_out ? stream_launch<FMT, DU, VU, 1, 1, FULL>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 1, 2, FULL>(c, t, a, p, st);
+  return a.dt_out ? stream_launch<FMT, DU, VU, 2, 1, FULL>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 2, 2, FULL>(c, t, a, p, st);
 }
 template <int FMT>
 int stream_sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
-  if (c.d <= 64 && c.dv <= 64) return stream_rows<FMT, 1, 1>(c, t, a, p, st);
-  if (c.d <= 128 && c.dv <= 128) return stream_rows<FMT, 2, 2>(c, t, a, p, st);
-  if (c.d <= 192 && c.dv <= 128) return stream_rows<FMT, 3, 2>(c, t, a, p, st);
-  if (c.d <= 128) return stream_rows<FMT, 2, 4>(c, t, a, p, st);
-  return stream_rows<FMT, 4, 4>(c, t, a, p, st);
+  const auto is = [&](int d, int dv) { return c.d == d && c.dv == dv; };
+  if (is(64, 64)) return stream_rows<FMT, 1, 1, true>(c, t, a, p, st);
+  if (is(128, 128)) return stream_rows<FMT, 2, 2, true>(c, t, a, p, st);
+  if (is(192, 128)) return stream_rows<FMT, 3, 2, true>(c, t, a, p, st);
+  if (is(128, 256)) return stream_rows<FMT, 2, 4, true>(c, t, a, p, st);
+  if (is(256, 256)) return stream_rows<FMT, 4, 4, true>(c, t, a, p, st);
+  return c.d <= 128 && c.dv <= 128 ? stream_rows<FMT, 2, 2, false>(c, t, a, p, st) : stream_rows<FMT, 4, 4, false>(c, t, a, p, st);
 }
 }  // namespace
 }  // namespace kb2seq
