@@ -44,7 +44,7 @@ struct StreamShape {
   static constexpr int MT = 8 * NQ;
   static constexpr int VB = VU % 2 ? 8 : 16, VC = VU * 8 / VB;            // a lane's bytes of a value row: VC times VB
   static constexpr int kK = 2 * DU * 512, kV = 4 * VU * 256, kStage = kK + kV + 128;
-  static constexpr bool kQShared = DU * 8 * NQ * PARTS > 32;              // registers of the queries
+  static constexpr bool kQShared = DU * 8 * NQ * PARTS > (NQ == 2 ? 16 : 32);      // registers of the queries; spilled ones cost more than those read again
   static constexpr int kQ = kQShared ? DU * 4 * PARTS * 2 * NQ * 128 : 0;
   static constexpr int kRing = kSWarps * kSStages * kStage, kRed = kSWarps * MT * VU * 64 * 4;
   static constexpr int kOffRow = kRing > kRed ? kRing : kRed, kOffStat = kOffRow + kSMostGroups * 4, kOffQ = kOffStat + kSWarps * MT * 4 * 4;
