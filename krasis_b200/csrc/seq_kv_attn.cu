@@ -44,10 +44,11 @@ struct StreamShape {
   static constexpr int MT = 8 * NQ;
   static constexpr int VB = VU % 2 ? 8 : 16, VC = VU * 8 / VB;            // a lane's bytes of a value row: VC times VB
   static constexpr int kK = 2 * DU * 512, kV = 4 * VU * 256, kStage = kK + kV + 128;
-  static constexpr bool kQShared = DU * 8 * NQ * PARTS > (NQ == 2 ? 16 : 32);      // registers of the queries; spilled ones cost more than those read again
-  static constexpr int kQ = kQShared ? DU * 4 * PARTS * 2 * NQ * 128 : 0;
-  static constexpr int kRing = kSWarps * kSStages * kStage, kRed = kSWarps * MT * VU * 64 * 4;
-  static constexpr int kOffRow = kRing > kRed ? kRing : kRed, kOffStat = kOffRow + kSMostGroups * 4, kOffQ = kOffStat + kSWarps * MT * 4 * 4;
+  static constexpr bool kQShared = NQ == 2 || DU * 8 * PARTS > 32;      // registers of the queries; spilled ones cost more than those read again
+  static constexpr int kQ = DU * 4 * PARTS * 2 * NQ * 128;
+  static constexpr int kRow = VU * 64 + 8;                                // numbers from row to row of a warp's share at the end: 32 bytes apart in the banks
+  static constexpr int kRing = kSWarps * kSStages * kStage, kRed = kSWarps * MT * kRow * 4;
+  static constexpr int kOffRow = kRing > kRed ? kRing : kRed, kOffStat = kOffRow + kSMostGroups * 4, kOffTok = kOffStat + kSWarps * MT * 4 * 4, kOffQ = kOffTok + MT * 16;
   static constexpr int kTotal = kOffQ + kQ;
   static constexpr int kBlocks = 2 * (kTotal + 1024) <= 227 * 1024 ? 2 : 1;
   static_assert(kTotal <= 227 * 1024 && kOffQ % 16 == 0 && kStage % 16 == 0, "shared memory");
@@ -72,6 +73,29 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * MT, nr = (int)min((long long)n * per - r0, (long long)MT);
   if (nr <= 0) return;
   const int t0 = c0 + r0 / per, t1 = c0 + (r0 + nr - 1) / per;
+
+  // queries: row r of the tile is head `r0 + r` mod per of a token.  kT threads have eight numbers each of a row (those of a row are neighbours in a warp); asked for first, as
+  // everything else waits for the tables
+  constexpr int kT = kSWarps * 32 / MT, kEach = (DU * 8 + kT - 1) / kT;
+  const int qr = threadIdx.x / kT, qx = threadIdx.x % kT;
+  float x[kEach][8];
+  {
+    const bool in = qr < nr;
+    const int rr = r0 + (in ? qr : 0), tk = c0 + rr / per, hd = head * per + rr % per;
+    const long long from = tk * a.ldq + hd * a.hq;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int e = (qx + i * kT) * 8;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float y[4];
+        query4(a, from + e + 4 * b, in ? c.d - e : 0, y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][4 * b + j] = y[j];
+      }
+    }
+    if (qx == 0) *reinterpret_cast<int2*>(smem + L::kOffTok + qr * 16) = make_int2(tk, in ? t.positions[tk] : -1);
+  }
   const KvSpan span = kv_span(c, t, s, t0, t1, a.window, a.first);
   const int total = span.groups(), np = min((total + a.piece - 1) / a.piece, a.pieces), z = blockIdx.z;
   if (z > 0 && z >= np) return;
@@ -82,6 +106,39 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   for (int i = threadIdx.x; i < u1 - u0; i += kSWarps * 32) {
     const long long r = kv_row(c, t, s, span.group(u0 + i) * kKvGroup);
     rows[i] = r < 0 ? -1 : (int)((r + ((long long)head << c.lps)) / kKvGroup);
+  }
+  // the queries as fragments: of a lane's 16 numbers of a unit, four products with four each
+  {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+#pragma unroll
+    for (int o = kT / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float up, down;
+    kv_row_scale(top, &up, &down);
+    if (qx == 0) *reinterpret_cast<float*>(smem + L::kOffTok + qr * 16 + 8) = a.scale * kLog2e * down;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int e = (qx + i * kT) * 8;
+      if (e >= DU * 64) continue;
+      const int at = (e >> 6) * 4 + ((e & 15) >> 2), to = (qr & 7) * 4 + ((e & 63) >> 4);        // product, lane
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float y0 = x[i][4 * k + 2 * b] * up, y1 = x[i][4 * k + 2 * b + 1] * up;
+          uint32_t p[PARTS];
+          p[0] = f16_pair(y0, y1);
+          if constexpr (PARTS == 2) {
+            const float2 f = f16_get(p[0]);
+            p[1] = f16_pair(y0 - f.x, y1 - f.y);
+          }
+#pragma unroll
+          for (int o = 0; o < PARTS; ++o) sts4(kb2::smem_u32(smem) + L::kOffQ + ((((at + k) * PARTS + o) * 32 + to) * 2 * NQ + b * NQ + (qr >> 3)) * 4, p[o]);
+        }
+    }
   }
   __syncthreads();
 
@@ -120,69 +177,32 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
 #pragma unroll
   for (int i = 0; i < kSStages; ++i) issue(u0 + warp + i * kSWarps, i);
 
-  // queries: row r of the tile is head `r0 + r` mod per of a token.  A lane's 16 numbers of a unit are its fragments of four products.
   constexpr int QR = L::kQShared ? 1 : DU * 4;
   uint32_t qf[QR][PARTS][2 * NQ];
+  if constexpr (!L::kQShared) {
+#pragma unroll
+    for (int i = 0; i < DU * 4; ++i)
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        const uint2 v = lds8(kb2::smem_u32(smem) + L::kOffQ + ((i * PARTS + p) * 32 + lane) * 8);
+        qf[i][p][0] = v.x;
+        qf[i][p][1] = v.y;
+      }
+  }
   float rf[NQ];
   int pos[NQ], tok[NQ];
   float m[NQ], l[NQ], ref[NQ], inv[NQ];
-  int pmin, pmax;
 #pragma unroll
   for (int h = 0; h < NQ; ++h) {
-    const int r = g8 + 8 * h;
-    const bool in = r < nr;
-    const int rr = r0 + (in ? r : 0), tk = c0 + rr / per, hd = head * per + rr % per;
-    tok[h] = tk;
-    pos[h] = in ? t.positions[tk] : -1;
+    const int4 v = *reinterpret_cast<const int4*>(smem + L::kOffTok + (g8 + 8 * h) * 16);
+    tok[h] = v.x;
+    pos[h] = v.y;
+    rf[h] = __int_as_float(v.z);
     m[h] = -INFINITY;
     l[h] = ref[h] = inv[h] = 0.f;
-    const long long from = tk * a.ldq + hd * a.hq;
-    float x[DU][16];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < DU; ++i) {
-      const int e = 64 * i + 16 * t4;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        float y[4];
-        query4(a, from + e + 4 * b, in ? c.d - e : 0, y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[i][4 * b + j] = y[j];
-          top = max(top, __float_as_uint(y[j]) & 0x7FFFFFFFu);
-        }
-      }
-    }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    float up, down;
-    kv_row_scale(top, &up, &down);
-    rf[h] = a.scale * kLog2e * down;
-#pragma unroll
-    for (int i = 0; i < DU; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {        // dimensions 4 k + 2 b, + 1 of the lane's 16
-          const float y0 = x[i][4 * k + 2 * b] * up, y1 = x[i][4 * k + 2 * b + 1] * up;
-          uint32_t p[PARTS];
-          p[0] = f16_pair(y0, y1);
-          if constexpr (PARTS == 2) {
-            const float2 f = f16_get(p[0]);
-            p[1] = f16_pair(y0 - f.x, y1 - f.y);
-          }
-#pragma unroll
-          for (int o = 0; o < PARTS; ++o) {
-            if constexpr (L::kQShared) {
-              if (warp == (i * 4 + k) % kSWarps) sts4(kb2::smem_u32(smem) + L::kOffQ + ((((i * 4 + k) * PARTS + o) * 32 + lane) * 2 * NQ + b * NQ + h) * 4, p[o]);
-            } else {
-              qf[i * 4 + k][o][b * NQ + h] = p[o];
-            }
-          }
-        }
   }
-  kv_reach(t, span, t0, t1, &pmin, &pmax);
-  if constexpr (L::kQShared) __syncthreads();
+  int pmin, pmax;
+  kv_reach(t, a, span, t0, t1, &pmin, &pmax);
 
   float o[MV][NQ][4];
 #pragma unroll
@@ -359,7 +379,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     if (t4 == 0) stat[warp * MT + g8 + 8 * h] = make_float4(m[h], l[h], ref[h], 0.f);
   }
   __syncthreads();                           // the rings are free from here on
-  float* red = reinterpret_cast<float*>(smem);                             // [warp][row][VU 64]
+  float* red = reinterpret_cast<float*>(smem);                             // [warp][row][tile of O^T][g8][2]
 #pragma unroll
   for (int h = 0; h < NQ; ++h)
 #pragma unroll
@@ -371,16 +391,15 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
       const float4 x = stat[warp * MT + q];
       const float f = x.x == -INFINITY ? 0.f : x.z * ex2(x.x - top);
 #pragma unroll
-      for (int i = 0; i < MV; ++i) {
-        const int dim = (i / (VB / 2)) * 8 * VB + VB * g8 + 2 * (i % (VB / 2));
-        *reinterpret_cast<float2*>(red + (warp * MT + q) * (VU * 64) + dim) = make_float2(o[i][h][e] * f, o[i][h][2 + e] * f);
-      }
+      for (int i = 0; i < MV; ++i) *reinterpret_cast<float2*>(red + (warp * MT + q) * L::kRow + (i * 8 + g8) * 2) = make_float2(o[i][h][e] * f, o[i][h][2 + e] * f);
     }
   __syncthreads();
   // a thread takes eight columns of a row
   constexpr int kCols = VU * 8;
   for (int i = threadIdx.x; i < MT * kCols; i += kSWarps * 32) {
     const int q = i / kCols, dim = (i - q * kCols) * 8;
+    // the eight columns are the pairs of four tiles of O^T, of one lane each
+    const int from = VB == 16 ? ((dim >> 7) * 8 + (dim >> 3 & 1) * 4) * 16 + ((dim & 127) >> 4) * 2 : (dim >> 6) * 64 + ((dim & 63) >> 3) * 2;
     if (q >= nr || dim >= c.dv) continue;
     float top = -INFINITY, sum = 0.f, acc[8] = {};
 #pragma unroll
@@ -389,10 +408,12 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     for (int w = 0; w < kSWarps; ++w) {
       const float4 x = stat[w * MT + q];
       sum += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top);                // a sum without a maximum is 0, or NaN from a row that holds one
-      const float4* r = reinterpret_cast<const float4*>(red + (w * MT + q) * (VU * 64) + dim);
-      const float4 lo = r[0], hi = r[1];
-      acc[0] += lo.x; acc[1] += lo.y; acc[2] += lo.z; acc[3] += lo.w;
-      acc[4] += hi.x; acc[5] += hi.y; acc[6] += hi.z; acc[7] += hi.w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 v = *reinterpret_cast<const float2*>(red + (w * MT + q) * L::kRow + from + 16 * e);
+        acc[2 * e] += v.x;
+        acc[2 * e + 1] += v.y;
+      }
     }
     const int rr = r0 + q, hd = head * per + rr % per;
     const long long row = (long long)(c0 + rr / per) * a.H + hd;

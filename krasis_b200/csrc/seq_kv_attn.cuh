@@ -61,12 +61,14 @@ __device__ __forceinline__ bool kv_sees(const KvStep& t, const KvAttn& a, const 
   }
   return spot <= pos && (pos - spot < a.window || spot < a.first);
 }
-// The least and the most position of the tokens t0 .. t1: the first and the last of a portion; of a tree the least is any that is no more.
-__device__ __forceinline__ void kv_reach(const KvStep& t, const KvSpan& span, int t0, int t1, int* least, int* most) {
-  *least = t.positions[t0];
+// The least and the most position of the tokens t0 .. t1: the first and the last of a portion; of a tree the least is any that is no more.  The most matters under a window.
+__device__ __forceinline__ void kv_reach(const KvStep& t, const KvAttn& a, const KvSpan& span, int t0, int t1, int* least, int* most) {
+  const bool tree = span.base < kKvNoWindow;
+  *least = tree ? span.base : t.positions[t0];
+  *most = *least;
+  if (a.window >= kKvNoWindow) return;
   *most = t.positions[t1];
-  if (span.base < kKvNoWindow) {
-    *least = span.base;
+  if (tree) {
     for (int x = t0; x < t1; ++x) *most = max(*most, t.positions[x]);
   }
 }
