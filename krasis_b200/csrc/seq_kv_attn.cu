@@ -557,18 +557,22 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
   p.least = least;
   p.most = most;
   p.rows = wide ? (kv_pairs(cache->d, cache->dv) ? 256 : 128) : rows <= 8 ? 8 : 16;
-  for (int s = 0; s < step->S; ++s) {
+  const auto tiles = [&](int s) {            // of a sequence of this kind
+    const long long r = (long long)step->layout[4 * s + 1] * per;
+    return r < least || r > most ? 0ll : (r + p.rows - 1) / p.rows;
+  };
+  const auto seen = [&](int s) {             // captured launches are run again with later positions: what the page lists hold
     const int* l = step->layout + 4 * s;
-    const long long r = (long long)l[1] * per;
-    same = same && l[1] == step->layout[1];
-    if (r < least || r > most || r == 0) continue;
-    const int tiles = (int)((r + p.rows - 1) / p.rows);
-    // captured launches are run again with later positions: what the page lists hold
     const long long end = step->replayed ? (long long)step->max_pages * cache->page_size : (long long)l[2] + l[1];
-    const long long g = groups_seen(end - l[1], l[1], window, first);
-    p.tiles += tiles;
-    top = std::max(top, g);
-    work += g * tiles;
+    return groups_seen(end - l[1], l[1], window, first);
+  };
+  for (int s = 0; s < step->S; ++s) {
+    same = same && step->layout[4 * s + 1] == step->layout[1];
+    const long long n = tiles(s);
+    if (n == 0) continue;
+    p.tiles += (int)n;
+    top = std::max(top, seen(s));
+    work += seen(s) * n;
   }
   if (p.tiles == 0) return p;
   p.per_seq = same ? p.tiles / step->S : 0;
@@ -579,10 +583,28 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
     piece = (piece + 7) / 8 * 8;
     if ((long long)p.tiles * cache->G >= want) piece = (top + 7) / 8 * 8;
   } else {
-    const long long want = 2ll * 2 * kb2::current_sms();
-    piece = std::max((work * cache->G + want - 1) / want, (top + 63) / 64);
-    piece = std::min<long long>((piece + kSWarps - 1) / kSWarps * kSWarps, kSMostGroups);
-    piece = std::max<long long>(piece, kSWarps);
+    // Blocks of one length in whole waves, as the last wave takes as long as the others: the length whose waves, with what a block costs beside its keys (some 16 groups), end
+    // first.  64 requests of 500 to 60000 rows (WAVES us, by four blocks a slot 284).
+    const long long slots = (long long)kb2::current_sms() * (cache->d <= 128 && cache->dv <= 128 ? 2 : 1);
+    long long best = 0, cost = 0;
+    for (int waves = 1; waves <= 4; ++waves) {
+      long long len = std::max<long long>((work * cache->G + waves * slots - 1) / (waves * slots), (top + 63) / 64);
+      for (int tries = 0; tries < 8; ++tries) {
+        len = std::max<long long>((len + kSWarps - 1) / kSWarps * kSWarps, kSWarps);
+        if (len >= kSMostGroups) break;
+        long long blocks = 0;
+        for (int s = 0; s < step->S; ++s) blocks += seen(s) ? tiles(s) * ((seen(s) + len - 1) / len) : 0;
+        if (blocks * cache->G <= waves * slots) break;
+        len += std::max<long long>(len / 16, 1);
+      }
+      len = std::min<long long>(len, kSMostGroups);
+      if (best == 0 || waves * (len + 16) < cost) {
+        best = len;
+        cost = waves * (len + 16);
+      }
+      if (len == kSWarps) break;
+    }
+    piece = best;
   }
   p.piece = (int)std::max(piece, 8ll);
   p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
@@ -686,7 +708,8 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
     if (int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, few, p.few, st) : stream_sizes<KV_INT8>(c, t, few, p.few, st)) return e;
   }
   if (p.few.pieces <= 1 && p.many.pieces <= 1) return KB2SEQ_OK;
-  const bool wide = std::max(p.few.pieces, p.many.pieces) > 8 && ((long long)t.T * H <= 16384 || std::max(p.few.pieces, p.many.pieces) > 32);
+  const int most = std::max(p.few.pieces, p.many.pieces);
+  const bool wide = (long long)t.T * H <= 4096 || (most > 8 && (long long)t.T * H <= 16384) || most > 32;
   auto join = wide ? kv_join_kernel<4> : kv_join_kernel<1>;
   kb2::launch_pdl(join, (unsigned)(wide ? (long long)t.T * H : ((long long)t.T * H + 3) / 4), 128, 0, st, c, t, few, many);
   SEQ_LAUNCHED();
