@@ -18,7 +18,9 @@
 namespace kb2seq {
 namespace {
 
-constexpr int kSWarps = 8, kSStages = 3, kSMostGroups = 1024, kMostPieces = 1024;
+constexpr int kSWarps = 8, kSStages = 3, kSMostGroups = 768, kMostPieces = 1024, kMostTiles = 768;
+constexpr int kPieceCost = 40;               // what a piece costs beside its keys, in groups of 16 (11 us against 0.25 a group, with two blocks on an SM)
+
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -48,8 +50,9 @@ struct StreamShape {
   static constexpr int kQ = DU * 4 * PARTS * 2 * NQ * 128;
   static constexpr int kRow = VU * 64 + 8;                                // numbers from row to row of a warp's share at the end: 32 bytes apart in the banks
   static constexpr int kRing = kSWarps * kSStages * kStage, kRed = kSWarps * MT * kRow * 4;
-  static constexpr int kOffRow = kRing > kRed ? kRing : kRed, kOffStat = kOffRow + kSMostGroups * 4, kOffTok = kOffStat + kSWarps * MT * 4 * 4, kOffQ = kOffTok + MT * 16;
-  static constexpr int kTotal = kOffQ + kQ;
+  static constexpr int kOffRow = kRing > kRed ? kRing : kRed, kOffStat = kOffRow + kSMostGroups * 4, kOffTok = kOffStat + kSWarps * MT * 4 * 4, kOffQ = kOffTok + MT * 16,
+                       kOffScan = kOffQ + kQ;
+  static constexpr int kTotal = kOffScan + (kMostTiles + 4) * 4;
   static constexpr int kBlocks = 2 * (kTotal + 1024) <= 227 * 1024 ? 2 : 1;
   static_assert(kTotal <= 227 * 1024 && kOffQ % 16 == 0 && kStage % 16 == 0, "shared memory");
 };
@@ -62,13 +65,94 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   extern __shared__ __align__(16) uint8_t smem[];
   kb2::pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-  const int per = a.H / c.G, head = blockIdx.y;
-  int s, tile;
-  if (a.per_seq) {
-    s = blockIdx.x / a.per_seq;
-    tile = blockIdx.x - s * a.per_seq;
-  } else if (!kv_find_tile(t, per, MT, a.least, a.most, blockIdx.x, &s, &tile)) {
-    return;
+  const int per = a.H / c.G;
+
+  // Many keys and few tiles: the groups of all tiles and heads in a row, each tile's behind its kPieceCost, are cut into chunks of one length, one for each block that fits
+  // the GPU at once, wherever a chunk's ends lie in a tile.  (Pieces of tiles: requests of 500 to 60000 rows left a quarter of the blocks idle.)
+  int* prefix = reinterpret_cast<int*>(smem + L::kOffScan);                // of the tiles' costs
+  const int tiles = a.per_seq * t.S;
+  long long chunk = 0, all = 0, at_cost = 0, to_cost = 0, next_chunk = blockIdx.x;
+  if (a.linear) {
+    int before = 0, most = 0;
+    int* part = reinterpret_cast<int*>(smem + L::kOffStat);
+    for (int b = 0; b < tiles; b += kSWarps * 32) {
+      const int x = b + threadIdx.x, q = x / a.per_seq, from = (x - q * a.per_seq) * MT;
+      int cost = 0;
+      if (x < tiles) {
+        const int f = t.cu[q], have = (int)min((long long)(t.cu[q + 1] - f) * per - from, (long long)MT);
+        if (have > 0) cost = kv_span(c, t, q, f + from / per, f + (from + have - 1) / per, a.window, a.first).groups() + kPieceCost;
+      }
+      most = max(most, cost);
+      int upto = cost;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      __syncthreads();
+      if (lane == 31) part[warp] = upto;
+      __syncthreads();
+      int ahead = before, whole = before;
+      for (int w = 0; w < kSWarps; ++w) {
+        ahead += w < warp ? part[w] : 0;
+        whole += part[w];
+      }
+      if (x < tiles) prefix[x] = ahead + upto - cost;
+      before = whole;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    __syncthreads();
+    if (lane == 0) part[warp] = most;
+    if (threadIdx.x == 0) prefix[tiles] = before;
+    __syncthreads();
+    for (int w = 0; w < kSWarps; ++w) most = max(most, part[w]);
+    all = (long long)before * c.G;
+    // no tile has more than a.pieces pieces, and no piece more groups than there is room for
+    chunk = min(max(max((all + gridDim.x - 1) / gridDim.x, (long long)(most + a.pieces - 2) / (a.pieces - 1)), 8ll), (long long)kSMostGroups);
+    __syncthreads();
+  }
+
+  for (bool once = true;; once = false) {
+  int s, tile, head, u0 = 0, u1 = 0, np = 0, z = blockIdx.z, number = 0;
+  if (a.linear) {
+    if (!once) __syncthreads();              // the last piece's shares have been read
+    if (at_cost >= to_cost) {
+      at_cost = next_chunk * chunk;
+      if (at_cost >= all) return;
+      to_cost = min(at_cost + chunk, all);
+      next_chunk += gridDim.x;
+    }
+    int lo = 0, hi = tiles;                  // the last tile that begins at or before this cost (of those without any, the one behind them)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((long long)prefix[mid] * c.G <= at_cost) lo = mid;
+      else hi = mid;
+    }
+    number = lo;
+    const int cost = prefix[lo + 1] - prefix[lo];
+    const long long begin = (long long)prefix[lo] * c.G, mine = begin + (at_cost - begin) / cost * cost, stop = min(mine + cost, to_cost);
+    head = (int)((at_cost - begin) / cost);
+    u0 = (int)max(at_cost - mine - kPieceCost, 0ll);
+    u1 = (int)max(stop - mine - kPieceCost, 0ll);
+    const bool start = at_cost == mine;
+    at_cost = stop;
+    const int groups = cost - kPieceCost;
+    if (groups == 0 ? !start : u1 == u0) continue;
+    const long long first = (mine + kPieceCost) / chunk;
+    np = groups == 0 ? 1 : (int)((mine + kPieceCost + groups - 1) / chunk - first) + 1;
+    z = groups == 0 ? 0 : (int)(next_chunk - gridDim.x - first);
+    s = number / a.per_seq;
+    tile = number - s * a.per_seq;
+    if (z == 0 && threadIdx.x == 0) a.counts[number * c.G + head] = np;
+  } else {
+    if (!once) return;
+    head = blockIdx.y;
+    if (a.per_seq) {
+      s = blockIdx.x / a.per_seq;
+      tile = blockIdx.x - s * a.per_seq;
+    } else if (!kv_find_tile(t, per, MT, a.least, a.most, blockIdx.x, &s, &tile)) {
+      return;
+    }
   }
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * MT, nr = (int)min((long long)n * per - r0, (long long)MT);
   if (nr <= 0) return;
@@ -97,9 +181,13 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     if (qx == 0) *reinterpret_cast<int2*>(smem + L::kOffTok + qr * 16) = make_int2(tk, in ? t.positions[tk] : -1);
   }
   const KvSpan span = kv_span(c, t, s, t0, t1, a.window, a.first);
-  const int total = span.groups(), np = min((total + a.piece - 1) / a.piece, a.pieces), z = blockIdx.z;
-  if (z > 0 && z >= np) return;
-  const int u0 = z * a.piece, u1 = min(total, u0 + a.piece);   // z = 0 of nothing to see: no group
+  if (!a.linear) {
+    const int total = span.groups();
+    np = min((total + a.piece - 1) / a.piece, a.pieces);
+    if (z > 0 && z >= np) return;
+    u0 = z * a.piece;
+    u1 = min(total, u0 + a.piece);           // z = 0 of nothing to see: no group
+  }
 
   // where the piece's groups lie: a row of this head in units of 16, or -1
   int* rows = reinterpret_cast<int*>(smem + L::kOffRow);
@@ -435,6 +523,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
       to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
     }
   }
+  }
 }
 
 // The pieces of a row (token, head), joined in a fixed order; rows that one piece finished are left alone.  x, y: the two kinds of sequences.  W warps a row take the pieces in
@@ -461,7 +550,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
   if (a.pieces <= 1) return;
   const int r0 = ((tok - c0) * per + hd % per) / a.rows * a.rows, nr = (int)min((long long)n * per - r0, (long long)a.rows);
   const KvSpan span = kv_span(c, t, s, c0 + r0 / per, c0 + (r0 + nr - 1) / per, a.window, a.first);
-  const int np = min((span.groups() + a.piece - 1) / a.piece, a.pieces);
+  const int np = a.linear ? a.counts[(s * a.per_seq + r0 / a.rows) * c.G + hd / per] : min((span.groups() + a.piece - 1) / a.piece, a.pieces);
   if (np <= 1) return;
   const long long p0 = row * a.pieces;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
@@ -537,7 +626,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
 constexpr int kTileFrom = 17;
 // How the sequences of one kind are cut: into tiles of rows, and the keys that a tile sees (in groups of 16) into pieces.
 struct KvPlan {
-  int least, most, rows, tiles, per_seq, piece, pieces;
+  int least, most, rows, tiles, per_seq, piece, pieces, blocks;            // blocks: of the even cut, 0 for pieces of tiles
   size_t floats;                             // workspace
 };
 // The most groups of 16 that the tokens start .. start + n - 1 see.
@@ -586,6 +675,12 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
     // Blocks of one length in whole waves, as the last wave takes as long as the others: the length whose waves, with what a block costs beside its keys (some 16 groups), end
     // first.  64 requests of 500 to 60000 rows (WAVES us, by four blocks a slot 284).
     const long long slots = (long long)kb2::current_sms() * (cache->d <= 128 && cache->dv <= 128 ? 2 : 1);
+    const long long even = (work + (long long)p.tiles * kPieceCost) * cache->G / slots;
+    if (p.per_seq && p.tiles <= kMostTiles && work * cache->G >= slots * kPieceCost) {
+      p.blocks = (int)slots;
+      // a captured step's keys may come to lie in one sequence: the kernel makes its pieces no more than this
+      p.pieces = (int)(step->replayed ? std::max(34ll, (top + kPieceCost) / kSMostGroups + 2) : (top + kPieceCost) / std::min<long long>(std::max(even, 8ll), kSMostGroups) + 2);
+    }
     long long best = 0, cost = 0;
     for (int waves = 1; waves <= 4; ++waves) {
       long long len = std::max<long long>((work * cache->G + waves * slots - 1) / (waves * slots), (top + 63) / 64);
@@ -607,8 +702,8 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
     piece = best;
   }
   p.piece = (int)std::max(piece, 8ll);
-  p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
-  p.floats = p.pieces > 1 ? ((size_t)step->T * H * p.pieces * (cache->dv + 2) + 3) / 4 * 4 : 0;      // what lies behind begins on 16 bytes too
+  if (!p.blocks) p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
+  p.floats = p.pieces > 1 ? ((size_t)step->T * H * p.pieces * (cache->dv + 2) + (p.blocks ? (size_t)p.tiles * cache->G : 0) + 3) / 4 * 4 : 0;      // what lies behind begins on 16 bytes too
   return p;
 }
 struct KvPlans {
@@ -631,6 +726,8 @@ inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, 
   a.pieces = p.pieces;
   a.part_o = work;
   a.part_ml = work + (size_t)rows_total * p.pieces * dv;
+  a.linear = p.blocks > 0;
+  a.counts = reinterpret_cast<int*>(a.part_ml + 2 * (size_t)rows_total * p.pieces);
   return a;
 }
 
@@ -639,7 +736,7 @@ int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPl
   using L = StreamShape<DU, VU, NQ, PARTS>;
   SEQ_CUDA((kb2::allow_smem<kv_stream_kernel<FMT, DU, VU, NQ, PARTS, FULL>>(L::kTotal)));
   auto kern = kv_stream_kernel<FMT, DU, VU, NQ, PARTS, FULL>;
-  kb2::launch_pdl(kern, dim3(p.tiles, c.G, p.pieces), kSWarps * 32, L::kTotal, st, c, t, a);
+  kb2::launch_pdl(kern, p.blocks ? dim3(p.blocks) : dim3(p.tiles, c.G, p.pieces), kSWarps * 32, L::kTotal, st, c, t, a);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }

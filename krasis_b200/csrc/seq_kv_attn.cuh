@@ -23,6 +23,8 @@ struct KvAttn {                              // what a call says beside the cach
                                              // each where the step's sequences bring as many tokens each, else 0
   int piece, pieces;                         // groups of 16 keys a piece; the most pieces of a tile
   float *part_o, *part_ml;                   // [T H][pieces][dv] and [T H][pieces][2]
+  bool linear;                               // all tiles' keys in a row are cut evenly, wherever the ends lie: `pieces` is then the most that a tile may have,
+  int* counts;                               // and this, [tiles][G], how many it has
 };
 
 __device__ __forceinline__ float ex2(float x) {
