@@ -16,77 +16,112 @@ namespace kb2seq {
 // ------------------------------------------------------------------------------------------------ writing
 // Four numbers of a row -> four codes.
 template <int FMT>
-__device__ __forceinline__ uint32_t kv_codes4(const float (&x)[4], float s, float inv, float up) {
+__device__ __forceinline__ uint32_t kv_codes4(const float* x, float s, float inv, float up) {
   if constexpr (FMT == KV_E4M3) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inv, x[1] * inv), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inv, x[3] * inv), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
   } else {
-    uint32_t c[4];
+    // x / s to a whole number: 1.5 2^23 leaves no room for a fraction, and the lowest byte of what comes is the code.  The reciprocal's rounding moves a quotient of at most
+    // 127 by 2^-16 or less, so only one that lies that near to the middle of two codes can have gone the other way: what is left over, x - code s, says so.
+    float t[4], far = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float y = x[e] * up;
-      float n = rintf(y * inv);                        // within one of the answer; what is left over says which it is
-      const float r = fmaf(-n, s, y), far = 2.f * fabsf(r);
-      if (far > s || (far == s && (((int)n) & 1))) n += copysignf(1.f, r);
-      n = fminf(fmaxf(n, -127.f), 127.f);
-      c[e] = (uint32_t)(int)n & 0xFFu;
+      t[e] = fmaf(x[e], inv, 12582912.f);
+      far = fmaxf(far, fabsf(fmaf(-(t[e] - 12582912.f), s, x[e])));
     }
-    return c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+    if (2.f * far >= s * 0.9999f || up != 1.f) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y = x[e] * up, u = s * up, w = fmaf(y, 1.f / u, 12582912.f), r = fmaf(-(w - 12582912.f), u, y), off = 2.f * fabsf(r);
+        int k = __float_as_int(w) - 0x4B400000;
+        if (off > u || (off == u && (k & 1))) k += r > 0.f ? 1 : -1;
+        t[e] = __int_as_float(0x4B400000 + min(max(k, -127), 127));
+      }
+    }
+    return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
   }
 }
 
-// One warp per row; lane l holds the numbers 4 l .. 4 l + 3 and 128 + 4 l ...
-template <int FMT, bool F32>
+// A lane has eight numbers of a row, so a row has n / 8 lanes (of a power of two of them), and a warp 32 / lanes rows at a time; kWriteRows times that are asked for at once.
+// What bounds it: bytes (8192 tokens of 4 + 4 heads of 128 in bf16: 25 MB, TIME us).  VEC: every eight numbers lie on 16 bytes.
+constexpr int kWriteRows = 2;
+template <int FMT, bool F32, bool VEC>
 __global__ void __launch_bounds__(256) kv_write_kernel(KvLayer c, KvStep t, const void* __restrict__ k, long long ldk, long long hk, const void* __restrict__ v,
                                                         long long ldv, long long hv) {
-  kb2::pdl_wait();
-  const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const bool val = at & 1;
-  const long long row = at >> 1;
-  const int tok = (int)(row / c.G), g = (int)(row - (long long)tok * c.G);
-  if (tok >= t.T || tok >= t.cu[t.S]) return;          // rows behind the last sequence
-  const int n = val ? c.dv : c.d;
-  const long long from = val ? tok * ldv + g * hv : tok * ldk + g * hk;
+  kb2::pdl_enter(k, v);
+  const bool val = blockIdx.y;
+  const int n = val ? c.dv : c.d, lanes = n <= 64 ? 8 : n <= 128 ? 16 : 32, rows = 256 / lanes, e = (threadIdx.x & (lanes - 1)) * 8;
   const void* src = val ? v : k;
-  float x[2][4];
-  uint32_t top = 0;
+  const long long ld = val ? ldv : ldk, hs = val ? hv : hk;
+  const unsigned total = (unsigned)t.T * c.G;
+  const int end = t.cu[t.S];                                               // behind the last sequence nothing is written; what lies there may be read
+  const unsigned first = blockIdx.x * (rows * kWriteRows) + threadIdx.x / lanes;
+  float x[kWriteRows][8];
+  int seq[kWriteRows], pos[kWriteRows], head[kWriteRows], token[kWriteRows];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = i * 128 + lane * 4;
+  for (int i = 0; i < kWriteRows; ++i) {
+    const unsigned row = first + i * rows;
+    seq[i] = pos[i] = head[i] = 0;
+    token[i] = 0x7FFFFFFF;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[i][j] = e < n ? (F32 ? ((const float*)src)[from + e + j] : __bfloat162float(((const bf16*)src)[from + e + j])) : 0.f;
-      top = max(top, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+    for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
+    if (row >= total) continue;
+    const int tok = (int)(row / (unsigned)c.G), g = head[i] = (int)(row - (unsigned)tok * c.G);
+    token[i] = tok;
+    seq[i] = t.seq_of[tok];
+    pos[i] = t.rows[tok];
+    if (e >= n) continue;
+    const long long from = (long long)tok * ld + g * hs + e;
+    if constexpr (F32) {
+      const float* p = (const float*)src + from;
+      if constexpr (VEC) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+        x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = p[j];
+      }
+    } else {
+      const bf16* p = (const bf16*)src + from;
+      if constexpr (VEC) {
+        unpack8(*reinterpret_cast<const uint4*>(p), x[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = __bfloat162float(p[j]);
+      }
     }
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  const long long r0 = kv_row(c, t, t.seq_of[tok], t.rows[tok]);
-  if (r0 < 0) return;
-  const long long r = r0 + ((long long)g << c.lps);
-  const float a = __uint_as_float(top);
-  float s, inv, up = 1.f;
-  if constexpr (FMT == KV_E4M3) {
-    const int e = max((int)(top >> 23) - 126 - 9 + ((top & 0x7FFFFFu) > 0x600000u), -126);      // a <= 448 2^e, 448 = 1.75 2^8
-    s = __uint_as_float((uint32_t)(e + 127) << 23);
-    inv = __uint_as_float((uint32_t)(127 - e) << 23);
-  } else {
-    s = a * (1.f / 127.f);
-    if (a < 1e-20f) up = 1.8446744073709552e19f;       // 2^64 on both: the reciprocal of a smallest scale does not exist
-    inv = 1.f / (s * up);
-  }
-  const bool bad = top >= 0x7F800000u;
-  if (bad) s = __uint_as_float(0x7FFFFFFFu);
-  else if (top == 0 || s == 0.f) s = 0.f;
-  const bool none = bad || s == 0.f;
-  uint8_t* codes = (val ? c.v : c.k) + r * n;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = i * 128 + lane * 4;
-    if (e < n) *reinterpret_cast<uint32_t*>(codes + e) = none ? 0u : kv_codes4<FMT>(x[i], s * up, inv, up);
+  for (int i = 0; i < kWriteRows; ++i) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+    for (int o = lanes / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (token[i] >= end) continue;
+    const long long r0 = kv_row(c, t, seq[i], pos[i]);
+    if (r0 < 0) continue;
+    const long long r = r0 + ((long long)head[i] << c.lps);
+    const float a = __uint_as_float(top);
+    float s, inv, up = 1.f;
+    if constexpr (FMT == KV_E4M3) {
+      const int b = max((int)(top >> 23) - 126 - 9 + ((top & 0x7FFFFFu) > 0x600000u), -126);      // a <= 448 2^b, 448 = 1.75 2^8
+      s = __uint_as_float((uint32_t)(b + 127) << 23);
+      inv = __uint_as_float((uint32_t)(127 - b) << 23);
+    } else {
+      s = a * (1.f / 127.f);
+      if (a < 1e-20f) up = 1.8446744073709552e19f;     // 2^64 on both: the reciprocal of a smallest scale does not exist
+      inv = __fdividef(1.f, s);
+    }
+    const bool bad = top >= 0x7F800000u, none = bad || top == 0 || s == 0.f;
+    if (none) s = bad ? __uint_as_float(0x7FFFFFFFu) : 0.f;
+    if (e < n) {
+      const uint32_t lo = none ? 0u : kv_codes4<FMT>(x[i], s, inv, up), hi = none ? 0u : kv_codes4<FMT>(x[i] + 4, s, inv, up);
+      *reinterpret_cast<uint2*>((val ? c.v : c.k) + r * n + e) = make_uint2(lo, hi);
+    }
+    if (e == 0) (val ? c.vs : c.ks)[r] = s;
   }
-  if (lane == 0) (val ? c.vs : c.ks)[r] = s;
 }
 
 // ------------------------------------------------------------------------------------------------ reading back
@@ -106,53 +141,66 @@ __device__ __forceinline__ void kv_unpack4(uint32_t w, float (&f)[4]) {
   }
 }
 
-// Rows first .. first + count - 1 of sequence s -> [count][G][d] and [count][G][dv]; a thread has 16 codes.
-template <int FMT, bool F32>
+// Rows first .. first + count - 1 of sequence s -> [count][G][d] and [count][G][dv]; a thread has 16 codes, AHEAD times.
+template <int FMT, bool F32, int AHEAD>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvLayer c, KvStep t, int s, int first, int count, void* __restrict__ ko, void* __restrict__ vo) {
-  kb2::pdl_wait();
+  kb2::pdl_enter(ko, vo);
   const int kd = c.d >> 4, w = kd + (c.dv >> 4);
-  const long long total = (long long)count * c.G * w;
-  for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long long)gridDim.x * 256) {
-    const long long rg = at / w;
-    const int x = (int)(at - rg * w), i = (int)(rg / c.G), g = (int)(rg - (long long)i * c.G);
+  const unsigned total = (unsigned)count * c.G * w, at = blockIdx.x * (256 * AHEAD) + threadIdx.x;
+  uint4 q[AHEAD];
+  float sc[AHEAD];
+  long long to[AHEAD];
+  bool val[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    const unsigned x = at + j * 256;
+    to[j] = -1;
+    q[j] = make_uint4(0, 0, 0, 0);
+    sc[j] = 0.f;
+    if (x >= total) continue;
+    const unsigned rg = x / (unsigned)w;
+    const int y = (int)(x - rg * w), i = (int)(rg / (unsigned)c.G), g = (int)(rg - (unsigned)i * c.G);
     const long long r0 = kv_row(c, t, s, first + i);
-    const bool val = x >= kd;
-    const int n = val ? c.dv : c.d, e = (val ? x - kd : x) * 16;
-    uint4 q = make_uint4(0, 0, 0, 0);
-    float sc = 0.f;
+    val[j] = y >= kd;
+    const int n = val[j] ? c.dv : c.d, e = (val[j] ? y - kd : y) * 16;
+    to[j] = (long long)rg * n + e;
     if (r0 >= 0) {
       const long long r = r0 + ((long long)g << c.lps);
-      q = *reinterpret_cast<const uint4*>((val ? c.v : c.k) + r * n + e);
-      sc = (val ? c.vs : c.ks)[r];
+      q[j] = ld_stream16((val[j] ? c.v : c.k) + r * n + e);
+      sc[j] = (val[j] ? c.vs : c.ks)[r];
     }
+  }
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    if (to[j] < 0) continue;
     float f[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int i = 0; i < 4; ++i) {
       float y[4];
-      kv_unpack4<FMT>(j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w, y);
+      kv_unpack4<FMT>(i == 0 ? q[j].x : i == 1 ? q[j].y : i == 2 ? q[j].z : q[j].w, y);
 #pragma unroll
-      for (int l = 0; l < 4; ++l) f[4 * j + l] = y[l] * sc;
+      for (int l = 0; l < 4; ++l) f[4 * i + l] = y[l] * sc[j];
     }
-    const long long to = rg * n + e;
     if constexpr (F32) {
-      float4* o = reinterpret_cast<float4*>((float*)(val ? vo : ko) + to);
+      float4* o = reinterpret_cast<float4*>((float*)(val[j] ? vo : ko) + to[j]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+      for (int i = 0; i < 4; ++i) o[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
     } else {
-      uint4* o = reinterpret_cast<uint4*>((bf16*)(val ? vo : ko) + to);
+      uint4* o = reinterpret_cast<uint4*>((bf16*)(val[j] ? vo : ko) + to[j]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        o[j] = make_uint4(kb2::bf16x2_bits_rn(f[8 * j + 1], f[8 * j]), kb2::bf16x2_bits_rn(f[8 * j + 3], f[8 * j + 2]),
-                          kb2::bf16x2_bits_rn(f[8 * j + 5], f[8 * j + 4]), kb2::bf16x2_bits_rn(f[8 * j + 7], f[8 * j + 6]));
+      for (int i = 0; i < 2; ++i)
+        o[i] = make_uint4(kb2::bf16x2_bits_rn(f[8 * i + 1], f[8 * i]), kb2::bf16x2_bits_rn(f[8 * i + 3], f[8 * i + 2]), kb2::bf16x2_bits_rn(f[8 * i + 5], f[8 * i + 4]),
+                          kb2::bf16x2_bits_rn(f[8 * i + 7], f[8 * i + 6]));
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ the accepted path
-// Block (sequence, layer): row base + path[i] -> row base + i.  A path rises, so path[i] >= i: what a thread writes at i no later step reads, and a thread
-// keeps its 16 bytes of every row, so it has read whatever it overwrites.
-constexpr int kKeepMost = 512;
-__global__ void __launch_bounds__(256) kv_keep_kernel(KvLayer c, long long layer_k, long long layer_v, long long layer_s, KvStep t, const int* __restrict__ path, int P) {
+// Block (sequence, kKeepLayers layers): row base + path[i] -> row base + i.  A path rises, so path[i] >= i: what a thread writes at i no later step reads, and a thread
+// keeps its 16 bytes of every row (eight rows on their way at once), so it has read whatever it overwrites.  What bounds it: the chain of tables ahead of the rows, so
+// a block has work for all its threads (64 paths of 8 in 48 layers: a layer a block 22 us, four TIME).
+constexpr int kKeepMost = 512, kKeepLayers = 8;
+__global__ void __launch_bounds__(256) kv_keep_kernel(KvLayer c, int layers, KvStep t, const int* __restrict__ path, int P) {
   __shared__ long long rows[2][kKeepMost];
   __shared__ int moved;
   kb2::pdl_wait();
@@ -170,29 +218,36 @@ __global__ void __launch_bounds__(256) kv_keep_kernel(KvLayer c, long long layer
     if (a < 0 || b < 0) atomicMin(&moved, i);          // the path ends here
   }
   __syncthreads();
-  const int m = moved, kd = c.d >> 4, w = kd + (c.dv >> 4);
-  const long long layer = blockIdx.y;
-  uint8_t *k = c.k + layer * layer_k, *v = c.v + layer * layer_v;
-  float *ks = c.ks + layer * layer_s, *vs = c.vs + layer * layer_s;
-  for (int x = threadIdx.x; x < c.G * w; x += 256) {
-    const int g = x / w, e = x - g * w;
-    const bool val = e >= kd;
-    const long long n16 = val ? c.dv : c.d, off = ((long long)g << c.lps) * n16 + (val ? e - kd : e) * 16;
-    uint8_t* p = val ? v : k;
-    for (int i0 = 0; i0 < m; i0 += 8) {
-      uint4 b[8];
+  const int m = moved, kd = c.d >> 4, w = kd + (c.dv >> 4), of = c.G * (w + 2), l0 = blockIdx.y * kKeepLayers, ln = min(kKeepLayers, layers - l0);
+  const long long all = ((long long)c.pages * c.G) << c.lps;               // rows of a layer
+  for (int x = threadIdx.x; x < of * ln; x += 256) {
+    const int layer = l0 + x / of, y = x % of, g = y / (w + 2), e = y - g * (w + 2);
+    const long long head = layer * all + ((long long)g << c.lps);
+    if (e < w) {
+      const bool val = e >= kd;
+      const long long n16 = val ? c.dv : c.d;
+      uint8_t* p = (val ? c.v : c.k) + head * n16 + (val ? e - kd : e) * 16;
+      for (int i0 = 0; i0 < m; i0 += 8) {
+        uint4 b[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i0 + i < m) b[i] = *reinterpret_cast<const uint4*>(p + rows[0][i0 + i] * n16 + off);
+        for (int i = 0; i < 8; ++i)
+          if (i0 + i < m) b[i] = *reinterpret_cast<const uint4*>(p + rows[0][i0 + i] * n16);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i0 + i < m) *reinterpret_cast<uint4*>(p + rows[1][i0 + i] * n16 + off) = b[i];
+        for (int i = 0; i < 8; ++i)
+          if (i0 + i < m) *reinterpret_cast<uint4*>(p + rows[1][i0 + i] * n16) = b[i];
+      }
+    } else {
+      float* p = (e > w ? c.vs : c.ks) + head;
+      for (int i0 = 0; i0 < m; i0 += 8) {
+        float b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i0 + i < m) b[i] = p[rows[0][i0 + i]];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i0 + i < m) p[rows[1][i0 + i]] = b[i];
+      }
     }
-  }
-  for (int x = threadIdx.x; x < 2 * c.G; x += 256) {
-    float* p = (x & 1) ? vs : ks;
-    const long long off = (long long)(x >> 1) << c.lps;
-    for (int i = 0; i < m; ++i) p[rows[1][i] + off] = p[rows[0][i] + off];
   }
 }
 }  // namespace kb2seq
@@ -210,11 +265,16 @@ KB2SEQ_API int kb2_seq_kv_write(const kb2_seq_kv_cache* cache, int layer, const 
   if (t.T == 0) return KB2SEQ_OK;
   OnDevice on(step->device);
   SEQ_CUDA(on.err);
-  const long long blocks = ((long long)t.T * c.G * 2 + 7) / 8;
-  if (blocks > 0x7FFFFFFFll) return failf(KB2SEQ_ERR_VALUE, "kv_write: too many rows");
-  auto kern = cache->fmt == KV_E4M3 ? (dt ? kv_write_kernel<KV_E4M3, false> : kv_write_kernel<KV_E4M3, true>)
-                                    : (dt ? kv_write_kernel<KV_INT8, false> : kv_write_kernel<KV_INT8, true>);
-  kb2::launch_pdl(kern, (unsigned)blocks, 256, 0, (cudaStream_t)stream, c, t, k, ldk, hk, v, ldv, hv);
+  const int most = std::max(c.d, c.dv), rows = 256 / (most <= 64 ? 8 : most <= 128 ? 16 : 32) * kWriteRows;      // the wider of the two: the other's last blocks have none
+  const long long blocks = ((long long)t.T * c.G + rows - 1) / rows;
+  if ((long long)t.T * c.G > 0x7FFFFFFFll - 4096) return failf(KB2SEQ_ERR_VALUE, "kv_write: too many rows");
+  const long long unit = dt ? 8 : 4;
+  const bool vec = !(((uintptr_t)k | (uintptr_t)v) & 15) && ldk % unit == 0 && ldv % unit == 0 && hk % unit == 0 && hv % unit == 0;
+  auto kern = cache->fmt == KV_E4M3 ? (dt ? (vec ? kv_write_kernel<KV_E4M3, false, true> : kv_write_kernel<KV_E4M3, false, false>)
+                                          : (vec ? kv_write_kernel<KV_E4M3, true, true> : kv_write_kernel<KV_E4M3, true, false>))
+                                    : (dt ? (vec ? kv_write_kernel<KV_INT8, false, true> : kv_write_kernel<KV_INT8, false, false>)
+                                          : (vec ? kv_write_kernel<KV_INT8, true, true> : kv_write_kernel<KV_INT8, true, false>));
+  kb2::launch_pdl(kern, dim3((unsigned)blocks, 2), 256, 0, (cudaStream_t)stream, c, t, k, ldk, hk, v, ldv, hv);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }
@@ -232,9 +292,13 @@ KB2SEQ_API int kb2_seq_kv_read(const kb2_seq_kv_cache* cache, int layer, const k
   OnDevice on(step->device);
   SEQ_CUDA(on.err);
   const long long total = (long long)count * c.G * ((c.d + c.dv) / 16);
-  const unsigned blocks = (unsigned)std::min((total + 255) / 256, kb2::current_sms() * 16ll);
-  auto kern = cache->fmt == KV_E4M3 ? (dt ? kv_read_kernel<KV_E4M3, false> : kv_read_kernel<KV_E4M3, true>)
-                                    : (dt ? kv_read_kernel<KV_INT8, false> : kv_read_kernel<KV_INT8, true>);
+  if (total > 0x7FFFFFFFll - 4096) return failf(KB2SEQ_ERR_VALUE, "kv_read: too many rows");
+  const bool ahead = total > kb2::current_sms() * 2048ll;                  // more than the GPU has threads: four pieces each are on their way at once
+  const unsigned blocks = (unsigned)((total + (ahead ? 1023 : 255)) / (ahead ? 1024 : 256));
+  auto kern = cache->fmt == KV_E4M3 ? (dt ? (ahead ? kv_read_kernel<KV_E4M3, false, 4> : kv_read_kernel<KV_E4M3, false, 1>)
+                                          : (ahead ? kv_read_kernel<KV_E4M3, true, 4> : kv_read_kernel<KV_E4M3, true, 1>))
+                                    : (dt ? (ahead ? kv_read_kernel<KV_INT8, false, 4> : kv_read_kernel<KV_INT8, false, 1>)
+                                          : (ahead ? kv_read_kernel<KV_INT8, true, 4> : kv_read_kernel<KV_INT8, true, 1>));
   kb2::launch_pdl(kern, blocks, 256, 0, (cudaStream_t)stream, c, t, s, first, count, k, v);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
@@ -246,11 +310,10 @@ KB2SEQ_API int kb2_seq_kv_keep(const kb2_seq_kv_cache* cache, const kb2_seq_kv_s
   if (int e = kv_args("kv_keep", cache, 0, step, &c, &t)) return e;
   if (P < 0 || P > kKeepMost || (P && !path)) return failf(KB2SEQ_ERR_VALUE, "kv_keep: a path of at most %d rows", kKeepMost);
   if (P == 0 || t.T == 0) return KB2SEQ_OK;
-  if (cache->layers > 65535) return failf(KB2SEQ_ERR_VALUE, "kv_keep: too many layers");
+  if (cache->layers > 65535 * kKeepLayers) return failf(KB2SEQ_ERR_VALUE, "kv_keep: too many layers");
   OnDevice on(step->device);
   SEQ_CUDA(on.err);
-  const long long rows = ((long long)c.pages * c.G) << c.lps;
-  kb2::launch_pdl(kv_keep_kernel, dim3(t.S, cache->layers), 256, 0, (cudaStream_t)stream, c, rows * c.d, rows * c.dv, rows, t, path, P);
+  kb2::launch_pdl(kv_keep_kernel, dim3(t.S, (cache->layers + kKeepLayers - 1) / kKeepLayers), 256, 0, (cudaStream_t)stream, c, cache->layers, t, path, P);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }
