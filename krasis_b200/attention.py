@@ -501,6 +501,7 @@ class CompactKVCache(PagedKVCache):
         self._free = list(range(max_pages - 1, -1, -1))
         self.args = seqops.KvCacheArgs(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), num_layers, max_pages, page_size,
                                        num_kv_heads, dim, vdim, code)
+        self.index, self.address = self.k.get_device(), C.addressof(self.args)       # for the C interface: the device's number, the structure's place
 
     def get_layer_caches(self, layer_offset: int):
         return self.k[layer_offset], self.v[layer_offset]

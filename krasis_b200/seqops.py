@@ -9,7 +9,7 @@ import os
 
 import torch
 
-from .streams import stream_of as _s
+from .streams import stream_of as _s, stream_on
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_lib", "libkrasis_b200_seq.so")
@@ -508,79 +508,94 @@ class DraftTables(StepTables):
 
 
 def _kv_step(tb: StepTables):
-    """The tables as the C interface takes them; made once per step, and again if the step's layout is set anew."""
-    kept = getattr(tb, "_kv_step", None)
-    if kept is not None and kept[1] is tb._layout_host:
-        return kept[0]
+    """The tables as the C interface takes them, and workspace sizes; made once per step, and again if the step's layout is set anew."""
     rows, bits = getattr(tb, "rows", None), getattr(tb, "bits", None)
     a = KvStepArgs(tb.positions.data_ptr(), tb.seq_of.data_ptr(), tb.cu.data_ptr(), tb.pages.data_ptr(), _ptr(rows), _ptr(bits), tb.layout_ptr,
                    tb.words if bits is not None else 0, tb.T, tb.S, tb.max_pages, int(tb.replayed), tb.buf.get_device())
-    tb._kv_step, tb._kv_sizes = (a, tb._layout_host), {}
-    return a
+    tb._kv = kept = (C.addressof(a), tb._layout_host, a.device, {}, a)
+    return kept
 
 
 def _kv_call(name, tb, cache, *tensors):
-    """(cache, tables) for the C interface; everything on one GPU."""
-    dev = tb.buf.get_device()
-    if dev < 0 or cache.k.get_device() != dev or any(t.get_device() != dev for t in tensors):
-        raise ValueError(f"{name}: the tables, the cache and the tensors belong on one CUDA device (krasis_b200 has no CPU path)")
-    return C.byref(cache.args), C.byref(_kv_step(tb))
+    """(address of the cache's structure, of the tables', device, workspace sizes) for the C interface; everything on one GPU."""
+    kept = getattr(tb, "_kv", None)
+    if kept is None or kept[1] is not tb._layout_host:
+        kept = _kv_step(tb)
+    dev = kept[2]
+    if dev < 0 or cache.index != dev:
+        _kv_refuse(name)
+    for t in tensors:
+        if t.get_device() != dev:
+            _kv_refuse(name)
+    return cache.address, kept[0], dev, kept[3]
 
 
-def _kv_rows(name, what, t, T, heads, width):
-    if t.dim() != 3 or t.shape[0] != T or t.shape[1] != heads or t.shape[2] != width:
-        raise ValueError(f"{name}: {what} has shape {tuple(t.shape)}, expected {(T, heads, width)}")
-    if t.stride(2) != 1 and width > 1:
+def _kv_refuse(name):
+    raise ValueError(f"{name}: the tables, the cache and the tensors belong on one CUDA device (krasis_b200 has no CPU path)")
+
+
+def _kv_rows(name, what, t, shape):
+    if t.shape != shape:
+        raise ValueError(f"{name}: {what} has shape {tuple(t.shape)}, expected {shape}")
+    if t.stride(2) != 1:
         raise ValueError(f"{name}: the numbers of a head of {what} lie side by side")
 
 
 def kv_write(k: torch.Tensor, v: torch.Tensor, tb: StepTables, cache, layer: int):
     """Quantises the step's keys k [T, G, d] and values v [T, G, dv] (fp32 or bfloat16, any strides with a unit last one) into the pages of a CompactKVCache."""
-    p, q = _kv_call("kv_write", tb, cache, k, v)
-    _kv_rows("kv_write", "k", k, tb.T, cache.num_kv_heads, cache.dim)
-    _kv_rows("kv_write", "v", v, tb.T, cache.num_kv_heads, cache.vdim)
-    if k.dtype != v.dtype:
+    p, q, dev, _ = _kv_call("kv_write", tb, cache, k, v)
+    _kv_rows("kv_write", "k", k, (tb.T, cache.num_kv_heads, cache.dim))
+    _kv_rows("kv_write", "v", v, (tb.T, cache.num_kv_heads, cache.vdim))
+    if k.dtype is not v.dtype:
         raise ValueError(f"kv_write: k is {k.dtype}, v {v.dtype}")
-    dt = dt_code(k.dtype)
-    check(load().kb2_seq_kv_write(p, layer, q, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dt, _s(k)))
+    dt, (ldk, hk, _), (ldv, hv, _) = dt_code(k.dtype), k.stride(), v.stride()
+    check(load().kb2_seq_kv_write(p, layer, q, k.data_ptr(), ldk, hk, v.data_ptr(), ldv, hv, dt, stream_on(dev)))
 
 
 def kv_read(tb: StepTables, s: int, first: int, count: int, cache, layer: int, dtype=torch.bfloat16):
     """Rows first .. first + count - 1 of the step's sequence s: (keys [count, G, d], values [count, G, dv]) in float32 or bfloat16."""
-    p, q = _kv_call("kv_read", tb, cache)
+    p, q, dev, _ = _kv_call("kv_read", tb, cache)
     if not 0 <= s < tb.S or first < 0 or count < 0:
         raise ValueError(f"kv_read: {count} rows from {first} of sequence {s} of {tb.S}")
-    dt, G = dt_code(dtype), cache.num_kv_heads
-    k = torch.empty((count, G, cache.dim), dtype=dtype, device=cache.k.device)
-    v = torch.empty((count, G, cache.vdim), dtype=dtype, device=cache.k.device)
-    check(load().kb2_seq_kv_read(p, layer, q, s, first, count, k.data_ptr(), v.data_ptr(), dt, _s(cache.k)))
+    dt, G, lib, device = dt_code(dtype), cache.num_kv_heads, load(), cache.k.device
+    k = torch.empty((count, G, cache.dim), dtype=dtype, device=device)
+    v = torch.empty((count, G, cache.vdim), dtype=dtype, device=device)
+    check(lib.kb2_seq_kv_read(p, layer, q, s, first, count, k.data_ptr(), v.data_ptr(), dt, stream_on(dev)))
     return k, v
 
 
 def _kv_attend(name, q, tb, cache, layer, scale, window, first, sinks, dtype, out):
-    p, st = _kv_call(name, tb, cache, q)
+    p, st, dev, sizes = _kv_call(name, tb, cache, q)
     H, G, T = q.shape[1] if q.dim() == 3 else 0, cache.num_kv_heads, tb.T
-    _kv_rows(name, "q", q, T, H, cache.dim)
+    _kv_rows(name, "q", q, (T, H, cache.dim))
     if H == 0 or H % G:
         raise ValueError(f"{name}: {H} heads on {G} key / value heads")
-    if (window is not None and window < 1) or first < 0:
-        raise ValueError(f"{name}: a window of {window} with {first} first tokens")
-    window = 0 if window is None else min(int(window), 1 << 30)
-    first = min(int(first), 1 << 30)
-    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != H or not sinks.is_contiguous() or sinks.get_device() != q.get_device()):
+    if window is None:
+        window = 0
+    elif window < 1:
+        raise ValueError(f"{name}: a window of {window}")
+    if first < 0:
+        raise ValueError(f"{name}: {first} first tokens")
+    window, first = min(int(window), 1 << 30), min(int(first), 1 << 30)
+    if sinks is not None and (sinks.dtype is not torch.float32 or sinks.numel() != H or not sinks.is_contiguous() or sinks.get_device() != dev):
         raise ValueError(f"{name}: one fp32 sink per head")
+    dq = dt_code(q.dtype)
     if out is None:
-        out = torch.empty((T, H, cache.vdim), dtype=q.dtype if dtype is None else dtype, device=q.device)
-    elif out.shape != (T, H, cache.vdim) or not out.is_contiguous() or out.get_device() != q.get_device() or (dtype is not None and out.dtype != dtype):
-        raise ValueError(f"{name}: out is a contiguous {(T, H, cache.vdim)}")
-    dq, do = dt_code(q.dtype), dt_code(out.dtype)
-    lib, key = load(), (G, cache.vdim, cache.page_size, H, window, first, do)
-    size = tb._kv_sizes.get(key)
+        dtype = q.dtype if dtype is None else dtype
+        do, device = dt_code(dtype), q.device
+        out = torch.empty((T, H, cache.vdim), dtype=dtype, device=device)
+    else:
+        if out.shape != (T, H, cache.vdim) or not out.is_contiguous() or out.get_device() != dev or (dtype is not None and out.dtype is not dtype):
+            raise ValueError(f"{name}: out is a contiguous {(T, H, cache.vdim)}")
+        do, device = dt_code(out.dtype), q.device
+    lib, key = load(), (G, cache.dim, cache.vdim, cache.page_size, H, window, first, do)
+    size = sizes.get(key)
     if size is None:
-        size = tb._kv_sizes[key] = lib.kb2_seq_kv_attn_workspace(p, st, H, window, first, do)
-    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    check(lib.kb2_seq_kv_attn(p, layer, st, q.data_ptr(), dq, q.stride(0), q.stride(1), H, float(scale), window, first, _ptr(sinks), out.data_ptr(), do,
-                              _ptr(work), size, _s(q)))
+        size = sizes[key] = lib.kb2_seq_kv_attn_workspace(p, st, H, window, first, do)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    ldq, hq, _ = q.stride()
+    check(lib.kb2_seq_kv_attn(p, layer, st, q.data_ptr(), dq, ldq, hq, H, scale, window, first, None if sinks is None else sinks.data_ptr(), out.data_ptr(), do,
+                              None if work is None else work.data_ptr(), size, stream_on(dev)))
     return out
 
 
@@ -606,7 +621,7 @@ def kv_keep(tb: DraftTables, path: torch.Tensor, cache):
     sequence, ended by -1 (or by any number that does not rise or is no token of the sequence).  The sequence then has start + (its path's length) rows."""
     if not isinstance(tb, DraftTables):
         raise ValueError("kv_keep: the step's tables are DraftTables")
-    p, q = _kv_call("kv_keep", tb, cache, path)
-    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != tb.S or not path.is_contiguous():
+    p, q, dev, _ = _kv_call("kv_keep", tb, cache, path)
+    if path.dtype is not torch.int32 or path.dim() != 2 or path.shape[0] != tb.S or not path.is_contiguous():
         raise ValueError(f"kv_keep: path is a contiguous int32 [{tb.S}, P]")
-    check(load().kb2_seq_kv_keep(p, q, path.data_ptr(), path.shape[1], _s(path)))
+    check(load().kb2_seq_kv_keep(p, q, path.data_ptr(), path.shape[1], stream_on(dev)))

@@ -50,7 +50,7 @@ def test_wrappers_refuse_the_cpu():
 @pytest.fixture
 def on_gpu(monkeypatch):
     """The wrappers' own checks: the device check is left out, and nothing may reach the library."""
-    monkeypatch.setattr(ops, "_kv_call", lambda name, tb, cache, *t: (None, ops._kv_step(tb)))
+    monkeypatch.setattr(ops, "_kv_call", lambda name, tb, cache, *t: (None, ops._kv_step(tb)[0], -1, {}))
 
     def load():
         raise AssertionError("the call should have been refused")
