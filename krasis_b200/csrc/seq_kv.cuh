@@ -33,6 +33,7 @@ __device__ __forceinline__ long long kv_row(const KvLayer& c, const KvStep& t, i
 struct KvSpan {
   int na, b0, nb, base;                      // base: the first drafted row, or past every position
   int lo, hi;                                // seen are the positions below `first` and lo .. hi - 1
+  int p0, p1;                                // positions of the first and the last token
   __device__ __forceinline__ int groups() const { return na + nb; }
   __device__ __forceinline__ int group(int i) const { return i < na ? i : b0 + i - na; }
 };
@@ -40,6 +41,8 @@ __device__ __forceinline__ KvSpan kv_span(const KvLayer& c, const KvStep& t, int
   KvSpan r;
   int lo, hi;
   const int most = t.max_pages << c.lps;     // fits: checked on the host
+  r.p0 = t.positions[t0];
+  r.p1 = t.positions[t1];
   if (t.bits != nullptr) {                   // a token's position is base + its depth, and its ancestors come before it
     const int c0 = t.cu[s];
     r.base = t.rows[c0];
@@ -47,8 +50,8 @@ __device__ __forceinline__ KvSpan kv_span(const KvLayer& c, const KvStep& t, int
     hi = r.base + (t1 - c0) + 1;
   } else {
     r.base = 0x7FFFFFFF;
-    lo = t.positions[t0];
-    hi = t.positions[t1] + 1;
+    lo = r.p0;
+    hi = r.p1 + 1;
   }
   hi = min(hi, most);
   lo = window < kKvNoWindow ? max(0, lo - window + 1) : 0;

@@ -18,7 +18,7 @@
 namespace kb2seq {
 namespace {
 
-constexpr int kSWarps = 8, kSStages = 3, kSMostGroups = 768, kMostPieces = 1024, kMostTiles = 768;
+constexpr int kSWarps = 8, kSStages = 3, kSMostGroups = 768, kMostPieces = 1024, kMostTiles = 768, kClusterMost = 8;
 constexpr int kPieceCost = 40;               // what a piece costs beside its keys, in groups of 16 (11 us against 0.25 a group, with two blocks on an SM)
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -49,13 +49,41 @@ struct StreamShape {
   static constexpr bool kQShared = NQ == 2 || DU * 8 * PARTS > 32;      // registers of the queries; spilled ones cost more than those read again
   static constexpr int kQ = DU * 4 * PARTS * 2 * NQ * 128;
   static constexpr int kRow = VU * 64 + 8;                                // numbers from row to row of a warp's share at the end: 32 bytes apart in the banks
-  static constexpr int kRing = kSWarps * kSStages * kStage, kRed = kSWarps * MT * kRow * 4;
+  static constexpr int kRing = kSWarps * kSStages * kStage, kShare = MT * (VU * 64 + 4) * 4, kRed = kSWarps * MT * kRow * 4 + kShare;      // kShare: what a block has for the others of its cluster
   static constexpr int kOffRow = kRing > kRed ? kRing : kRed, kOffStat = kOffRow + kSMostGroups * 4, kOffTok = kOffStat + kSWarps * MT * 4 * 4, kOffQ = kOffTok + MT * 16,
                        kOffScan = kOffQ + kQ;
   static constexpr int kTotal = kOffScan + (kMostTiles + 4) * 4;
   static constexpr int kBlocks = 2 * (kTotal + 1024) <= 227 * 1024 ? 2 : 1;
   static_assert(kTotal <= 227 * 1024 && kOffQ % 16 == 0 && kStage % 16 == 0, "shared memory");
 };
+
+// Four numbers at this place in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ float4 lds_of(const float* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(kb2::cluster_addr(p, rank)));
+  return v;
+}
+// Eight columns of a row: finished, or as piece z with its maximum and sum.
+__device__ __forceinline__ void store8(const KvLayer& c, const KvAttn& a, const float (&acc)[8], float top, float sum, long long row, int hd, int dim, int z) {
+  float y[8];
+  float by = 1.f;
+  if (z < 0) {
+    if (a.sinks != nullptr && top != -INFINITY) sum += ex2(fmaf(a.sinks[hd], kLog2e, -top));
+    by = sum == 0.f ? 0.f : 1.f / sum;
+  } else if (dim == 0) {
+    *reinterpret_cast<float2*>(a.part_ml + 2 * (row * a.pieces + z)) = make_float2(top, sum);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = acc[e] * by;
+  if (z < 0 && a.dt_out) {
+    *reinterpret_cast<uint4*>((bf16*)a.out + row * c.dv + dim) =
+        make_uint4(kb2::bf16x2_bits_rn(y[1], y[0]), kb2::bf16x2_bits_rn(y[3], y[2]), kb2::bf16x2_bits_rn(y[5], y[4]), kb2::bf16x2_bits_rn(y[7], y[6]));
+  } else {
+    float4* to = reinterpret_cast<float4*>(z < 0 ? (float*)a.out + row * c.dv + dim : a.part_o + (row * a.pieces + z) * c.dv + dim);
+    to[0] = make_float4(y[0], y[1], y[2], y[3]);
+    to[1] = make_float4(y[4], y[5], y[6], y[7]);
+  }
+}
 
 // FULL: d and dv are whole units, and every copy's address is one of two a lane has plus a constant.
 template <int FMT, int DU, int VU, int NQ, int PARTS, bool FULL>
@@ -183,9 +211,9 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   const KvSpan span = kv_span(c, t, s, t0, t1, a.window, a.first);
   if (!a.linear) {
     const int total = span.groups();
-    np = min((total + a.piece - 1) / a.piece, a.pieces);
+    np = a.cluster ? a.pieces : min((total + a.piece - 1) / a.piece, a.pieces);
     if (z > 0 && z >= np) return;
-    u0 = z * a.piece;
+    u0 = min(z * a.piece, total);
     u1 = min(total, u0 + a.piece);           // z = 0 of nothing to see: no group
   }
 
@@ -473,13 +501,8 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int q = 8 * h + 2 * t4 + e;
-      float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kSWarps; ++w) top = fmaxf(top, stat[w * MT + q].x);
-      const float4 x = stat[warp * MT + q];
-      const float f = x.x == -INFINITY ? 0.f : x.z * ex2(x.x - top);
-#pragma unroll
-      for (int i = 0; i < MV; ++i) *reinterpret_cast<float2*>(red + (warp * MT + q) * L::kRow + (i * 8 + g8) * 2) = make_float2(o[i][h][e] * f, o[i][h][2 + e] * f);
+      for (int i = 0; i < MV; ++i) *reinterpret_cast<float2*>(red + (warp * MT + q) * L::kRow + (i * 8 + g8) * 2) = make_float2(o[i][h][e], o[i][h][2 + e]);
     }
   __syncthreads();
   // a thread takes eight columns of a row
@@ -495,33 +518,57 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
 #pragma unroll
     for (int w = 0; w < kSWarps; ++w) {
       const float4 x = stat[w * MT + q];
-      sum += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top);                // a sum without a maximum is 0, or NaN from a row that holds one
+      const float g = x.x == -INFINITY ? 0.f : ex2(x.x - top), f = x.z * g;
+      sum += x.x == -INFINITY ? x.y : x.y * g;                             // a sum without a maximum is 0, or NaN from a row that holds one
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 v = *reinterpret_cast<const float2*>(red + (w * MT + q) * L::kRow + from + 16 * e);
-        acc[2 * e] += v.x;
-        acc[2 * e + 1] += v.y;
+        acc[2 * e] = fmaf(v.x, f, acc[2 * e]);
+        acc[2 * e + 1] = fmaf(v.y, f, acc[2 * e + 1]);
       }
     }
-    const int rr = r0 + q, hd = head * per + rr % per;
-    const long long row = (long long)(c0 + rr / per) * a.H + hd;
-    if (np <= 1) {
-      if (a.sinks != nullptr && top != -INFINITY) sum += ex2(fmaf(a.sinks[hd], kLog2e, -top));
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (a.cluster) {                         // the tile's pieces are the blocks of a cluster: they meet in shared memory
+      float* share = red + kSWarps * MT * L::kRow + q * (VU * 64 + 4);
+      *reinterpret_cast<float4*>(share + dim) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(share + dim + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (dim == 0) *reinterpret_cast<float4*>(share + VU * 64) = make_float4(top, sum, 0.f, 0.f);
+      continue;
+    }
+    store8(c, a, acc, top, sum, (long long)(c0 + (r0 + q) / per) * a.H + head * per + (r0 + q) % per, head * per + (r0 + q) % per, dim, np <= 1 ? -1 : z);
+  }
+  if (a.cluster) {
+    kb2::cluster_sync_all();
+    const int rank = (int)kb2::cluster_rank(), i = threadIdx.x * np + rank, q = i / kCols, dim = (i - q * kCols) * 8;
+    if (q < nr && dim < c.dv) {
+      const float* share = red + kSWarps * MT * L::kRow + q * (VU * 64 + 4);
+      float top = -INFINITY, sum = 0.f, acc[8] = {};
+      float4 ml[kClusterMost], v[kClusterMost][2];                         // all asked for at once: one after another they took half of a small call's time
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] *= inv;
-    } else if (dim == 0) {
-      a.part_ml[2 * (row * a.pieces + z)] = top;
-      a.part_ml[2 * (row * a.pieces + z) + 1] = sum;
+      for (int b = 0; b < kClusterMost; ++b) {
+        const int of = min(b, np - 1);
+        ml[b] = lds_of(share + VU * 64, of);
+        v[b][0] = lds_of(share + dim, of);
+        v[b][1] = lds_of(share + dim + 4, of);
+      }
+#pragma unroll
+      for (int b = 0; b < kClusterMost; ++b) top = fmaxf(top, ml[b].x);
+#pragma unroll
+      for (int b = 0; b < kClusterMost; ++b) {
+        if (b >= np) continue;
+        const float f = ml[b].x == -INFINITY ? 1.f : ex2(ml[b].x - top);   // a piece without a maximum holds zeros, or NaN
+        sum += ml[b].y * f;
+        acc[0] = fmaf(v[b][0].x, f, acc[0]);
+        acc[1] = fmaf(v[b][0].y, f, acc[1]);
+        acc[2] = fmaf(v[b][0].z, f, acc[2]);
+        acc[3] = fmaf(v[b][0].w, f, acc[3]);
+        acc[4] = fmaf(v[b][1].x, f, acc[4]);
+        acc[5] = fmaf(v[b][1].y, f, acc[5]);
+        acc[6] = fmaf(v[b][1].z, f, acc[6]);
+        acc[7] = fmaf(v[b][1].w, f, acc[7]);
+      }
+      store8(c, a, acc, top, sum, (long long)(c0 + (r0 + q) / per) * a.H + head * per + (r0 + q) % per, head * per + (r0 + q) % per, dim, -1);
     }
-    if (np <= 1 && a.dt_out) {
-      *reinterpret_cast<uint4*>((bf16*)a.out + row * c.dv + dim) =
-          make_uint4(kb2::bf16x2_bits_rn(acc[1], acc[0]), kb2::bf16x2_bits_rn(acc[3], acc[2]), kb2::bf16x2_bits_rn(acc[5], acc[4]), kb2::bf16x2_bits_rn(acc[7], acc[6]));
-    } else {
-      float4* to = reinterpret_cast<float4*>(np <= 1 ? (float*)a.out + row * c.dv + dim : a.part_o + (row * a.pieces + z) * c.dv + dim);
-      to[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-    }
+    kb2::cluster_sync_all();                 // nobody leaves while its share is read
   }
   }
 }
@@ -547,7 +594,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
   if (tok >= t.cu[t.S]) return;
   const int per = x.H / c.G, s = t.seq_of[tok], c0 = t.cu[s], n = t.cu[s + 1] - c0;
   const KvAttn& a = n * per <= x.most ? x : y;
-  if (a.pieces <= 1) return;
+  if (a.pieces <= 1 || a.cluster) return;
   const int r0 = ((tok - c0) * per + hd % per) / a.rows * a.rows, nr = (int)min((long long)n * per - r0, (long long)a.rows);
   const KvSpan span = kv_span(c, t, s, c0 + r0 / per, c0 + (r0 + nr - 1) / per, a.window, a.first);
   const int np = a.linear ? a.counts[(s * a.per_seq + r0 / a.rows) * c.G + hd / per] : min((span.groups() + a.piece - 1) / a.piece, a.pieces);
@@ -627,6 +674,7 @@ constexpr int kTileFrom = 17;
 // How the sequences of one kind are cut: into tiles of rows, and the keys that a tile sees (in groups of 16) into pieces.
 struct KvPlan {
   int least, most, rows, tiles, per_seq, piece, pieces, blocks;            // blocks: of the even cut, 0 for pieces of tiles
+  bool cluster;                              // the pieces of a tile are a cluster, which joins them itself
   size_t floats;                             // workspace
 };
 // The most groups of 16 that the tokens start .. start + n - 1 see.
@@ -681,6 +729,15 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
       // a captured step's keys may come to lie in one sequence: the kernel makes its pieces no more than this
       p.pieces = (int)(step->replayed ? std::max(34ll, (top + kPieceCost) / kSMostGroups + 2) : (top + kPieceCost) / std::min<long long>(std::max(even, 8ll), kSMostGroups) + 2);
     }
+    // Few keys: up to eight blocks a tile meet in shared memory, without a second launch and a workspace (four requests of 1028 visible rows: TIME us, with a join 9.8);
+    // more than that, a warp would have too many keys one after another (6144 a tile).
+    if (!p.blocks && top > kSWarps && top <= 48 * kClusterMost && (long long)p.tiles * cache->G * kClusterMost <= slots) {
+      p.cluster = true;
+      p.pieces = (int)std::min<long long>(kClusterMost, (top + kSWarps - 1) / kSWarps);
+      p.piece = (int)((top + p.pieces - 1) / p.pieces);
+      if (p.piece <= kSMostGroups) return p;
+      p.cluster = false;
+    }
     long long best = 0, cost = 0;
     for (int waves = 1; waves <= 4; ++waves) {
       long long len = std::max<long long>((work * cache->G + waves * slots - 1) / (waves * slots), (top + 63) / 64);
@@ -727,6 +784,7 @@ inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, 
   a.part_o = work;
   a.part_ml = work + (size_t)rows_total * p.pieces * dv;
   a.linear = p.blocks > 0;
+  a.cluster = p.cluster;
   a.counts = reinterpret_cast<int*>(a.part_ml + 2 * (size_t)rows_total * p.pieces);
   return a;
 }
@@ -736,7 +794,7 @@ int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPl
   using L = StreamShape<DU, VU, NQ, PARTS>;
   SEQ_CUDA((kb2::allow_smem<kv_stream_kernel<FMT, DU, VU, NQ, PARTS, FULL>>(L::kTotal)));
   auto kern = kv_stream_kernel<FMT, DU, VU, NQ, PARTS, FULL>;
-  kb2::launch_pdl(kern, p.blocks ? dim3(p.blocks) : dim3(p.tiles, c.G, p.pieces), kSWarps * 32, L::kTotal, st, c, t, a);
+  kb2::launch_pdl_clusters(kern, p.blocks ? dim3(p.blocks) : dim3(p.tiles, c.G, p.pieces), kSWarps * 32, L::kTotal, st, dim3(1, 1, p.cluster ? p.pieces : 1), c, t, a);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }
@@ -804,7 +862,7 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   if (p.few.tiles) {
     if (int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, few, p.few, st) : stream_sizes<KV_INT8>(c, t, few, p.few, st)) return e;
   }
-  if (p.few.pieces <= 1 && p.many.pieces <= 1) return KB2SEQ_OK;
+  if ((p.few.pieces <= 1 || p.few.cluster) && p.many.pieces <= 1) return KB2SEQ_OK;
   const int most = std::max(p.few.pieces, p.many.pieces);
   const bool wide = (long long)t.T * H <= 4096 || (most > 8 && (long long)t.T * H <= 16384) || most > 32;
   auto join = wide ? kv_join_kernel<4> : kv_join_kernel<1>;

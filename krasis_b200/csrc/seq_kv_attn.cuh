@@ -23,6 +23,7 @@ struct KvAttn {                              // what a call says beside the cach
                                              // each where the step's sequences bring as many tokens each, else 0
   int piece, pieces;                         // groups of 16 keys a piece; the most pieces of a tile
   float *part_o, *part_ml;                   // [T H][pieces][dv] and [T H][pieces][2]
+  bool cluster;                              // a tile's pieces are the blocks of a cluster, which joins them itself
   bool linear;                               // all tiles' keys in a row are cut evenly, wherever the ends lie: `pieces` is then the most that a tile may have,
   int* counts;                               // and this, [tiles][G], how many it has
 };
@@ -66,10 +67,10 @@ __device__ __forceinline__ bool kv_sees(const KvStep& t, const KvAttn& a, const 
 // The least and the most position of the tokens t0 .. t1: the first and the last of a portion; of a tree the least is any that is no more.  The most matters under a window.
 __device__ __forceinline__ void kv_reach(const KvStep& t, const KvAttn& a, const KvSpan& span, int t0, int t1, int* least, int* most) {
   const bool tree = span.base < kKvNoWindow;
-  *least = tree ? span.base : t.positions[t0];
+  *least = tree ? span.base : span.p0;
   *most = *least;
   if (a.window >= kKvNoWindow) return;
-  *most = t.positions[t1];
+  *most = span.p1;
   if (tree) {
     for (int x = t0; x < t1; ++x) *most = max(*most, t.positions[x]);
   }

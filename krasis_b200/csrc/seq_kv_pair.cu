@@ -188,7 +188,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     int least, most;
     {                                        // of the warp's rows
       const int w0 = row - lane, ra = min(r0 + w0, r0 + nr - 1), rb = min(r0 + w0 + 31, r0 + nr - 1);
-      kv_reach(t, a, span, c0 + ra / per, c0 + rb / per, &least, &most);
+      KvSpan own = span;
+      own.p0 = t.positions[c0 + ra / per];
+      own.p1 = t.positions[c0 + rb / per];
+      kv_reach(t, a, own, c0 + ra / per, c0 + rb / per, &least, &most);
     }
     const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16), s_at = lane_at + grp * (2 * FK), o_at = lane_at + kColO + grp * (64 * NV);
     // queries, a warp a row: scaled by a power of two, rounded to fp16, in the operand's layout (rows of 64 numbers, 16-byte pieces swizzled by the row).  A warp brings

@@ -329,7 +329,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     int least, most;
     {                                        // of the warp's rows
       const int ra = min(r0 + quarter * 32, r0 + nr - 1), rb = min(r0 + quarter * 32 + 31, r0 + nr - 1);
-      kv_reach(t, a, span, c0 + ra / per, c0 + rb / per, &least, &most);
+      KvSpan own = span;
+      own.p0 = t.positions[c0 + ra / per];
+      own.p1 = t.positions[c0 + rb / per];
+      kv_reach(t, a, own, c0 + ra / per, c0 + rb / per, &least, &most);
     }
     const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
     float* xchg = reinterpret_cast<float*>(smem + L::kOffX);
