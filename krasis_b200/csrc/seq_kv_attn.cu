@@ -597,7 +597,9 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
   if (a.pieces <= 1 || a.cluster) return;
   const int r0 = ((tok - c0) * per + hd % per) / a.rows * a.rows, nr = (int)min((long long)n * per - r0, (long long)a.rows);
   const KvSpan span = kv_span(c, t, s, c0 + r0 / per, c0 + (r0 + nr - 1) / per, a.window, a.first);
-  const int np = a.linear ? a.counts[(s * a.per_seq + r0 / a.rows) * c.G + hd / per] : min((span.groups() + a.piece - 1) / a.piece, a.pieces);
+  int length = a.piece;
+  if (a.rows > 16) kv_cut(c, t, a, s, &length);
+  const int np = a.linear ? a.counts[(s * a.per_seq + r0 / a.rows) * c.G + hd / per] : min((span.groups() + length - 1) / length, a.pieces);
   if (np <= 1) return;
   const long long p0 = row * a.pieces;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
@@ -671,9 +673,10 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
 // ------------------------------------------------------------------------------------------------ host
 // Rows per kv head (a sequence's tokens times the heads that share one) from which a sequence runs on the tensor cores' tiles of 128.
 constexpr int kTileFrom = 17;
+constexpr long long kWideWaves = 2;          // pieces for each SM, of such sequences (sixteen trees of 57 to 64 tokens: 2 530 us, 3 548, 4 571, 6 638)
 // How the sequences of one kind are cut: into tiles of rows, and the keys that a tile sees (in groups of 16) into pieces.
 struct KvPlan {
-  int least, most, rows, tiles, per_seq, piece, pieces, blocks;            // blocks: of the even cut, 0 for pieces of tiles
+  int least, most, rows, tiles, per_seq, piece, pieces, blocks;            // blocks: of the even cut (0 for pieces of tiles); of tiles on the tensor cores, pieces and all
   bool cluster;                              // the pieces of a tile are a cluster, which joins them itself
   size_t floats;                             // workspace
 };
@@ -714,11 +717,15 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
   if (p.tiles == 0) return p;
   p.per_seq = same ? p.tiles / step->S : 0;
   long long piece;
-  if (wide) {                                // one block an SM, two to four tiles of keys a piece at least
-    const long long want = 2ll * kb2::current_sms();
+  if (wide) {                                // one block an SM; a piece of at least four tiles of keys
+    const long long want = kWideWaves * kb2::current_sms();
     piece = std::max((work * cache->G + want - 1) / want, std::max(16ll, (top + 63) / 64));
-    piece = (piece + 7) / 8 * 8;
-    if ((long long)p.tiles * cache->G >= want) piece = (top + 7) / 8 * 8;
+    if ((long long)p.tiles * cache->G >= 2ll * kb2::current_sms() && same) piece = top;
+    p.piece = (int)std::max(piece, 8ll);
+    p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
+    for (int s = 0; s < step->S; ++s) p.blocks += tiles(s) ? (int)(tiles(s) * std::max(1ll, (seen(s) + p.piece - 1) / p.piece)) : 0;
+    p.floats = p.pieces > 1 ? ((size_t)step->T * H * p.pieces * (cache->dv + 2) + 3) / 4 * 4 : 0;
+    return p;
   } else {
     // Blocks of one length in whole waves, as the last wave takes as long as the others: the length whose waves, with what a block costs beside its keys (some 16 groups), end
     // first.  64 requests of 500 to 60000 rows (WAVES us, by four blocks a slot 284).
@@ -783,7 +790,7 @@ inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, 
   a.pieces = p.pieces;
   a.part_o = work;
   a.part_ml = work + (size_t)rows_total * p.pieces * dv;
-  a.linear = p.blocks > 0;
+  a.linear = p.blocks > 0 && p.rows <= 16;
   a.cluster = p.cluster;
   a.counts = reinterpret_cast<int*>(a.part_ml + 2 * (size_t)rows_total * p.pieces);
   return a;
@@ -857,7 +864,7 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   const KvAttn few = with_plan(a, p.few, (float*)work, t.T * H, c.dv), many = with_plan(a, p.many, (float*)work + p.few.floats, t.T * H, c.dv);
   const cudaStream_t st = (cudaStream_t)stream;
   if (p.many.tiles) {
-    if (int e = (kv_pairs(c.d, c.dv) ? kv_pair_attend : kv_tile_attend)(cache->fmt, c, t, many, p.many.tiles, st)) return e;
+    if (int e = (kv_pairs(c.d, c.dv) ? kv_pair_attend : kv_tile_attend)(cache->fmt, c, t, many, p.many.blocks, st)) return e;
   }
   if (p.few.tiles) {
     if (int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, few, p.few, st) : stream_sizes<KV_INT8>(c, t, few, p.few, st)) return e;

@@ -76,6 +76,48 @@ __device__ __forceinline__ void kv_reach(const KvStep& t, const KvAttn& a, const
   }
 }
 
+// Tiles on the tensor cores: into how many pieces of how many groups the keys of a sequence's tiles are cut.  All of a sequence's tiles alike, by what its tokens see together.
+__device__ __forceinline__ int kv_cut(const KvLayer& c, const KvStep& t, const KvAttn& a, int s, int* length) {
+  const int c0 = t.cu[s], c1 = t.cu[s + 1];
+  const int groups = c1 > c0 ? kv_span(c, t, s, c0, c1 - 1, a.window, a.first).groups() : 0;
+  const int n = max(min((groups + a.piece - 1) / a.piece, a.pieces), 1);
+  *length = max((groups + n - 1) / n, 1);
+  *length = (*length + 3) / 4 * 4;                                         // whole tiles of 64 keys
+  return n;
+}
+// The (sequence, tile, piece) number `at`, the pieces of one sequence behind those of the one before, a piece's tiles together (they read the same keys).  One warp; false
+// behind the last.
+__device__ __forceinline__ bool kv_find_piece(const KvLayer& c, const KvStep& t, const KvAttn& a, int per, int at, int* seq, int* tile, int* piece, int* length) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < t.S; s0 += 32) {
+    const int s = s0 + lane;
+    int tiles = 0, len = 1, n = 0;
+    if (s < t.S) {
+      const int have = (t.cu[s + 1] - t.cu[s]) * per;
+      tiles = have >= a.least && have <= a.most ? (have + a.rows - 1) / a.rows : 0;
+      if (tiles) n = tiles * (a.pieces > 1 ? kv_cut(c, t, a, s, &len) : 1);
+    }
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > at);
+    if (hit) {
+      const int l = __ffs(hit) - 1, of = __shfl_sync(0xffffffffu, tiles, l), i = at - before - __shfl_sync(0xffffffffu, upto - n, l);
+      *length = __shfl_sync(0xffffffffu, len, l);
+      *seq = s0 + l;
+      *piece = i / of;
+      *tile = i - *piece * of;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
+}
+
 // 2^e that brings a row's largest magnitude (its bits: top) below 2^15, and 2^-e.  Of a row of smallest numbers or one that is not finite both stay within fp32.
 __device__ __forceinline__ void kv_row_scale(uint32_t top, float* up, float* down) {
   const int e = min(max(141 - (int)(top >> 23), -113), 100);

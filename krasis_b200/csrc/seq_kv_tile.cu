@@ -103,13 +103,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
 
   // which tile, and what its rows see: the same in every warp
   const int per = a.H / c.G, head = blockIdx.y;
-  int s = 0, tile = 0;
+  int s = 0, tile = 0, z = 0, length = 0x7FFFFFFF;
   bool in = true;
-  if (a.per_seq) {
+  if (a.per_seq && a.pieces == 1) {
     s = blockIdx.x / a.per_seq;
     tile = blockIdx.x - s * a.per_seq;
   } else {
-    in = kv_find_tile(t, per, kRows, a.least, a.most, blockIdx.x, &s, &tile);
+    in = kv_find_piece(c, t, a, per, blockIdx.x, &s, &tile, &z, &length);
   }
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * kRows, nr = in ? (int)min((long long)n * per - r0, (long long)kRows) : 0;
   int u0 = 0, u1 = 0, np = 0, t0 = c0, t1 = c0;
@@ -118,11 +118,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     t0 = c0 + r0 / per;
     t1 = c0 + (r0 + nr - 1) / per;
     span = kv_span(c, t, s, t0, t1, a.window, a.first);
-    np = min((span.groups() + a.piece - 1) / a.piece, a.pieces);
-    u0 = blockIdx.z * a.piece;
-    u1 = min(span.groups(), u0 + a.piece);
+    np = a.pieces == 1 ? 1 : min((span.groups() + length - 1) / length, a.pieces);
+    u0 = a.pieces == 1 ? 0 : z * length;
+    u1 = a.pieces == 1 ? span.groups() : min(span.groups(), u0 + length);
   }
-  const bool work = nr > 0 && (blockIdx.z == 0 || (int)blockIdx.z < np);   // piece 0 of a tile that sees nothing writes its zeros
+  const bool work = nr > 0 && (z == 0 || z < np);   // piece 0 of a tile that sees nothing writes its zeros
   const int n_tiles = work ? max(0, (u1 - u0 + GT - 1) / GT) : 0;
 
   // queries, 8 rows a warp: scaled by a power of two, rounded to fp16, in the operand's layout (rows of 64 numbers, 16-byte pieces swizzled by the row)
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     if (n_tiles >= 2) pv_wait(n_tiles - 2);
     pv_wait(n_tiles - 1);
     const int hd = head * per + rr % per;
-    const long long orow = (long long)tok * a.H + hd, part = orow * a.pieces + blockIdx.z;
+    const long long orow = (long long)tok * a.H + hd, part = orow * a.pieces + z;
     const bool whole = np <= 1;
     if (whole && live && a.sinks != nullptr && m != -INFINITY) l += ex2(fmaf(a.sinks[hd], kLog2e, -m));
     const float by = whole ? (l == 0.f ? 0.f : ref / l) : ref;
@@ -497,7 +497,7 @@ int launch(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaSt
   using L = TileShape<NC, NV>;
   SEQ_CUDA((kb2::allow_smem<kv_tile_kernel<FMT, NC, NV>>(L::kTotal)));
   auto kern = kv_tile_kernel<FMT, NC, NV>;
-  kb2::launch_pdl(kern, dim3(tiles, c.G, a.pieces), kThreads, L::kTotal, st, c, t, a);
+  kb2::launch_pdl(kern, dim3(tiles, c.G), kThreads, L::kTotal, st, c, t, a);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }
