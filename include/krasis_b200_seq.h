@@ -334,12 +334,13 @@ typedef struct {
 /* The tables of a step (see above; layout and replayed as in kb2_seq_attention_step).  For drafted tokens rows [T] says where a token's key and value lie, behind
  * the committed rows of its sequence in the order of the tokens, positions holds first row + depth, and bits [T][words] which tokens of its sequence a token sees: bit i
  * is set for token i if that is the token itself or one of its ancestors, which come before it.  rows and bits null: positions and order of a portion.
+ * tiles_from: from how many rows per kv head (tokens times H / G) a sequence's attention runs on the tensor cores' tiles where its result is bf16; 0: the library's rule.
  * Tokens behind cu[S] are left alone by every call below.  Pages that are not in the pool hold nothing: no row is written there or seen. */
 typedef struct {
   const int *positions, *seq_of, *cu, *pages, *rows;
   const unsigned* bits;
   const int* layout;
-  int words, T, S, max_pages, replayed, device;
+  int words, T, S, max_pages, replayed, device, tiles_from;
 } kb2_seq_kv_step;
 /* The step's keys k [T][G][d] and values v [T][G][dv] (dt; numbers of a head side by side, ld* and h* numbers from token to token and head to head) into the pages. */
 KB2SEQ_API int kb2_seq_kv_write(const kb2_seq_kv_cache* cache, int layer, const kb2_seq_kv_step* step, const void* k, long long ldk, long long hk, const void* v,

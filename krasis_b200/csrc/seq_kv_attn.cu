@@ -671,8 +671,10 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// Rows per kv head (a sequence's tokens times the heads that share one) from which a sequence runs on the tensor cores' tiles of 128.
-constexpr int kTileFrom = 17;
+// Rows per kv head (a sequence's tokens times the heads that share one) from which a sequence may run on the tensor cores' tiles.  Fewer are faster on the kernel for few rows
+// (us there / on tiles, 16 / 2 heads of 128, int8: 24 rows after 2000 keys 13 / 20, eight sequences of 32 rows after 16000 51 / 62); more are where there is enough to do to
+// make up for the tiles' longer start (64 rows after 2000 14 / 21, eight of 64 after 16000 81 / 65; 128 rows after 2000 17 / 23, after 16000 33 / 27).
+constexpr int kTileFrom = 48;
 constexpr long long kWideWaves = 2;          // pieces for each SM, of such sequences (sixteen trees of 57 to 64 tokens: 2 530 us, 3 548, 4 571, 6 638)
 // How the sequences of one kind are cut: into tiles of rows, and the keys that a tile sees (in groups of 16) into pieces.
 struct KvPlan {
@@ -775,10 +777,27 @@ struct KvPlans {
   size_t bytes() const { return (few.floats + many.floats) * 4; }
 };
 KvPlans kv_plans(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int dt_out) {
-  const int split = dt_out ? kTileFrom - 1 : 0x7FFFFFFF;                   // fp32 results carry 22 bits: the tiles have 11
+  int split = 0x7FFFFFFF;                    // fp32 results carry 22 bits: the tiles have 11
   KvPlans p{};
+  if (dt_out && step->tiles_from > 0) {
+    split = step->tiles_from - 1;
+  } else if (dt_out) {
+    long long few = 0, many = 0;             // groups of 16 keys times tiles, either way
+    const int per = H / cache->G, rows = kv_pairs(cache->d, cache->dv) ? 256 : 128;
+    for (int s = 0; s < step->S; ++s) {
+      const int* l = step->layout + 4 * s;
+      const long long r = (long long)l[1] * per, end = step->replayed ? (long long)step->max_pages * cache->page_size : (long long)l[2] + l[1];
+      if (r < kTileFrom) continue;
+      const long long g = groups_seen(end - l[1], l[1], window, first) * cache->G;
+      few += (r + 15) / 16 * g;
+      many += (r + rows - 1) / rows * g;
+    }
+    // 0.27 us a group on one of two blocks an SM, 0.3 on the one of the tiles, and 8 us
+    const long long sms = kb2::current_sms();
+    if (few * 27 > 2 * (many * 30 + 800 * sms)) split = kTileFrom - 1;
+  }
   p.few = kv_plan(cache, step, H, window, first, 1, split, false);
-  if (dt_out) p.many = kv_plan(cache, step, H, window, first, split + 1, 0x7FFFFFFF, true);
+  if (split < 0x7FFFFFFF) p.many = kv_plan(cache, step, H, window, first, split + 1, 0x7FFFFFFF, true);
   return p;
 }
 inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, int dv) {

@@ -461,7 +461,10 @@ class KvCacheArgs(C.Structure):
 
 class KvStepArgs(C.Structure):
     """kb2_seq_kv_step."""
-    _fields_ = [(n, _P) for n in ("positions", "seq_of", "cu", "pages", "rows", "bits", "layout")] + [(n, _I) for n in ("words", "T", "S", "max_pages", "replayed", "device")]
+    _fields_ = [(n, _P) for n in ("positions", "seq_of", "cu", "pages", "rows", "bits", "layout")] + [(n, _I) for n in ("words", "T", "S", "max_pages", "replayed", "device", "tiles_from")]
+
+
+KV_TILES_FROM = 0      # rows per kv head from which attention over the 8-bit cache runs on the tensor cores' tiles (bf16 results), for tables made from now on; 0: by size
 
 
 class DraftTables(StepTables):
@@ -511,7 +514,7 @@ def _kv_step(tb: StepTables):
     """The tables as the C interface takes them, and workspace sizes; made once per step, and again if the step's layout is set anew."""
     rows, bits = getattr(tb, "rows", None), getattr(tb, "bits", None)
     a = KvStepArgs(tb.positions.data_ptr(), tb.seq_of.data_ptr(), tb.cu.data_ptr(), tb.pages.data_ptr(), _ptr(rows), _ptr(bits), tb.layout_ptr,
-                   tb.words if bits is not None else 0, tb.T, tb.S, tb.max_pages, int(tb.replayed), tb.buf.get_device())
+                   tb.words if bits is not None else 0, tb.T, tb.S, tb.max_pages, int(tb.replayed), tb.buf.get_device(), KV_TILES_FROM)
     tb._kv = kept = (C.addressof(a), tb._layout_host, a.device, {}, a)
     return kept
 

@@ -41,6 +41,19 @@ def _step(lens, page_size, seed=0, spare=2, parents=None):
     return (ops.DraftTables if parents else ops.StepTables)(entries, "cuda"), seqs, sum(need) + spare
 
 
+@pytest.fixture
+def forms(monkeypatch):
+    """Runs a call by the library's choice of kernels and with every sequence of more than 16 rows per kv head on the tiles of the tensor cores (bf16 results)."""
+    from krasis_b200 import seqops as ops
+
+    def both(tb, call):
+        for rows in (0, 17):
+            monkeypatch.setattr(ops, "KV_TILES_FROM", rows)
+            tb._kv = None
+            yield call()
+    return both
+
+
 def _check(got, q, cache, seqs, layer=0, known=None, **kw):
     want, *sizes = known = known or kv_plain.attention(q, cache, layer, seqs, **kw)
     keys = max(n + s for n, s, _, _ in seqs)
@@ -151,7 +164,7 @@ STEPS = {"one": [(1, 0)], "few": [(1, 63), (1, 64), (1, 300)], "ragged": [(1, 0)
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("H,G,d,dv", SIZES)
 @pytest.mark.parametrize("step", sorted(STEPS))
-def test_attention(fmt, H, G, d, dv, step):
+def test_attention(fmt, H, G, d, dv, step, forms):
     from krasis_b200 import seqops as ops
     i = SIZES.index((H, G, d, dv)) + sorted(STEPS).index(step)
     page_size = (64, 16, 128)[i % 3]
@@ -161,22 +174,23 @@ def test_attention(fmt, H, G, d, dv, step):
         for dq in (F32, BF):
             q, known = torch.randn(tb.T, H, d, generator=_gen(i)).to(dq).cuda(), None
             for do in (F32, BF):
-                got = ops.kv_attn(q, tb, c, 1, d ** -0.5, window=window, first=first, dtype=do)
-                known = _check(got, q, c, seqs, 1, known=known, scale=d ** -0.5, window=window, first=first)
+                for got in forms(tb, lambda: ops.kv_attn(q, tb, c, 1, d ** -0.5, window=window, first=first, dtype=do)):
+                    known = _check(got, q, c, seqs, 1, known=known, scale=d ** -0.5, window=window, first=first)
 
 
 @pytest.mark.parametrize("window,first", [(1, 0), (1, 1), (1, 64), (16, 16), (15, 17), (5000, 3), (2, 100000)])
-def test_windows(window, first):
+def test_windows(window, first, forms):
     from krasis_b200 import seqops as ops
     tb, seqs, pages = _step([(1, 0), (50, 0), (1, 31), (1, 500), (20, 90)], 16, 5)
     c = _cache(2, 64, 64, pages, "int8", 16)
     q = torch.randn(tb.T, 6, 64, generator=_gen(6)).cuda()
+    known = None
     for do in (BF, F32):
-        got = ops.kv_attn(q, tb, c, 0, 0.125, window=window, first=first, dtype=do)
-        _check(got, q, c, seqs, scale=0.125, window=window, first=first)
+        for got in forms(tb, lambda: ops.kv_attn(q, tb, c, 0, 0.125, window=window, first=first, dtype=do)):
+            known = _check(got, q, c, seqs, known=known, scale=0.125, window=window, first=first)
 
 
-def test_sinks_and_scales():
+def test_sinks_and_scales(forms):
     """Scores far apart, a negative scale, sinks below and above all scores, rows of values whose scales are 1e8 apart."""
     from krasis_b200 import seqops as ops
     tb, seqs, pages = _step([(3, 400), (1, 3000)], 64, 7)
@@ -188,11 +202,71 @@ def test_sinks_and_scales():
         for s in (None, sinks):
             got = ops.kv_attn(q, tb, c, 0, scale, sinks=s, dtype=F32)
             _check(got, q, c, seqs, scale=scale, sinks=s)
+    # on tiles a value row keeps its bits down to 2^-21 of its tile's largest scale
+    tb, seqs, pages = _step([(13, 400), (40, 21), (1, 3000)], 64, 7)
+    c = _cache(2, 128, 128, pages, "int8")
+    c.v_scale[0, :, 0] *= torch.exp2(torch.randint(-6, 6, c.v_scale[0, :, 0].shape, generator=_gen(8)).float()).cuda()
+    q = (torch.randn(tb.T, 8, 128, generator=_gen(9)) * torch.exp2(torch.randint(-6, 3, (tb.T, 8, 1), generator=_gen(10)).float())).cuda()
+    for scale in (0.09, -0.09, 0.0):
+        for s in (None, sinks):
+            known = None
+            for got in forms(tb, lambda: ops.kv_attn(q, tb, c, 0, scale, sinks=s, dtype=BF)):
+                known = _check(got, q, c, seqs, known=known, scale=scale, sinks=s)
+
+
+@pytest.mark.parametrize("H,G,d,dv", [(16, 2, 128, 128), (8, 2, 256, 256), (14, 2, 96, 96)])
+def test_one_key_far_above_the_others(H, G, d, dv, forms):
+    """Keys whose scores lie 100 powers of e above all others come late, twice: what was summed before counts for nothing then."""
+    from krasis_b200 import seqops as ops
+    tb, seqs, pages = _step([(20, 1000), (1, 700)], 64, 29)
+    c = _cache(G, d, dv, pages, "int8")
+    q = torch.randn(tb.T, H, d, generator=_gen(30)).cuda()
+    for s, (n, start, pl, _) in enumerate(seqs):
+        t = 0 if s == 0 else 20
+        for g in range(G):
+            for j, gain in ((300, 60.0), (start - 70, 100.0)):
+                x = q[t, g * (H // G)] * gain / float(q[t, g * (H // G)].square().sum()) / d ** -0.5
+                top = float(x.abs().max())
+                c.k[0, pl[j // 64], g, j % 64] = torch.round(x * 127 / top).to(torch.int8)
+                c.k_scale[0, pl[j // 64], g, j % 64] = top / 127
+    known = None
+    for do in (F32, BF):
+        for got in forms(tb, lambda: ops.kv_attn(q, tb, c, 0, d ** -0.5, dtype=do)):
+            known = _check(got, q, c, seqs, known=known, scale=d ** -0.5)
+
+
+@pytest.mark.parametrize("lens,H,G,d", [([(1, 30000), (1, 0), (1, 17), (1, 4000), (1, 900)], 16, 8, 64), ([(1, 20000 + 97 * i) for i in range(3)], 12, 12, 128),
+                                        ([(2, 7000)] * 5, 16, 4, 256), ([(1, 50000)], 64, 4, 128), ([(1, 9000 * (i % 3)) for i in range(40)], 7, 7, 128)])
+def test_many_keys(lens, H, G, d):
+    """Requests with so many keys that these are cut evenly over the GPU, wherever the ends lie in the requests."""
+    from krasis_b200 import seqops as ops
+    tb, seqs, pages = _step(lens, 64, 3)
+    c = _cache(G, d, d, pages, "int8")
+    q = torch.randn(tb.T, H, d, generator=_gen(1)).cuda()
+    for window, first in ((None, 0), (8000, 5)):
+        known = None
+        for do in (F32, BF):
+            known = _check(ops.kv_attn(q, tb, c, 0, d ** -0.5, dtype=do, window=window, first=first), q, c, seqs, known=known, scale=d ** -0.5, window=window, first=first)
+
+
+def test_a_row_is_the_same_however_it_is_cut(monkeypatch):
+    """One request alone, beside many others, as a single token and within a portion: the same numbers up to roundings."""
+    from krasis_b200 import seqops as ops
+    lens = [(1, 3000)] + [(1, 100 * i) for i in range(30)] + [(70, 900)]
+    tb, seqs, pages = _step(lens, 64, 31)
+    c = _cache(2, 128, 128, pages, "e4m3")
+    q = torch.randn(tb.T, 16, 128, generator=_gen(32)).cuda()
+    whole = ops.kv_attn(q, tb, c, 0, 0.09, dtype=F32)
+    for i in (0, 7, 31):
+        n, start, pl, _ = seqs[i]
+        at = sum(x for x, _ in lens[:i])
+        alone = ops.kv_attn(q[at:at + n], ops.StepTables([([0] * n, start, 0, pl)], "cuda"), c, 0, 0.09, dtype=F32)
+        assert float((alone - whole[at:at + n]).abs().max()) < 1e-5 * float(whole.abs().max())
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("lens,H,G,d", [([(1, 130), (40, 21), (1, 700)], 8, 2, 64), ([(150, 77)], 16, 2, 128)])
-def test_rows_that_are_not_numbers(fmt, lens, H, G, d):
+def test_rows_that_are_not_numbers(fmt, lens, H, G, d, forms):
     """A token with a NaN in its key (or an infinity in its value) makes NaN for the tokens and heads that see it and for no others."""
     from krasis_b200 import seqops as ops
     tb, seqs, pages = _step(lens, 16, 11)
@@ -207,14 +281,14 @@ def test_rows_that_are_not_numbers(fmt, lens, H, G, d):
         q = torch.randn(tb.T, H, d, generator=g).cuda()
         for window, first in ((None, 0), (9, 2)):
             for do in (BF, F32):
-                got = ops.kv_attn(q, tb, c, 0, 0.1, window=window, first=first, dtype=do).cpu()
                 see = torch.zeros(tb.T, H, dtype=torch.bool)
                 last = sum(n for n, _ in lens[:s + 1]) if window is None else min(at + window, sum(n for n, _ in lens[:s + 1]))
                 see[at:last, H // G:2 * (H // G)] = True
-                assert torch.equal(torch.isnan(got).all(-1), see) and bool(torch.isfinite(got[~see]).all())
+                for got in forms(tb, lambda: ops.kv_attn(q, tb, c, 0, 0.1, window=window, first=first, dtype=do).cpu()):
+                    assert torch.equal(torch.isnan(got).all(-1), see) and bool(torch.isfinite(got[~see]).all())
 
 
-def test_what_nobody_sees_changes_nothing():
+def test_what_nobody_sees_changes_nothing(forms):
     """Rows behind the sequences, ahead of the windows and in strange pages hold codes of another life and NaN scales: the bits stay."""
     from krasis_b200 import seqops as ops
     lens = [(1, 777), (30, 200), (1, 3), (200, 50)]
@@ -222,7 +296,7 @@ def test_what_nobody_sees_changes_nothing():
     for fmt in ("e4m3", "int8"):
         c = _cache(2, 128, 128, pages, fmt, seed=1)
         q = torch.randn(tb.T, 16, 128, generator=_gen(14)).cuda()
-        calls = [lambda do=do: ops.kv_attn(q, tb, c, 0, 0.09, window=60, first=5, dtype=do) for do in (BF, F32)]
+        calls = [lambda do=do: list(forms(tb, lambda: ops.kv_attn(q, tb, c, 0, 0.09, window=60, first=5, dtype=do))) for do in (BF, F32)]
         before = [f() for f in calls]
         mark = torch.ones(pages, 64, dtype=torch.bool)
         for n, start, pl, _ in seqs:
@@ -233,7 +307,7 @@ def test_what_nobody_sees_changes_nothing():
         for sc in (c.k_scale, c.v_scale):
             sc[0].transpose(1, 2)[mark] = float("nan")
         for a, f in zip(before, calls):
-            assert torch.equal(a, f())
+            assert all(torch.equal(x, y) for x, y in zip(a, f()))
 
 
 def test_pages_outside_the_pool():
@@ -316,7 +390,7 @@ def _tree(n, seed, span):
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("H,G,d,dv", [(16, 2, 128, 128), (4, 4, 64, 64), (24, 8, 192, 128), (32, 1, 128, 256), (6, 2, 256, 256)])
 @pytest.mark.parametrize("lens", [[(1, 0)], [(16, 700)], [(5, 0), (33, 64), (1, 500), (64, 90)], [(70, 1000), (300, 40)]])
-def test_tree(fmt, H, G, d, dv, lens):
+def test_tree(fmt, H, G, d, dv, lens, forms):
     from krasis_b200 import seqops as ops
     i = H + len(lens)
     tb, seqs, pages = _step(lens, (64, 16)[i % 2], i, parents=[_tree(n, i + n, 4) for n, _ in lens])
@@ -324,8 +398,9 @@ def test_tree(fmt, H, G, d, dv, lens):
     for window, first in ((None, 0), (30, 7), (2, 0)):
         for dq, do in ((F32, BF), (BF, BF), (F32, F32)):
             q = torch.randn(tb.T, H, d, generator=_gen(i)).to(dq).cuda()
-            got = ops.kv_tree_attn(q, tb, c, 1, d ** -0.5, window=window, first=first, dtype=do)
-            _check(got, q, c, seqs, 1, scale=d ** -0.5, window=window, first=first)
+            known = None
+            for got in forms(tb, lambda: ops.kv_tree_attn(q, tb, c, 1, d ** -0.5, window=window, first=first, dtype=do)):
+                known = _check(got, q, c, seqs, 1, known=known, scale=d ** -0.5, window=window, first=first)
 
 
 def test_tree_tables():
@@ -474,6 +549,73 @@ def test_captured_decode():
             eager = ops.kv_attn(q, ops.StepTables([([0], s, i, lists[i]) for i, s in enumerate(starts)], "cuda"), c, 0, 0.09, window=40, first=2, dtype=F32)
         other.synchronize()
         _check(eager, q, c, seqs, scale=0.09, window=40, first=2)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_captured_portions(tree, monkeypatch):
+    """A captured step of portions or trees (tiles of the tensor cores, pieces and their join) runs again with later positions."""
+    from krasis_b200 import seqops as ops
+    from krasis_b200.graphs import capture
+    monkeypatch.setattr(ops, "KV_TILES_FROM", 17)
+    H, G, d, ns = 8, 2, 128, (24, 9)
+    c, g = _cache(G, d, d, 64, "int8", 16), _gen(33)
+    pages = torch.randperm(64, generator=g).tolist()
+    lists, T = [pages[0:32], pages[32:64]], sum(ns)
+    q = torch.randn(T, H, d, generator=g).cuda()
+    parents = [_tree(n, n, 3) for n in ns]
+    buf = torch.zeros(3 * T + 3 + 2 + 2 * 32, dtype=torch.int32, device="cuda")
+    draft = torch.zeros(2 * T, dtype=torch.int32, device="cuda")
+
+    def tables(starts):
+        e = [([0] * n, s, i, lists[i]) for i, (n, s) in enumerate(zip(ns, starts))]
+        return ops.DraftTables([x + (p,) for x, p in zip(e, parents)], "cuda", device_buf=buf, draft_buf=draft) if tree else ops.StepTables(e, "cuda", device_buf=buf)
+    call = ops.kv_tree_attn if tree else ops.kv_attn
+    tb = tables((3, 40))
+    graph, out = capture(lambda: call(q, tb, c, 0, 0.09, window=200, first=3, dtype=BF), "cuda")
+    for starts in ((3, 40), (480, 0), (0, 500)):
+        kept = tables(starts)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, q, c, [(n, s, lists[i], parents[i] if tree else None) for i, (n, s) in enumerate(zip(ns, starts))], scale=0.09, window=200, first=3)
+        del kept
+
+
+def test_captured_many_keys():
+    """A captured decode step whose page lists have room for many keys: cut evenly by whatever the positions are when it runs."""
+    from krasis_b200 import seqops as ops
+    from krasis_b200.graphs import capture
+    H, G, d, S, room = 16, 8, 64, 2, 400
+    c, g = _cache(G, d, d, 2 * room, "e4m3", 64), _gen(34)
+    lists = [list(range(0, room)), list(range(2 * room - 1, room - 1, -1))]
+    q = torch.randn(S, H, d, generator=g).cuda()
+    buf = torch.zeros(3 * S + S + 1 + S + S * room, dtype=torch.int32, device="cuda")
+    tables = lambda starts: ops.StepTables([([0], s, i, lists[i]) for i, s in enumerate(starts)], "cuda", device_buf=buf)  # noqa: E731
+    tb = tables((25000, 25000))
+    graph, out = capture(lambda: ops.kv_attn(q, tb, c, 0, 0.1, dtype=F32), "cuda")
+    for starts in ((25000, 25000), (0, 25599), (0, 0), (130, 7000)):
+        kept = tables(starts)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, q, c, [(1, s, lists[i], None) for i, s in enumerate(starts)], scale=0.1)
+        del kept
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with its own results and workspaces, and tables that both read."""
+    from krasis_b200 import seqops as ops
+    tb, seqs, pages = _step([(1, 6000), (1, 90), (60, 2000)], 64, 35)
+    c = _cache(2, 128, 128, pages, "int8")
+    q = torch.randn(tb.T, 16, 128, generator=_gen(36)).cuda()
+    want = [ops.kv_attn(q * f, tb, c, 0, 0.09, dtype=do) for f, do in ((1.0, BF), (0.5, F32))]
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for i, (s, f, do) in enumerate(zip(streams, (1.0, 0.5), (BF, F32))):
+            with torch.cuda.stream(s):
+                got[i].append(ops.kv_attn(q * f, tb, c, 0, 0.09, dtype=do))
+    torch.cuda.synchronize()
+    for w, xs in zip(want, got):
+        assert all(torch.equal(w, x) for x in xs)
 
 
 def test_same_call_same_bits():

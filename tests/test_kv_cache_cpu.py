@@ -98,7 +98,7 @@ def test_draft_tables():
 def _structs(**kw):
     layout = np.array(kw.pop("layout", [[0, 2, 3, 1]]), dtype=np.int32)
     c = dict(k=4096, v=4096, k_scale=4096, v_scale=4096, layers=2, pages=6, page_size=16, G=2, d=64, dv=32, fmt=1)
-    s = dict(positions=4096, seq_of=4096, cu=4096, pages=4096, rows=None, bits=None, layout=layout.ctypes.data, words=0, T=2, S=len(layout), max_pages=1, replayed=0, device=0)
+    s = dict(positions=4096, seq_of=4096, cu=4096, pages=4096, rows=None, bits=None, layout=layout.ctypes.data, words=0, T=2, S=len(layout), max_pages=1, replayed=0, device=0, tiles_from=0)
     step_pages = kw.pop("step_pages", 4096)
     for k, v in kw.items():
         (c if k in c else s)[k] = v
