@@ -350,7 +350,7 @@ KB2SEQ_API int kb2_seq_kv_read(const kb2_seq_kv_cache* cache, int layer, const k
                                void* stream);
 /* out [T][H][dv] in dt_out: softmax(scale q k^T) v over the rows j <= pos of a token's sequence with pos - j < window (0: no window) or j < first; a drafted token sees
  * the committed rows by that rule and of the drafted ones its ancestors and itself, whose place in the rule is their position.  Nothing to see: zeros.
- * sinks [H] (may be null): the softmax denominator of head h also holds exp(sinks[h]).  The step's own rows have been written before.  q [T][H][d] in dt_q as k above; out and work on 16 bytes. */
+ * scale is finite.  sinks [H] (may be null): the softmax denominator of head h also holds exp(sinks[h]).  The step's own rows have been written before.  q [T][H][d] in dt_q as k above; out and work on 16 bytes. */
 KB2SEQ_API size_t kb2_seq_kv_attn_workspace(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int dt_out);
 KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const kb2_seq_kv_step* step, const void* q, int dt_q, long long ldq, long long hq, int H,
                                float scale, int window, int first, const float* sinks, void* out, int dt_out, void* work, size_t work_bytes, void* stream);

@@ -44,7 +44,8 @@ __device__ __forceinline__ uint32_t kv_codes4(const float* x, float s, float inv
 }
 
 // A lane has eight numbers of a row, so a row has n / 8 lanes (of a power of two of them), and a warp 32 / lanes rows at a time; kWriteRows times that are asked for at once.
-// What bounds it: bytes (8192 tokens of 4 + 4 heads of 128 in bf16: 25 MB, TIME us).  VEC: every eight numbers lie on 16 bytes.
+// What bounds it: 8192 tokens of 4 + 4 heads of 128 in bf16 (25 MB, 3.9 us at the copy rate) take 12.6 us as int8, 9.1 without making the codes: two rounds of loads a thread
+// (rows and tables, then the page list) and the codes' arithmetic.  Four rows a thread 13.3, one 12.7.  VEC: every eight numbers lie on 16 bytes.
 constexpr int kWriteRows = 2;
 template <int FMT, bool F32, bool VEC>
 __global__ void __launch_bounds__(256) kv_write_kernel(KvLayer c, KvStep t, const void* __restrict__ k, long long ldk, long long hk, const void* __restrict__ v,
@@ -142,6 +143,7 @@ __device__ __forceinline__ void kv_unpack4(uint32_t w, float (&f)[4]) {
 }
 
 // Rows first .. first + count - 1 of sequence s -> [count][G][d] and [count][G][dv]; a thread has 16 codes, AHEAD times.
+// What bounds it: bytes, two thirds of them written (40001 rows of 4 + 4 heads of 128 to bf16: 124 MB in 24.5 us, 5.1 TB/s).
 template <int FMT, bool F32, int AHEAD>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvLayer c, KvStep t, int s, int first, int count, void* __restrict__ ko, void* __restrict__ vo) {
   kb2::pdl_enter(ko, vo);
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvLayer c, KvStep t, int s
 // ------------------------------------------------------------------------------------------------ the accepted path
 // Block (sequence, kKeepLayers layers): row base + path[i] -> row base + i.  A path rises, so path[i] >= i: what a thread writes at i no later step reads, and a thread
 // keeps its 16 bytes of every row (eight rows on their way at once), so it has read whatever it overwrites.  What bounds it: the chain of tables ahead of the rows, so
-// a block has work for all its threads (64 paths of 8 in 48 layers: a layer a block 22 us, four TIME).
+// a block has work for all its threads (64 paths of 8 in 48 layers: a layer a block 22 us, four 15.5, eight 13.7; 7.9 at the copy rate).
 constexpr int kKeepMost = 512, kKeepLayers = 8;
 __global__ void __launch_bounds__(256) kv_keep_kernel(KvLayer c, int layers, KvStep t, const int* __restrict__ path, int P) {
   __shared__ long long rows[2][kKeepMost];

@@ -124,6 +124,8 @@ inline int kv_args(const char* name, const kb2_seq_kv_cache* cache, int layer, c
   if ((long long)cache->pages * cache->G * (ps / kKvGroup) > 0x7FFFFFFFll) return failf(KB2SEQ_ERR_VALUE, "%s: too many rows in a layer", name);
   for (int s = 0; s < step->S; ++s) {        // ahead of the first launch: the kernels go by the page lists alone
     const int* l = step->layout + 4 * s;
+    if (step->bits && l[1] > 32ll * step->words)
+      return failf(KB2SEQ_ERR_VALUE, "%s: sequence %d: %d words of bits for %d drafted tokens", name, s, step->words, l[1]);
     if (l[1] > 0 && (long long)l[2] + l[1] > (long long)l[3] * ps)
       return failf(KB2SEQ_ERR_RANGE, "%s: sequence %d: %d pages of %d rows do not hold %lld positions", name, s, l[3], ps, (long long)l[2] + l[1]);
   }

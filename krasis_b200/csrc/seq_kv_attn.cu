@@ -7,12 +7,17 @@
 // so that S's accumulators are P's fragments where they stand, without a shuffle.  Dimensions and keys may be summed in any order, so a lane takes 16 neighbouring
 // bytes of a key row and 8 or 16 of a value row for its fragments: everything a lane multiplies it has copied itself (cp.async into its own slots), no warp waits for
 // another, and no byte is read from shared memory twice.
-// What bounds it: the cache's bytes.  16 keys of 128 + 128 dimensions are 4.2 KB a warp and iteration; 3 stages x 16 warps an SM keep 200 KB on the way.
+// What bounds it: the cache's bytes.  16 keys of 128 + 128 dimensions are 4.2 KB a warp and iteration; 3 stages x 16 warps an SM keep 200 KB on the way.  64 requests of 500 to
+// 60000 rows, 64 / 4 heads of 128, int8 (862 MB, 131 us at the copy rate): 216 us, the copies alone 170 or so; 32 / 4 heads (811 MB) 176, the copies alone 162.  What is left
+// beside them is arithmetic on codes (a conversion is a half-rate instruction for two codes), which 16 query rows cannot hide behind four warps a scheduler.
+// Tried and left out: int8 keys as whole numbers (mma.s8 on queries of 15 bits: no conversion, no faster), the next keys' scores beside these keys' products (no faster).
 //
 // Rounding.  q: a row is scaled by a power of two to the top of fp16's range, bf16 numbers keep their 8 bits, fp32 ones are rounded to 11 (PARTS 1) or split into two
 // fp16 numbers with 22 together (PARTS 2, for fp32 results).  Scores, maxima and sums are fp32; the key's scale multiplies the fp32 score.  The weight times the value's
 // scale is rounded to fp16, relative to a reference R of its own that follows the largest such product (2^6 to 2^15 of it), so that small scales or weights do not
 // fall out of fp16's range: 11 bits, or 22 with PARTS 2, down to 2^-30 of the largest.
+#include <cmath>
+
 #include "seq_kv_attn.cuh"
 
 namespace kb2seq {
@@ -730,7 +735,7 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
     return p;
   } else {
     // Blocks of one length in whole waves, as the last wave takes as long as the others: the length whose waves, with what a block costs beside its keys (some 16 groups), end
-    // first.  64 requests of 500 to 60000 rows (WAVES us, by four blocks a slot 284).
+    // first.  A mixed fp32 step on heads of 256: 73 -> 61 us.
     const long long slots = (long long)kb2::current_sms() * (cache->d <= 128 && cache->dv <= 128 ? 2 : 1);
     const long long even = (work + (long long)p.tiles * kPieceCost) * cache->G / slots;
     if (p.per_seq && p.tiles <= kMostTiles && work * cache->G >= slots * kPieceCost) {
@@ -738,7 +743,7 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
       // a captured step's keys may come to lie in one sequence: the kernel makes its pieces no more than this
       p.pieces = (int)(step->replayed ? std::max(34ll, (top + kPieceCost) / kSMostGroups + 2) : (top + kPieceCost) / std::min<long long>(std::max(even, 8ll), kSMostGroups) + 2);
     }
-    // Few keys: up to eight blocks a tile meet in shared memory, without a second launch and a workspace (four requests of 1028 visible rows: TIME us, with a join 9.8);
+    // Few keys: up to eight blocks a tile meet in shared memory, without a second launch and a workspace (four requests of 1028 visible rows: 9.0 us, with a join 9.8; 11.0 against 15 with what the host does);
     // more than that, a warp would have too many keys one after another (6144 a tile).
     if (!p.blocks && top > kSWarps && top <= 48 * kClusterMost && (long long)p.tiles * cache->G * kClusterMost <= slots) {
       p.cluster = true;
@@ -848,6 +853,7 @@ extern "C" {
 
 KB2SEQ_API size_t kb2_seq_kv_attn_workspace(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int dt_out) {
   if (!cache || !step || !step->layout || cache->G < 1 || H < cache->G || bad_dt(dt_out)) return 0;
+  OnDevice on(step->device);
   return kv_plans(cache, step, H, window > 0 ? std::min(window, kKvNoWindow) : kKvNoWindow, first, dt_out).bytes();
 }
 
@@ -856,7 +862,7 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   KvLayer c;
   KvStep t;
   if (int e = kv_args("kv_attn", cache, layer, step, &c, &t)) return e;
-  if (!q || !out || ((uintptr_t)out & 15) || bad_dt(dt_q) || bad_dt(dt_out) || H < c.G || H % c.G || window < 0 || first < 0)
+  if (!q || !out || ((uintptr_t)out & 15) || bad_dt(dt_q) || bad_dt(dt_out) || H < c.G || H % c.G || window < 0 || first < 0 || !std::isfinite(scale))
     return failf(KB2SEQ_ERR_VALUE, "kv_attn: bad argument");
   if (c.G > 65535 || (long long)t.T * H > 0x7FFFFFFFll / 2) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many heads or tokens");
   if (t.T == 0) return KB2SEQ_OK;

@@ -8,8 +8,11 @@
 // Key tiles of 64 with two buffers of scores per row tile, so that the next scores are made while a tile's are worked on; four buffers of keys and of values.
 // Tensor memory: S 2 x 2 x 64 | O 2 x 64 NV.
 //
-// What bounds it: for 128 keys and 256 rows 32768 exponentials take 2048 cycles (16 a cycle), and shared memory's 128 bytes a cycle are taken for 2560 (the first product
-// reads Q again for every 64 keys: 192 KB, the second V: 64 KB, decoding writes 64 KB).
+// What bounds it: the tensor pipe.  A product of 128 x 64 x 16 with both operands in shared memory takes 75 cycles (64 x 16 of K and 128 x 16 of Q are read each time), one of
+// 128 x 128 x 16 with P in tensor memory 76, so 128 keys and 256 rows take 3616; their 32768 exponentials take 2048 (16 a cycle).  A portion of 4096 tokens after 5001, window
+// 4096, 64 / 4 heads of 128: 606 us, 4400 cycles for those 128 keys, 552 GFLOP at 0.55 of the measured cuBLAS rate.  On the way there: one row tile a CTA with 128 keys a tile
+// 989, two 722, softmax groups in turn 679, tiles of 64 keys with two buffers of scores 688 with one warp for the tensor cores, which spends 300 cycles between two batches of
+// products while the pipe takes two ahead, and 606 with two.
 //
 // Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value unit are fp16 (11 bits).  A row's factor is its scale over a unit, a power of two
 // near the tile's largest scale (exact for scales that are powers of two); the units join the softmax's factors.  Weights are rounded relative to a reference R per row that
@@ -28,7 +31,7 @@ template <int NC, int NV>                    // chunks of 64 of d and dv
 struct PairShape {
   static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128, kKeys = NC > 2 ? 2 : kBufs;      // kKeys: buffers of keys
   static constexpr int kOffQ = 0, kOffK = 2 * kQ, kOffV = kOffK + kKeys * kK, kOffFac = kOffV + kBufs * kV, kOffGroup = kOffFac + kPlans * 512,
-                       kOffBar = kOffGroup + kPlans * 32, kOffUnit = kOffBar + 320, kOffTmem = kOffUnit + kUnits * 8, kOffRow = kOffTmem + 16, kTotal = kOffRow + 256 * 4;
+                       kOffBar = kOffGroup + kPlans * 32, kOffUnit = kOffBar + 320, kOffTmem = kOffUnit + kUnits * 16, kOffRow = kOffTmem + 16, kTotal = kOffRow + 256 * 4;
   static_assert(kTotal <= 227 * 1024 && 4 * FK + 128 * NV <= 512, "memory");
   static_assert(128 * (64 * NV + 1) * 4 + 128 * 12 <= 2 * kQ + kKeys * kK + kBufs * kV, "the second group's share at the end");
 };
@@ -79,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
            *plan_empty = bars + 28 + kPlans, *q_full = bars + 28 + 2 * kPlans;
   uint32_t* factors = reinterpret_cast<uint32_t*>(smem + L::kOffFac);      // [kPlans][128] fp16: of the row's key codes, of its value codes
   int* groups = reinterpret_cast<int*>(smem + L::kOffGroup);               // [kPlans][8] where the groups lie (rows / 16), -1: nowhere
-  float2* units = reinterpret_cast<float2*>(smem + L::kOffUnit);           // [kUnits] of keys, of values
+  float4* units = reinterpret_cast<float4*>(smem + L::kOffUnit);           // [kUnits] of keys, of values; four bits a group: whether it lies nowhere
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
   float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [256] what the queries' own scaling is undone with
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -241,7 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       const uint32_t x_at = s_at + (k & 1) * FK;
       mbar_wait(&s_full[b], turn);
       tc_fence_after_sync();
-      const float2 unit = units[(it >> 1) % kUnits];
+      const float4 unit = units[(it >> 1) % kUnits];
+      const uint32_t gone = __float_as_uint(unit.z) >> (it & 1) * 16 & 0xFFFFu;
       float x[FK];
       {
         uint32_t r[FK / 16][16];
@@ -253,13 +257,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       }
       const int ua = u0 + it * GT, ub = min(ua + GT, u1) - 1;              // groups of the tile
       const int pa = span.group(ua) * kKvGroup, pb = span.group(ub) * kKvGroup + kKvGroup - 1;
-      const bool all = ub == ua + GT - 1 && pb < span.base && pb <= least && (pb < a.first || (ua >= span.na && most - pa < a.window));
+      const bool all = gone == 0 && ub == ua + GT - 1 && pb < span.base && pb <= least && (pb < a.first || (ua >= span.na && most - pa < a.window));
       if (!all) {
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
           const int u = ua + g, j0 = span.group(u) * kKvGroup;
           uint32_t see = 0;
-          if (u < u1 && live) {
+          if (u < u1 && live && !(gone >> 4 * g & 1u)) {
             if (j0 + kKvGroup <= span.base) {                              // the positions of a group that are no further than the row's, and near enough or among the first
               see = pos < j0 ? 0u : pos - j0 >= 15 ? 0xFFFFu : (2u << (pos - j0)) - 1;
               const int far = pos - a.window - j0 + 1;                     // these of the group lie ahead of the window
@@ -440,7 +444,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
         mbar_wait(&plan_empty[slot], (p / kPlans & 1) ^ 1);
         *reinterpret_cast<uint4*>(factors + slot * 128 + lane * 4) = make_uint4(f[0], f[1], f[2], f[3]);
         if ((lane & 3) == 0) groups[slot * 8 + lane / 4] = r < 0 ? -1 : (int)(r / kKvGroup);
-        if (lane == 0) units[p % kUnits] = make_float2(kp, vt ? vp : 0.f);
+        const uint32_t gone = __ballot_sync(0xffffffffu, r < 0);
+        if (lane == 0) units[p % kUnits] = make_float4(kp, vt ? vp : 0.f, __uint_as_float(gone), 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&plan_full[slot]);
         r = next;

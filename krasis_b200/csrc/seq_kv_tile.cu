@@ -1,14 +1,14 @@
-// Attention over the 8-bit cache for many query rows per key / value head (portions of prompts, trees of drafted tokens) on tcgen05.
+// Attention over the 8-bit cache for many query rows per key / value head (portions of prompts, trees of drafted tokens) on tcgen05, where a head has more than 192 (keys) or
+// 128 (values) numbers: tensor memory has room for one output of 128 rows there (seq_kv_pair.cu has two).
 //
 // A tile is 128 (token, head) rows of one sequence and kv head: the H / G heads that share keys fill it together, so a key tile is decoded once for all of them.  Roles of
 // a CTA of 16 warps:
 //   warp  1      brings codes and scales from the pages into a ring of three half tiles (bulk copies of 16 rows)
-//   warps 12-15  decode: codes as fp16 into the swizzled operand tiles.  A row's scale over a power of two
-//                near the tile's largest one is multiplied in there (one packed product for two codes; exact for scales that are powers of two), the power joins the
-//                softmax's factor
+//   warps 12-15  decode: codes as fp16 into the swizzled operand tiles.  A row's scale over a power of two near the tile's largest one is multiplied in there (one packed
+//                product for two codes; exact for scales that are powers of two), the power joins the softmax's factor
 //   warp  0      tcgen05.mma: S = Q K^T, O += P V (P from tensor memory)
 //   warps 4-11   softmax, two threads a row
-// S and P have two buffers each.  FK = 128 keys a tile, 64 where d or dv is above 128 (tensor memory: 3 FK + dv columns).
+// S and P have two buffers each; 64 keys a tile (tensor memory: 3 FK + dv columns).
 //
 // Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value scale are fp16 (11 bits).  Weights are rounded relative to a reference R per row
 // that follows the largest weight times scale (2^6 to 2^15 of it), as in the kernel for few rows; maxima, weights and their sum are fp32.
@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
            *c_full = bars + 16, *c_empty = bars + 19;
   float2* refs = reinterpret_cast<float2*>(smem + L::kOffRef);             // [4] tile's units: keys, values
   uint32_t* have = reinterpret_cast<uint32_t*>(refs + 4);                  // [3] a slot's groups that are there, a bit each
+  uint32_t* gone = have + 3;                                               // [4] a tile's groups that are not
   uint32_t* tmem_at = have + 3;
   float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [128] what the queries' own scaling is undone with
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -212,7 +213,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       }
       mbar_wait(&k_empty[b], (it >> 1 & 1) ^ 1);
       decode<FMT, NR, NC>(smem + L::kOffK + b * L::kK, from, c.d, ct, fk, see);
-      if (ct == 0) refs[it & 3] = make_float2(kp, vt ? vp : 0.f);
+      if (ct == 0) {
+        refs[it & 3] = make_float2(kp, vt ? vp : 0.f);
+        gone[it & 3] = ~groups & ((1u << GT) - 1);
+      }
       if (lane == 0) {
         mbar_arrive(&k_full[b]);
         mbar_arrive(&c_empty[slot]);
@@ -239,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ codes and scales from the pages, in the decoders' order.  A run of groups that one page holds is one run of
-    // bytes in each pool, and one bulk copy (one a group: 1083 us for a portion of 4096 tokens); scales go 16 bytes a lane.
+    // bytes in each pool, and one bulk copy (heads of 128, 4096 tokens: one a group 1083 us, one a run 989); scales go 16 bytes a lane.
     const auto at_row = [&](int it) {        // lane's group of a tile
       const int u = u0 + it * GT + lane;
       const long long r = lane < GT && it < n_tiles && u < u1 ? kv_row(c, t, s, span.group(u) * kKvGroup) : -1;
@@ -353,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       mbar_wait(&s_full[b], it >> 1 & 1);
       tc_fence_after_sync();
       const float2 p2 = refs[it & 3];        // written ahead of the keys; the tile after next writes none before this one's scores are taken
+      const uint32_t away = gone[it & 3];
       float x[NB][32];
       {
         uint32_t r[NB][2][16];
@@ -370,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       tell(&s_cons[b]);
       const int ua = u0 + it * GT, ub = min(ua + GT, u1) - 1;              // groups of the tile
       const int pa = span.group(ua) * kKvGroup, pb = span.group(ub) * kKvGroup + kKvGroup - 1;
-      const bool all = ub == ua + GT - 1 && pb < span.base && pb <= least && (pb < a.first || (ua >= span.na && most - pa < a.window));
+      const bool all = away == 0 && ub == ua + GT - 1 && pb < span.base && pb <= least && (pb < a.first || (ua >= span.na && most - pa < a.window));
       if (!all) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
           for (int g = 0; g < 2; ++g) {
             const int u = ua + i * 4 + hf * 2 + g, j0 = span.group(u) * kKvGroup;
             uint32_t see = 0;
-            if (u < u1 && live) {
+            if (u < u1 && live && !(away >> (u - ua) & 1u)) {
 #pragma unroll 1
               for (int j = 0; j < 16; ++j) see |= (uint32_t)kv_sees(t, a, span, c0, n, tok, pos, j0 + j) << j;
             }

@@ -339,6 +339,32 @@ def test_pages_outside_the_pool():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("d,dv", [(64, 64), (192, 128), (256, 256)])
+@pytest.mark.parametrize("tokens", [40, 8])
+def test_pages_outside_the_pool_on_tiles(d, dv, tokens, monkeypatch):
+    """The same where the tensor cores' tiles take the rows: a missing page's rows have no weight, not even that of a score of 0."""
+    from krasis_b200 import seqops as ops
+    monkeypatch.setattr(ops, "KV_TILES_FROM", 1)
+    for bad in (6, -1):
+        pages = [5, 3, 1, 0]
+        tb = ops.StepTables([([0] * tokens, 190, 0, pages)], "cuda")
+        tb.pages[1] = bad                                  # positions 64 .. 127
+        c = _cache(2, d, dv, 6, "int8", seed=2)
+        q = (torch.randn(tokens, 8, d, generator=_gen(15)) - 0.5).to(BF).cuda()
+        (k, v), codes = kv_plain.held(c, 0), c.v[0].double().abs().cpu()
+        for window, first in ((None, 0), (150, 70)):
+            got = ops.kv_attn(q, tb, c, 0, 0.125, window=window, first=first)
+            for t in range(tokens):
+                rows = [j for j in range(190 + t + 1) if not 64 <= j < 128 and (window is None or 190 + t - j < window or j < first)]
+                at = torch.tensor([pages[j // 64] for j in rows]), torch.tensor([j % 64 for j in rows])
+                for h in range(8):
+                    kk, vv, x = k[at[0], h // 4, at[1]], v[at[0], h // 4, at[1]], q[t, h].double().cpu()
+                    w = torch.softmax(kk @ x * 0.125, 0)
+                    off = kv_plain.off_by(BF, BF, 256, d, w @ vv, w @ vv.abs(), (kk.abs() @ x.abs()).max() * 0.125,
+                                          (w * c.v_scale[0].double().cpu()[at[0], h // 4, at[1]]).max() * codes[at[0], h // 4, at[1]].sum(0), decoded=True)
+                    assert bool(((got[t, h].double().cpu() - w @ vv).abs() <= off).all())
+
+
 def test_rows_behind_the_last_sequence():
     from krasis_b200 import seqops as ops
     tb, seqs, pages = _step([(2, 40), (3, 7)], 64, 16)

@@ -111,6 +111,7 @@ def _structs(**kw):
     ({"d": 40}, 2), ({"dv": 512}, 2), ({"layers": 0}, 2), ({"positions": None}, 2), ({"cu": None}, 2), ({"step_pages": None}, 2), ({"layout": [[0, 2, 15, 1]]}, 4),
     ({"layout": [[0, 1, 0, 1], [1, 1, 0, 0]]}, 4), ({"layout": [[0, 2, 2147483647, 1]]}, 4), ({"S": 0}, 2), ({"T": -1}, 2), ({"max_pages": 0}, 2), ({"bits": 4096, "words": 1}, 2),
     ({"bits": 4096, "words": 0, "rows": 4096}, 2), ({"pages": 1 << 30}, 2),
+    ({"bits": 4096, "words": 1, "rows": 4096, "T": 33, "layout": [[0, 33, 3, 3]], "max_pages": 3}, 2),
 ])
 def test_interface_refuses(kw, code):
     lib = ops.load()
@@ -133,6 +134,8 @@ def test_interface_refuses_arguments():
     assert lib.kb2_seq_kv_read(p, 0, q, 0, 0, 1, 4100, 4096, 0, None) == 2
     for H, window, first, dq, do in ((3, 0, 0, 0, 0), (1, 0, 0, 0, 0), (4, -1, 0, 0, 0), (4, 0, -1, 0, 0), (4, 0, 0, 2, 0), (4, 0, 0, 0, -1)):
         assert lib.kb2_seq_kv_attn(p, 0, q, 4096, dq, 256, 64, H, 1.0, window, first, None, 4096, do, None, 0, None) == 2
+    for scale in (float("nan"), float("inf"), float("-inf")):
+        assert lib.kb2_seq_kv_attn(p, 0, q, 4096, 0, 256, 64, 4, scale, 0, 0, None, 4096, 0, None, 0, None) == 2
     assert lib.kb2_seq_kv_keep(p, q, 4096, 513, None) == 2 and lib.kb2_seq_kv_keep(p, q, 4096, -1, None) == 2 and lib.kb2_seq_kv_keep(p, q, None, 1, None) == 2
     big, layout = 200000, [[0, 1, 199999, 12500]]
     c, s, keep = _structs(pages=12500, max_pages=12500, layout=layout, T=1)
