@@ -8,7 +8,8 @@ Two targets, so that a model only compiles what it runs on:
                                   before the window, rotated values, distance penalty), gated and ungated linear units, router and
                                   routed experts,
                                   gated linear attention, matrix memory (mLSTM), selective scan and real-gated linear recurrent unit with
-                                  state slots, side-by-side mixers, depth average, several mixed copies of the residual stream
+                                  state slots, side-by-side mixers, depth average, several mixed copies of the residual stream;
+                                  a paged cache of keys and values in 8 bits: writing, reading, windowed and tree attention, moving rows
 nvcc cross-compiles without a GPU.  The .so files are git-ignored; a missing or stale one is rebuilt on demand.
 """
 import hashlib
