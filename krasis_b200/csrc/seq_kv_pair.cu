@@ -10,9 +10,9 @@
 //
 // What bounds it: the tensor pipe.  A product of 128 x 64 x 16 with both operands in shared memory takes 75 cycles (64 x 16 of K and 128 x 16 of Q are read each time), one of
 // 128 x 128 x 16 with P in tensor memory 76, so 128 keys and 256 rows take 3616; their 32768 exponentials take 2048 (16 a cycle).  A portion of 4096 tokens after 5001, window
-// 4096, 64 / 4 heads of 128: 606 us, 4400 cycles for those 128 keys, 552 GFLOP at 0.55 of the measured cuBLAS rate.  On the way there: one row tile a CTA with 128 keys a tile
+// 4096, 64 / 4 heads of 128: 617 us, 4480 cycles for those 128 keys, 552 GFLOP at 0.54 of the measured cuBLAS rate.  On the way there: one row tile a CTA with 128 keys a tile
 // 989, two 722, softmax groups in turn 679, tiles of 64 keys with two buffers of scores 688 with one warp for the tensor cores, which spends 300 cycles between two batches of
-// products while the pipe takes two ahead, and 606 with two.
+// products while the pipe takes two ahead, and 606 with two; groups of pages that are not there, looked for in each tile, cost the rest.
 //
 // Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value unit are fp16 (11 bits).  A row's factor is its scale over a unit, a power of two
 // near the tile's largest scale (exact for scales that are powers of two); the units join the softmax's factors.  Weights are rounded relative to a reference R per row that
