@@ -28,9 +28,9 @@ struct TileShape {
   static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128;
   static constexpr int kSlots = 3, kCodes = FK * 64 * (NC > NV ? NC : NV), kSlot = kCodes + FK * 8;       // codes as they come | scales of keys | of values
   static constexpr int kOffQ = 0, kOffK = kQ, kOffV = kOffK + 2 * kK, kOffSlot = kOffV + VS * kV, kOffBar = kOffSlot + kSlots * kSlot, kOffRef = kOffBar + 192,
-                       kOffX = kOffRef + 64, kOffRow = kOffX + 2 * 2 * 128 * 4;
+                       kOffHave = kOffRef + 4 * 8, kOffGone = kOffHave + kSlots * 4, kOffTmem = kOffGone + 4 * 4, kOffX = kOffTmem + 4, kOffRow = kOffX + 2 * 2 * 128 * 4;
   static constexpr int kTotal = kOffRow + 128 * 4;
-  static_assert(kTotal <= 227 * 1024 && 3 * FK + 64 * NV <= 512 && kSlot % 128 == 0, "memory");
+  static_assert(kTotal <= 227 * 1024 && 3 * FK + 64 * NV <= 512 && kSlot % 128 == 0 && kOffRef % 8 == 0 && kOffX % 16 == 0, "memory");
 };
 
 // Codes of a tile from `from` (rows of `width` bytes) into the operand at `to`.  A thread has the rows ct / 4 + 32 i and 16 bytes of each chunk of 64 of those, f times the
@@ -77,9 +77,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *s_cons = bars + 10, *p_full = bars + 12, *pv_done = bars + 14,
            *c_full = bars + 16, *c_empty = bars + 19;
   float2* refs = reinterpret_cast<float2*>(smem + L::kOffRef);             // [4] tile's units: keys, values
-  uint32_t* have = reinterpret_cast<uint32_t*>(refs + 4);                  // [3] a slot's groups that are there, a bit each
-  uint32_t* gone = have + 3;                                               // [4] a tile's groups that are not
-  uint32_t* tmem_at = have + 3;
+  uint32_t* have = reinterpret_cast<uint32_t*>(smem + L::kOffHave);        // [3] a slot's groups that are there, a bit each
+  uint32_t* gone = reinterpret_cast<uint32_t*>(smem + L::kOffGone);        // [4] a tile's groups that are not
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
   float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [128] what the queries' own scaling is undone with
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
