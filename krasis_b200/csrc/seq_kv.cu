@@ -205,7 +205,7 @@ constexpr int kKeepMost = 512, kKeepLayers = 8;
 __global__ void __launch_bounds__(256) kv_keep_kernel(KvLayer c, int layers, KvStep t, const int* __restrict__ path, int P) {
   __shared__ long long rows[2][kKeepMost];
   __shared__ int moved;
-  kb2::pdl_wait();
+  kb2::pdl_enter(path);
   const int s = blockIdx.x, base_tok = t.cu[s], n = t.cu[s + 1] - base_tok;
   if (n <= 0) return;
   const int base = t.rows[base_tok];
