@@ -400,9 +400,10 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = p[h][e] * (__uint_as_float(word(vq, e)) * inv[h]);
+          x[e] = p[h][e] * __uint_as_float(word(vq, e));
           if (!all && y[h][e] == -INFINITY) x[e] = 0.f;                    // a row that nobody sees may hold anything
           big = fmaxf(big, x[e]);
+          x[e] *= inv[h];                    // not times the scale first: of a small reference that may be infinite, and the weight zero
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -412,7 +413,8 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
             w[h][PARTS - 1][b] = f16_pair(x[2 * b] - f.x, x[2 * b + 1] - f.y);
           }
         }
-        return top > 8.f || big > 32768.f;   // a weight above 2^8, a product above fp16's range
+        // a weight above 2^8, a product above fp16's range, or one where there is no reference yet: all values so far were zero, or their weights have become so
+        return top > 8.f || big * inv[h] > 32768.f || (inv[h] == 0.f && big > 1e-37f);
       };
       bool again = false;
 #pragma unroll
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
           grow[h] = 1.f;
-          if (big > ref[h] * 32768.f && big > 1e-37f) {
+          if (big > 1e-37f && (ref[h] < 1e-37f || big > ref[h] * 32768.f)) {
             const float r = fmaxf(big * 0.015625f, 1e-37f);
             grow[h] = ref[h] / r;
             ref[h] = r;

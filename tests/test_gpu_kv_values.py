@@ -1,0 +1,65 @@
+"""Attention over the 8-bit cache where rows of values are zero or far apart, and where a step's tables hold fewer tokens than its layout."""
+import pytest
+import torch
+
+from tests import kv_plain
+from tests.test_gpu_kv_cache import BF, F32, _cache, _check, _gen, _step, _tree, forms, waits  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def _zero(c, seqs, rows):
+    """Zero values in the rows that `rows` says of every sequence."""
+    for n, start, pages, _ in seqs:
+        for j in rows(start + n):
+            c.v[0, pages[j // c.page_size], :, j % c.page_size] = 0
+            c.v_scale[0, pages[j // c.page_size], :, j % c.page_size] = 0
+
+
+GROUPS = {"first": lambda n: range(min(n, 16)), "of the first warps": lambda n: [j for j in range(n) if j < 128 and j // 16 % 3],
+          "of all warps": lambda n: range(min(n, 128)), "of each piece": lambda n: [j for j in range(n) if j // 16 % 16 < 9], "every other": lambda n: [j for j in range(n) if j // 16 % 2 == 0],
+          "the first row": lambda n: [0], "all but the last": lambda n: range(n - 1)}
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("H,G,d,dv", [(16, 2, 128, 128), (4, 4, 64, 64), (6, 2, 256, 256)])
+@pytest.mark.parametrize("groups", sorted(GROUPS))
+def test_rows_of_zero_values(fmt, H, G, d, dv, groups, forms):  # noqa: F811
+    """Rows whose values are all zero weigh in the sum and take nothing from the rows behind them."""
+    from krasis_b200 import seqops as ops
+    tb, seqs, pages = _step([(1, 500), (1, 20), (30, 300), (1, 3000)], 64, 40)
+    c = _cache(G, d, dv, pages, fmt, seed=41)
+    _zero(c, seqs, GROUPS[groups])
+    q = torch.randn(tb.T, H, d, generator=_gen(42)).cuda()
+    for window, first in ((None, 0), (200, 1), (40, 16)):
+        known = None
+        for do in (F32, BF):
+            for got in forms(tb, lambda: ops.kv_attn(q, tb, c, 0, d ** -0.5, window=window, first=first, dtype=do)):
+                known = _check(got, q, c, seqs, known=known, scale=d ** -0.5, window=window, first=first)
+
+
+@pytest.mark.parametrize("groups", ["first", "of all warps", "every other"])
+def test_rows_of_zero_values_ahead_of_drafts(groups, forms):  # noqa: F811
+    from krasis_b200 import seqops as ops
+    lens = [(16, 5000), (40, 64), (3, 300)]
+    tb, seqs, pages = _step(lens, 64, 43, parents=[_tree(n, n, 4) for n, _ in lens])
+    c = _cache(2, 128, 128, pages, "int8", seed=44)
+    _zero(c, seqs, GROUPS[groups])
+    q = torch.randn(tb.T, 16, 128, generator=_gen(45)).cuda()
+    known = None
+    for do in (F32, BF):
+        for got in forms(tb, lambda: ops.kv_tree_attn(q, tb, c, 0, 0.09, dtype=do)):
+            known = _check(got, q, c, seqs, known=known, scale=0.09)
+
+
+def test_many_keys_behind_rows_of_zero_values():
+    """Keys that are cut evenly over the GPU, and a captured-size step of few keys that clusters join."""
+    from krasis_b200 import seqops as ops
+    for lens, H, G, d in (([(1, 20000 + 97 * i) for i in range(3)], 12, 12, 128), ([(2, 7000)] * 5, 16, 4, 256), ([(1, 900)] * 4, 16, 2, 128)):
+        tb, seqs, pages = _step(lens, 64, 46)
+        c = _cache(G, d, d, pages, "int8", seed=47)
+        _zero(c, seqs, lambda n: [j for j in range(n) if j // 16 % 32 < 20])
+        q = torch.randn(tb.T, H, d, generator=_gen(48)).cuda()
+        known = None
+        for do in (F32, BF):
+            known = _check(ops.kv_attn(q, tb, c, 0, d ** -0.5, dtype=do), q, c, seqs, known=known, scale=d ** -0.5)
