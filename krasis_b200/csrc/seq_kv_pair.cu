@@ -284,19 +284,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       const float fac = fminf(fmaxf(down * unit.x, 1e-37f), 1e37f);
       const float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * fac;
       // a new maximum, or values whose unit may take a weight beyond fp16: seldom after the first tiles
-      if (__any_sync(0xffffffffu, mt > m || unit.y > ref * 32768.f)) {
+      if (__any_sync(0xffffffffu, mt > m || unit.y > (inv_ref == 0.f ? 0.f : ref * 32768.f))) {
         const float mn = fmaxf(m, mt), from = mn == -INFINITY ? 0.f : mn, back = ex2(m - from);
         m = mn;
         l *= back;
         ref *= back;
         const float big = ex2(mt - from) * unit.y;                         // the tile's largest weight times unit
         float grow = 1.f;
-        if (big > ref * 32768.f && big > 1e-37f) {
-          const float r = fmaxf(big * 0.015625f, 1e-37f);
+        const float least = fmaxf(unit.y * 7.8886091e-31f, 1e-37f);        // 2^-100 of the unit: 1 / ref times it stays within fp32
+        if (big > 1e-37f && (big > ref * 32768.f || ref < least)) {
+          const float r = fmaxf(big * 0.015625f, least);
           grow = ref / r;
           ref = r;
         }
-        inv_ref = ref >= 1e-37f ? 1.f / ref : 0.f;
+        inv_ref = ref >= least ? 1.f / ref : 0.f;                          // no reference: what the tile's weights come to is nothing
         if (k > 0 && __any_sync(0xffffffffu, grow != 1.f)) {
           mbar_wait(&pv_done[grp * 2 + ((k - 1) & 1)], (k - 1) >> 1 & 1);  // O holds every product so far
           tc_fence_after_sync();

@@ -411,13 +411,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       const float big = ex2(mt - from) * p2.y;                             // the tile's largest weight times scale
       float grow = 1.f;
       bool again = false;
-      if (big > ref * 32768.f && big > 1e-37f) {
-        const float r = fmaxf(big * 0.015625f, 1e-37f);
+      const float least = fmaxf(p2.y * 7.8886091e-31f, 1e-37f);            // 2^-100 of the unit: 1 / ref times it stays within fp32
+      if (big > 1e-37f && (big > ref * 32768.f || ref < least)) {
+        const float r = fmaxf(big * 0.015625f, least);
         grow = ref / r;
         again = it > 0;                      // a reference that has shrunk to nothing as well: what O holds is then far below
         ref = r;
       }
-      const float f = ref >= 1e-37f ? p2.y * __frcp_rn(ref) : 0.f;
+      const float f = ref >= least ? p2.y * __frcp_rn(ref) : 0.f;
       const uint64_t fac2 = pair_of(fac, fac), neg2 = pair_of(-from, -from), f2 = pair_of(f, f);
       uint64_t sum[2] = {0, 0};
       uint32_t pk[NB][16];

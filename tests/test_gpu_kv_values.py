@@ -63,3 +63,35 @@ def test_many_keys_behind_rows_of_zero_values():
         known = None
         for do in (F32, BF):
             known = _check(ops.kv_attn(q, tb, c, 0, d ** -0.5, dtype=do), q, c, seqs, known=known, scale=d ** -0.5)
+@pytest.mark.parametrize("H,G,d,dv", [(16, 2, 128, 128), (4, 4, 64, 64), (6, 2, 256, 256)])
+@pytest.mark.parametrize("above", [60.0, 83.0, 84.5, 85.5, 86.5, 90.0])
+def test_a_zero_value_far_above_large_ones(H, G, d, dv, above, forms):  # noqa: F811
+    """One key takes nearly all of the weight and its value is zero, as are those around it: the others' large values count for next to nothing, and for a number."""
+    from krasis_b200 import seqops as ops
+    tb, seqs, pages = _step([(1, 700), (40, 900)], 64, 49)
+    c = _cache(G, d, dv, pages, "int8", seed=50)
+    c.k.copy_(torch.randint(-3, 4, c.k.shape, generator=_gen(51), dtype=torch.int8))
+    c.k_scale.fill_(1.0)
+    c.v_scale[0].copy_(torch.exp2(torch.randint(13, 17, c.v_scale[0].shape, generator=_gen(52)).float()))
+    c.v_scale[0, :, :, ::7] *= 2.0 ** 20
+    _zero(c, seqs, lambda n: range(256, 400))
+    for n, start, pl, _ in seqs:
+        c.k[0, pl[300 // 64], :, 300 % 64] = 100
+    q = torch.ones(tb.T, H, d).cuda()
+    scale = above / (100 * d)
+    want, *sizes = kv_plain.attention(q, c, 0, seqs, scale)
+    # Beside off_by.  Weights are fp32 numbers relative to the row's largest, and the exponential gives 0 below 2^-126: each is off by as much, and the result by that times
+    # the sum of |v|.  A reference is at least 2^-100 of the unit that it divides (on tiles), and a product is off by half of fp16's least step, 2^-25, times it: 2^-125 of |v|.
+    # Products of weight and unit up to 1e-37 may be left out, the unit at least 2^-7 of the row's scale: 1e-37 times 2^7 times the sum of the codes.
+    numbers, codes = kv_plain.held(c, 0)[1].abs(), c.v[0].cpu().double().abs()
+    lost, at = torch.zeros_like(want), 0
+    for n, start, pl, _ in seqs:
+        for x, f in ((numbers, 3 * 2.0 ** -126), (codes, 2.0 ** 7 * 1e-37)):
+            lost[at:at + n] += f * x[pl].transpose(1, 2).reshape(-1, G, dv)[:start + n].sum(0).repeat_interleave(H // G, 0)
+        at += n
+    for do in (F32, BF):
+        off = kv_plain.off_by(F32, do, 940, d, want, *sizes, decoded=True) + lost
+        for got in forms(tb, lambda: ops.kv_attn(q, tb, c, 0, scale, dtype=do)):
+            assert bool(torch.isfinite(got).all())
+            err = (got.double().cpu() - want).abs()
+            assert bool((err <= off).all()), (float((err / off).max()), float(err.max()))
