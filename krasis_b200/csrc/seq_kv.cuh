@@ -63,8 +63,17 @@ __device__ __forceinline__ KvSpan kv_span(const KvLayer& c, const KvStep& t, int
   return r;
 }
 
-// Tile number `at` of the sequences that have least .. most rows, `per` a token and `rows` a tile.  One warp; false behind the last tile.
-__device__ __forceinline__ bool kv_find_tile(const KvStep& t, int per, int rows, int least, int most, int at, int* seq, int* tile) {
+// Which sequences run on the tensor cores' tiles, as the host's layout has it: the device's table may end early, and a sequence's rows there are then fewer than those that
+// it was planned with.  A bit for each 2^shift sequences; every: 0 none, 1 all, 2 by the bits.
+constexpr int kKvKindBits = 2048;
+struct KvKinds {
+  uint32_t on[kKvKindBits / 32];
+  int shift, every;
+  __host__ __device__ __forceinline__ bool on_tiles(int s) const { return every < 2 ? every : on[s >> shift >> 5] >> (s >> shift & 31) & 1u; }
+};
+
+// Tile number `at` of the sequences that are not on the tensor cores' tiles, of `per` rows a token and `rows` a tile.  One warp; false behind the last tile.
+__device__ __forceinline__ bool kv_find_tile(const KvStep& t, const KvKinds& kinds, int per, int rows, int at, int* seq, int* tile) {
   const int lane = threadIdx.x & 31;
   int before = 0;
   for (int s0 = 0; s0 < t.S; s0 += 32) {
@@ -72,7 +81,7 @@ __device__ __forceinline__ bool kv_find_tile(const KvStep& t, int per, int rows,
     int n = 0;
     if (s < t.S) {
       const int have = (t.cu[s + 1] - t.cu[s]) * per;
-      n = have >= least && have <= most ? (have + rows - 1) / rows : 0;
+      n = have > 0 && !kinds.on_tiles(s) ? (have + rows - 1) / rows : 0;
     }
     int upto = n;                            // tiles up to and with sequence s
 #pragma unroll

@@ -92,7 +92,7 @@ __device__ __forceinline__ void store8(const KvLayer& c, const KvAttn& a, const 
 
 // FULL: d and dv are whole units, and every copy's address is one of two a lane has plus a constant.
 template <int FMT, int DU, int VU, int NQ, int PARTS, bool FULL>
-__global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>::kBlocks)) kv_stream_kernel(KvLayer c, KvStep t, KvAttn a) {
+__global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>::kBlocks)) kv_stream_kernel(KvLayer c, KvStep t, KvAttn a, const __grid_constant__ KvKinds kinds) {
   using L = StreamShape<DU, VU, NQ, PARTS>;
   constexpr int MT = L::MT, VB = L::VB, VC = L::VC, MV = VU * 4;         // MV: 16-row tiles of O^T
   extern __shared__ __align__(16) uint8_t smem[];
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     if (a.per_seq) {
       s = blockIdx.x / a.per_seq;
       tile = blockIdx.x - s * a.per_seq;
-    } else if (!kv_find_tile(t, per, MT, a.least, a.most, blockIdx.x, &s, &tile)) {
+    } else if (!kv_find_tile(t, kinds, per, MT, blockIdx.x, &s, &tile)) {
       return;
     }
   }
@@ -580,11 +580,11 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   }
 }
 
-// The pieces of a row (token, head), joined in a fixed order; rows that one piece finished are left alone.  x, y: the two kinds of sequences.  W warps a row take the pieces in
+// The pieces of a row (token, head), joined in a fixed order; rows that one piece finished are left alone.  x, y: sequences of few rows, and those on tiles.  W warps a row take the pieces in
 // turn, four of a warp's on their way at once (one at a time 64 pieces took 27 us).  One request of 30000 rows, 16 / 2 heads: four warps a row 17 us in all, one 38 at the time;
 // 62000 rows of few pieces: four warps 50 us more than one.
 template <int W>
-__global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAttn x, KvAttn y) {
+__global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAttn x, KvAttn y, const __grid_constant__ KvKinds kinds) {
   __shared__ float weights[W > 1 ? kMostPieces : 4 * 32];
   __shared__ __align__(16) float share[3][256];
   __shared__ float total[4];
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
   if (tok >= t.T) return;
   if (tok >= t.cu[t.S]) return;
   const int per = x.H / c.G, s = t.seq_of[tok], c0 = t.cu[s], n = t.cu[s + 1] - c0;
-  const KvAttn& a = n * per <= x.most ? x : y;
+  const KvAttn& a = kinds.on_tiles(s) ? y : x;
   if (a.pieces <= 1 || a.cluster) return;
   const int r0 = ((tok - c0) * per + hd % per) / a.rows * a.rows, nr = (int)min((long long)n * per - r0, (long long)a.rows);
   const KvSpan span = kv_span(c, t, s, c0 + r0 / per, c0 + (r0 + nr - 1) / per, a.window, a.first);
@@ -685,7 +685,7 @@ constexpr int kTileFrom = 48;
 constexpr long long kWideWaves = 2;          // pieces for each SM, of such sequences (sixteen trees of 57 to 64 tokens: 2 530 us, 3 548, 4 571, 6 638)
 // How the sequences of one kind are cut: into tiles of rows, and the keys that a tile sees (in groups of 16) into pieces.
 struct KvPlan {
-  int least, most, rows, tiles, per_seq, piece, pieces, blocks;            // blocks: of the even cut (0 for pieces of tiles); of tiles on the tensor cores, pieces and all
+  int rows, tiles, per_seq, piece, pieces, blocks;                         // blocks: of the even cut (0 for pieces of tiles); of tiles on the tensor cores, pieces and all
   bool cluster;                              // the pieces of a tile are a cluster, which joins them itself
   size_t floats;                             // workspace
 };
@@ -694,21 +694,19 @@ inline long long groups_seen(long long start, long long n, int window, int first
   const long long lo = window < kKvNoWindow ? std::max(0ll, start - window + 1) : 0;
   return (start + n - lo + 30) / 16 + (std::min<long long>(first, lo) + 15) / 16;
 }
-KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int least, int most, bool wide) {
+KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, const KvKinds& kinds, bool wide) {
   KvPlan p{};
   const int per = H / cache->G;
   long long top = 0, work = 0, rows = 0;
   bool same = true;
   for (int s = 0; s < step->S; ++s) {
     const long long r = (long long)step->layout[4 * s + 1] * per;
-    if (r >= least && r <= most) rows = std::max(rows, r);
+    if (kinds.on_tiles(s) == wide) rows = std::max(rows, r);
   }
-  p.least = least;
-  p.most = most;
   p.rows = wide ? (kv_pairs(cache->d, cache->dv) ? 256 : 128) : rows <= 8 ? 8 : 16;
   const auto tiles = [&](int s) {            // of a sequence of this kind
     const long long r = (long long)step->layout[4 * s + 1] * per;
-    return r < least || r > most ? 0ll : (r + p.rows - 1) / p.rows;
+    return kinds.on_tiles(s) == wide ? (r + p.rows - 1) / p.rows : 0ll;
   };
   const auto seen = [&](int s) {             // captured launches are run again with later positions: what the page lists hold
     const int* l = step->layout + 4 * s;
@@ -781,6 +779,7 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
 }
 struct KvPlans {
   KvPlan few, many;
+  KvKinds kinds;
   size_t bytes() const { return (few.floats + many.floats) * 4; }
 };
 KvPlans kv_plans(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int dt_out) {
@@ -803,13 +802,30 @@ KvPlans kv_plans(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int
     const long long sms = kb2::current_sms();
     if (few * 27 > 2 * (many * 30 + 800 * sms)) split = kTileFrom - 1;
   }
-  p.few = kv_plan(cache, step, H, window, first, 1, split, false);
-  if (split < 0x7FFFFFFF) p.many = kv_plan(cache, step, H, window, first, split + 1, 0x7FFFFFFF, true);
+  // more than `split` rows: on tiles.  Of steps with more sequences than there are bits, neighbours are if all of them that have tokens do.
+  KvKinds& kinds = p.kinds;
+  int wide = 0, all = 0;
+  if (split < 0x7FFFFFFF) {
+    while ((step->S - 1) >> kinds.shift >= kKvKindBits) ++kinds.shift;
+    for (int s0 = 0; s0 < step->S; s0 += 1 << kinds.shift) {
+      int n = 0, on = 0;
+      for (int s = s0; s < std::min(s0 + (1 << kinds.shift), step->S); ++s) {
+        const long long r = (long long)step->layout[4 * s + 1] * (H / cache->G);
+        n += r > 0;
+        on += r > split;
+      }
+      all += n;
+      if (on == 0 || on < n) continue;
+      wide += on;
+      kinds.on[s0 >> kinds.shift >> 5] |= 1u << (s0 >> kinds.shift & 31);
+    }
+    kinds.every = wide == 0 ? 0 : wide == all ? 1 : 2;
+  }
+  if (kinds.every != 1) p.few = kv_plan(cache, step, H, window, first, kinds, false);
+  if (kinds.every) p.many = kv_plan(cache, step, H, window, first, kinds, true);
   return p;
 }
 inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, int dv) {
-  a.least = p.least;
-  a.most = p.most;
   a.rows = p.rows;
   a.per_seq = p.per_seq;
   a.piece = p.piece;
@@ -823,28 +839,28 @@ inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, 
 }
 
 template <int FMT, int DU, int VU, int NQ, int PARTS, bool FULL>
-int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
+int stream_launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, const KvKinds& kinds, cudaStream_t st) {
   using L = StreamShape<DU, VU, NQ, PARTS>;
   SEQ_CUDA((kb2::allow_smem<kv_stream_kernel<FMT, DU, VU, NQ, PARTS, FULL>>(L::kTotal)));
   auto kern = kv_stream_kernel<FMT, DU, VU, NQ, PARTS, FULL>;
-  kb2::launch_pdl_clusters(kern, p.blocks ? dim3(p.blocks) : dim3(p.tiles, c.G, p.pieces), kSWarps * 32, L::kTotal, st, dim3(1, 1, p.cluster ? p.pieces : 1), c, t, a);
+  kb2::launch_pdl_clusters(kern, p.blocks ? dim3(p.blocks) : dim3(p.tiles, c.G, p.pieces), kSWarps * 32, L::kTotal, st, dim3(1, 1, p.cluster ? p.pieces : 1), c, t, a, kinds);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }
 template <int FMT, int DU, int VU, bool FULL>
-int stream_rows(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
-  if (p.rows == 8) return a.dt_out ? stream_launch<FMT, DU, VU, 1, 1, FULL>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 1, 2, FULL>(c, t, a, p, st);
-  return a.dt_out ? stream_launch<FMT, DU, VU, 2, 1, FULL>(c, t, a, p, st) : stream_launch<FMT, DU, VU, 2, 2, FULL>(c, t, a, p, st);
+int stream_rows(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, const KvKinds& kinds, cudaStream_t st) {
+  if (p.rows == 8) return a.dt_out ? stream_launch<FMT, DU, VU, 1, 1, FULL>(c, t, a, p, kinds, st) : stream_launch<FMT, DU, VU, 1, 2, FULL>(c, t, a, p, kinds, st);
+  return a.dt_out ? stream_launch<FMT, DU, VU, 2, 1, FULL>(c, t, a, p, kinds, st) : stream_launch<FMT, DU, VU, 2, 2, FULL>(c, t, a, p, kinds, st);
 }
 template <int FMT>
-int stream_sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, cudaStream_t st) {
+int stream_sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvPlan& p, const KvKinds& kinds, cudaStream_t st) {
   const auto is = [&](int d, int dv) { return c.d == d && c.dv == dv; };
-  if (is(64, 64)) return stream_rows<FMT, 1, 1, true>(c, t, a, p, st);
-  if (is(128, 128)) return stream_rows<FMT, 2, 2, true>(c, t, a, p, st);
-  if (is(192, 128)) return stream_rows<FMT, 3, 2, true>(c, t, a, p, st);
-  if (is(128, 256)) return stream_rows<FMT, 2, 4, true>(c, t, a, p, st);
-  if (is(256, 256)) return stream_rows<FMT, 4, 4, true>(c, t, a, p, st);
-  return c.d <= 128 && c.dv <= 128 ? stream_rows<FMT, 2, 2, false>(c, t, a, p, st) : stream_rows<FMT, 4, 4, false>(c, t, a, p, st);
+  if (is(64, 64)) return stream_rows<FMT, 1, 1, true>(c, t, a, p, kinds, st);
+  if (is(128, 128)) return stream_rows<FMT, 2, 2, true>(c, t, a, p, kinds, st);
+  if (is(192, 128)) return stream_rows<FMT, 3, 2, true>(c, t, a, p, kinds, st);
+  if (is(128, 256)) return stream_rows<FMT, 2, 4, true>(c, t, a, p, kinds, st);
+  if (is(256, 256)) return stream_rows<FMT, 4, 4, true>(c, t, a, p, kinds, st);
+  return c.d <= 128 && c.dv <= 128 ? stream_rows<FMT, 2, 2, false>(c, t, a, p, kinds, st) : stream_rows<FMT, 4, 4, false>(c, t, a, p, kinds, st);
 }
 }  // namespace
 }  // namespace kb2seq
@@ -891,16 +907,16 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   const KvAttn few = with_plan(a, p.few, (float*)work, t.T * H, c.dv), many = with_plan(a, p.many, (float*)work + p.few.floats, t.T * H, c.dv);
   const cudaStream_t st = (cudaStream_t)stream;
   if (p.many.tiles) {
-    if (int e = (kv_pairs(c.d, c.dv) ? kv_pair_attend : kv_tile_attend)(cache->fmt, c, t, many, p.many.blocks, st)) return e;
+    if (int e = (kv_pairs(c.d, c.dv) ? kv_pair_attend : kv_tile_attend)(cache->fmt, c, t, many, p.kinds, p.many.blocks, st)) return e;
   }
   if (p.few.tiles) {
-    if (int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, few, p.few, st) : stream_sizes<KV_INT8>(c, t, few, p.few, st)) return e;
+    if (int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, few, p.few, p.kinds, st) : stream_sizes<KV_INT8>(c, t, few, p.few, p.kinds, st)) return e;
   }
   if ((p.few.pieces <= 1 || p.few.cluster) && p.many.pieces <= 1) return KB2SEQ_OK;
   const int most = std::max(p.few.pieces, p.many.pieces);
   const bool wide = (long long)t.T * H <= 4096 || (most > 8 && (long long)t.T * H <= 16384) || most > 32;
   auto join = wide ? kv_join_kernel<4> : kv_join_kernel<1>;
-  kb2::launch_pdl(join, (unsigned)(wide ? (long long)t.T * H : ((long long)t.T * H + 3) / 4), 128, 0, st, c, t, few, many);
+  kb2::launch_pdl(join, (unsigned)(wide ? (long long)t.T * H : ((long long)t.T * H + 3) / 4), 128, 0, st, c, t, few, many, p.kinds);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }

@@ -19,8 +19,7 @@ struct KvAttn {                              // what a call says beside the cach
   const float* sinks;
   void* out;
   int dt_out;
-  int least, most, rows, per_seq;            // the sequences that have least .. most rows (tokens times heads per kv head), in tiles of `rows`; per_seq: the tiles of
-                                             // each where the step's sequences bring as many tokens each, else 0
+  int rows, per_seq;                         // rows (tokens times heads per kv head) a tile; per_seq: the tiles of each sequence where the step's bring as many tokens each, else 0
   int piece, pieces;                         // groups of 16 keys a piece; the most pieces of a tile
   float *part_o, *part_ml;                   // [T H][pieces][dv] and [T H][pieces][2]
   bool cluster;                              // a tile's pieces are the blocks of a cluster, which joins them itself
@@ -87,7 +86,8 @@ __device__ __forceinline__ int kv_cut(const KvLayer& c, const KvStep& t, const K
 }
 // The (sequence, tile, piece) number `at`, the pieces of one sequence behind those of the one before, a piece's tiles together (they read the same keys).  One warp; false
 // behind the last.
-__device__ __forceinline__ bool kv_find_piece(const KvLayer& c, const KvStep& t, const KvAttn& a, int per, int at, int* seq, int* tile, int* piece, int* length) {
+__device__ __forceinline__ bool kv_find_piece(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, int per, int at, int* seq, int* tile, int* piece,
+                                              int* length) {
   const int lane = threadIdx.x & 31;
   int before = 0;
   for (int s0 = 0; s0 < t.S; s0 += 32) {
@@ -95,7 +95,7 @@ __device__ __forceinline__ bool kv_find_piece(const KvLayer& c, const KvStep& t,
     int tiles = 0, len = 1, n = 0;
     if (s < t.S) {
       const int have = (t.cu[s + 1] - t.cu[s]) * per;
-      tiles = have >= a.least && have <= a.most ? (have + a.rows - 1) / a.rows : 0;
+      tiles = have > 0 && kinds.on_tiles(s) ? (have + a.rows - 1) / a.rows : 0;
       if (tiles) n = tiles * (a.pieces > 1 ? kv_cut(c, t, a, s, &len) : 1);
     }
     int upto = n;
@@ -158,8 +158,8 @@ __device__ __forceinline__ void query4(const KvAttn& a, long long from, int left
 }
 
 // Tiles on the tensor cores: 256 rows (seq_kv_pair.cu), 128 where tensor memory has no room for two outputs (seq_kv_tile.cu).
-int kv_pair_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t stream);
-int kv_tile_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t stream);
+int kv_pair_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, int tiles, cudaStream_t stream);
+int kv_tile_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, int tiles, cudaStream_t stream);
 inline bool kv_pairs(int d, int dv) { return d <= 192 && dv <= 128; }
 
 }  // namespace kb2seq

@@ -73,7 +73,7 @@ __device__ __forceinline__ void pair_store(uint8_t* to, int ct, const uint32_t (
 }
 
 template <int FMT, int NC, int NV>
-__global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep t, KvAttn a) {
+__global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep t, KvAttn a, const __grid_constant__ KvKinds kinds) {
   using L = PairShape<NC, NV>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     s = blockIdx.x / a.per_seq;
     tile = blockIdx.x - s * a.per_seq;
   } else {
-    in = kv_find_piece(c, t, a, per, blockIdx.x, &s, &tile, &z, &length);
+    in = kv_find_piece(c, t, a, kinds, per, blockIdx.x, &s, &tile, &z, &length);
   }
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * 256, nr = in ? (int)min((long long)n * per - r0, 256ll) : 0;
   int u0 = 0, u1 = 0, np = 0, t0 = c0;
@@ -506,23 +506,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
 }
 
 template <int FMT, int NC, int NV>
-int launch(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t st) {
+int launch(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, int tiles, cudaStream_t st) {
   using L = PairShape<NC, NV>;
   SEQ_CUDA((kb2::allow_smem<kv_pair_kernel<FMT, NC, NV>>(L::kTotal)));
   auto kern = kv_pair_kernel<FMT, NC, NV>;
-  kb2::launch_pdl(kern, dim3(tiles, c.G), kThreads, L::kTotal, st, c, t, a);
+  kb2::launch_pdl(kern, dim3(tiles, c.G), kThreads, L::kTotal, st, c, t, a, kinds);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }
 template <int FMT>
-int sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t st) {
-  if (c.d <= 64 && c.dv <= 64) return launch<FMT, 1, 1>(c, t, a, tiles, st);
-  return c.d <= 128 ? launch<FMT, 2, 2>(c, t, a, tiles, st) : launch<FMT, 3, 2>(c, t, a, tiles, st);
+int sizes(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, int tiles, cudaStream_t st) {
+  if (c.d <= 64 && c.dv <= 64) return launch<FMT, 1, 1>(c, t, a, kinds, tiles, st);
+  return c.d <= 128 ? launch<FMT, 2, 2>(c, t, a, kinds, tiles, st) : launch<FMT, 3, 2>(c, t, a, kinds, tiles, st);
 }
 }  // namespace
 
-int kv_pair_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, int tiles, cudaStream_t stream) {
-  return fmt == KV_E4M3 ? sizes<KV_E4M3>(c, t, a, tiles, stream) : sizes<KV_INT8>(c, t, a, tiles, stream);
+int kv_pair_attend(int fmt, const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, int tiles, cudaStream_t stream) {
+  return fmt == KV_E4M3 ? sizes<KV_E4M3>(c, t, a, kinds, tiles, stream) : sizes<KV_INT8>(c, t, a, kinds, tiles, stream);
 }
 
 }  // namespace kb2seq

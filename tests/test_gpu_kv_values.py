@@ -95,3 +95,47 @@ def test_a_zero_value_far_above_large_ones(H, G, d, dv, above, forms):  # noqa: 
             assert bool(torch.isfinite(got).all())
             err = (got.double().cpu() - want).abs()
             assert bool((err <= off).all()), (float((err / off).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("lens,keep,tiles_from", [([(1, 300), (30, 200), (12, 100)], 39, 40), ([(20, 500)], 3, 17), ([(1, 900), (1, 20), (50, 700), (13, 0), (40, 31)], 66, 33),
+                                                  ([(12, 700)] * 3, 26, 48), ([(64, 2000), (64, 3000)], 70, 0), ([(1, 4000), (12, 3000), (20, 0)], 5, 24)])
+@pytest.mark.parametrize("H,G,d", [(8, 2, 128), (8, 2, 256)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_fewer_tokens_than_the_layout_has(lens, keep, tiles_from, H, G, d, tree, monkeypatch):
+    """The device's table of first tokens ends early: what is left of a sequence that was planned for the tiles has few rows, and is attended to all the same."""
+    from krasis_b200 import seqops as ops
+    monkeypatch.setattr(ops, "KV_TILES_FROM", tiles_from)
+    tb, seqs, pages = _step(lens, 64, 53, parents=[_tree(n, n, 4) for n, _ in lens] if tree else None)
+    c = _cache(G, d, d, pages, "int8", seed=54)
+    T, at = tb.T, 0
+    tb.cu.clamp_(max=keep)
+    for i, (n, start, pl, parents) in enumerate(seqs):
+        left = max(0, min(n, keep - at))
+        at += n
+        seqs[i] = (left, start, pl, parents[:left] if tree else None)
+    q = torch.randn(T, H, d, generator=_gen(55)).to(BF).cuda()
+    call = ops.kv_tree_attn if tree else ops.kv_attn
+    for window, first in ((None, 0), (150, 20)):
+        want, *sizes = kv_plain.attention(q[:keep], c, 0, [s for s in seqs if s[0]], d ** -0.5, window, first)
+        for do in (BF, F32):
+            out = torch.full((T, H, d), 7.0, dtype=do, device="cuda")
+            call(q, tb, c, 0, d ** -0.5, window=window, first=first, out=out)
+            assert bool((out[keep:] == 7).all())
+            off = kv_plain.off_by(BF, do, max(n + s for n, s, _, _ in seqs), d, want, *sizes, decoded=True)      # the tiles take what the layout gives them
+            err = (out[:keep].double().cpu() - want).abs()
+            assert bool((err <= off).all()), (float((err / off).max()), float(err.max()))
+
+
+def test_more_sequences_than_there_are_bits(monkeypatch):
+    """Steps of thousands of sequences, some of them for the tiles: alone between others of few rows, and in a long run."""
+    from krasis_b200 import seqops as ops
+    monkeypatch.setattr(ops, "KV_TILES_FROM", 17)
+    lens = [(5 if i in (7, 2050, 4099) or 3000 <= i < 3040 else 1, i * 7 % 40) for i in range(4100)]
+    tb, seqs, pages = _step(lens, 16, 56)
+    c = _cache(1, 64, 64, pages, "e4m3", 16, seed=57)
+    q = torch.randn(tb.T, 4, 64, generator=_gen(58)).to(BF).cuda()
+    want, *sizes = kv_plain.attention(q, c, 0, seqs, 0.125)
+    got = ops.kv_attn(q, tb, c, 0, 0.125)
+    off = kv_plain.off_by(BF, BF, 45, 64, want, *sizes, decoded=True)
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= off).all()), (float((err / off).max()), float(err.max()))
