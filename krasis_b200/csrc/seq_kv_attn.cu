@@ -56,8 +56,8 @@ struct StreamShape {
   static constexpr int kRow = VU * 64 + 8;                                // numbers from row to row of a warp's share at the end: 32 bytes apart in the banks
   static constexpr int kRing = kSWarps * kSStages * kStage, kShare = MT * (VU * 64 + 4) * 4, kRed = kSWarps * MT * kRow * 4 + kShare;      // kShare: what a block has for the others of its cluster
   static constexpr int kOffRow = kRing > kRed ? kRing : kRed, kOffStat = kOffRow + kSMostGroups * 4, kOffTok = kOffStat + kSWarps * MT * 4 * 4, kOffQ = kOffTok + MT * 16,
-                       kOffScan = kOffQ + kQ;
-  static constexpr int kTotal = kOffScan + (kMostTiles + 4) * 4;
+                       kOffScan = kOffQ + kQ, kOffParts = kOffScan + (kMostTiles + 4) * 4;
+  static constexpr int kTotal = kOffParts + 16;
   static constexpr int kBlocks = 2 * (kTotal + 1024) <= 227 * 1024 ? 2 : 1;
   static_assert(kTotal <= 227 * 1024 && kOffQ % 16 == 0 && kStage % 16 == 0, "shared memory");
 };
@@ -68,23 +68,24 @@ __device__ __forceinline__ float4 lds_of(const float* p, int rank) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(kb2::cluster_addr(p, rank)));
   return v;
 }
-// Eight columns of a row: finished, or as piece z with its maximum and sum.
-__device__ __forceinline__ void store8(const KvLayer& c, const KvAttn& a, const float (&acc)[8], float top, float sum, long long row, int hd, int dim, int z) {
+// Eight columns of a row: finished (part < 0), or as a partial result with its maximum and sum.
+__device__ __forceinline__ void store8(const KvLayer& c, const KvAttn& a, const float (&acc)[8], float top, float sum, long long row, int hd, int dim, long long part) {
   float y[8];
   float by = 1.f;
-  if (z < 0) {
+  if (part >= a.parts) return;
+  if (part < 0) {
     if (a.sinks != nullptr && top != -INFINITY) sum += ex2(fmaf(a.sinks[hd], kLog2e, -top));
     by = sum == 0.f ? 0.f : 1.f / sum;
   } else if (dim == 0) {
-    *reinterpret_cast<float2*>(a.part_ml + 2 * (row * a.pieces + z)) = make_float2(top, sum);
+    *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(top, sum);
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = acc[e] * by;
-  if (z < 0 && a.dt_out) {
+  if (part < 0 && a.dt_out) {
     *reinterpret_cast<uint4*>((bf16*)a.out + row * c.dv + dim) =
         make_uint4(kb2::bf16x2_bits_rn(y[1], y[0]), kb2::bf16x2_bits_rn(y[3], y[2]), kb2::bf16x2_bits_rn(y[5], y[4]), kb2::bf16x2_bits_rn(y[7], y[6]));
   } else {
-    float4* to = reinterpret_cast<float4*>(z < 0 ? (float*)a.out + row * c.dv + dim : a.part_o + (row * a.pieces + z) * c.dv + dim);
+    float4* to = reinterpret_cast<float4*>(part < 0 ? (float*)a.out + row * c.dv + dim : a.part_o + part * c.dv + dim);
     to[0] = make_float4(y[0], y[1], y[2], y[3]);
     to[1] = make_float4(y[4], y[5], y[6], y[7]);
   }
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     z = groups == 0 ? 0 : (int)(next_chunk - gridDim.x - first);
     s = number / a.per_seq;
     tile = number - s * a.per_seq;
-    if (z == 0 && threadIdx.x == 0) a.counts[number * c.G + head] = np;
+    if (z == 0 && threadIdx.x == 0) a.counts[number * c.G + head] = make_int2(np, (int)first);
   } else {
     if (!once) return;
     head = blockIdx.y;
@@ -297,6 +298,16 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   };
 #pragma unroll
   for (int i = 0; i < kSStages; ++i) issue(u0 + warp + i * kSWarps, i);
+
+  // where this piece's results go, those of row 0 of the tile (an even cut) or of the sequence, and how far apart rows are; looked up while the first keys are on their way
+  KvParts* mine = reinterpret_cast<KvParts*>(smem + L::kOffParts);
+  if (warp == 0 && !a.cluster) {
+    KvParts parts{-1, 0};
+    if (np > 1 && a.linear) parts = {(next_chunk - gridDim.x + number * c.G + head) * MT, 1};
+    else if (np > 1) parts = kv_parts(c, t, a, kinds, false, s);
+    if (np > 1 && !a.linear) parts.first += z;
+    if (lane == 0) *mine = parts;
+  }
 
   constexpr int QR = L::kQShared ? 1 : DU * 4;
   uint32_t qf[QR][PARTS][2 * NQ];
@@ -541,7 +552,11 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
       if (dim == 0) *reinterpret_cast<float4*>(share + VU * 64) = make_float4(top, sum, 0.f, 0.f);
       continue;
     }
-    store8(c, a, acc, top, sum, (long long)(c0 + (r0 + q) / per) * a.H + head * per + (r0 + q) % per, head * per + (r0 + q) % per, dim, np <= 1 ? -1 : z);
+    const int hd = head * per + (r0 + q) % per;
+    const long long row = (long long)((r0 + q) / per) * a.H + hd;          // of the sequence
+    const KvParts parts = *mine;
+    const long long part = parts.first < 0 ? -1 : parts.first + (a.linear ? q : row * parts.pieces);
+    store8(c, a, acc, top, sum, (long long)c0 * a.H + row, hd, dim, part);
   }
   if (a.cluster) {
     kb2::cluster_sync_all();
@@ -582,36 +597,81 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
 
 // The pieces of a row (token, head), joined in a fixed order; rows that one piece finished are left alone.  x, y: sequences of few rows, and those on tiles.  W warps a row take the pieces in
 // turn, four of a warp's on their way at once (one at a time 64 pieces took 27 us).  One request of 30000 rows, 16 / 2 heads: four warps a row 17 us in all, one 38 at the time;
-// 62000 rows of few pieces: four warps 50 us more than one.
+// 62000 rows of few pieces: four warps 50 us more than one.  `rows`: of the sequences that are cut, one behind the other.
 template <int W>
-__global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAttn x, KvAttn y, const __grid_constant__ KvKinds kinds) {
+__global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAttn x, KvAttn y, const __grid_constant__ KvKinds kinds, int rows) {
   __shared__ float weights[W > 1 ? kMostPieces : 4 * 32];
   __shared__ __align__(16) float share[3][256];
   __shared__ float total[4];
   kb2::pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wr = warp % W, at = wr * 32 + lane;
-  const long long row = (long long)blockIdx.x * (4 / W) + warp / W;
-  const int tok = (int)(row / x.H), hd = (int)(row - (long long)tok * x.H);
+  int at_row = (int)(blockIdx.x * (4 / W) + warp / W);
   float* weight = weights + (W > 1 ? 0 : warp * 32);
   const auto meet = [&] {
     if (W > 1) __syncthreads();
     else __syncwarp();
   };
-  if (tok >= t.T) return;
-  if (tok >= t.cu[t.S]) return;
-  const int per = x.H / c.G, s = t.seq_of[tok], c0 = t.cu[s], n = t.cu[s + 1] - c0;
+  if (at_row >= rows) return;
+  int s = -1;
+  KvParts parts{};
+  if (x.linear) {                            // all sequences are
+    const int tok = at_row / x.H;
+    if (tok >= t.cu[t.S]) return;
+    s = t.seq_of[tok];
+    at_row -= t.cu[s] * x.H;
+  } else {
+    int before = 0;
+    long long ahead[2] = {};                 // parts of sequences of few rows, of those on tiles
+    for (int s0 = 0; s0 < t.S; s0 += 32) {
+      const int q = s0 + lane;
+      const bool tiles = q < t.S && kinds.on_tiles(q);
+      const int cut = q < t.S ? kv_pieces(c, t, tiles ? y : x, q) : 1, n = cut > 1 ? (t.cu[q + 1] - t.cu[q]) * x.H : 0;
+      int upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > at_row);
+      const int l = hit ? __ffs(hit) - 1 : 32;
+      const bool kind = __shfl_sync(0xffffffffu, tiles, l & 31);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        long long take = lane < l && tiles == (k == 1) ? (long long)n * cut : 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) take += __shfl_xor_sync(0xffffffffu, take, o);
+        ahead[k] += take;
+      }
+      if (hit) {
+        s = s0 + l;
+        parts = {kind ? ahead[1] : ahead[0], __shfl_sync(0xffffffffu, cut, l)};
+        at_row -= before + __shfl_sync(0xffffffffu, upto - n, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (s < 0) return;
+  }
+  const int per = x.H / c.G, c0 = t.cu[s], n = t.cu[s + 1] - c0, tok = c0 + at_row / x.H, hd = at_row % x.H;
+  const long long row = (long long)tok * x.H + hd;
   const KvAttn& a = kinds.on_tiles(s) ? y : x;
-  if (a.pieces <= 1 || a.cluster) return;
-  const int r0 = ((tok - c0) * per + hd % per) / a.rows * a.rows, nr = (int)min((long long)n * per - r0, (long long)a.rows);
+  const int in_seq = (tok - c0) * per + hd % per, r0 = in_seq / a.rows * a.rows, nr = (int)min((long long)n * per - r0, (long long)a.rows);
   const KvSpan span = kv_span(c, t, s, c0 + r0 / per, c0 + (r0 + nr - 1) / per, a.window, a.first);
   int length = a.piece;
   if (a.rows > 16) kv_cut(c, t, a, s, &length);
-  const int np = a.linear ? a.counts[(s * a.per_seq + r0 / a.rows) * c.G + hd / per] : min((span.groups() + length - 1) / length, a.pieces);
-  if (np <= 1) return;
-  const long long p0 = row * a.pieces;
+  int np = min((span.groups() + length - 1) / length, a.pieces), step = 1;
+  long long p0 = parts.first + (long long)at_row * parts.pieces;
+  if (a.linear) {
+    const int number = (s * a.per_seq + r0 / a.rows) * c.G + hd / per;
+    const int2 v = a.counts[number];
+    np = v.x;
+    step = a.rows;
+    p0 = (long long)(v.y + number) * step + in_seq - r0;
+  }
+  if (np <= 1 || p0 + (long long)(np - 1) * step >= a.parts) return;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
   float top = -INFINITY, sum = 0.f;
-  for (int i = at; i < np; i += 32 * W) top = fmaxf(top, ml[i].x);
+  for (int i = at; i < np; i += 32 * W) top = fmaxf(top, ml[i * step].x);
   top = warp_max(top);
   if (W > 1) {
     if (lane == 0) total[warp] = top;
@@ -620,7 +680,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
     meet();
   }
   for (int i = at; i < np; i += 32 * W) {
-    const float2 v = ml[i];
+    const float2 v = ml[i * step];
     const bool none = v.x == -INFINITY;      // a piece without a maximum holds zeros, or NaN
     weight[i] = none ? 1.f : ex2(v.x - top);
     sum += none ? v.y : v.y * weight[i];
@@ -636,7 +696,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        v[i][h] = i0 + W * i < np && h * 128 + lane * 4 < c.dv ? *reinterpret_cast<const float4*>(a.part_o + (p0 + i0 + W * i) * c.dv + h * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[i][h] = i0 + W * i < np && h * 128 + lane * 4 < c.dv ? *reinterpret_cast<const float4*>(a.part_o + (p0 + (i0 + W * i) * step) * c.dv + h * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float f = i0 + W * i < np ? weight[i0 + W * i] : 0.f;
@@ -687,7 +747,11 @@ constexpr long long kWideWaves = 2;          // pieces for each SM, of such sequ
 struct KvPlan {
   int rows, tiles, per_seq, piece, pieces, blocks;                         // blocks: of the even cut (0 for pieces of tiles); of tiles on the tensor cores, pieces and all
   bool cluster;                              // the pieces of a tile are a cluster, which joins them itself
+  long long parts, joined;                   // partial results; rows (token, head) of the sequences that are cut
   size_t floats;                             // workspace
+  void size(int H, int G, int dv, bool wide) {       // what lies behind begins on 16 bytes too
+    floats = ((size_t)parts * (dv + 2) + (blocks && !wide ? 2 * (size_t)tiles * G : 0) + 3) / 4 * 4;
+  }
 };
 // The most groups of 16 that the tokens start .. start + n - 1 see.
 inline long long groups_seen(long long start, long long n, int window, int first) {
@@ -723,6 +787,11 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
   }
   if (p.tiles == 0) return p;
   p.per_seq = same ? p.tiles / step->S : 0;
+  const auto cut = [&](int s, long long n) { // into n pieces
+    const long long rows = n > 1 ? (long long)step->layout[4 * s + 1] * H : 0;
+    p.joined += rows;
+    p.parts += rows * n;
+  };
   long long piece;
   if (wide) {                                // one block an SM; a piece of at least four tiles of keys
     const long long want = kWideWaves * kb2::current_sms();
@@ -730,8 +799,12 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
     if ((long long)p.tiles * cache->G >= 2ll * kb2::current_sms() && same) piece = top;
     p.piece = (int)std::max(piece, 8ll);
     p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
-    for (int s = 0; s < step->S; ++s) p.blocks += tiles(s) ? (int)(tiles(s) * std::max(1ll, (seen(s) + p.piece - 1) / p.piece)) : 0;
-    p.floats = p.pieces > 1 ? ((size_t)step->T * H * p.pieces * (cache->dv + 2) + 3) / 4 * 4 : 0;
+    for (int s = 0; s < step->S; ++s) {
+      const long long n = tiles(s) ? std::max(1ll, (seen(s) + p.piece - 1) / p.piece) : 0;
+      p.blocks += (int)(tiles(s) * n);
+      cut(s, n);
+    }
+    p.size(H, cache->G, cache->dv, wide);
     return p;
   } else {
     // Blocks of one length in whole waves, as the last wave takes as long as the others: the length whose waves, with what a block costs beside its keys (some 16 groups), end
@@ -773,8 +846,15 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
     piece = best;
   }
   p.piece = (int)std::max(piece, 8ll);
-  if (!p.blocks) p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
-  p.floats = p.pieces > 1 ? ((size_t)step->T * H * p.pieces * (cache->dv + 2) + (p.blocks ? (size_t)p.tiles * cache->G : 0) + 3) / 4 * 4 : 0;      // what lies behind begins on 16 bytes too
+  if (p.blocks) {                            // a chunk for each block, or each kSMostGroups groups where that is more; a piece ends a chunk or a tile of a head
+    const long long all = (work + (long long)p.tiles * kPieceCost) * cache->G;
+    p.parts = (std::max<long long>(p.blocks, (all + kSMostGroups - 1) / kSMostGroups) + (long long)p.tiles * cache->G) * p.rows;
+    p.joined = (long long)step->T * H;
+  } else {
+    p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
+    for (int s = 0; s < step->S; ++s) cut(s, tiles(s) ? (seen(s) + p.piece - 1) / p.piece : 0);
+  }
+  p.size(H, cache->G, cache->dv, wide);
   return p;
 }
 struct KvPlans {
@@ -825,16 +905,17 @@ KvPlans kv_plans(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int
   if (kinds.every) p.many = kv_plan(cache, step, H, window, first, kinds, true);
   return p;
 }
-inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int rows_total, int dv) {
+inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int dv) {
   a.rows = p.rows;
   a.per_seq = p.per_seq;
   a.piece = p.piece;
   a.pieces = p.pieces;
   a.part_o = work;
-  a.part_ml = work + (size_t)rows_total * p.pieces * dv;
+  a.part_ml = work + (size_t)p.parts * dv;
+  a.parts = p.parts;
   a.linear = p.blocks > 0 && p.rows <= 16;
   a.cluster = p.cluster;
-  a.counts = reinterpret_cast<int*>(a.part_ml + 2 * (size_t)rows_total * p.pieces);
+  a.counts = reinterpret_cast<int2*>(a.part_ml + 2 * (size_t)p.parts);
   return a;
 }
 
@@ -904,7 +985,7 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   a.sinks = sinks;
   a.out = out;
   a.dt_out = dt_out;
-  const KvAttn few = with_plan(a, p.few, (float*)work, t.T * H, c.dv), many = with_plan(a, p.many, (float*)work + p.few.floats, t.T * H, c.dv);
+  const KvAttn few = with_plan(a, p.few, (float*)work, c.dv), many = with_plan(a, p.many, (float*)work + p.few.floats, c.dv);
   const cudaStream_t st = (cudaStream_t)stream;
   if (p.many.tiles) {
     if (int e = (kv_pairs(c.d, c.dv) ? kv_pair_attend : kv_tile_attend)(cache->fmt, c, t, many, p.kinds, p.many.blocks, st)) return e;
@@ -912,11 +993,12 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   if (p.few.tiles) {
     if (int e = cache->fmt == KV_E4M3 ? stream_sizes<KV_E4M3>(c, t, few, p.few, p.kinds, st) : stream_sizes<KV_INT8>(c, t, few, p.few, p.kinds, st)) return e;
   }
-  if ((p.few.pieces <= 1 || p.few.cluster) && p.many.pieces <= 1) return KB2SEQ_OK;
-  const int most = std::max(p.few.pieces, p.many.pieces);
-  const bool wide = (long long)t.T * H <= 4096 || (most > 8 && (long long)t.T * H <= 16384) || most > 32;
+  const long long rows = p.few.joined + p.many.joined;
+  if (rows == 0) return KB2SEQ_OK;
+  const int most = std::max(p.few.cluster ? 1 : p.few.pieces, p.many.pieces);
+  const bool wide = rows <= 4096 || (most > 8 && rows <= 16384) || most > 32;
   auto join = wide ? kv_join_kernel<4> : kv_join_kernel<1>;
-  kb2::launch_pdl(join, (unsigned)(wide ? (long long)t.T * H : ((long long)t.T * H + 3) / 4), 128, 0, st, c, t, few, many, p.kinds);
+  kb2::launch_pdl(join, (unsigned)(wide ? rows : (rows + 3) / 4), 128, 0, st, c, t, few, many, p.kinds, (int)rows);
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }

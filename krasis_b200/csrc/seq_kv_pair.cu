@@ -31,7 +31,7 @@ template <int NC, int NV>                    // chunks of 64 of d and dv
 struct PairShape {
   static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128, kKeys = NC > 2 ? 2 : kBufs;      // kKeys: buffers of keys
   static constexpr int kOffQ = 0, kOffK = 2 * kQ, kOffV = kOffK + kKeys * kK, kOffFac = kOffV + kBufs * kV, kOffGroup = kOffFac + kPlans * 512,
-                       kOffBar = kOffGroup + kPlans * 32, kOffUnit = kOffBar + 320, kOffTmem = kOffUnit + kUnits * 16, kOffRow = kOffTmem + 16, kTotal = kOffRow + 256 * 4;
+                       kOffBar = kOffGroup + kPlans * 32, kOffParts = kOffBar + 304, kOffUnit = kOffParts + 16, kOffTmem = kOffUnit + kUnits * 16, kOffRow = kOffTmem + 16, kTotal = kOffRow + 256 * 4;
   static_assert(kTotal <= 227 * 1024 && 4 * FK + 128 * NV <= 512, "memory");
   static_assert(128 * (64 * NV + 1) * 4 + 128 * 12 <= 2 * kQ + kKeys * kK + kBufs * kV, "the second group's share at the end");
 };
@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
   int* groups = reinterpret_cast<int*>(smem + L::kOffGroup);               // [kPlans][8] where the groups lie (rows / 16), -1: nowhere
   float4* units = reinterpret_cast<float4*>(smem + L::kOffUnit);           // [kUnits] of keys, of values; four bits a group: whether it lies nowhere
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
+  KvParts* seq_parts = reinterpret_cast<KvParts*>(smem + L::kOffParts);    // where the sequence's partial results lie
   float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [256] what the queries' own scaling is undone with
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (warp == 2) tmem_alloc(tmem_at, 512);
@@ -97,7 +98,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     s = blockIdx.x / a.per_seq;
     tile = blockIdx.x - s * a.per_seq;
   } else {
-    in = kv_find_piece(c, t, a, kinds, per, blockIdx.x, &s, &tile, &z, &length);
+    KvParts parts{};
+    in = kv_find_piece(c, t, a, kinds, per, blockIdx.x, &s, &tile, &z, &length, &parts);
+    if (threadIdx.x == 0) *seq_parts = parts;
   }
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * 256, nr = in ? (int)min((long long)n * per - r0, 256ll) : 0;
   int u0 = 0, u1 = 0, np = 0, t0 = c0;
@@ -340,8 +343,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       tc_fence_after_sync();
     }
     const int hd = head * per + rr % per;
-    const long long orow = (long long)tok * a.H + hd, part = orow * a.pieces + z;
     const bool whole = np <= 1;
+    const long long orow = (long long)tok * a.H + hd, part = whole ? 0 : seq_parts->first + (orow - (long long)c0 * a.H) * seq_parts->pieces + z;
+    const bool kept = live && (whole || part < a.parts);
     float ref1 = 0.f;
     constexpr int kPad = 64 * NV + 1;        // numbers a row, an odd number: a row a thread meets every bank once
     float* share = reinterpret_cast<float*>(smem + L::kOffQ) + (quarter * 32 + lane) * kPad;
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     if (two || grp == 0) {
       if (whole && live && a.sinks != nullptr && m != -INFINITY) l += ex2(fmaf(a.sinks[hd], kLog2e, -m));
       const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f, by = ref * inv, by1 = ref1 * inv, none = l != l ? l : 0.f;      // a NaN may have a reference of 0
-      if (!whole && live) {
+      if (!whole && kept) {
         a.part_ml[2 * part] = m;
         a.part_ml[2 * part + 1] = l;
       }
@@ -384,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
         __syncwarp();                          // the warp reads tensor memory together
         tmem_ld16(o_at + o, r);
         tmem_ld_wait();
-        if (!live || o >= c.dv) continue;
+        if (!kept || o >= c.dv) continue;
         float y[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]) * by + none;

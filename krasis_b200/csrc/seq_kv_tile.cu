@@ -27,7 +27,7 @@ struct TileShape {
   static constexpr int VS = NC + NV > 6 ? 1 : 2;                           // buffers of values
   static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128;
   static constexpr int kSlots = 3, kCodes = FK * 64 * (NC > NV ? NC : NV), kSlot = kCodes + FK * 8;       // codes as they come | scales of keys | of values
-  static constexpr int kOffQ = 0, kOffK = kQ, kOffV = kOffK + 2 * kK, kOffSlot = kOffV + VS * kV, kOffBar = kOffSlot + kSlots * kSlot, kOffRef = kOffBar + 192,
+  static constexpr int kOffQ = 0, kOffK = kQ, kOffV = kOffK + 2 * kK, kOffSlot = kOffV + VS * kV, kOffBar = kOffSlot + kSlots * kSlot, kOffParts = kOffBar + 176, kOffRef = kOffParts + 16,
                        kOffHave = kOffRef + 4 * 8, kOffGone = kOffHave + kSlots * 4, kOffTmem = kOffGone + 4 * 4, kOffX = kOffTmem + 4, kOffRow = kOffX + 2 * 2 * 128 * 4;
   static constexpr int kTotal = kOffRow + 128 * 4;
   static_assert(kTotal <= 227 * 1024 && 3 * FK + 64 * NV <= 512 && kSlot % 128 == 0 && kOffRef % 8 == 0 && kOffX % 16 == 0, "memory");
@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
   uint32_t* have = reinterpret_cast<uint32_t*>(smem + L::kOffHave);        // [3] a slot's groups that are there, a bit each
   uint32_t* gone = reinterpret_cast<uint32_t*>(smem + L::kOffGone);        // [4] a tile's groups that are not
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
+  KvParts* seq_parts = reinterpret_cast<KvParts*>(smem + L::kOffParts);    // where the sequence's partial results lie
   float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [128] what the queries' own scaling is undone with
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -110,7 +111,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     s = blockIdx.x / a.per_seq;
     tile = blockIdx.x - s * a.per_seq;
   } else {
-    in = kv_find_piece(c, t, a, kinds, per, blockIdx.x, &s, &tile, &z, &length);
+    KvParts parts{};
+    in = kv_find_piece(c, t, a, kinds, per, blockIdx.x, &s, &tile, &z, &length, &parts);
+    if (threadIdx.x == 0) *seq_parts = parts;
   }
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * kRows, nr = in ? (int)min((long long)n * per - r0, (long long)kRows) : 0;
   int u0 = 0, u1 = 0, np = 0, t0 = c0, t1 = c0;
@@ -461,11 +464,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     if (n_tiles >= 2) pv_wait(n_tiles - 2);
     pv_wait(n_tiles - 1);
     const int hd = head * per + rr % per;
-    const long long orow = (long long)tok * a.H + hd, part = orow * a.pieces + z;
     const bool whole = np <= 1;
+    const long long orow = (long long)tok * a.H + hd, part = whole ? 0 : seq_parts->first + (orow - (long long)c0 * a.H) * seq_parts->pieces + z;
+    const bool kept = live && (whole || part < a.parts);
     if (whole && live && a.sinks != nullptr && m != -INFINITY) l += ex2(fmaf(a.sinks[hd], kLog2e, -m));
     const float by = whole ? (l == 0.f ? 0.f : ref / l) : ref;
-    if (!whole && live && hf == 0) {
+    if (!whole && kept && hf == 0) {
       a.part_ml[2 * part] = m;
       a.part_ml[2 * part + 1] = l;
     }
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       __syncwarp();                          // the warp reads tensor memory together
       tmem_ld16(lane_at + kColO + o, r);
       tmem_ld_wait();
-      if (!live || o >= c.dv) continue;
+      if (!kept || o >= c.dv) continue;
       float y[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]) * by + (l != l ? l : 0.f);         // a sum that is NaN has a zero for its reference, maybe
