@@ -263,7 +263,7 @@ KB2SEQ_API int kb2_seq_kv_write(const kb2_seq_kv_cache* cache, int layer, const 
   KvLayer c;
   KvStep t;
   if (int e = kv_args("kv_write", cache, layer, step, &c, &t)) return e;
-  if (!k || !v || bad_dt(dt)) return failf(KB2SEQ_ERR_VALUE, "kv_write: bad argument");
+  if (bad_dt(dt) || (t.T > 0 && (!k || !v))) return failf(KB2SEQ_ERR_VALUE, "kv_write: bad argument");
   if (t.T == 0) return KB2SEQ_OK;
   OnDevice on(step->device);
   SEQ_CUDA(on.err);

@@ -118,7 +118,8 @@ struct OnDevice {
 
 // The two structures of the C interface as the kernels take them.
 inline int kv_args(const char* name, const kb2_seq_kv_cache* cache, int layer, const kb2_seq_kv_step* step, KvLayer* c, KvStep* t) {
-  if (!cache || !step || !cache->k || !cache->v || !cache->k_scale || !cache->v_scale || !step->positions || !step->seq_of || !step->cu || !step->pages || !step->layout)
+  if (!cache || !step || !cache->k || !cache->v || !cache->k_scale || !cache->v_scale || !step->cu || !step->pages || !step->layout ||
+      (step->T > 0 && (!step->positions || !step->seq_of)))                // of no tokens there are none
     return failf(KB2SEQ_ERR_VALUE, "%s: a pointer is missing", name);
   if (((uintptr_t)cache->k | (uintptr_t)cache->v | (uintptr_t)cache->k_scale | (uintptr_t)cache->v_scale) & 15)
     return failf(KB2SEQ_ERR_VALUE, "%s: the pools begin on 16 bytes", name);

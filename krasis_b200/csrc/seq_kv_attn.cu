@@ -951,7 +951,7 @@ using namespace kb2seq;
 extern "C" {
 
 KB2SEQ_API size_t kb2_seq_kv_attn_workspace(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H, int window, int first, int dt_out) {
-  if (!cache || !step || !step->layout || cache->G < 1 || H < cache->G || bad_dt(dt_out)) return 0;
+  if (!cache || !step || !step->layout || step->T < 1 || cache->G < 1 || H < cache->G || bad_dt(dt_out)) return 0;
   OnDevice on(step->device);
   return kv_plans(cache, step, H, window > 0 ? std::min(window, kKvNoWindow) : kKvNoWindow, first, dt_out).bytes();
 }
@@ -961,7 +961,7 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   KvLayer c;
   KvStep t;
   if (int e = kv_args("kv_attn", cache, layer, step, &c, &t)) return e;
-  if (!q || !out || ((uintptr_t)out & 15) || bad_dt(dt_q) || bad_dt(dt_out) || H < c.G || H % c.G || window < 0 || first < 0 || !std::isfinite(scale))
+  if ((t.T > 0 && (!q || !out)) || ((uintptr_t)out & 15) || bad_dt(dt_q) || bad_dt(dt_out) || H < c.G || H % c.G || window < 0 || first < 0 || !std::isfinite(scale))
     return failf(KB2SEQ_ERR_VALUE, "kv_attn: bad argument");
   if (c.G > 65535 || (long long)t.T * H > 0x7FFFFFFFll / 2) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many heads or tokens");
   if (t.T == 0) return KB2SEQ_OK;

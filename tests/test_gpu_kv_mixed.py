@@ -87,3 +87,27 @@ def test_captured_mixed_steps(monkeypatch):
         for w, do, (_, out) in graphs:
             _check(out, q, c, seqs, scale=0.09, window=w, first=3)
         del kept
+
+
+def test_steps_without_tokens():
+    """Every call on a step that brings no tokens, and rows read back through such tables."""
+    from krasis_b200 import seqops as ops
+    c = _cache(2, 64, 32, 4, "int8", seed=71)
+    entries = [([], 100, 0, [2, 0]), ([], 0, 1, [])]
+    tb, dt = ops.StepTables(entries, "cuda"), ops.DraftTables([e + ([],) for e in entries], "cuda")
+    before = [t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale)]
+    k, v, q = (torch.zeros(0, h, n, device="cuda") for h, n in ((2, 64), (2, 32), (4, 64)))
+    for tables in (tb, dt):
+        ops.kv_write(k, v, tables, c, 0)
+    ops.kv_keep(dt, torch.zeros(2, 3, dtype=torch.int32, device="cuda"), c)
+    for a, b in zip(before, (c.k, c.v, c.k_scale, c.v_scale)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for do in (BF, F32):
+        assert ops.kv_attn(q, tb, c, 0, 0.1, dtype=do).shape == ops.kv_tree_attn(q, dt, c, 0, 0.1, dtype=do).shape == (0, 4, 32)
+    want = kv_plain.held(c, 0)
+    for tables in (tb, dt):
+        for got, x in zip(ops.kv_read(tables, 0, 60, 40, c, 0, dtype=F32), want):
+            rows = x[[2, 0]].transpose(1, 2).reshape(-1, 2, x.shape[-1])[60:100]
+            assert bool(((got.double().cpu() - rows).abs() <= rows.abs() * 2.0 ** -24).all())
+        with pytest.raises(IndexError):
+            ops.kv_read(tables, 1, 0, 1, c, 0)

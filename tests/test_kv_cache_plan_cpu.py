@@ -49,3 +49,37 @@ def test_fp32_results_ask_for_what_is_cut(lens):
     """Portions with fp32 results beside a long request: at most 64 pieces for the request, and none for a portion whose keys one piece holds (768 groups of 16)."""
     cut = sum(n * 64 * min(64, max(1, (n + start + 15) // 16 // 8)) for n, start in lens if n == 1 or n + start > 768 * 16)
     assert _workspace(lens, 64, 4, 128, 128, dt_out=0) <= max(cut, 296 * 16 + 64 * 4) * 130 * 4 + 1024
+
+
+# ------------------------------------------------------------------------------------------------ steps without tokens
+
+def _empty(positions=None, **kw):
+    layout = np.array([[0, 0, 5, 1]], dtype=np.int32)
+    cache = ops.KvCacheArgs(4096, 4096, 4096, 4096, 2, 6, 16, 2, 64, 32, 1)
+    step = dict(positions=positions, seq_of=positions, cu=4096, pages=4096, rows=None, bits=None, layout=layout.ctypes.data, words=0, T=0, S=1, max_pages=1, replayed=0, device=0, tiles_from=0)
+    step.update(kw)
+    return cache, ops.KvStepArgs(**step), layout
+
+
+def test_a_step_without_tokens_does_nothing():
+    """Empty tensors have no address."""
+    lib = ops.load()
+    cache, step, keep = _empty()
+    p, q = C.byref(cache), C.byref(step)
+    assert lib.kb2_seq_kv_write(p, 0, q, None, 128, 64, None, 64, 32, 0, None) == 0
+    assert lib.kb2_seq_kv_attn_workspace(p, q, 4, 0, 0, 1) == 0
+    assert lib.kb2_seq_kv_attn(p, 0, q, None, 0, 256, 64, 4, 1.0, 0, 0, None, None, 0, None, 0, None) == 0
+    assert lib.kb2_seq_kv_keep(p, q, 4096, 1, None) == 0
+    assert lib.kb2_seq_kv_read(p, 0, q, 0, 0, 0, None, None, 0, None) == 0
+    # what has tokens or bad arguments is refused as before
+    assert lib.kb2_seq_kv_write(p, 2, q, None, 128, 64, None, 64, 32, 0, None) == 4 and lib.kb2_seq_kv_write(p, 0, q, None, 128, 64, None, 64, 32, 2, None) == 2
+    assert lib.kb2_seq_kv_attn(p, 0, q, None, 0, 256, 64, 3, 1.0, 0, 0, None, None, 0, None, 0, None) == 2
+    for kw in (dict(cu=None), dict(pages=None), dict(layout=None), dict(T=1), dict(T=1, positions=4096, seq_of=None)):
+        cache, step, keep = _empty(**kw)
+        assert lib.kb2_seq_kv_write(C.byref(cache), 0, C.byref(step), 4096, 128, 64, 4096, 64, 32, 0, None) == 2
+
+
+def test_rows_are_read_through_tables_without_tokens():
+    """Tables that were made to read a sequence back: what they do not have is not asked for, what the pages do not hold is refused."""
+    cache, step, keep = _empty()
+    assert ops.load().kb2_seq_kv_read(C.byref(cache), 0, C.byref(step), 0, 0, 17, 4096, 4096, 0, None) == 4
