@@ -965,13 +965,13 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
     return failf(KB2SEQ_ERR_VALUE, "kv_attn: bad argument");
   if (c.G > 65535 || (long long)t.T * H > 0x7FFFFFFFll / 2) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many heads or tokens");
   if (t.T == 0) return KB2SEQ_OK;
-  OnDevice on(step->device);
-  SEQ_CUDA(on.err);
+  OnDevice on(step->device);                 // ahead of the plan, which goes by the device's size
   const int win = window > 0 ? std::min(window, kKvNoWindow) : kKvNoWindow;
   const KvPlans p = kv_plans(cache, step, H, win, first, dt_out);
   if (work_bytes < p.bytes() || (p.bytes() && (!work || ((uintptr_t)work & 15))))
     return failf(KB2SEQ_ERR_VALUE, "kv_attn: workspace of %zu bytes, %zu needed", work_bytes, p.bytes());
   if (std::max(p.few.pieces, p.many.pieces) > kMostPieces) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many rows in a sequence");
+  SEQ_CUDA(on.err);
   KvAttn a{};
   a.q = q;
   a.ldq = ldq;

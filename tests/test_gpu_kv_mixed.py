@@ -111,3 +111,21 @@ def test_steps_without_tokens():
             assert bool(((got.double().cpu() - rows).abs() <= rows.abs() * 2.0 ** -24).all())
         with pytest.raises(IndexError):
             ops.kv_read(tables, 1, 0, 1, c, 0)
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    """With a buffer of the size that is needed, of which one byte less is declared."""
+    import ctypes as C
+
+    from krasis_b200 import seqops as ops
+    tb, seqs, pages = _step([(1, 5000), (70, 900)], 64, 72)
+    c = _cache(2, 128, 128, pages, "int8", seed=73)
+    q, out = torch.randn(tb.T, 16, 128, generator=_gen(74)).cuda(), torch.full((tb.T, 16, 128), 7.0, device="cuda")
+    lib, st = ops.load(), ops._kv_step(tb)[0]
+    size = lib.kb2_seq_kv_attn_workspace(c.address, st, 16, 0, 0, 0)
+    work = torch.empty(size, dtype=torch.uint8, device="cuda")
+    call = lambda n: lib.kb2_seq_kv_attn(c.address, 0, st, q.data_ptr(), 0, 16 * 128, 128, 16, C.c_float(0.09), 0, 0, None, out.data_ptr(), 0, work.data_ptr(), n,  # noqa: E731
+                                         torch.cuda.current_stream().cuda_stream)
+    assert size > 0 and call(size - 1) == 2 and bool((out == 7).all())
+    assert call(size) == 0
+    _check(out, q, c, seqs, scale=0.09)

@@ -3,6 +3,7 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
 from krasis_b200 import seqops as ops
 
@@ -83,3 +84,19 @@ def test_rows_are_read_through_tables_without_tokens():
     """Tables that were made to read a sequence back: what they do not have is not asked for, what the pages do not hold is refused."""
     cache, step, keep = _empty()
     assert ops.load().kb2_seq_kv_read(C.byref(cache), 0, C.byref(step), 0, 0, 17, 4096, 4096, 0, None) == 4
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up")
+@pytest.mark.parametrize("lens,do,kw", [([(1, 199999)], 0, {}), ([(40, 3000), (1, 5000)], 1, {"tiles_from": 17}), ([(1, 9000)] * 40, 1, {})])
+def test_a_workspace_that_is_too_small_is_refused(lens, do, kw):
+    """Ahead of everything that needs a GPU."""
+    lib = ops.load()
+    pages, rows = [(n + start + 15) // 16 for n, start in lens], np.cumsum([0] + [n for n, _ in lens])
+    layout = np.array([[r, n, start, p] for r, (n, start), p in zip(rows, lens, pages)], dtype=np.int32)
+    cache = ops.KvCacheArgs(4096, 4096, 4096, 4096, 2, sum(pages), 16, 2, 64, 32, 1)
+    step = ops.KvStepArgs(4096, 4096, 4096, 4096, None, None, layout.ctypes.data, 0, int(rows[-1]), len(lens), max(pages), 0, 0, kw.get("tiles_from", 0))
+    p, q = C.byref(cache), C.byref(step)
+    size = lib.kb2_seq_kv_attn_workspace(p, q, 8, 0, 0, do)
+    assert size > 0
+    for work, n in ((4096, size - 1), (4096, 0), (None, size), (4100, size)):
+        assert lib.kb2_seq_kv_attn(p, 0, q, 4096, 0, 512, 64, 8, 1.0, 0, 0, None, 4096, do, work, n, None) == 2
