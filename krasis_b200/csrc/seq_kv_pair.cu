@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     if (work && warp >= 4 && warp < 12) {                                  // nothing to see (no piece shares this tile): zeros
       for (int i = (warp - 4) * 32 + lane; i < nr * c.dv; i += 256) {
         const int r = i / c.dv, rr = r0 + r;
-        st_dt(a.out, a.dt_out, ((long long)(c0 + rr / per) * a.H + head * per + rr % per) * c.dv + i - r * c.dv, 0.f);
+        ((bf16*)a.out)[((long long)(c0 + rr / per) * a.H + head * per + rr % per) * c.dv + i - r * c.dv] = __float2bfloat16_rn(0.f);
       }
     }
   } else if (warp >= 12) {
@@ -396,14 +396,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
 #pragma unroll
           for (int j = 0; j < 16; ++j) y[j] = fmaf(share[o + j], by1, y[j]);
         }
-        if (whole && a.dt_out) {
+        if (whole) {
           uint4* to = reinterpret_cast<uint4*>((bf16*)a.out + orow * c.dv + o);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
             to[j] = make_uint4(bf16x2_bits_rn(y[8 * j + 1], y[8 * j]), bf16x2_bits_rn(y[8 * j + 3], y[8 * j + 2]), bf16x2_bits_rn(y[8 * j + 5], y[8 * j + 4]),
                                bf16x2_bits_rn(y[8 * j + 7], y[8 * j + 6]));
         } else {
-          float4* to = reinterpret_cast<float4*>(whole ? (float*)a.out + orow * c.dv + o : a.part_o + part * c.dv + o);
+          float4* to = reinterpret_cast<float4*>(a.part_o + part * c.dv + o);
 #pragma unroll
           for (int j = 0; j < 4; ++j) to[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
         }

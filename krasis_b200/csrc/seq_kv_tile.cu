@@ -8,7 +8,7 @@
 //                product for two codes; exact for scales that are powers of two), the power joins the softmax's factor
 //   warp  0      tcgen05.mma: S = Q K^T, O += P V (P from tensor memory)
 //   warps 4-11   softmax, two threads a row
-// S and P have two buffers each; 64 keys a tile (tensor memory: 3 FK + dv columns).
+// S and P have two buffers each; 64 keys a tile (tensor memory: 3 x 64 + 256 columns).
 //
 // Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value scale are fp16 (11 bits).  Weights are rounded relative to a reference R per row
 // that follows the largest weight times scale (2^6 to 2^15 of it), as in the kernel for few rows; maxima, weights and their sum are fp32.
@@ -19,11 +19,10 @@ namespace kb2seq {
 namespace {
 using namespace kb2;
 
-constexpr int kThreads = 512, kRows = 128;
+constexpr int kThreads = 512, kRows = 128, FK = 64, GT = FK / kKvGroup, NR = FK / 32;      // keys of a tile, their groups, a decoding thread's rows
 
 template <int NC, int NV>                    // chunks of 64 of d and dv
 struct TileShape {
-  static constexpr int FK = NC > 2 || NV > 2 ? 64 : 128;
   static constexpr int VS = NC + NV > 6 ? 1 : 2;                           // buffers of values
   static constexpr int kQ = NC * 128 * 128, kK = NC * FK * 128, kV = NV * FK * 128;
   static constexpr int kSlots = 3, kCodes = FK * 64 * (NC > NV ? NC : NV), kSlot = kCodes + FK * 8;       // codes as they come | scales of keys | of values
@@ -33,11 +32,12 @@ struct TileShape {
   static_assert(kTotal <= 227 * 1024 && 3 * FK + 64 * NV <= 512 && kSlot % 128 == 0 && kOffRef % 8 == 0 && kOffX % 16 == 0, "memory");
 };
 
-// Codes of a tile from `from` (rows of `width` bytes) into the operand at `to`.  A thread has the rows ct / 4 + 32 i and 16 bytes of each chunk of 64 of those, f times the
-// codes where see.  Odd rows take their chunks in another order: eight lanes that are served together then read 128 neighbouring bytes or two rows' halves, and the stores
+// Codes of a tile from `from` (rows of `width` bytes) into the operand at `to`.  A thread has the rows ct / 4 and ct / 4 + 32 and 16 bytes of each chunk of 64 of those, f times
+// the codes where see.  Odd rows take their chunks in another order: eight lanes that are served together then read 128 neighbouring bytes or two rows' halves, and the stores
 // of 16 bytes meet 8 rows' swizzles, two of them in eight lanes: no bank twice either way.
-template <int FMT, int NR, int CH>
+template <int FMT, int CH>
 __device__ __forceinline__ void decode(uint8_t* to, const uint8_t* from, int width, int ct, const float (&f)[NR], const bool (&see)[NR]) {
+  static_assert(CH % 2 == 0, "odd rows begin with the second chunk of two");
   const int q = ct & 3;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
@@ -45,7 +45,7 @@ __device__ __forceinline__ void decode(uint8_t* to, const uint8_t* from, int wid
     const uint32_t m = f16_pair(f[i], f[i]);
 #pragma unroll
     for (int h0 = 0; h0 < CH; ++h0) {
-      const int h = CH % 2 ? h0 : h0 ^ (row & 1), e0 = h * 64 + q * 16;
+      const int h = h0 ^ (row & 1), e0 = h * 64 + q * 16;
       const uint4 v = see[i] && e0 < width ? *reinterpret_cast<const uint4*>(from + row * width + e0) : make_uint4(0, 0, 0, 0);
       uint32_t y[8];
 #pragma unroll
@@ -71,7 +71,6 @@ __device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {
 template <int FMT, int NC, int NV>
 __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep t, KvAttn a, const __grid_constant__ KvKinds kinds) {
   using L = TileShape<NC, NV>;
-  constexpr int FK = L::FK, GT = FK / kKvGroup;                            // groups a tile
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *s_cons = bars + 10, *p_full = bars + 12, *pv_done = bars + 14,
@@ -172,13 +171,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     if (work && warp >= 4 && warp < 12) {                                  // nothing to see (no piece shares this tile): zeros
       for (int i = (warp - 4) * 32 + lane; i < nr * c.dv; i += 256) {
         const int r = i / c.dv, rr = r0 + r;
-        st_dt(a.out, a.dt_out, ((long long)(c0 + rr / per) * a.H + head * per + rr % per) * c.dv + i - r * c.dv, 0.f);
+        ((bf16*)a.out)[((long long)(c0 + rr / per) * a.H + head * per + rr % per) * c.dv + i - r * c.dv] = __float2bfloat16_rn(0.f);
       }
     }
   } else if (warp >= 12) {
     // ------------------------------------------------------------ decode: K(0), then K(it + 1) and V(it) in turn
     const int ct = threadIdx.x - 384;
-    constexpr int NR = FK / 32;
     bool see[NR], see_v[NR];
     float fk[NR], fv[NR], fv_next[NR];
     int job = 0;
@@ -215,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
         fv_next[i] = y != y ? 0.f : y * vi;
       }
       mbar_wait(&k_empty[b], (it >> 1 & 1) ^ 1);
-      decode<FMT, NR, NC>(smem + L::kOffK + b * L::kK, from, c.d, ct, fk, see);
+      decode<FMT, NC>(smem + L::kOffK + b * L::kK, from, c.d, ct, fk, see);
       if (ct == 0) {
         refs[it & 3] = make_float2(kp, vt ? vp : 0.f);
         gone[it & 3] = ~groups & ((1u << GT) - 1);
@@ -237,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       const int b = it % L::VS, slot = job % L::kSlots;
       mbar_wait(&c_full[slot], job / L::kSlots & 1);
       mbar_wait(&v_empty[b], (it / L::VS & 1) ^ 1);
-      decode<FMT, NR, NV>(smem + L::kOffV + b * L::kV, smem + L::kOffSlot + slot * L::kSlot, c.dv, ct, fv, see_v);
+      decode<FMT, NV>(smem + L::kOffV + b * L::kV, smem + L::kOffSlot + slot * L::kSlot, c.dv, ct, fv, see_v);
       if (lane == 0) {
         mbar_arrive(&v_full[b]);
         mbar_arrive(&c_empty[slot]);
@@ -344,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
     float* xchg = reinterpret_cast<float*>(smem + L::kOffX);
     const float down = rows_down[row];
-    constexpr int NB = FK / 64, OH = 32 * NV;
+    constexpr int OH = 32 * NV;
     float m = -INFINITY, l = 0.f, ref = 0.f;
     const auto tell = [&](uint64_t* bar) {
       tc_fence_before_sync();
@@ -361,19 +359,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       tc_fence_after_sync();
       const float2 p2 = refs[it & 3];        // written ahead of the keys; the tile after next writes none before this one's scores are taken
       const uint32_t away = gone[it & 3];
-      float x[NB][32];
+      float x[32];
       {
-        uint32_t r[NB][2][16];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          tmem_ld16(lane_at + kColS + b * FK + i * 64 + hf * 32, r[i][0]);
-          tmem_ld16(lane_at + kColS + b * FK + i * 64 + hf * 32 + 16, r[i][1]);
-        }
+        uint32_t r[2][16];
+        tmem_ld16(lane_at + kColS + b * FK + hf * 32, r[0]);
+        tmem_ld16(lane_at + kColS + b * FK + hf * 32 + 16, r[1]);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int j = 0; j < 32; ++j) x[i][j] = __uint_as_float(r[i][j / 16][j % 16]);
+        for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(r[j / 16][j % 16]);
       }
       tell(&s_cons[b]);
       const int ua = u0 + it * GT, ub = min(ua + GT, u1) - 1;              // groups of the tile
@@ -381,25 +374,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       const bool all = away == 0 && ub == ua + GT - 1 && pb < span.base && pb <= least && (pb < a.first || (ua >= span.na && most - pa < a.window));
       if (!all) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const int u = ua + i * 4 + hf * 2 + g, j0 = span.group(u) * kKvGroup;
-            uint32_t see = 0;
-            if (u < u1 && live && !(away >> (u - ua) & 1u)) {
+        for (int g = 0; g < 2; ++g) {
+          const int u = ua + hf * 2 + g, j0 = span.group(u) * kKvGroup;
+          uint32_t see = 0;
+          if (u < u1 && live && !(away >> (u - ua) & 1u)) {
 #pragma unroll 1
-              for (int j = 0; j < 16; ++j) see |= (uint32_t)kv_sees(t, a, span, c0, n, tok, pos, j0 + j) << j;
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (!(see >> j & 1u)) x[i][16 * g + j] = -INFINITY;
+            for (int j = 0; j < 16; ++j) see |= (uint32_t)kv_sees(t, a, span, c0, n, tok, pos, j0 + j) << j;
           }
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (!(see >> j & 1u)) x[16 * g + j] = -INFINITY;
+        }
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], x[i][j], x[i][j + 1]);
+      for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], x[j], x[j + 1]);
       float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
       float* xb = xchg + b * 256;
       xb[hf * 128 + row] = mt;
@@ -424,17 +413,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       const float f = ref >= least ? p2.y * __frcp_rn(ref) : 0.f;
       const uint64_t fac2 = pair_of(fac, fac), neg2 = pair_of(-from, -from), f2 = pair_of(f, f);
       uint64_t sum[2] = {0, 0};
-      uint32_t pk[NB][16];
+      uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const float2 e = pair_get(pair_fma(pair_of(x[i][j], x[i][j + 1]), fac2, neg2));
-          const uint64_t p = pair_of(ex2(e.x), ex2(e.y));
-          sum[j >> 1 & 1] = pair_add(sum[j >> 1 & 1], p);
-          const float2 y = pair_get(pair_mul(p, f2));
-          pk[i][j / 2] = f16_pair(y.x, y.y);
-        }
+      for (int j = 0; j < 32; j += 2) {
+        const float2 e = pair_get(pair_fma(pair_of(x[j], x[j + 1]), fac2, neg2));
+        const uint64_t p = pair_of(ex2(e.x), ex2(e.y));
+        sum[j >> 1 & 1] = pair_add(sum[j >> 1 & 1], p);
+        const float2 y = pair_get(pair_mul(p, f2));
+        pk[j / 2] = f16_pair(y.x, y.y);
+      }
       const float2 s2 = pair_get(pair_add(sum[0], sum[1]));
       l += s2.x + s2.y;
       if (it >= 2) pv_wait(it - 2);          // PV(it - 2) has read this P buffer
@@ -451,8 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
           tmem_st16(lane_at + kColO + o, r);
         }
       }
-#pragma unroll
-      for (int i = 0; i < NB; ++i) tmem_st16(lane_at + kColP + b * (FK / 2) + i * 32 + hf * 16, pk[i]);
+      tmem_st16(lane_at + kColP + b * (FK / 2) + hf * 16, pk);
       tmem_st_wait();
       tell(&p_full[b]);
     }
@@ -483,14 +469,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
       float y[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]) * by + (l != l ? l : 0.f);         // a sum that is NaN has a zero for its reference, maybe
-      if (whole && a.dt_out) {
+      if (whole) {
         uint4* to = reinterpret_cast<uint4*>((bf16*)a.out + orow * c.dv + o);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           to[j] = make_uint4(bf16x2_bits_rn(y[8 * j + 1], y[8 * j]), bf16x2_bits_rn(y[8 * j + 3], y[8 * j + 2]), bf16x2_bits_rn(y[8 * j + 5], y[8 * j + 4]),
                              bf16x2_bits_rn(y[8 * j + 7], y[8 * j + 6]));
       } else {
-        float4* to = reinterpret_cast<float4*>(whole ? (float*)a.out + orow * c.dv + o : a.part_o + part * c.dv + o);
+        float4* to = reinterpret_cast<float4*>(a.part_o + part * c.dv + o);
 #pragma unroll
         for (int j = 0; j < 4; ++j) to[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
       }
