@@ -139,3 +139,41 @@ def test_more_sequences_than_there_are_bits(monkeypatch):
     off = kv_plain.off_by(BF, BF, 45, 64, want, *sizes, decoded=True)
     err = (got.double().cpu() - want).abs()
     assert bool((err <= off).all()), (float((err / off).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("dq", [BF, F32])
+@pytest.mark.parametrize("H,G,d,dv", [(16, 2, 128, 128), (6, 2, 256, 256), (8, 2, 48, 32)])
+def test_queries_at_odd_offsets(dq, H, G, d, dv, forms):  # noqa: F811
+    """Queries as part of a projection, at addresses that hold no four of them whole, heads apart by more than their numbers."""
+    from krasis_b200 import seqops as ops
+    tb, seqs, pages = _step([(1, 300), (40, 200)], 64, 80)
+    c = _cache(G, d, dv, pages, "e4m3", seed=81)
+    proj = torch.randn(tb.T, 3 + H * (d + 5), generator=_gen(82)).to(dq).cuda()
+    q = proj[:, 3:].unflatten(1, (H, d + 5))[..., :d]
+    known = None
+    for do in (BF, F32):
+        for got in forms(tb, lambda: ops.kv_attn(q, tb, c, 0, d ** -0.5, dtype=do)):
+            known = _check(got, q, c, seqs, known=known, scale=d ** -0.5)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("H,G,d,dv", [(16, 2, 128, 128), (8, 2, 256, 256), (24, 8, 192, 128)])
+def test_each_sequence_by_the_bound_of_its_kernel(fmt, H, G, d, dv, monkeypatch):
+    """Codes and scales are held whole where a sequence has few rows, beside others on tiles or alone: the rounding of decoded numbers belongs to the tiles' sequences."""
+    from krasis_b200 import seqops as ops
+    lens = [(1, 700), (50, 300), (2, 33), (1, 2500), (30, 900)]
+    tb, seqs, pages = _step(lens, 64, 83)
+    c = _cache(G, d, dv, pages, fmt, seed=84)
+    q = torch.randn(tb.T, H, d, generator=_gen(85)).to(BF).cuda()
+    for window, first in ((None, 0), (500, 4)):
+        want, *sizes = kv_plain.attention(q, c, 0, seqs, d ** -0.5, window, first)
+        for tiles_from in (17, 1 << 30):
+            monkeypatch.setattr(ops, "KV_TILES_FROM", tiles_from)
+            tb._kv, at = None, 0
+            got = ops.kv_attn(q, tb, c, 0, d ** -0.5, window=window, first=first).double().cpu()
+            for n, start in lens:
+                rows = slice(at, at + n)
+                off = kv_plain.off_by(BF, BF, n + start, d, want[rows], *(x[rows] for x in sizes), decoded=n * H // G >= tiles_from)
+                err = (got[rows] - want[rows]).abs()
+                assert bool((err <= off).all()), (n, start, tiles_from, float((err / off).max()))
+                at += n
