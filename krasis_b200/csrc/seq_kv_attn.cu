@@ -69,7 +69,7 @@ __device__ __forceinline__ float4 lds_of(const float* p, int rank) {
   return v;
 }
 // Eight columns of a row: finished (part < 0), or as a partial result with its maximum and sum.
-__device__ __forceinline__ void store8(const KvLayer& c, const KvAttn& a, const float (&acc)[8], float top, float sum, long long row, int hd, int dim, long long part) {
+__device__ __forceinline__ void store8(const KvLayer& c, const KvAttn& a, const float (&acc)[8], float top, float sum, long long row, int hd, int dim, int part) {
   float y[8];
   float by = 1.f;
   if (part >= a.parts) return;
@@ -77,7 +77,7 @@ __device__ __forceinline__ void store8(const KvLayer& c, const KvAttn& a, const 
     if (a.sinks != nullptr && top != -INFINITY) sum += ex2(fmaf(a.sinks[hd], kLog2e, -top));
     by = sum == 0.f ? 0.f : 1.f / sum;
   } else if (dim == 0) {
-    *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(top, sum);
+    *reinterpret_cast<float2*>(a.part_ml + 2ll * part) = make_float2(top, sum);
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = acc[e] * by;
@@ -85,7 +85,7 @@ __device__ __forceinline__ void store8(const KvLayer& c, const KvAttn& a, const 
     *reinterpret_cast<uint4*>((bf16*)a.out + row * c.dv + dim) =
         make_uint4(kb2::bf16x2_bits_rn(y[1], y[0]), kb2::bf16x2_bits_rn(y[3], y[2]), kb2::bf16x2_bits_rn(y[5], y[4]), kb2::bf16x2_bits_rn(y[7], y[6]));
   } else {
-    float4* to = reinterpret_cast<float4*>(part < 0 ? (float*)a.out + row * c.dv + dim : a.part_o + part * c.dv + dim);
+    float4* to = reinterpret_cast<float4*>(part < 0 ? (float*)a.out + row * c.dv + dim : a.part_o + (long long)part * c.dv + dim);
     to[0] = make_float4(y[0], y[1], y[2], y[3]);
     to[1] = make_float4(y[4], y[5], y[6], y[7]);
   }
@@ -302,10 +302,10 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
   // where this piece's results go, those of row 0 of the tile (an even cut) or of the sequence, and how far apart rows are; looked up while the first keys are on their way
   KvParts* mine = reinterpret_cast<KvParts*>(smem + L::kOffParts);
   if (warp == 0 && !a.cluster) {
-    KvParts parts{-1, 0};
-    if (np > 1 && a.linear) parts = {(next_chunk - gridDim.x + number * c.G + head) * MT, 1};
-    else if (np > 1) parts = kv_parts(c, t, a, kinds, false, s);
-    if (np > 1 && !a.linear) parts.first += z;
+    KvParts parts{-1, 1};
+    int length;
+    if (np > 1 && a.linear) parts.first = ((int)next_chunk - gridDim.x + number * c.G + head) * MT;
+    else if (np > 1) parts = {kv_parts_ahead(c, t, a, kinds, s) + z, nr == n * per ? np : kv_cut(c, t, a, s, &length)};
     if (lane == 0) *mine = parts;
   }
 
@@ -553,10 +553,9 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
       continue;
     }
     const int hd = head * per + (r0 + q) % per;
-    const long long row = (long long)((r0 + q) / per) * a.H + hd;          // of the sequence
+    const int row = (r0 + q) / per * a.H + hd;                             // of the sequence
     const KvParts parts = *mine;
-    const long long part = parts.first < 0 ? -1 : parts.first + (a.linear ? q : row * parts.pieces);
-    store8(c, a, acc, top, sum, (long long)c0 * a.H + row, hd, dim, part);
+    store8(c, a, acc, top, sum, (long long)c0 * a.H + row, hd, dim, parts.first < 0 ? -1 : parts.first + (a.linear ? q : row * parts.pieces));
   }
   if (a.cluster) {
     kb2::cluster_sync_all();
@@ -612,7 +611,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
     else __syncwarp();
   };
   if (at_row >= rows) return;
-  int s = -1;
+  int s = -1, length = 1;
   KvParts parts{};
   if (x.linear) {                            // all sequences are
     const int tok = at_row / x.H;
@@ -620,12 +619,14 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
     s = t.seq_of[tok];
     at_row -= t.cu[s] * x.H;
   } else {
-    int before = 0;
-    long long ahead[2] = {};                 // parts of sequences of few rows, of those on tiles
+    int before = 0, ahead[2] = {};           // parts of sequences of few rows, of those on tiles
     for (int s0 = 0; s0 < t.S; s0 += 32) {
       const int q = s0 + lane;
       const bool tiles = q < t.S && kinds.on_tiles(q);
-      const int cut = q < t.S ? kv_pieces(c, t, tiles ? y : x, q) : 1, n = cut > 1 ? (t.cu[q + 1] - t.cu[q]) * x.H : 0;
+      const KvAttn& z = tiles ? y : x;
+      int cut = 1, len = 1;
+      if (q < t.S && z.pieces > 1 && !z.cluster) cut = kv_cut(c, t, z, q, &len);
+      const int n = cut > 1 ? (t.cu[q + 1] - t.cu[q]) * x.H : 0;
       int upto = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -636,15 +637,11 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
       const int l = hit ? __ffs(hit) - 1 : 32;
       const bool kind = __shfl_sync(0xffffffffu, tiles, l & 31);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        long long take = lane < l && tiles == (k == 1) ? (long long)n * cut : 0;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) take += __shfl_xor_sync(0xffffffffu, take, o);
-        ahead[k] += take;
-      }
+      for (int k = 0; k < 2; ++k) ahead[k] += __reduce_add_sync(0xffffffffu, lane < l && tiles == (k == 1) ? n * cut : 0);
       if (hit) {
         s = s0 + l;
         parts = {kind ? ahead[1] : ahead[0], __shfl_sync(0xffffffffu, cut, l)};
+        length = __shfl_sync(0xffffffffu, len, l);
         at_row -= before + __shfl_sync(0xffffffffu, upto - n, l);
         break;
       }
@@ -657,18 +654,15 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
   const KvAttn& a = kinds.on_tiles(s) ? y : x;
   const int in_seq = (tok - c0) * per + hd % per, r0 = in_seq / a.rows * a.rows, nr = (int)min((long long)n * per - r0, (long long)a.rows);
   const KvSpan span = kv_span(c, t, s, c0 + r0 / per, c0 + (r0 + nr - 1) / per, a.window, a.first);
-  int length = a.piece;
-  if (a.rows > 16) kv_cut(c, t, a, s, &length);
-  int np = min((span.groups() + length - 1) / length, a.pieces), step = 1;
-  long long p0 = parts.first + (long long)at_row * parts.pieces;
+  int np = min((span.groups() + length - 1) / length, a.pieces), step = 1, p0 = parts.first + at_row * parts.pieces;
   if (a.linear) {
     const int number = (s * a.per_seq + r0 / a.rows) * c.G + hd / per;
     const int2 v = a.counts[number];
     np = v.x;
     step = a.rows;
-    p0 = (long long)(v.y + number) * step + in_seq - r0;
+    p0 = (v.y + number) * step + in_seq - r0;
   }
-  if (np <= 1 || p0 + (long long)(np - 1) * step >= a.parts) return;
+  if (np <= 1 || p0 < 0 || p0 + (long long)(np - 1) * step >= a.parts) return;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
   float top = -INFINITY, sum = 0.f;
   for (int i = at; i < np; i += 32 * W) top = fmaxf(top, ml[i * step].x);
@@ -696,7 +690,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        v[i][h] = i0 + W * i < np && h * 128 + lane * 4 < c.dv ? *reinterpret_cast<const float4*>(a.part_o + (p0 + (i0 + W * i) * step) * c.dv + h * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[i][h] = i0 + W * i < np && h * 128 + lane * 4 < c.dv ? *reinterpret_cast<const float4*>(a.part_o + (long long)(p0 + (i0 + W * i) * step) * c.dv + h * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float f = i0 + W * i < np ? weight[i0 + W * i] : 0.f;
@@ -912,7 +906,7 @@ inline KvAttn with_plan(KvAttn a, const KvPlan& p, float* work, int dv) {
   a.pieces = p.pieces;
   a.part_o = work;
   a.part_ml = work + (size_t)p.parts * dv;
-  a.parts = p.parts;
+  a.parts = (int)p.parts;
   a.linear = p.blocks > 0 && p.rows <= 16;
   a.cluster = p.cluster;
   a.counts = reinterpret_cast<int2*>(a.part_ml + 2 * (size_t)p.parts);
@@ -971,6 +965,7 @@ KB2SEQ_API int kb2_seq_kv_attn(const kb2_seq_kv_cache* cache, int layer, const k
   if (work_bytes < p.bytes() || (p.bytes() && (!work || ((uintptr_t)work & 15))))
     return failf(KB2SEQ_ERR_VALUE, "kv_attn: workspace of %zu bytes, %zu needed", work_bytes, p.bytes());
   if (std::max(p.few.pieces, p.many.pieces) > kMostPieces) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many rows in a sequence");
+  if (std::max(p.few.parts, p.many.parts) > 0x7FFFFFFFll) return failf(KB2SEQ_ERR_VALUE, "kv_attn: too many rows that are cut");
   SEQ_CUDA(on.err);
   KvAttn a{};
   a.q = q;

@@ -24,15 +24,14 @@ struct KvAttn {                              // what a call says beside the cach
   // Partial results, an output of dv numbers and its maximum and sum each: of the rows (token, head) that are cut alone.  Sequences that are cut lie one behind the other, in
   // each its rows, in each row its pieces (KvParts).
   float *part_o, *part_ml;                   // [parts][dv] and [parts][2]
-  long long parts;
+  int parts;
   bool cluster;                              // a tile's pieces are the blocks of a cluster, which joins them itself
   bool linear;                               // all tiles' keys in a row are cut evenly, wherever the ends lie: `pieces` is then the most that a tile may have,
   int2* counts;                              // and this, [tiles][G], how many it has and the chunk of its first.  A piece's results lie at number chunk + tile G + head, which
                                              // no two share (from piece to piece the chunk or the tile moves on), `rows` to each
 };
 struct KvParts {                             // of a sequence
-  long long first;                           // where they begin
-  int pieces;                                // of each row; one: nothing is cut
+  int first, pieces;                         // where they begin; of each row (one: nothing is cut)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -83,55 +82,38 @@ __device__ __forceinline__ void kv_reach(const KvStep& t, const KvAttn& a, const
   }
 }
 
-// Tiles on the tensor cores: into how many pieces of how many groups the keys of a sequence's tiles are cut.  All of a sequence's tiles alike, by what its tokens see together.
+// Into how many pieces (at most) of how many groups the keys of a sequence's tiles are cut, by what its tokens see together.  Tiles on the tensor cores have them all alike.
 __device__ __forceinline__ int kv_cut(const KvLayer& c, const KvStep& t, const KvAttn& a, int s, int* length) {
   const int c0 = t.cu[s], c1 = t.cu[s + 1];
   const int groups = c1 > c0 ? kv_span(c, t, s, c0, c1 - 1, a.window, a.first).groups() : 0;
   const int n = max(min((groups + a.piece - 1) / a.piece, a.pieces), 1);
-  *length = max((groups + n - 1) / n, 1);
-  *length = (*length + 3) / 4 * 4;                                         // whole tiles of 64 keys
+  *length = a.rows <= 16 ? a.piece : (max((groups + n - 1) / n, 1) + 3) / 4 * 4;      // whole tiles of 64 keys
   return n;
 }
-// The same for tiles of either kind: into how many pieces at most a tile of the sequence is cut.
-__device__ __forceinline__ int kv_pieces(const KvLayer& c, const KvStep& t, const KvAttn& a, int s) {
-  int length;
-  if (a.pieces <= 1 || a.cluster) return 1;
-  if (a.rows > 16) return kv_cut(c, t, a, s, &length);
-  const int c0 = t.cu[s], c1 = t.cu[s + 1];
-  return c1 > c0 ? max(min((kv_span(c, t, s, c0, c1 - 1, a.window, a.first).groups() + a.piece - 1) / a.piece, a.pieces), 1) : 1;
-}
-// The parts of sequence `seq`, of those that are on tiles or of the others.  One warp.
-__device__ __forceinline__ KvParts kv_parts(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, bool tiles, int seq) {
-  const int lane = threadIdx.x & 31;
-  long long ahead = 0;
-  int mine = 1;
-  for (int s0 = 0; s0 <= seq; s0 += 32) {
-    const int s = s0 + lane;
-    const int n = s <= seq && kinds.on_tiles(s) == tiles ? kv_pieces(c, t, a, s) : 1;
-    if (s < seq && n > 1) ahead += (long long)(t.cu[s + 1] - t.cu[s]) * a.H * n;
-    if (s0 + 32 > seq) mine = __shfl_sync(0xffffffffu, n, seq & 31);
+// Where the parts of sequence `seq` begin, which is one of few rows.  One warp.
+__device__ __forceinline__ int kv_parts_ahead(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, int seq) {
+  int ahead = 0, length;
+  for (int s = threadIdx.x & 31; s < seq; s += 32) {
+    const int n = kinds.on_tiles(s) ? 1 : kv_cut(c, t, a, s, &length);
+    if (n > 1) ahead += (t.cu[s + 1] - t.cu[s]) * a.H * n;
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
-  return {ahead, mine};
+  return __reduce_add_sync(0xffffffffu, ahead);
 }
 // The (sequence, tile, piece) number `at`, the pieces of one sequence behind those of the one before, a piece's tiles together (they read the same keys), and the sequence's
 // parts.  One warp; false behind the last.
 __device__ __forceinline__ bool kv_find_piece(const KvLayer& c, const KvStep& t, const KvAttn& a, const KvKinds& kinds, int per, int at, int* seq, int* tile, int* piece,
                                               int* length, KvParts* parts) {
   const int lane = threadIdx.x & 31;
-  int before = 0;
-  long long ahead = 0;
+  int before = 0, ahead = 0;
   for (int s0 = 0; s0 < t.S; s0 += 32) {
     const int s = s0 + lane;
-    int tiles = 0, len = 1, n = 0, cut = 1;
-    long long take = 0;
+    int tiles = 0, len = 1, n = 0, cut = 1, take = 0;
     if (s < t.S) {
       const int tokens = t.cu[s + 1] - t.cu[s], have = tokens * per;
       tiles = have > 0 && kinds.on_tiles(s) ? (have + a.rows - 1) / a.rows : 0;
       if (tiles && a.pieces > 1) cut = kv_cut(c, t, a, s, &len);
       n = tiles * cut;
-      if (cut > 1) take = (long long)tokens * a.H * cut;
+      if (cut > 1) take = tokens * a.H * cut;
     }
     int upto = n;
 #pragma unroll
@@ -146,16 +128,11 @@ __device__ __forceinline__ bool kv_find_piece(const KvLayer& c, const KvStep& t,
       *seq = s0 + l;
       *piece = i / of;
       *tile = i - *piece * of;
-      if (lane >= l) take = 0;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) take += __shfl_xor_sync(0xffffffffu, take, o);
-      *parts = {ahead + take, __shfl_sync(0xffffffffu, cut, l)};
+      *parts = {ahead + __reduce_add_sync(0xffffffffu, lane < l ? take : 0), __shfl_sync(0xffffffffu, cut, l)};
       return true;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) take += __shfl_xor_sync(0xffffffffu, take, o);
-    ahead += take;
+    ahead += __reduce_add_sync(0xffffffffu, take);
   }
   return false;
 }

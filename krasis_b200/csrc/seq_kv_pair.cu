@@ -344,8 +344,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     }
     const int hd = head * per + rr % per;
     const bool whole = np <= 1;
-    const long long orow = (long long)tok * a.H + hd, part = whole ? 0 : seq_parts->first + (orow - (long long)c0 * a.H) * seq_parts->pieces + z;
-    const bool kept = live && (whole || part < a.parts);
+    const long long orow = (long long)tok * a.H + hd;
+    const int part = whole ? 0 : seq_parts->first + ((tok - c0) * a.H + hd) * seq_parts->pieces + z;
+    const bool kept = live && (whole || (unsigned)part < (unsigned)a.parts);
     float ref1 = 0.f;
     constexpr int kPad = 64 * NV + 1;        // numbers a row, an odd number: a row a thread meets every bank once
     float* share = reinterpret_cast<float*>(smem + L::kOffQ) + (quarter * 32 + lane) * kPad;
@@ -379,8 +380,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       if (whole && live && a.sinks != nullptr && m != -INFINITY) l += ex2(fmaf(a.sinks[hd], kLog2e, -m));
       const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f, by = ref * inv, by1 = ref1 * inv, none = l != l ? l : 0.f;      // a NaN may have a reference of 0
       if (!whole && kept) {
-        a.part_ml[2 * part] = m;
-        a.part_ml[2 * part + 1] = l;
+        a.part_ml[2ll * part] = m;
+        a.part_ml[2ll * part + 1] = l;
       }
 #pragma unroll 2
       for (int o = 0; o < 64 * NV; o += 16) {
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
             to[j] = make_uint4(bf16x2_bits_rn(y[8 * j + 1], y[8 * j]), bf16x2_bits_rn(y[8 * j + 3], y[8 * j + 2]), bf16x2_bits_rn(y[8 * j + 5], y[8 * j + 4]),
                                bf16x2_bits_rn(y[8 * j + 7], y[8 * j + 6]));
         } else {
-          float4* to = reinterpret_cast<float4*>(a.part_o + part * c.dv + o);
+          float4* to = reinterpret_cast<float4*>(a.part_o + (long long)part * c.dv + o);
 #pragma unroll
           for (int j = 0; j < 4; ++j) to[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
         }

@@ -451,13 +451,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     pv_wait(n_tiles - 1);
     const int hd = head * per + rr % per;
     const bool whole = np <= 1;
-    const long long orow = (long long)tok * a.H + hd, part = whole ? 0 : seq_parts->first + (orow - (long long)c0 * a.H) * seq_parts->pieces + z;
-    const bool kept = live && (whole || part < a.parts);
+    const long long orow = (long long)tok * a.H + hd;
+    const int part = whole ? 0 : seq_parts->first + ((tok - c0) * a.H + hd) * seq_parts->pieces + z;
+    const bool kept = live && (whole || (unsigned)part < (unsigned)a.parts);
     if (whole && live && a.sinks != nullptr && m != -INFINITY) l += ex2(fmaf(a.sinks[hd], kLog2e, -m));
     const float by = whole ? (l == 0.f ? 0.f : ref / l) : ref;
     if (!whole && kept && hf == 0) {
-      a.part_ml[2 * part] = m;
-      a.part_ml[2 * part + 1] = l;
+      a.part_ml[2ll * part] = m;
+      a.part_ml[2ll * part + 1] = l;
     }
 #pragma unroll 2
     for (int o = hf * OH; o < (hf + 1) * OH; o += 16) {
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
           to[j] = make_uint4(bf16x2_bits_rn(y[8 * j + 1], y[8 * j]), bf16x2_bits_rn(y[8 * j + 3], y[8 * j + 2]), bf16x2_bits_rn(y[8 * j + 5], y[8 * j + 4]),
                              bf16x2_bits_rn(y[8 * j + 7], y[8 * j + 6]));
       } else {
-        float4* to = reinterpret_cast<float4*>(a.part_o + part * c.dv + o);
+        float4* to = reinterpret_cast<float4*>(a.part_o + (long long)part * c.dv + o);
 #pragma unroll
         for (int j = 0; j < 4; ++j) to[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
       }
