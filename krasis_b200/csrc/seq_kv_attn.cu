@@ -15,7 +15,8 @@
 // Rounding.  q: a row is scaled by a power of two to the top of fp16's range, bf16 numbers keep their 8 bits, fp32 ones are rounded to 11 (PARTS 1) or split into two
 // fp16 numbers with 22 together (PARTS 2, for fp32 results).  Scores, maxima and sums are fp32; the key's scale multiplies the fp32 score.  The weight times the value's
 // scale is rounded to fp16, relative to a reference R of its own that follows the largest such product (2^6 to 2^15 of it), so that small scales or weights do not
-// fall out of fp16's range: 11 bits, or 22 with PARTS 2, down to 2^-30 of the largest.
+// fall out of fp16's range: 11 bits, or 22 with PARTS 2, down to 2^-30 of the largest.  R is never less than kLeastRef: where all values so far were zero, or weigh nothing
+// beside a zero one, the next product that counts is above fp16's range and asks for a new R.
 #include <cmath>
 
 #include "seq_kv_attn.cuh"
@@ -24,6 +25,7 @@ namespace kb2seq {
 namespace {
 
 constexpr int kSWarps = 8, kSStages = 3, kSMostGroups = 768, kMostPieces = 1024, kMostTiles = 768, kClusterMost = 8;
+constexpr float kLeastRef = 1e-37f;
 constexpr int kPieceCost = 40;               // what a piece costs beside its keys, in groups of 16 (11 us against 0.25 a group, with two blocks on an SM)
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -331,7 +333,9 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
     pos[h] = v.y;
     rf[h] = __int_as_float(v.z);
     m[h] = -INFINITY;
-    l[h] = ref[h] = inv[h] = 0.f;
+    l[h] = 0.f;
+    ref[h] = kLeastRef;
+    inv[h] = 1.f / kLeastRef;
   }
   int pmin, pmax;
   kv_reach(t, a, span, t0, t1, &pmin, &pmax);
@@ -411,10 +415,9 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = p[h][e] * __uint_as_float(word(vq, e));
+          x[e] = p[h][e] * __uint_as_float(word(vq, e)) * inv[h];          // the scale not times 1 / R first: that may be infinite, and the weight zero
           if (!all && y[h][e] == -INFINITY) x[e] = 0.f;                    // a row that nobody sees may hold anything
           big = fmaxf(big, x[e]);
-          x[e] *= inv[h];                    // not times the scale first: of a small reference that may be infinite, and the weight zero
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -424,8 +427,7 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
             w[h][PARTS - 1][b] = f16_pair(x[2 * b] - f.x, x[2 * b + 1] - f.y);
           }
         }
-        // a weight above 2^8, a product above fp16's range, or one where there is no reference yet: all values so far were zero, or their weights have become so
-        return top > 8.f || big * inv[h] > 32768.f || (inv[h] == 0.f && big > 1e-37f);
+        return top > 8.f || big > 32768.f;   // a weight above 2^8, a product above fp16's range
       };
       bool again = false;
 #pragma unroll
@@ -447,13 +449,10 @@ __global__ void __launch_bounds__(kSWarps * 32, (StreamShape<DU, VU, NQ, PARTS>:
             if (y[h][e] != -INFINITY) big = fmaxf(big, ex2(y[h][e] - from) * __uint_as_float(word(vq, e)));
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-          grow[h] = 1.f;
-          if (big > 1e-37f && (ref[h] < 1e-37f || big > ref[h] * 32768.f)) {
-            const float r = fmaxf(big * 0.015625f, 1e-37f);
-            grow[h] = ref[h] / r;
-            ref[h] = r;
-          }
-          inv[h] = ref[h] >= 1e-37f ? 1.f / ref[h] : 0.f;
+          const float r = fmaxf(big > ref[h] * 32768.f ? big * 0.015625f : ref[h], kLeastRef);
+          grow[h] = ref[h] / r;
+          ref[h] = r;
+          inv[h] = 1.f / r;
           weigh(h);
         }
 #pragma unroll
