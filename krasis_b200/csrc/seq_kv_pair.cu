@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
   int* groups = reinterpret_cast<int*>(smem + L::kOffGroup);               // [kPlans][8] where the groups lie (rows / 16), -1: nowhere
   float4* units = reinterpret_cast<float4*>(smem + L::kOffUnit);           // [kUnits] of keys, of values; four bits a group: whether it lies nowhere
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
-  KvParts* seq_parts = reinterpret_cast<KvParts*>(smem + L::kOffParts);    // where the sequence's partial results lie
+  KvParts* seq_parts = reinterpret_cast<KvParts*>(smem + L::kOffParts);    // where the piece's partial results lie, those of the sequence's row 0; -1: there are none, the tile has one piece
   float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [256] what the queries' own scaling is undone with
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (warp == 2) tmem_alloc(tmem_at, 512);
@@ -94,13 +94,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
   const int per = a.H / c.G, head = blockIdx.y;
   int s = 0, tile = 0, z = 0, length = 0x7FFFFFFF;
   bool in = true;
+  KvParts parts{};
   if (a.per_seq && a.pieces == 1) {
     s = blockIdx.x / a.per_seq;
     tile = blockIdx.x - s * a.per_seq;
   } else {
-    KvParts parts{};
     in = kv_find_piece(c, t, a, kinds, per, blockIdx.x, &s, &tile, &z, &length, &parts);
-    if (threadIdx.x == 0) *seq_parts = parts;
   }
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * 256, nr = in ? (int)min((long long)n * per - r0, 256ll) : 0;
   int u0 = 0, u1 = 0, np = 0, t0 = c0;
@@ -112,6 +111,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
     u0 = a.pieces == 1 ? 0 : z * length;
     u1 = a.pieces == 1 ? span.groups() : min(span.groups(), u0 + length);
   }
+  if (threadIdx.x == 0) *seq_parts = {np <= 1 ? -1 : parts.first + z, parts.pieces};
   const bool work = nr > 0 && (z == 0 || z < np);   // piece 0 of a tile that sees nothing writes its zeros
   const int n_tiles = work ? max(0, (u1 - u0 + GT - 1) / GT) : 0;
   const bool two = nr > 128;                 // two row tiles; else one whose key tiles go to both groups in turn
@@ -343,9 +343,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_pair_kernel(KvLayer c, KvStep 
       tc_fence_after_sync();
     }
     const int hd = head * per + rr % per;
-    const bool whole = np <= 1;
+    const bool whole = seq_parts->first < 0;
     const long long orow = (long long)tok * a.H + hd;
-    const int part = whole ? 0 : seq_parts->first + ((tok - c0) * a.H + hd) * seq_parts->pieces + z;
+    const int part = whole ? 0 : seq_parts->first + ((tok - c0) * a.H + hd) * seq_parts->pieces;
     const bool kept = live && (whole || (unsigned)part < (unsigned)a.parts);
     float ref1 = 0.f;
     constexpr int kPad = 64 * NV + 1;        // numbers a row, an odd number: a row a thread meets every bank once

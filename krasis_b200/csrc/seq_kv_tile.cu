@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
   uint32_t* have = reinterpret_cast<uint32_t*>(smem + L::kOffHave);        // [3] a slot's groups that are there, a bit each
   uint32_t* gone = reinterpret_cast<uint32_t*>(smem + L::kOffGone);        // [4] a tile's groups that are not
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
-  KvParts* seq_parts = reinterpret_cast<KvParts*>(smem + L::kOffParts);    // where the sequence's partial results lie
+  KvParts* seq_parts = reinterpret_cast<KvParts*>(smem + L::kOffParts);    // where the piece's partial results lie, those of the sequence's row 0; -1: there are none, the tile has one piece
   float* rows_down = reinterpret_cast<float*>(smem + L::kOffRow);          // [128] what the queries' own scaling is undone with
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -106,13 +106,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
   const int per = a.H / c.G, head = blockIdx.y;
   int s = 0, tile = 0, z = 0, length = 0x7FFFFFFF;
   bool in = true;
+  KvParts parts{};
   if (a.per_seq && a.pieces == 1) {
     s = blockIdx.x / a.per_seq;
     tile = blockIdx.x - s * a.per_seq;
   } else {
-    KvParts parts{};
     in = kv_find_piece(c, t, a, kinds, per, blockIdx.x, &s, &tile, &z, &length, &parts);
-    if (threadIdx.x == 0) *seq_parts = parts;
   }
   const int c0 = t.cu[s], n = t.cu[s + 1] - c0, r0 = tile * kRows, nr = in ? (int)min((long long)n * per - r0, (long long)kRows) : 0;
   int u0 = 0, u1 = 0, np = 0, t0 = c0, t1 = c0;
@@ -125,6 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     u0 = a.pieces == 1 ? 0 : z * length;
     u1 = a.pieces == 1 ? span.groups() : min(span.groups(), u0 + length);
   }
+  if (threadIdx.x == 0) *seq_parts = {np <= 1 ? -1 : parts.first + z, parts.pieces};
   const bool work = nr > 0 && (z == 0 || z < np);   // piece 0 of a tile that sees nothing writes its zeros
   const int n_tiles = work ? max(0, (u1 - u0 + GT - 1) / GT) : 0;
 
@@ -450,9 +450,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_tile_kernel(KvLayer c, KvStep 
     if (n_tiles >= 2) pv_wait(n_tiles - 2);
     pv_wait(n_tiles - 1);
     const int hd = head * per + rr % per;
-    const bool whole = np <= 1;
+    const bool whole = seq_parts->first < 0;
     const long long orow = (long long)tok * a.H + hd;
-    const int part = whole ? 0 : seq_parts->first + ((tok - c0) * a.H + hd) * seq_parts->pieces + z;
+    const int part = whole ? 0 : seq_parts->first + ((tok - c0) * a.H + hd) * seq_parts->pieces;
     const bool kept = live && (whole || (unsigned)part < (unsigned)a.parts);
     if (whole && live && a.sinks != nullptr && m != -INFINITY) l += ex2(fmaf(a.sinks[hd], kLog2e, -m));
     const float by = whole ? (l == 0.f ? 0.f : ref / l) : ref;
