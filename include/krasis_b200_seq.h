@@ -335,7 +335,8 @@ typedef struct {
  * the committed rows of its sequence in the order of the tokens, positions holds first row + depth, and bits [T][words] which tokens of its sequence a token sees: bit i
  * is set for token i if that is the token itself or one of its ancestors, which come before it.  rows and bits null: positions and order of a portion.
  * tiles_from: from how many rows per kv head (tokens times H / G) a sequence's attention runs on the tensor cores' tiles where its result is bf16; 0: the library's rule.
- * Tokens behind cu[S] are left alone by every call below: cu may end before the layout does (which says how the work is cut), it may not give a sequence more.  Pages that are not in the pool hold nothing: no row is written there or seen. */
+ * Tokens behind cu[S] are left alone by every call below: cu may end before the layout does, which says how the work is cut, but gives no sequence more.  Pages that are not
+ * in the pool hold nothing: no row is written there or seen.  Of a step without tokens positions, seq_of and the tensors may be null. */
 typedef struct {
   const int *positions, *seq_of, *cu, *pages, *rows;
   const unsigned* bits;

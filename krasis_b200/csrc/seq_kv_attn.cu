@@ -8,8 +8,9 @@
 // bytes of a key row and 8 or 16 of a value row for its fragments: everything a lane multiplies it has copied itself (cp.async into its own slots), no warp waits for
 // another, and no byte is read from shared memory twice.
 // What bounds it: the cache's bytes.  16 keys of 128 + 128 dimensions are 4.2 KB a warp and iteration; 3 stages x 16 warps an SM keep 200 KB on the way.  64 requests of 500 to
-// 60000 rows, 64 / 4 heads of 128, int8 (862 MB, 131 us at the copy rate): 216 us, the copies alone 170 or so; 32 / 4 heads (811 MB) 176, the copies alone 162.  What is left
-// beside them is arithmetic on codes (a conversion is a half-rate instruction for two codes), which 16 query rows cannot hide behind four warps a scheduler.
+// 60000 rows, 64 / 4 heads of 128, int8 (862 MB, 131 us at the copy rate): 219 us, the copies alone 170 or so; 64 of 12000, 32 / 4 heads (811 MB) 182, the copies alone 162.
+// What is left beside them is arithmetic on codes (a conversion is a half-rate instruction for two codes), which 16 query rows cannot hide behind four warps a scheduler; heads of
+// 128 with 16 rows take all 128 registers of two blocks an SM and spill 60 bytes.
 // Tried and left out: int8 keys as whole numbers (mma.s8 on queries of 15 bits: no conversion, no faster), the next keys' scores beside these keys' products (no faster).
 //
 // Rounding.  q: a row is scaled by a power of two to the top of fp16's range, bf16 numbers keep their 8 bits, fp32 ones are rounded to 11 (PARTS 1) or split into two
@@ -732,8 +733,10 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvLayer c, KvStep t, KvAtt
 
 // ------------------------------------------------------------------------------------------------ host
 // Rows per kv head (a sequence's tokens times the heads that share one) from which a sequence may run on the tensor cores' tiles.  Fewer are faster on the kernel for few rows
-// (us there / on tiles, 16 / 2 heads of 128, int8: 24 rows after 2000 keys 13 / 20, eight sequences of 32 rows after 16000 51 / 62); more are where there is enough to do to
-// make up for the tiles' longer start (64 rows after 2000 14 / 21, eight of 64 after 16000 81 / 65; 128 rows after 2000 17 / 23, after 16000 33 / 27).
+// (us there / on tiles, 16 / 2 heads of 128, int8: 24 rows after 2000 keys 13 / 20, eight sequences of 32 rows after 16000 51 / 62, of 48 after 30000 106 / 120); more are where
+// there is enough to do to make up for the tiles' longer start (64 rows after 2000 13 / 23, eight of 64 after 30000 133 / 123; 128 rows after 2000 18 / 25, after 30000 49 / 34).
+// One rule for all heads, made for those of 128; for others both kernels cost more a group.  Of 48 to 512 rows, one sequence or eight, after 2000, 8000 and 30000 keys it loses at
+// most 14 % of the better kernel's time on heads of 128, 34 % on 192 / 128 (256 rows after 8000: 47 / 35), 27 % on 128 / 256 and 21 % on 256.
 constexpr int kTileFrom = 48;
 constexpr long long kWideWaves = 2;          // pieces for each SM, of such sequences (sixteen trees of 57 to 64 tokens: 2 530 us, 3 548, 4 571, 6 638)
 // How the sequences of one kind are cut: into tiles of rows, and the keys that a tile sees (in groups of 16) into pieces.
@@ -742,7 +745,7 @@ struct KvPlan {
   bool cluster;                              // the pieces of a tile are a cluster, which joins them itself
   long long parts, joined;                   // partial results; rows (token, head) of the sequences that are cut
   size_t floats;                             // workspace
-  void size(int H, int G, int dv, bool wide) {       // what lies behind begins on 16 bytes too
+  void size(int G, int dv, bool wide) {      // what lies behind begins on 16 bytes too
     floats = ((size_t)parts * (dv + 2) + (blocks && !wide ? 2 * (size_t)tiles * G : 0) + 3) / 4 * 4;
   }
 };
@@ -797,7 +800,7 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
       p.blocks += (int)(tiles(s) * n);
       cut(s, n);
     }
-    p.size(H, cache->G, cache->dv, wide);
+    p.size(cache->G, cache->dv, wide);
     return p;
   } else {
     // Blocks of one length in whole waves, as the last wave takes as long as the others: the length whose waves, with what a block costs beside its keys (some 16 groups), end
@@ -809,7 +812,7 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
       // a captured step's keys may come to lie in one sequence: the kernel makes its pieces no more than this
       p.pieces = (int)(step->replayed ? std::max(34ll, (top + kPieceCost) / kSMostGroups + 2) : (top + kPieceCost) / std::min<long long>(std::max(even, 8ll), kSMostGroups) + 2);
     }
-    // Few keys: up to eight blocks a tile meet in shared memory, without a second launch and a workspace (four requests of 1028 visible rows: 9.0 us, with a join 9.8; 11.0 against 15 with what the host does);
+    // Few keys: up to eight blocks a tile meet in shared memory, without a second launch and a workspace (four requests of 1028 visible rows: 9.0 us, with a join 9.8; 11.0 against 15 with what the host does, as measured then);
     // more than that, a warp would have too many keys one after another (6144 a tile).
     if (!p.blocks && top > kSWarps && top <= 48 * kClusterMost && (long long)p.tiles * cache->G * kClusterMost <= slots) {
       p.cluster = true;
@@ -847,7 +850,7 @@ KvPlan kv_plan(const kb2_seq_kv_cache* cache, const kb2_seq_kv_step* step, int H
     p.pieces = (int)std::max(1ll, (top + p.piece - 1) / p.piece);
     for (int s = 0; s < step->S; ++s) cut(s, tiles(s) ? (seen(s) + p.piece - 1) / p.piece : 0);
   }
-  p.size(H, cache->G, cache->dv, wide);
+  p.size(cache->G, cache->dv, wide);
   return p;
 }
 struct KvPlans {

@@ -1,4 +1,4 @@
-// Attention over the 8-bit cache: what its two kernels and their join share.
+// Attention over the 8-bit cache: what its three kernels and their join share.
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

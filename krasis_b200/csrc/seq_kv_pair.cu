@@ -10,13 +10,15 @@
 //
 // What bounds it: the tensor pipe.  A product of 128 x 64 x 16 with both operands in shared memory takes 75 cycles (64 x 16 of K and 128 x 16 of Q are read each time), one of
 // 128 x 128 x 16 with P in tensor memory 76, so 128 keys and 256 rows take 3616; their 32768 exponentials take 2048 (16 a cycle).  A portion of 4096 tokens after 5001, window
-// 4096, 64 / 4 heads of 128: 617 us, 4480 cycles for those 128 keys, 552 GFLOP at 0.54 of the measured cuBLAS rate.  On the way there: one row tile a CTA with 128 keys a tile
+// 4096, 64 / 4 heads of 128: 621 us, 4510 cycles for those 128 keys, 552 GFLOP at 0.54 of the measured cuBLAS rate.  On the way there: one row tile a CTA with 128 keys a tile
 // 989, two 722, softmax groups in turn 679, tiles of 64 keys with two buffers of scores 688 with one warp for the tensor cores, which spends 300 cycles between two batches of
-// products while the pipe takes two ahead, and 606 with two; groups of pages that are not there, looked for in each tile, cost the rest.
+// products while the pipe takes two ahead, and 606 with two; groups of pages that are not there, looked for in each tile, cost most of the rest.
+// Heads of 192 spill 264 bytes a thread (a portion of 2048 after 3000, 64 / 4 heads of 192 / 128: 440 us, 338 GFLOP at 0.46 of that rate), those of 64 24.
 //
 // Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value unit are fp16 (11 bits).  A row's factor is its scale over a unit, a power of two
 // near the tile's largest scale (exact for scales that are powers of two); the units join the softmax's factors.  Weights are rounded relative to a reference R per row that
-// follows the largest weight times unit (2^6 to 2^15 of it), as in the kernel for few rows; maxima, weights and their sum are fp32.
+// follows the largest weight times unit (2^6 to 2^15 of it); maxima, weights and their sum are fp32.  The largest weight's own value may be zero (the kernel for few rows goes by
+// each row's scale): weights below 2^-20 of the row's largest lose bits all the same.
 // A row whose scale is NaN gets NaN keys and zero values: scores that nobody sees are replaced, and those that see it carry the NaN into the sum.
 #include "seq_kv_tc.cuh"
 

@@ -9,9 +9,11 @@
 //   warp  0      tcgen05.mma: S = Q K^T, O += P V (P from tensor memory)
 //   warps 4-11   softmax, two threads a row
 // S and P have two buffers each; 64 keys a tile (tensor memory: 3 x 64 + 256 columns).
+// What bounds it: a tile of keys is decoded for 128 rows, half as many as in seq_kv_pair.cu, and no pipe is near its limit (tensor 18 %, issue slots 30 %).  A portion of 2048
+// tokens after 3000: 16 / 2 heads of 256 440 us (135 GFLOP, 0.19 of the measured cuBLAS rate), 32 / 4 heads of 128 / 256 411 (203 GFLOP, 0.30).
 //
 // Rounding, for bf16 results: queries, decoded numbers and weights times their tile's value scale are fp16 (11 bits).  Weights are rounded relative to a reference R per row
-// that follows the largest weight times scale (2^6 to 2^15 of it), as in the kernel for few rows; maxima, weights and their sum are fp32.
+// that follows the largest weight times unit (2^6 to 2^15 of it); maxima, weights and their sum are fp32.  Weights below 2^-20 of the row's largest lose bits, whatever that one's value.
 // A row whose scale is NaN gets NaN keys and zero values: scores that nobody sees are replaced, and those that see it carry the NaN into the sum.
 #include "seq_kv_tc.cuh"
 

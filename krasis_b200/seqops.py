@@ -464,7 +464,7 @@ class KvStepArgs(C.Structure):
     _fields_ = [(n, _P) for n in ("positions", "seq_of", "cu", "pages", "rows", "bits", "layout")] + [(n, _I) for n in ("words", "T", "S", "max_pages", "replayed", "device", "tiles_from")]
 
 
-KV_TILES_FROM = 0      # rows per kv head from which attention over the 8-bit cache runs on the tensor cores' tiles (bf16 results), for tables made from now on; 0: by size
+KV_TILES_FROM = 0      # rows per kv head from which attention over the 8-bit cache runs on the tensor cores' tiles (bf16 results), for tables that no call has used yet; 0: by size
 
 
 class DraftTables(StepTables):
@@ -605,7 +605,9 @@ def _kv_attend(name, q, tb, cache, layer, scale, window, first, sinks, dtype, ou
 def kv_attn(q: torch.Tensor, tb: StepTables, cache, layer: int, scale: float, window=None, first: int = 0, sinks=None, dtype=None, out=None) -> torch.Tensor:
     """Softmax attention of q [T, H, d] (fp32 or bfloat16) over a CompactKVCache that holds the step's own rows already (kv_write): [T, H, dv] in `dtype` (q's own).
     A token at position p sees row j <= p if p - j < window (None: no window) or j < first: the sequence's first tokens stay visible.  sinks [H] fp32: exp(sinks[h])
-    joins head h's softmax denominator.  float32 results carry 22 bits of queries and weights, bfloat16 ones 11."""
+    joins head h's softmax denominator.  float32 results carry 22 bits of queries and weights, bfloat16 ones 11; codes and scales are held whole.  bfloat16 results of sequences
+    with many rows per key / value head (tokens times heads, from 48, by size) run on the tensor cores' tiles, where a key's or value's code times its scale is rounded to 11 bits
+    as well (int8: the scale before it), and where weights below 2^-20 of a row's largest, or scales below 2^-21 of those around them, lose bits."""
     if isinstance(tb, DraftTables):
         raise ValueError("kv_attn: drafted tokens see a tree: kv_tree_attn")
     return _kv_attend("kv_attn", q, tb, cache, layer, scale, window, first, sinks, dtype, out)
