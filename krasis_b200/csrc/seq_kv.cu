@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvLayer c, KvStep t, int s
 // ------------------------------------------------------------------------------------------------ the accepted path
 // Block (sequence, kKeepLayers layers): row base + path[i] -> row base + i.  A path rises, so path[i] >= i: what a thread writes at i no later step reads, and a thread
 // keeps its 16 bytes of every row (eight rows on their way at once), so it has read whatever it overwrites.  What bounds it: the chain of tables ahead of the rows, so
-// a block has work for all its threads (64 paths of 8 in 48 layers: a layer a block 22 us, four 15.5, eight 13.7; 7.9 at the copy rate).
+// a block has work for all its threads (64 paths of 8 in 48 layers: a layer a block 22 us, four 15.5, eight 14; 7.9 at the copy rate).
 constexpr int kKeepMost = 512, kKeepLayers = 8;
 __global__ void __launch_bounds__(256) kv_keep_kernel(KvLayer c, int layers, KvStep t, const int* __restrict__ path, int P) {
   __shared__ long long rows[2][kKeepMost];
