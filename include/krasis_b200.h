@@ -266,6 +266,32 @@ KB2_API int kb2_linear_f32(const float* x_dev, int64_t x_ld, int64_t x_group, co
                            int64_t out_ld, int64_t out_group, int32_t M, int32_t N, int32_t K, int32_t groups, void* workspace_dev,
                            size_t workspace_bytes, int32_t device, void* stream);
 
+/* ---- Products of 8-bit floating-point numbers (e4m3) with a scale per block of 128 (activations: 128 numbers of a row; weights: 128 x 128; the last
+ * blocks may be cut short).  With a = max |x| over a block: scale 2^k, k the least whole number >= -126 with a <= 448 2^k, codes e4m3(x / scale), ties to
+ * even; a = 0: scale 0, codes 0; a number that is not finite: scale NaN, codes 0.  The products take any fp32 scales.
+ * K (W) % 16 == 0.  x_f32 0: bf16, 1: fp32 rows of any stride; out_f32 likewise.  Codes, weights, outputs and workspaces on 16 bytes. */
+/* x [M][K] (row stride ldx) -> codes [M][K], scales[b * ld_scales + m] for the blocks b of a row (ld_scales >= M). */
+KB2_API int kb2_fp8_quantize_rows(const void* x_dev, int32_t x_f32, int64_t ldx, int32_t M, int32_t K, void* codes_dev, float* scales_dev, int64_t ld_scales,
+                                  int32_t device, void* stream);
+/* w [groups][N][K] -> codes of that shape, scales [groups][ceil(N / 128)][ceil(K / 128)]. */
+KB2_API int kb2_fp8_quantize_blocks(const void* w_dev, int32_t w_f32, int32_t groups, int32_t N, int32_t K, void* codes_dev, float* scales_dev, int32_t device,
+                                    void* stream);
+/* out [M][N] = x . w^T (+ bias [N] f32, may be NULL) of rows as kb2_fp8_quantize_rows leaves them (scales on 16 bytes, ld_scales % 4 == 0).  A block's
+ * products are summed in fp32, as are the blocks' sums times their scales. */
+KB2_API int kb2_fp8_linear_rows(const void* codes_dev, const float* scales_dev, int64_t ld_scales, const void* w_dev, const float* w_scales_dev, const float* bias_dev,
+                                void* out_dev, int32_t out_f32, int32_t M, int32_t N, int32_t K, int32_t device, void* stream);
+/* Both in one: the rows are quantised into the workspace.  A workspace serves one call at a time. */
+KB2_API size_t kb2_fp8_linear_workspace(int32_t M, int32_t K);
+KB2_API int kb2_fp8_linear(const void* x_dev, int32_t x_f32, int64_t ldx, const void* w_dev, const float* w_scales_dev, const float* bias_dev, void* out_dev,
+                           int32_t out_f32, int32_t M, int32_t N, int32_t K, void* work_dev, size_t work_bytes, int32_t device, void* stream);
+/* Routed experts: out [T][W] = sum_j weights[t][j] down_e(q(silu(gate_e x) * up_e x)) with e = ids[t][j], x = q(h[t]), q the quantisation of rows and the products
+ * in fp32.  w1 [E][2 F][W] = [gate ; up], w2 [E][W][F] with their scales; ids [T][top] int32, those outside [0, E) bring nothing.  F % 128 == 0, E <= 1024.
+ * An expert's rows are rounded to bf16 ahead of the weighted sum (fp32) where out is bf16. */
+KB2_API size_t kb2_fp8_experts_workspace(int32_t T, int32_t top, int32_t E, int32_t W, int32_t F, int32_t out_f32);
+KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const int32_t* ids_dev, const float* weights_dev, const void* w1_dev, const float* s1_dev,
+                            const void* w2_dev, const float* s2_dev, void* out_dev, int32_t out_f32, int32_t T, int32_t top, int32_t E, int32_t W, int32_t F,
+                            void* work_dev, size_t work_bytes, int32_t device, void* stream);
+
 /* flashinfer.norm.rmsnorm (residual_dev == NULL) / fused_add_rmsnorm (residual_dev != NULL: residual += x, in place)
  * as used at python/krasis/layer.py:163-183,283-308.  x, residual, out: [M][H] bf16 (out may alias x); weight [H] f32. */
 KB2_API int kb2_rmsnorm(void* x_dev, void* residual_dev, const float* weight_dev, void* out_dev, int32_t M, int32_t H,

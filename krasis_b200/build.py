@@ -1,15 +1,16 @@
 """Build the C-ABI CUDA libraries in-tree (krasis_b200/_lib/) for sm_100a.
 
 Two targets, so that a model only compiles what it runs on:
-  "core"  libkrasis_b200.so       MoE prefill path: grouped / dense tcgen05 GEMMs, Gated DeltaNet, GQA / MLA attention, NCCL glue
-  "seq"   libkrasis_b200_seq.so   ragged-batch sequence operators (csrc/seq_ops.cu, seq_mix.cu, seq_rec.cu, seq_kv.cu, seq_kv_attn.cu, seq_kv_tile.cu, seq_kv_pair.cu): norms, generic GEMM, windowed
+  "core"  libkrasis_b200.so       MoE prefill path: grouped / dense tcgen05 GEMMs, products of 8-bit floating point, Gated DeltaNet, GQA / MLA attention, NCCL glue
+  "seq"   libkrasis_b200_seq.so   ragged-batch sequence operators (csrc/seq_ops.cu, seq_mix.cu, seq_rec.cu, seq_kv.cu, seq_kv_attn.cu, seq_kv_tile.cu, seq_kv_pair.cu, seq_logp.cu): norms, generic GEMM, windowed
                                   latent attention with an optional sink, short convolution + gated delta rule (decay per head or per
                                   key channel) with state slots, per-head paged multi-map attention (score cap, sink, pooled blocks
                                   before the window, rotated values, distance penalty), gated and ungated linear units, router and
                                   routed experts,
                                   gated linear attention, matrix memory (mLSTM), selective scan and real-gated linear recurrent unit with
                                   state slots, side-by-side mixers, depth average, several mixed copies of the residual stream;
-                                  a paged cache of keys and values in 8 bits: writing, reading, windowed and tree attention, moving rows
+                                  a paged cache of keys and values in 8 bits: writing, reading, windowed and tree attention, moving rows;
+                                  log probabilities of given tokens with entropy and the largest alternatives
 nvcc cross-compiles without a GPU.  The .so files are git-ignored; a missing or stale one is rebuilt on demand.
 """
 import hashlib
@@ -22,8 +23,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "libkrasis_b200.so")
 SEQ_LIB = os.path.join(LIBDIR, "libkrasis_b200_seq.so")
-SEQ_SOURCES = ["seq_ops.cu", "seq_mix.cu", "seq_rec.cu", "seq_kv.cu", "seq_kv_attn.cu", "seq_kv_tile.cu", "seq_kv_pair.cu"]
-SOURCES = ["grouped_gemm.cu", "router_gemm.cu", "dense_gemm.cu", "split_gemm.cu", "gdn.cu", "gdn_tc.cu", "gqa.cu", "elementwise.cu", "moe_kernels.cu", "capi.cu", "capi_attn.cu", "capi_comm.cu"]
+SEQ_SOURCES = ["seq_ops.cu", "seq_mix.cu", "seq_rec.cu", "seq_kv.cu", "seq_kv_attn.cu", "seq_kv_tile.cu", "seq_kv_pair.cu", "seq_logp.cu"]
+SOURCES = ["grouped_gemm.cu", "router_gemm.cu", "dense_gemm.cu", "split_gemm.cu", "gdn.cu", "gdn_tc.cu", "gqa.cu", "elementwise.cu", "moe_kernels.cu", "capi.cu", "capi_attn.cu", "capi_comm.cu",
+           "fp8_rows.cu", "fp8_gemm.cu", "fp8_moe.cu", "capi_fp8.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

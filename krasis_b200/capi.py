@@ -123,6 +123,13 @@ SIGNATURES = {
     "kb2_linear_glu_bf16_binned": (C.c_int, [C.c_void_p] * 3 + [C.c_int32] * 4 + [C.c_float, C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32,
                                                                                   C.c_int32, C.c_void_p]),
     "kb2_linear_bf16_grouped": (C.c_int, [C.c_void_p] * 3 + [C.c_int32] * 4 + [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
+    "kb2_fp8_quantize_rows": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
+    "kb2_fp8_quantize_blocks": (C.c_int, [C.c_void_p] + [C.c_int32] * 4 + [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
+    "kb2_fp8_linear_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64] + [C.c_void_p] * 4 + [C.c_int32] * 5 + [C.c_void_p]),
+    "kb2_fp8_linear_workspace": (C.c_size_t, [C.c_int32] * 2),
+    "kb2_fp8_linear": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 4 + [C.c_int32] * 4 + [C.c_void_p, C.c_size_t, C.c_int32, C.c_void_p]),
+    "kb2_fp8_experts_workspace": (C.c_size_t, [C.c_int32] * 6),
+    "kb2_fp8_experts": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 7 + [C.c_int32] * 6 + [C.c_void_p, C.c_size_t, C.c_int32, C.c_void_p]),
     "kb2_fmha_maps": (C.c_int, [C.c_void_p] * 4 + [C.c_int32] * 7 + [C.c_float, C.c_int32, C.c_int32, C.c_void_p]),
     "kb2_fmha_maps_softcap": (C.c_int, [C.c_void_p] * 4 + [C.c_int32] * 7 + [C.c_float, C.c_float, C.c_int32, C.c_int32, C.c_void_p]),
     "kb2_fmha_maps_slopes": (C.c_int, [C.c_void_p] * 4 + [C.c_int32] * 7 + [C.c_float, C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,

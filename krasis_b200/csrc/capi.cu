@@ -58,7 +58,8 @@ const char* const kKernelNames[K_NUM] = {
     "router_gemm", "router_topk", "binning(count+scan+scatter)", "grouped_gemm<gate_up+silu_mul>", "grouped_gemm<down>", "combine",
     "dense_gemm<bf16>", "dense_gemm<int8>", "gdn_prep(conv+l2norm+gates)", "gdn_conv_state", "gdn_chunk_prepare", "gdn_chunk_scan",
     "gdn_post(gated_rmsnorm)", "gqa_prep(norm+rope+fp8_append)", "kv_gather(fp8->bf16)", "fmha", "mla_prep", "rmsnorm", "quant_rows_int8",
-    "silu_and_mul", "sigmoid_gate_mul", "add_bf16", "quantize_group", "retile"};
+    "silu_and_mul", "sigmoid_gate_mul", "add_bf16", "quantize_group", "retile",
+    "fp8_quantize", "fp8_product"};
 }  // namespace
 
 namespace kb2 {

@@ -44,4 +44,20 @@ inline cudaError_t allow_smem(int bytes) {
   return e;
 }
 
+// The call's device is the current one until the call returns.
+struct OnDevice {
+  int before = -1;
+  cudaError_t err;
+  explicit OnDevice(int device) {
+    err = cudaGetDevice(&before);
+    if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+    else before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+};
+
 }  // namespace kb2

@@ -1,0 +1,66 @@
+// 8-bit floating-point operands with a scale per block of 128, shared by fp8_rows.cu (making them), fp8_gemm.cu (products) and capi_fp8.cu.
+//
+// A block is 128 numbers of a row (activations) or 128 x 128 numbers of a matrix (weights); the last ones of a row or column may be cut short.  With a = max |x| over
+// the block: scale 2^k, k the least whole number >= -126 with a <= 448 2^k, codes e4m3(x / scale), ties to even.  A power of two costs a floating format nothing and
+// makes x / scale exact.  a = 0: scale 0, codes 0.  A number that is not finite: scale NaN, codes 0.  The products take any fp32 scales.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "moe_common.cuh"
+
+namespace kb2 {
+
+constexpr int kFp8Block = 128;
+__host__ __device__ constexpr int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+// What the bits of a block's largest magnitude say: its scale, and the reciprocal that numbers are multiplied by (0 where the codes are zeros).
+struct Fp8Scale {
+  float scale, inv;
+};
+__device__ __forceinline__ Fp8Scale fp8_scale(uint32_t a) {
+  const int e = (int)(a >> 23) - 127, k = max(e - 8 + ((a & 0x7FFFFFu) > 0x600000u ? 1 : 0), -126);      // 448 = 1.75 2^8
+  Fp8Scale s;
+  s.scale = __uint_as_float((uint32_t)(k + 127) << 23);
+  s.inv = __uint_as_float((uint32_t)(127 - k) << 23);
+  if (a == 0) s.scale = s.inv = 0.f;
+  if (a >= 0x7F800000u) {
+    s.scale = __uint_as_float(0x7FC00000u);
+    s.inv = 0.f;
+  }
+  return s;
+}
+// Four numbers -> four codes.  inv 0: zeros, whatever the numbers are.
+__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float inv) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
+  return inv == 0.f ? 0u : lo | hi << 16;
+}
+
+// out[m] = sum over the blocks of scales x codes of row m times those of w, per matrix of `groups` ones.  x [.][K] codes with scales xs[b * ldxs + row],
+// w [groups][N][K] with scales ws [groups][blocks of N][blocks of K].
+struct Fp8Product {
+  const void* x = nullptr;
+  const float* xs = nullptr;
+  long long ldxs = 0;
+  const void* w = nullptr;
+  const float* ws = nullptr;
+  const float* bias = nullptr;      // [N], one matrix only
+  void* out = nullptr;              // [M][N], bf16 or fp32
+  bool out_f32 = false;
+  int M = 0, N = 0, K = 0;
+  int groups = 1;
+  // runs of rows that share a matrix (null: all M rows, one matrix), at most max_chunks of them
+  const ChunkDesc* chunks = nullptr;
+  const int* n_chunks = nullptr;
+  int max_chunks = 0;
+};
+
+cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K, void* codes, float* scales, long long ld_scales, cudaStream_t s);
+cudaError_t launch_fp8_blocks(const void* w, bool f32, int groups, int N, int K, void* codes, float* scales, cudaStream_t s);
+cudaError_t launch_fp8_product(const Fp8Product& p, int num_sms, cudaStream_t s);
+
+}  // namespace kb2

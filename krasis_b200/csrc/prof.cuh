@@ -10,7 +10,8 @@ namespace kb2 {
 enum KernelId : int {
   K_ROUTER_GEMM = 0, K_ROUTER_TOPK, K_BINNING, K_GEMM1_GATE_UP, K_GEMM2_DOWN, K_COMBINE, K_DENSE_BF16, K_DENSE_I8,
   K_GDN_PREP, K_GDN_CONV_STATE, K_GDN_PREPARE, K_GDN_SCAN, K_GDN_POST, K_GQA_PREP, K_KV_GATHER, K_FMHA, K_MLA_PREP,
-  K_RMSNORM, K_QUANT_ROWS, K_SILU_MUL, K_SIGMOID_GATE, K_ADD, K_QUANTIZE_GROUP, K_RETILE, K_NUM
+  K_RMSNORM, K_QUANT_ROWS, K_SILU_MUL, K_SIGMOID_GATE, K_ADD, K_QUANTIZE_GROUP, K_RETILE,
+  K_FP8_QUANTIZE, K_FP8_PRODUCT, K_NUM
 };
 
 void kernel_span_begin(int id, cudaStream_t s, int n_launches, int* slot);

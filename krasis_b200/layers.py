@@ -112,6 +112,139 @@ def silu_and_mul(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# ------------------------------------------------------------------------------------------------ 8-bit floating-point products, a scale per block of 128
+
+FP8_BLOCK = 128
+
+
+def _fp8_blocks(n: int) -> int:
+    return (n + FP8_BLOCK - 1) // FP8_BLOCK
+
+
+def _f32_code(t, name) -> int:
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{name}: {t.dtype}, expected bfloat16 or float32")
+    return int(t.dtype is torch.float32)
+
+
+def _fp8_device(name, *tensors) -> int:
+    """The CUDA device that all tensors (None: not given) are on."""
+    dev = tensors[0].get_device()
+    if dev < 0 or any(t is not None and t.get_device() != dev for t in tensors):
+        raise ValueError(f"{name}: the tensors belong on one CUDA device (krasis_b200 has no CPU path)")
+    return dev
+
+
+def _fp8_input(name, x):
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] != 1):
+        raise ValueError(f"{name}: rows [M, K] whose numbers lie side by side, got {tuple(x.shape)} with strides {x.stride()}")
+    if x.shape[1] == 0 or x.shape[1] % 16:
+        raise ValueError(f"{name}: rows of {x.shape[1]} numbers, a multiple of 16 is needed")
+
+
+def _fp8_matrix(name, w, scales, shape):
+    """Codes of `shape` and a scale per block of 128 x 128 of its last two axes."""
+    want = tuple(shape[:-2]) + (_fp8_blocks(shape[-2]), _fp8_blocks(shape[-1]))
+    if w.dtype is not torch.float8_e4m3fn or tuple(w.shape) != tuple(shape) or not w.is_contiguous():
+        raise ValueError(f"{name}: contiguous float8_e4m3fn weights {tuple(shape)}, got {w.dtype} {tuple(w.shape)}")
+    if scales.dtype is not torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous():
+        raise ValueError(f"{name}: contiguous float32 scales {want}, got {scales.dtype} {tuple(scales.shape)}")
+
+
+def quantize_fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows [M, K] (bfloat16 or float32, any row stride, K a multiple of 16) in 8 bits: (codes [M, K] float8_e4m3fn, scales [M, ceil(K / 128)] float32, one for
+    each 128 numbers of a row).  A block's scale is the least 2^k, k >= -126, that its largest magnitude is at most 448 times of; a block of zeros has scale 0, one
+    with a number that is not finite scale NaN and codes 0.  The scales of one block of all rows lie side by side: strides (1, rows rounded up to 4)."""
+    _fp8_input("quantize_fp8_rows", x)
+    f32, dev, (m, k) = _f32_code(x, "quantize_fp8_rows"), _fp8_device("quantize_fp8_rows", x), x.shape
+    codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
+    ld = (m + 3) // 4 * 4
+    scales = torch.empty((_fp8_blocks(k), ld), dtype=torch.float32, device=x.device)
+    capi.check(capi.load().kb2_fp8_quantize_rows(x.data_ptr(), f32, x.stride(0), m, k, codes.data_ptr(), scales.data_ptr(), ld, dev, stream_on(dev)))
+    return codes, scales.t()[:m]
+
+
+def quantize_fp8_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A matrix [N, K] or a stack of them [E, N, K] (bfloat16 or float32, contiguous, K a multiple of 16) in 8 bits: codes of that shape, and a scale for each block of
+    128 x 128 by the rule of quantize_fp8_rows."""
+    if w.dim() not in (2, 3) or not w.is_contiguous() or w.shape[-1] == 0 or w.shape[-2] == 0 or w.shape[-1] % 16:
+        raise ValueError(f"quantize_fp8_blocks: contiguous [N, K] or [E, N, K] with K a multiple of 16, got {tuple(w.shape)}")
+    f32, dev, (n, k) = _f32_code(w, "quantize_fp8_blocks"), _fp8_device("quantize_fp8_blocks", w), w.shape[-2:]
+    codes = torch.empty(w.shape, dtype=torch.float8_e4m3fn, device=w.device)
+    scales = torch.empty(tuple(w.shape[:-2]) + (_fp8_blocks(n), _fp8_blocks(k)), dtype=torch.float32, device=w.device)
+    capi.check(capi.load().kb2_fp8_quantize_blocks(w.data_ptr(), f32, w.shape[0] if w.dim() == 3 else 1, n, k, codes.data_ptr(), scales.data_ptr(), dev, stream_on(dev)))
+    return codes, scales
+
+
+def _fp8_out(name, x, n, bias, out_dtype):
+    if bias is not None and (bias.dtype is not torch.float32 or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
+        raise ValueError(f"{name}: a float32 bias [{n}]")
+    out = torch.empty((x.shape[0], n), dtype=out_dtype, device=x.device)
+    return out, _f32_code(out, name)
+
+
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, bias: Optional[torch.Tensor] = None, out_dtype=None) -> torch.Tensor:
+    """x [M, K] (bfloat16 or float32) times a matrix that is held in 8 bits, weight [N, K] float8_e4m3fn with any fp32 scales [ceil(N / 128), ceil(K / 128)], plus bias
+    [N] float32: [M, N] in out_dtype (x's own).  The rows are quantised as by quantize_fp8_rows; sums are fp32."""
+    _fp8_input("fp8_linear", x)
+    (m, k), n = x.shape, weight.shape[0]
+    _fp8_matrix("fp8_linear", weight, weight_scales, (n, k))
+    f32, dev = _f32_code(x, "fp8_linear"), _fp8_device("fp8_linear", x, weight, weight_scales, bias)
+    out, o32 = _fp8_out("fp8_linear", x, n, bias, x.dtype if out_dtype is None else out_dtype)
+    lib = capi.load()
+    size = lib.kb2_fp8_linear_workspace(m, k)
+    work = torch.empty(size, dtype=torch.uint8, device=x.device)
+    capi.check(lib.kb2_fp8_linear(x.data_ptr(), f32, x.stride(0), weight.data_ptr(), weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), o32,
+                                  m, n, k, work.data_ptr(), size, dev, stream_on(dev)))
+    return out
+
+
+def fp8_linear_rows(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                    out_dtype=torch.bfloat16) -> torch.Tensor:
+    """fp8_linear on rows that are quantised already: codes [M, K] float8_e4m3fn and scales [M, ceil(K / 128)] float32 (in the order that quantize_fp8_rows leaves them;
+    others are copied into it)."""
+    _fp8_input("fp8_linear_rows", codes)
+    (m, k), n = codes.shape, weight.shape[0]
+    if codes.dtype is not torch.float8_e4m3fn or not codes.is_contiguous() or scales.dtype is not torch.float32 or tuple(scales.shape) != (m, _fp8_blocks(k)):
+        raise ValueError(f"fp8_linear_rows: contiguous float8_e4m3fn codes [M, K] and float32 scales [M, {_fp8_blocks(k)}]")
+    _fp8_matrix("fp8_linear_rows", weight, weight_scales, (n, k))
+    dev = _fp8_device("fp8_linear_rows", codes, scales, weight, weight_scales, bias)
+    out, o32 = _fp8_out("fp8_linear_rows", codes, n, bias, out_dtype)
+    if scales.stride(0) != 1 or scales.stride(1) % 4 or scales.stride(1) < m or scales.data_ptr() % 16:
+        kept = torch.empty((scales.shape[1], (m + 3) // 4 * 4), dtype=torch.float32, device=codes.device)
+        scales = kept.t()[:m].copy_(scales)
+    capi.check(capi.load().kb2_fp8_linear_rows(codes.data_ptr(), scales.data_ptr(), scales.stride(1), weight.data_ptr(), weight_scales.data_ptr(),
+                                               None if bias is None else bias.data_ptr(), out.data_ptr(), o32, m, n, k, dev, stream_on(dev)))
+    return out
+
+
+def fp8_experts(h: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate_up: torch.Tensor, s_gate_up: torch.Tensor, w_down: torch.Tensor, s_down: torch.Tensor,
+                out_dtype=None) -> torch.Tensor:
+    """Routed experts whose matrices are held in 8 bits: out[t] = sum_j weights[t, j] down_e(q(silu(gate_e q(h[t])) * up_e q(h[t]))) with e = ids[t, j] and q the
+    quantisation of quantize_fp8_rows.  h [T, W] bfloat16 or float32; ids [T, top] int32, those outside [0, E) bring nothing; weights [T, top] float32; w_gate_up
+    [E, 2 F, W] = [gate ; up] and w_down [E, W, F] float8_e4m3fn, with a scale for each block of 128 x 128; W a multiple of 16, F of 128, at most 1024 experts.
+    [T, W] in out_dtype (h's own); for bfloat16 each expert's row is rounded to it ahead of the weighted sum."""
+    _fp8_input("fp8_experts", h)
+    T, W = h.shape
+    if w_gate_up.dim() != 3 or w_gate_up.shape[1] % 256 or w_gate_up.shape[1] == 0:
+        raise ValueError(f"fp8_experts: gate and up projections [E, 2 F, W] with F a multiple of 128, got {tuple(w_gate_up.shape)}")
+    E, F = w_gate_up.shape[0], w_gate_up.shape[1] // 2
+    _fp8_matrix("fp8_experts", w_gate_up, s_gate_up, (E, 2 * F, W))
+    _fp8_matrix("fp8_experts", w_down, s_down, (E, W, F))
+    if ids.dtype is not torch.int32 or ids.dim() != 2 or ids.shape[0] != T or ids.shape[1] == 0 or not ids.is_contiguous():
+        raise ValueError(f"fp8_experts: contiguous int32 ids [{T}, top]")
+    if weights.dtype is not torch.float32 or weights.shape != ids.shape or not weights.is_contiguous():
+        raise ValueError(f"fp8_experts: contiguous float32 weights {tuple(ids.shape)}")
+    dev = _fp8_device("fp8_experts", h, ids, weights, w_gate_up, s_gate_up, w_down, s_down)
+    out = torch.empty((T, W), dtype=h.dtype if out_dtype is None else out_dtype, device=h.device)
+    f32, o32, top, lib = _f32_code(h, "fp8_experts"), _f32_code(out, "fp8_experts"), ids.shape[1], capi.load()
+    size = lib.kb2_fp8_experts_workspace(T, top, E, W, F, o32)
+    work = torch.empty(size, dtype=torch.uint8, device=h.device)
+    capi.check(lib.kb2_fp8_experts(h.data_ptr(), f32, h.stride(0), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(), s_gate_up.data_ptr(), w_down.data_ptr(),
+                                   s_down.data_ptr(), out.data_ptr(), o32, T, top, E, W, F, work.data_ptr(), size, dev, stream_on(dev)))
+    return out
+
+
 class SharedExpert:
     """TransformerLayer._shared_expert_forward (layer.py:508-524): INT8 gate_up / down + optional sigmoid gate."""
 

@@ -6,6 +6,7 @@ ImportError that names the build command.
 """
 import ctypes as C
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -19,6 +20,7 @@ SIGNATURES = {
     "kb2_seq_last_error": (C.c_char_p, []),
     "kb2_seq_total_launches": (C.c_longlong, []),
     "kb2_seq_wait_timeouts": (_I, [_I, _I, C.POINTER(C.c_int)]),
+    "kb2_seq_token_logprobs": (_I, [_P, _I, _L, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P]),
     "kb2_seq_embed": (_I, [_P, _I, _P, _P, _I, _I, _F, _P]),
     "kb2_seq_gemm": (_I, [_P, _I, _L, _P, _I, _L, _P, _I, _L, _I, _I, _I, _I, _L, _L, _L, _P]),
     "kb2_seq_residual_norm": (_I, [_P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _P]),
@@ -630,3 +632,38 @@ def kv_keep(tb: DraftTables, path: torch.Tensor, cache):
     if path.dtype is not torch.int32 or path.dim() != 2 or path.shape[0] != tb.S or not path.is_contiguous():
         raise ValueError(f"kv_keep: path is a contiguous int32 [{tb.S}, P]")
     check(load().kb2_seq_kv_keep(p, q, path.data_ptr(), path.shape[1], stream_on(dev)))
+
+
+# ------------------------------------------------------------------------------------------------ what a step's logits say
+
+class TokenLogprobs(NamedTuple):
+    """Of rows of logits: the given tokens' log probabilities [T], the entropies [T] (nats), and the largest alternatives [T, top] with theirs, the largest first."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+MAX_TOP_LOGPROBS = 64
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """logits [T, V] (fp32 or bfloat16, any row stride) and tokens [T] (int64 or int32): log softmax at the tokens, the entropy of the softmax, and the `top` largest
+    logits' ids (int32) and log probabilities, the lowest id first among equals.  All in fp32.  A token outside [0, V) has log probability -inf; logits of -inf weigh
+    nothing; a row with a NaN or +inf, or with nothing but -inf, gives NaN and ids of -1."""
+    _cuda(logits, "token_logprobs")
+    if logits.dim() != 2 or logits.shape[1] == 0 or (logits.stride(1) != 1 and logits.shape[1] != 1):
+        raise ValueError(f"token_logprobs: logits [T, V] whose numbers lie side by side, got {tuple(logits.shape)} with strides {logits.stride()}")
+    T, V = logits.shape
+    if tuple(tokens.shape) != (T,) or tokens.dtype not in (torch.int64, torch.int32) or tokens.get_device() != logits.get_device():
+        raise ValueError(f"token_logprobs: one int64 or int32 token per row, [{T}] on the logits' device")
+    top = int(top)
+    if not 0 <= top <= min(V, MAX_TOP_LOGPROBS):
+        raise ValueError(f"token_logprobs: {top} alternatives of {V}, at most {MAX_TOP_LOGPROBS}")
+    tokens = tokens.to(torch.int64).contiguous()
+    dev, dt = logits.device, dt_code(logits.dtype)
+    out = torch.empty(T * (2 + 2 * top), dtype=torch.float32, device=dev)          # one allocation
+    lp, en, best, ids = out[:T], out[T:2 * T], out[2 * T:(2 + top) * T].view(T, top), out[(2 + top) * T:].view(torch.int32).view(T, top)
+    check(load().kb2_seq_token_logprobs(logits.data_ptr(), dt, logits.stride(0), T, V, tokens.data_ptr(), top, lp.data_ptr(), en.data_ptr(), ids.data_ptr(),
+                                        best.data_ptr(), dev.index, _s(logits)))
+    return TokenLogprobs(lp, en, ids, best)
