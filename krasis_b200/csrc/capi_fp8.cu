@@ -12,7 +12,6 @@ cudaError_t launch_binning(const int* ids, const float* wts, int M, int top_k, i
                            cudaStream_t s);
 cudaError_t launch_fp8_gather(const void* codes, const float* scales, long long lds, const int* token_of, const int* slots, int max_slots, int K, void* out,
                               float* out_scales, long long ldo, cudaStream_t s);
-cudaError_t launch_fp8_glu(const float* gu, const int* slots, int max_slots, int F, void* codes, float* scales, long long lds, cudaStream_t s);
 cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s);
 }  // namespace kb2
 
@@ -121,7 +120,7 @@ KB2_API int kb2_fp8_linear(const void* x_dev, int32_t x_f32, int64_t ldx, const 
 // ---- routed experts
 struct ExpertsWork {
   uint8_t *hc, *xc, *ac;
-  float *hs, *xs, *as, *gu, *sorted_w;
+  float *hs, *xs, *as, *sorted_w;
   void* y;
   ChunkDesc* chunks;
   int *n_chunks, *counts, *offsets, *cursor, *slot_of, *token_of;
@@ -135,12 +134,11 @@ static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F,
   const size_t slots = (size_t)T * top;
   k.ldh = scale_ld(T);
   k.ldx = scale_ld((long long)slots);
-  k.max_chunks = (int)std::min<size_t>(slots, slots / kMaxChunkTokens + E);
+  k.max_chunks = (int)std::min<size_t>(slots, slots / kFp8Run + E);
   k.hc = c.take<uint8_t>((size_t)T * W);
   k.hs = c.take<float>((size_t)k.ldh * fp8_blocks(W));
   k.xc = c.take<uint8_t>(slots * W);
   k.xs = c.take<float>((size_t)k.ldx * fp8_blocks(W));
-  k.gu = c.take<float>(slots * 2 * F);
   k.ac = c.take<uint8_t>(slots * F);
   k.as = c.take<float>((size_t)k.ldx * fp8_blocks(F));
   k.y = c.take<uint8_t>(slots * W * (out_f32 ? 4 : 2));
@@ -159,6 +157,7 @@ static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F,
 static int experts_sizes(long long T, int top, int E, int W, int F) {
   if (T < 0 || top <= 0 || E <= 0 || E > 1024 || W <= 0 || W % 16 || F <= 0 || F % kFp8Block || W > 65535 * 128 || F > 65535 * 64)
     return failf(KB2_ERR_VALUE, "fp8_experts: need T >= 0, top > 0, 1 to 1024 experts, W %% 16 == 0, F %% 128 == 0 (T=%lld top=%d E=%d W=%d F=%d)", T, top, E, W, F);
+  if ((long long)E * std::max(2 * F, W) > INT32_MAX / 2) return failf(KB2_ERR_VALUE, "fp8_experts: E=%d W=%d F=%d is too large", E, W, F);
   if (T * top > INT32_MAX / 4) return failf(KB2_ERR_VALUE, "fp8_experts: %lld tokens of %d choices are too many", T, top);
   return KB2_OK;
 }
@@ -180,16 +179,15 @@ KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const
   CUDA_TRY(on.err);
   cudaStream_t s = (cudaStream_t)stream;
   const int slots = T * top;
-  CUDA_TRY(launch_binning(ids_dev, weights_dev, T, top, 0, E, kMaxChunkTokens, k.counts, k.offsets, k.cursor, k.chunks, k.n_chunks, k.sorted_w, k.slot_of, nullptr, k.token_of,
+  CUDA_TRY(launch_binning(ids_dev, weights_dev, T, top, 0, E, kFp8Run, k.counts, k.offsets, k.cursor, k.chunks, k.n_chunks, k.sorted_w, k.slot_of, nullptr, k.token_of,
                           nullptr, nullptr, 0, s));
   CUDA_TRY(launch_fp8_rows(h_dev, h_f32 != 0, ldh, T, W, k.hc, k.hs, k.ldh, s));
   CUDA_TRY(launch_fp8_gather(k.hc, k.hs, k.ldh, k.token_of, k.offsets + E, slots, W, k.xc, k.xs, k.ldx, s));
   Fp8Product p;
-  p.x = k.xc; p.xs = k.xs; p.ldxs = k.ldx; p.w = w1_dev; p.ws = s1_dev; p.out = k.gu; p.out_f32 = true;
+  p.x = k.xc; p.xs = k.xs; p.ldxs = k.ldx; p.w = w1_dev; p.ws = s1_dev; p.out = k.ac;
   p.M = slots; p.N = 2 * F; p.K = W; p.groups = E;
   p.chunks = k.chunks; p.n_chunks = k.n_chunks; p.max_chunks = k.max_chunks;
-  CUDA_TRY(launch_fp8_product(p, current_sms(), s));
-  CUDA_TRY(launch_fp8_glu(k.gu, k.offsets + E, slots, F, k.ac, k.as, k.ldx, s));
+  CUDA_TRY(launch_fp8_gated(p, k.as, k.ldx, current_sms(), s));
   p.x = k.ac; p.xs = k.as; p.w = w2_dev; p.ws = s2_dev; p.out = k.y; p.out_f32 = out_f32 != 0;
   p.N = W; p.K = F;
   CUDA_TRY(launch_fp8_product(p, current_sms(), s));

@@ -15,6 +15,7 @@
 namespace kb2 {
 
 constexpr int kFp8Block = 128;
+constexpr int kFp8Run = 256;      // the most rows of a run
 __host__ __device__ constexpr int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 
 // What the bits of a block's largest magnitude say: its scale, and the reciprocal that numbers are multiplied by (0 where the codes are zeros).
@@ -53,7 +54,7 @@ struct Fp8Product {
   bool out_f32 = false;
   int M = 0, N = 0, K = 0;
   int groups = 1;
-  // runs of rows that share a matrix (null: all M rows, one matrix), at most max_chunks of them
+  // runs of up to kFp8Run rows that share a matrix (null: all M rows, one matrix), at most max_chunks of them
   const ChunkDesc* chunks = nullptr;
   const int* n_chunks = nullptr;
   int max_chunks = 0;
@@ -62,5 +63,7 @@ struct Fp8Product {
 cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K, void* codes, float* scales, long long ld_scales, cudaStream_t s);
 cudaError_t launch_fp8_blocks(const void* w, bool f32, int groups, int N, int K, void* codes, float* scales, cudaStream_t s);
 cudaError_t launch_fp8_product(const Fp8Product& p, int num_sms, cudaStream_t s);
+// Runs of rows times matrices [gate: N / 2 | up: N / 2]: silu(gate) up in fp32, quantised by rows: codes [M][N / 2] in p.out, out_scales[b * ld + row].  N % 256 == 0.
+cudaError_t launch_fp8_gated(const Fp8Product& p, float* out_scales, long long ld_out_scales, int num_sms, cudaStream_t s);
 
 }  // namespace kb2

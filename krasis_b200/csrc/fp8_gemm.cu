@@ -1,76 +1,478 @@
 // Products of 8-bit floating-point operands with a scale per block of 128 (fp8.cuh): out[m][n] = sum_b xs[m][b] ws[n / 128][b] sum_{k in block b} x[m][k] w[n][k].
-// A block's 128 products are summed in fp32, then multiplied by the two scales and added up.
+//
+// The tensor cores' accumulators cannot be rescaled on the way, so each block of 128 products per result is a sum of its own in tensor memory (two of them in turn),
+// which the other warps multiply by its scales and add up in registers while the next one runs.
+#include <cuda.h>
+
 #include "fp8.cuh"
 #include "prof.cuh"
+#include "ptx.cuh"
+#include "seq_act.cuh"
 
 namespace kb2 {
 
-constexpr int kFTile = 64, kFStep = 32;
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// a b + c for two numbers at once
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// the larger of the number at a place of either CTA's shared memory and v
+__device__ __forceinline__ void max_cluster(uint32_t addr, uint32_t v) { asm volatile("red.shared::cluster.max.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// mbar_wait for what the other CTA has written and told
+__device__ __forceinline__ void mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+  mbar_wait(bar, parity);
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+}
+cudaError_t make_tmap_u8_rows(void* out_tmap, const void* base, long long rows, long long cols, int box_rows);
+cudaError_t make_tmap_u8_gate_up(void* out_tmap, const void* base, long long groups, long long F, long long cols);
 
-// 64 x 64 results of a thread block, 4 x 4 of a thread.
-__global__ void __launch_bounds__(256) fp8_product_kernel(const Fp8Product p) {
+// ---- many rows: pairs of CTAs, 256 weight rows x up to 256 rows of x
+// The weights are the M side of the instruction: a CTA has 128 of them, of one block of 128 (one scale), and half the rows of x, 32 KB for 512 cycles of MMAs.  The N side,
+// rows of x, goes in steps of 32, so runs of rows (an expert's) need little padding.  Eight warps hold the tile's sums, 128 a thread; a thread has four weight rows and
+// pairs of neighbouring rows of x, whose scales it gets as four numbers per 16 bytes.
+constexpr int kFStages = 6, kFRows = 128, kFBox = 16, kFABytes = kFRows * 128, kFStage = 2 * kFABytes;
+constexpr int kFMost = kFp8Run;                       // rows of x per tile
+constexpr int kFScales = 4;                        // blocks whose scales are at hand
+constexpr int kFThreads = 384, kFWarps = 8;
+constexpr int kFStageOut = 2560;                   // a warp's results on their way out
+constexpr int kFOffOut = kFStages * kFStage, kFOffScale = kFOffOut + kFWarps * kFStageOut, kFOffMax = kFOffScale + kFScales * 2 * kFMost * 4,
+              kFOffBar = kFOffMax + 2 * kFMost * 4, kFSmem = kFOffBar + 256;
+static_assert(kFSmem >= 512 * 430 - 1024 && kFSmem <= 227 * 1024, "what a CTA of a cluster takes for 512 columns (tmem_smem)");
+
+struct PairArgs {
+  Fp8Product p;
+  int w_tiles, row_tile;                           // tiles of 256 weight rows (gated: 128 of either half); rows of x per tile (one matrix)
+  // gated units: out is codes [M][N / 2] with scales
+  float* out_scales;
+  long long ld_out_scales;
+};
+
+// Where column c of a tile finds its scale: the numbers that a thread wants of 16 columns lie side by side.
+__device__ __forceinline__ int scale_place(int c) { return (c & ~15) | (c >> 1 & 3) << 2 | (c >> 3 & 1) << 1 | (c & 1); }
+
+template <bool kGlu, bool kOutF32>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
+    fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const PairArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFOffBar);       // of the first CTA: both CTAs' loads
+  uint64_t* empty = full + kFStages;
+  uint64_t* acc_full = empty + kFStages;           // [2]
+  uint64_t* acc_empty = acc_full + 2;              // [2], of the first CTA: both CTAs' read-outs
+  uint64_t* s_full = acc_empty + 2;                // [kFScales]
+  uint64_t* s_empty = s_full + kFScales;
+  uint64_t* max_full = s_empty + kFScales;         // [2]
+  uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(max_full + 2);
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const Fp8Product& p = a.p;
+  if (threadIdx.x == 32) {
+    if (smem_u32(smem) & 1023u) __trap();
+    for (int i = 0; i < kFStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * kFWarps);
+      mbar_init(&max_full[i], 2 * kFWarps);
+    }
+    for (int i = 0; i < kFScales; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], kFWarps);
+    }
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 64) {
+    prefetch_tmap(&tmap_x);
+    prefetch_tmap(&tmap_w);
+  }
+  if (kGlu)
+    for (int i = threadIdx.x; i < 2 * kFMost; i += kFThreads) reinterpret_cast<uint32_t*>(smem + kFOffMax)[i] = 0;
+  if (warp == 0) tmem_alloc_pair(tmem_ptr_smem, 512);
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();                              // the other CTA's barriers are there
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_ptr_smem;
   pdl_wait();
-  __shared__ __align__(16) float xs[kFStep][kFTile + 4], ws[kFStep][kFTile + 4];
-  int row0 = 0, rows = p.M, group = 0;
-  if (p.chunks) {
-    if ((int)blockIdx.z >= p.n_chunks[0]) return;
-    const ChunkDesc c = p.chunks[blockIdx.z];
-    row0 = c.slot_begin;
-    rows = c.n_tok;
-    group = c.expert;
-  }
-  const int m0 = blockIdx.y * kFTile, n0 = blockIdx.x * kFTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, nb = fp8_blocks(p.K);
-  if (m0 >= rows) return;
-  const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x) + (long long)row0 * p.K;
-  const uint8_t* w = reinterpret_cast<const uint8_t*>(p.w) + (long long)group * p.N * p.K;
-  const auto number = [](uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); };
-  float acc[4][4] = {};
-  for (int b = 0; b < nb; ++b) {
-    float part[4][4] = {};
-    for (int k0 = b * kFp8Block; k0 < min(p.K, (b + 1) * kFp8Block); k0 += kFStep) {
-      for (int i = threadIdx.x; i < kFTile * kFStep; i += 256) {
-        const int r = i / kFStep, k = i % kFStep;
-        xs[k][r] = m0 + r < rows && k0 + k < p.K ? number(x[(long long)(m0 + r) * p.K + k0 + k]) : 0.f;
-        ws[k][r] = n0 + r < p.N && k0 + k < p.K ? number(w[(long long)(n0 + r) * p.K + k0 + k]) : 0.f;
+  const int F = p.N / 2, nb = fp8_blocks(p.K);
+  const int units = p.chunks ? p.n_chunks[0] : (p.M + a.row_tile - 1) / a.row_tile, total = units * a.w_tiles;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  struct Item {
+    int row0, rows, group, wt, nt;
+  };
+  // weight tiles first, so that pairs that run at once share the rows of x
+  const auto item = [&](int t) {
+    Item i;
+    const int u = t / a.w_tiles;
+    i.wt = t - u * a.w_tiles;
+    if (p.chunks) {
+      const ChunkDesc c = p.chunks[u];
+      i.row0 = c.slot_begin;
+      i.rows = c.n_tok;
+      i.group = c.expert;
+    } else {
+      i.row0 = u * a.row_tile;
+      i.rows = min(a.row_tile, p.M - i.row0);
+      i.group = 0;
+    }
+    i.nt = __shfl_sync(0xffffffffu, (i.rows + 31) & ~31, 0);
+    return i;
+  };
+
+  if (warp >= 4) {
+    more_registers<216>();
+    const int q = warp & 3, h = (warp - 4) >> 2, l = lane & 3, r = lane >> 2;
+    const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16);
+    uint8_t* out_at = smem + kFOffOut + (warp - 4) * kFStageOut;
+    int b = 0;
+    uint32_t aphase = 0, slot = 0, sphase = 0, tile = 0;
+    for (int t = first; t < total; t += step, ++tile) {
+      const Item i = item(t);
+      const int c0 = h * (i.nt / 2), cols = i.nt / 2, steps = (cols + 31) / 32;
+      uint64_t acc[4][2][4][2];                    // [32 columns][rows 16 apart][8 columns][rows 8 apart]
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[s][j >> 3][j >> 1 & 3][j & 1] = 0;
+      for (int kb = 0; kb < nb; ++kb) {
+        const float* sc = reinterpret_cast<const float*>(smem + kFOffScale) + slot * 2 * kFMost + c0 + 4 * l;
+        mbar_wait(&s_full[slot], sphase);
+        mbar_wait(&acc_full[b], aphase);
+        tc_fence_after_sync();
+        const uint32_t from = lanes + b * 256 + c0;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if (s >= steps) break;
+          uint32_t v[2][16];
+          tmem_ld_rows16(from + s * 32, v[0]);
+          tmem_ld_rows16(from + s * 32 + (16u << 16), v[1]);
+          uint4 g[2], u[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            g[j] = *reinterpret_cast<const uint4*>(sc + s * 32 + j * 16);
+            if (kGlu) u[j] = *reinterpret_cast<const uint4*>(sc + kFMost + s * 32 + j * 16);
+          }
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint64_t sg = j & 1 ? pack2(g[j / 2].z, g[j / 2].w) : pack2(g[j / 2].x, g[j / 2].y);
+            const uint64_t su = !kGlu ? sg : j & 1 ? pack2(u[j / 2].z, u[j / 2].w) : pack2(u[j / 2].x, u[j / 2].y);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              acc[s][e][j][0] = fma2(pack2(v[e][4 * j], v[e][4 * j + 1]), sg, acc[s][e][j][0]);
+              acc[s][e][j][1] = fma2(pack2(v[e][4 * j + 2], v[e][4 * j + 3]), su, acc[s][e][j][1]);
+            }
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_cluster(cluster_addr(&acc_empty[b], 0));
+          mbar_arrive(&s_empty[slot]);
+        }
+        if (++slot == kFScales) { slot = 0; sphase ^= 1; }
+        b ^= 1;
+        aphase ^= b == 0;
       }
-      __syncthreads();
+      // thread (r, l) has of columns c0 + 32 s + 8 j + 2 l and the one behind it the weight rows 32 q + 16 e + 8 k + r
+      if constexpr (kGlu) {
+        // rows 16 e + r of the 32 are gate, 16 e + 8 + r up of the unit 64 rank + 16 q + 8 e + r of the tile
+        uint32_t* most = reinterpret_cast<uint32_t*>(smem + kFOffMax) + (tile & 1) * kFMost;
+        uint32_t* other = reinterpret_cast<uint32_t*>(smem + kFOffMax) + (~tile & 1) * kFMost;
+        named_bar_sync(1, 32 * kFWarps);           // everyone has read the last tile's maxima
+        if (warp == 4)
+          for (int c = lane; c < kFMost; c += 32) other[c] = 0;
+        const uint32_t peer = cluster_addr(most, rank ^ 1);
 #pragma unroll
-      for (int k = 0; k < kFStep; ++k) {
-        const float4 a = *reinterpret_cast<const float4*>(&xs[k][ty * 4]), c = *reinterpret_cast<const float4*>(&ws[k][tx * 4]);
-        const float av[4] = {a.x, a.y, a.z, a.w}, cv[4] = {c.x, c.y, c.z, c.w};
+        for (int s = 0; s < 4; ++s) {
+          if (s >= steps) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int j = 0; j < 4; ++j) {
+            uint32_t m0 = 0, m1 = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][j] = fmaf(av[i], cv[j], part[i][j]);
+            for (int e = 0; e < 2; ++e) {
+              float g0, g1, u0, u1;
+              unpack2(acc[s][e][j][0], g0, g1);
+              unpack2(acc[s][e][j][1], u0, u1);
+              const float v0 = kb2act::silu(g0) * u0, v1 = kb2act::silu(g1) * u1;
+              acc[s][e][j][0] = pack2(__float_as_uint(v0), __float_as_uint(v1));
+              m0 = max(m0, __float_as_uint(v0) & 0x7FFFFFFFu);
+              m1 = max(m1, __float_as_uint(v1) & 0x7FFFFFFFu);
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+              m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+              m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+            }
+            const int c = s * 32 + j * 8 + 2 * l;
+            if (r < 2 && c < cols) {               // lanes of r 0 tell their own CTA, those of r 1 the other
+              const uint32_t to = (r ? peer : smem_u32(most)) + (c0 + c) * 4;
+              if (r) {
+                max_cluster(to, m0);
+                max_cluster(to + 4, m1);
+              } else {
+                atomicMax(&most[c0 + c], m0);
+                atomicMax(&most[c0 + c + 1], m1);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_cluster(cluster_addr(&max_full[tile & 1], rank));
+          mbar_arrive_cluster(cluster_addr(&max_full[tile & 1], rank ^ 1));
+        }
+        mbar_wait_cluster(&max_full[tile & 1], tile >> 1 & 1);
+        uint8_t* codes = reinterpret_cast<uint8_t*>(p.out);
+        const int f0 = i.wt * 128 + rank * 64 + q * 16;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if (s >= steps) break;
+          uint32_t w[2][2];                        // [8 columns of gate and up][16 columns]: this thread's codes of them, a pair of columns in 16 bits
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = c0 + s * 32 + j * 8 + 2 * l;
+            const Fp8Scale s0 = fp8_scale(most[min(c, kFMost - 2)]), s1 = fp8_scale(most[min(c, kFMost - 2) + 1]);
+            if (q == 0 && rank == 0 && r == 0 && c - c0 < cols) {
+              if (c < i.rows) a.out_scales[i.wt * a.ld_out_scales + i.row0 + c] = s0.scale;
+              if (c + 1 < i.rows) a.out_scales[i.wt * a.ld_out_scales + i.row0 + c + 1] = s1.scale;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v0, v1;
+              unpack2(acc[s][e][j][0], v0, v1);
+              v0 = s0.inv == 0.f ? 0.f : v0 * s0.inv;
+              v1 = s1.inv == 0.f ? 0.f : v1 * s1.inv;
+              const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v0, v1), __NV_SATFINITE, __NV_E4M3);
+              w[e][j >> 1] = j & 1 ? w[e][j >> 1] | two << 16 : two;
+            }
+          }
+          // matrix (e, j / 2): its column 2 l' + i is the pair l' of the eight columns 2 (j / 2) + i
+          __syncwarp();
+          stmatrix4_t(smem_u32(out_at) + (lane & 7) * 80 + (lane >> 3) * 16, w[0][0], w[0][1], w[1][0], w[1][1]);
+          __syncwarp();
+          // a thread takes row `lane & 7` of matrix lane >> 3: eight units of two columns
+          const uint4 x = *reinterpret_cast<const uint4*>(out_at + (lane & 7) * 80 + (lane >> 3) * 16);
+          const int c = s * 32 + (lane >> 3 & 1) * 16 + (lane & 1) * 8 + (lane >> 1 & 3) * 2;
+          const int m = c0 + c;
+          if (c < cols) {
+            uint8_t* to = codes + (long long)(i.row0 + m) * F + f0 + (lane >> 4) * 8;
+            if (m < i.rows) *reinterpret_cast<uint2*>(to) = make_uint2(__byte_perm(x.x, x.y, 0x6420), __byte_perm(x.z, x.w, 0x6420));
+            if (m + 1 < i.rows) *reinterpret_cast<uint2*>(to + F) = make_uint2(__byte_perm(x.x, x.y, 0x7531), __byte_perm(x.z, x.w, 0x7531));
+          }
+        }
+      } else {
+        const int n0 = i.wt * 256 + rank * 128 + q * 32;
+        float bias[2][2] = {};
+        if (p.bias != nullptr)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) bias[k >> 1][k & 1] = n0 + k * 8 + r < p.N ? p.bias[n0 + k * 8 + r] : 0.f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if (s >= steps) break;
+          const int m0 = c0 + s * 32, have = min(i.rows, c0 + cols) - m0;
+          if constexpr (kOutF32) {
+            float* st = reinterpret_cast<float*>(out_at);                  // [16 columns][36]
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if ((j & 1) == 0) __syncwarp();
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float v0, v1;
+                unpack2(acc[s][e >> 1][j][e & 1], v0, v1);
+                float* to = st + ((j & 1) * 8 + 2 * l) * 36 + e * 8 + r;
+                to[0] = v0 + bias[e >> 1][e & 1];
+                to[36] = v1 + bias[e >> 1][e & 1];
+              }
+              if (j & 1) {
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const int c = k * 4 + (lane >> 3), m = (j >> 1) * 16 + c, n = n0 + (lane & 7) * 4;
+                  if (m >= have || n >= p.N) continue;
+                  const float4 x = *reinterpret_cast<const float4*>(st + c * 36 + (lane & 7) * 4);
+                  float* to = reinterpret_cast<float*>(p.out) + (long long)(i.row0 + m0 + m) * p.N + n;
+                  if ((p.N & 3) == 0) *reinterpret_cast<float4*>(to) = x;
+                  else {
+                    to[0] = x.x;
+                    if (n + 1 < p.N) to[1] = x.y;
+                    if (n + 2 < p.N) to[2] = x.z;
+                    if (n + 3 < p.N) to[3] = x.w;
+                  }
+                }
+              }
+            }
+          } else {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float v0, v1;
+                unpack2(acc[s][e >> 1][j][e & 1], v0, v1);
+                w[e] = bf16x2_bits_rn(v1 + bias[e >> 1][e & 1], v0 + bias[e >> 1][e & 1]);
+              }
+              stmatrix4_t(smem_u32(out_at) + (j * 8 + (lane & 7)) * 80 + (lane >> 3) * 16, w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int m = k * 8 + (lane >> 2), n = n0 + l * 8;
+              if (m >= have || n >= p.N) continue;
+              const uint4 x = *reinterpret_cast<const uint4*>(out_at + m * 80 + l * 16);
+              __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(p.out) + (long long)(i.row0 + m0 + m) * p.N + n;
+              if ((p.N & 7) == 0) *reinterpret_cast<uint4*>(to) = x;
+              else {
+                const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                  if (n + y < p.N) to[y] = __ushort_as_bfloat16((unsigned short)(u[y >> 1] >> (y & 1) * 16));
+              }
+            }
+          }
+        }
       }
-      __syncthreads();
     }
-    const float sw = p.ws[((long long)group * fp8_blocks(p.N) + n0 / kFp8Block) * nb + b];
+  } else if (fewer_registers<64>(), warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int t = first; t < total; t += step) {
+      const Item i = item(t);
+      const uint32_t bytes = 2 * kFABytes + i.nt * 128;
+      const int x0 = i.row0 + rank * (i.nt / 2);
+      for (int kb = 0; kb < nb; ++kb) {
+        mbar_wait(&empty[stage], phase ^ 1);
+        uint8_t* at = smem + stage * kFStage;
+        if (elect_one()) {
+          const uint32_t bar = cluster_addr(&full[stage], 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+          if constexpr (kGlu) tma_load_5d_pair(at, &tmap_w, kb * 128, 0, 0, (i.wt * 128 + (int)rank * 64) / 8, i.group, bar);
+          else tma_load_2d_pair(at, &tmap_w, kb * 128, i.group * p.N + i.wt * 256 + rank * 128, bar);
+          for (int r = 0; r < i.nt / 2; r += kFBox) tma_load_2d_pair(at + kFABytes + r * 128, &tmap_x, kb * 128, x0 + r, bar);
+        }
+        __syncwarp();
+        if (++stage == kFStages) { stage = 0; phase ^= 1; }
+      }
+    }
+    for (int i = 0; i < kFStages; ++i) {           // the last reports of freed stages have arrived, too
+      mbar_wait(&empty[stage], phase ^ 1);
+      if (++stage == kFStages) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      int stage = 0, b = 0;
+      uint32_t phase = 0, aphase = 0;
+      for (int t = first; t < total; t += step) {
+        const uint32_t idesc = umma_idesc_e4m3(256, item(t).nt);
+        for (int kb = 0; kb < nb; ++kb) {
+          mbar_wait(&acc_empty[b], aphase ^ 1);
+          mbar_wait(&full[stage], phase);
+          tc_fence_after_sync();
+          const uint32_t addr = smem_u32(smem + stage * kFStage);
+          const uint64_t ad = umma_desc_k_sw128(addr), bd = umma_desc_k_sw128(addr + kFABytes);
+          if (elect_one()) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int m = m0 + ty * 4 + i;
-      const float s = m < rows ? p.xs[b * p.ldxs + row0 + m] * sw : 0.f;
+            for (int k = 0; k < 4; ++k) umma_f8_pair(tmem_base + b * 256, ad + 2 * k, bd + 2 * k, idesc, k > 0 ? 1u : 0u);
+            umma_commit_pair(&empty[stage]);
+            umma_commit_pair(&acc_full[b]);
+          }
+          __syncwarp();
+          if (++stage == kFStages) { stage = 0; phase ^= 1; }
+          b ^= 1;
+          aphase ^= b == 0;
+        }
+      }
+    }
+  } else if (warp < 4) {
+    // the scales of a block: those of the rows of x times the weights', by two warps in turn
+    int turn = 0;
+    uint32_t slot = 0, phase = 0;
+    for (int t = first; t < total; t += step) {
+      const Item i = item(t);
+      const int blocks = fp8_blocks(p.N), n0 = kGlu ? i.wt : min(i.wt * 2 + (int)rank, blocks - 1);
+      const float* ws = p.ws + ((long long)i.group * blocks + n0) * nb;
+      for (int kb = 0; kb < nb; ++kb, turn ^= 1) {
+        if (turn == warp - 2) {
+          float v[kFMost / 32];
+          const float g = ws[kb], u = kGlu ? ws[(long long)(F / kFp8Block) * nb + kb] : 0.f;
+          const float* xs = p.xs + kb * p.ldxs + i.row0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(part[i][j], s, acc[i][j]);
+          for (int j = 0; j < kFMost / 32; ++j) v[j] = j * 32 + lane < i.rows ? xs[j * 32 + lane] : 0.f;
+          mbar_wait(&s_empty[slot], phase ^ 1);
+          float* to = reinterpret_cast<float*>(smem + kFOffScale) + slot * 2 * kFMost;
+#pragma unroll
+          for (int j = 0; j < kFMost / 32; ++j)
+            if (j * 32 < i.nt) {
+              to[scale_place(j * 32 + lane)] = v[j] * g;
+              if (kGlu) to[kFMost + scale_place(j * 32 + lane)] = v[j] * u;
+            }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_full[slot]);
+        }
+        if (++slot == kFScales) { slot = 0; phase ^= 1; }
+      }
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m >= rows || n >= p.N) continue;
-      const float v = acc[i][j] + (p.bias ? p.bias[n] : 0.f);
-      const long long at = (long long)(row0 + m) * p.N + n;
-      if (p.out_f32) reinterpret_cast<float*>(p.out)[at] = v;
-      else reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();                              // nobody leaves while the other may still report to its barriers
+  tc_fence_after_sync();
+  if (warp == 0) tmem_dealloc_pair(tmem_base, 512);
+}
+
+// Rows of x per tile of one matrix: what takes the fewest rounds of the chip's pairs, weighed by a block's time, which is that of 256 weight rows on their way (as much as
+// 96 rows of x in MMAs) at least.
+static int pair_rows(int M, int w_tiles, int pairs) {
+  int best = kFMost;
+  long long least = -1;
+  for (int nt = kFMost; nt >= 32; nt -= 32) {
+    const long long rounds = ((long long)((M + nt - 1) / nt) * w_tiles + pairs - 1) / pairs, time = rounds * (nt > 96 ? nt : 96);
+    if (least < 0 || time < least) {
+      least = time;
+      best = nt;
     }
+  }
+  return best;
+}
+
+template <bool kGlu, bool kOutF32>
+static cudaError_t launch_pair(const PairArgs& a, int num_sms, cudaStream_t s) {
+  const Fp8Product& p = a.p;
+  alignas(64) CUtensorMap tx, tw;
+  cudaError_t e = make_tmap_u8_rows(&tx, p.x, p.M, p.K, kFBox);
+  if (e == cudaSuccess) e = kGlu ? make_tmap_u8_gate_up(&tw, p.w, p.groups, p.N / 2, p.K) : make_tmap_u8_rows(&tw, p.w, (long long)p.groups * p.N, p.K, kFRows);
+  if (e == cudaSuccess) e = allow_smem<fp8_pair_kernel<kGlu, kOutF32>>(kFSmem);
+  if (e != cudaSuccess) return e;
+  const long long total = (long long)a.w_tiles * (p.chunks ? p.max_chunks : (p.M + a.row_tile - 1) / a.row_tile);
+  const int pairs = (int)(total < num_sms / 2 ? total : num_sms / 2);
+  return launch_pdl(fp8_pair_kernel<kGlu, kOutF32>, 2 * pairs, kFThreads, kFSmem, s, tx, tw, a);
 }
 
 cudaError_t launch_fp8_product(const Fp8Product& p, int num_sms, cudaStream_t s) {
   KernelSpan ks(K_FP8_PRODUCT, s);
-  const int most = p.chunks ? kMaxChunkTokens : p.M;
-  return launch_pdl(fp8_product_kernel, dim3((p.N + kFTile - 1) / kFTile, (most + kFTile - 1) / kFTile, p.chunks ? p.max_chunks : 1), 256, 0, s, p);
+  PairArgs a{p, (p.N + 255) / 256, 0, nullptr, 0};
+  if (!p.chunks) a.row_tile = pair_rows(p.M, a.w_tiles, num_sms / 2);
+  return p.out_f32 ? launch_pair<false, true>(a, num_sms, s) : launch_pair<false, false>(a, num_sms, s);
+}
+
+cudaError_t launch_fp8_gated(const Fp8Product& p, float* out_scales, long long ld_out_scales, int num_sms, cudaStream_t s) {
+  KernelSpan ks(K_FP8_PRODUCT, s);
+  const PairArgs a{p, p.N / 256, 0, out_scales, ld_out_scales};
+  return launch_pair<true, false>(a, num_sms, s);
 }
 
 }  // namespace kb2

@@ -1,7 +1,6 @@
-// Routed experts on 8-bit operands (fp8.cuh): what lies between and behind their two products.
+// Routed experts on 8-bit operands (fp8.cuh): what lies ahead of and behind their two products.
 #include "fp8.cuh"
 #include "prof.cuh"
-#include "seq_act.cuh"
 
 namespace kb2 {
 
@@ -14,27 +13,6 @@ __global__ void __launch_bounds__(256) fp8_gather_kernel(const uint8_t* codes, c
   const int t = token_of[slot];
   for (int k = lane * 16; k < K; k += 512) *reinterpret_cast<uint4*>(out + (long long)slot * K + k) = *reinterpret_cast<const uint4*>(codes + (long long)t * K + k);
   for (int b = lane; b < fp8_blocks(K); b += 32) out_scales[b * ldo + slot] = scales[b * lds + t];
-}
-
-// silu(gate) up of rows [gate: F | up: F] in fp32, quantised; sixteen lanes have a block of 128.
-__global__ void __launch_bounds__(256) fp8_glu_kernel(const float* gu, const int* slots, int F, uint8_t* codes, float* scales, long long lds) {
-  pdl_wait();
-  const int lane = threadIdx.x & 15, slot = blockIdx.x * 16 + (threadIdx.x >> 4), b = blockIdx.y, f = b * kFp8Block + lane * 8;
-  const bool in = slot < slots[0];
-  float v[8];
-  uint32_t a = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const long long at = (long long)slot * 2 * F + f + i;
-    v[i] = in ? kb2act::silu(gu[at]) * gu[at + F] : 0.f;
-    a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  }
-#pragma unroll
-  for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-  if (!in) return;
-  const Fp8Scale s = fp8_scale(a);
-  *reinterpret_cast<uint2*>(codes + (long long)slot * F + f) = make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], s.inv), fp8_codes4(v[4], v[5], v[6], v[7], s.inv));
-  if (lane == 0) scales[b * lds + slot] = s.scale;
 }
 
 // out[t] = sum_j weights[t][j] y[slot_of[t][j]] in the order of j; entries without a slot bring nothing.
@@ -60,10 +38,6 @@ cudaError_t launch_fp8_gather(const void* codes, const float* scales, long long 
                               float* out_scales, long long ldo, cudaStream_t s) {
   KernelSpan ks(K_FP8_QUANTIZE, s);
   return launch_pdl(fp8_gather_kernel, (max_slots + 7) / 8, 256, 0, s, (const uint8_t*)codes, scales, lds, token_of, slots, K, (uint8_t*)out, out_scales, ldo);
-}
-cudaError_t launch_fp8_glu(const float* gu, const int* slots, int max_slots, int F, void* codes, float* scales, long long lds, cudaStream_t s) {
-  KernelSpan ks(K_FP8_QUANTIZE, s);
-  return launch_pdl(fp8_glu_kernel, dim3((max_slots + 15) / 16, F / kFp8Block), 256, 0, s, gu, slots, F, (uint8_t*)codes, scales, lds);
 }
 cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s) {
   KernelSpan ks(K_COMBINE, s);
