@@ -39,15 +39,16 @@ cudaError_t make_tmap_u8_gate_up(void* out_tmap, const void* base, long long gro
 
 // ---- many rows: pairs of CTAs, 256 weight rows x up to 256 rows of x
 // The weights are the M side of the instruction: a CTA has 128 of them, of one block of 128 (one scale), and half the rows of x, 32 KB for 512 cycles of MMAs.  The N side,
-// rows of x, goes in steps of 32, so runs of rows (an expert's) need little padding.  Eight warps hold the tile's sums, 128 a thread; a thread has four weight rows and
-// pairs of neighbouring rows of x, whose scales it gets as four numbers per 16 bytes.
+// rows of x, goes in steps of 32, so runs of rows (an expert's) need little padding.  Eight warps hold the tile's sums, 128 a thread: one weight row and
+// half the rows of x, whose scales come four at a time from shared memory.
 constexpr int kFStages = 6, kFRows = 128, kFBox = 16, kFABytes = kFRows * 128, kFStage = 2 * kFABytes;
 constexpr int kFMost = kFp8Run;                       // rows of x per tile
-constexpr int kFScales = 4;                        // blocks whose scales are at hand
+constexpr int kFScales = 4;                        // blocks whose scales are at hand: those with gate's, and from kFUp on with up's (other banks)
+constexpr int kFUp = kFMost + 8, kFSlot = 2 * kFMost + 16;
 constexpr int kFThreads = 384, kFWarps = 8;
-constexpr int kFStageOut = 2560;                   // a warp's results on their way out
-constexpr int kFOffOut = kFStages * kFStage, kFOffScale = kFOffOut + kFWarps * kFStageOut, kFOffMax = kFOffScale + kFScales * 2 * kFMost * 4,
-              kFOffBar = kFOffMax + 2 * kFMost * 4, kFSmem = kFOffBar + 256;
+constexpr int kFStageOut = 2304;                   // a warp's results on their way out
+constexpr int kFOffOut = kFStages * kFStage, kFOffScale = kFOffOut + kFWarps * kFStageOut, kFOffMax = kFOffScale + kFScales * kFSlot * 4,
+              kFOffInv = kFOffMax + 2 * kFMost * 4, kFOffBar = kFOffInv + kFMost * 4, kFSmem = kFOffBar + 256;
 static_assert(kFSmem >= 512 * 430 - 1024 && kFSmem <= 227 * 1024, "what a CTA of a cluster takes for 512 columns (tmem_smem)");
 
 struct PairArgs {
@@ -57,9 +58,6 @@ struct PairArgs {
   float* out_scales;
   long long ld_out_scales;
 };
-
-// Where column c of a tile finds its scale: the numbers that a thread wants of 16 columns lie side by side.
-__device__ __forceinline__ int scale_place(int c) { return (c & ~15) | (c >> 1 & 3) << 2 | (c >> 3 & 1) << 1 | (c & 1); }
 
 template <bool kGlu, bool kOutF32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
@@ -110,44 +108,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
   const int units = p.chunks ? p.n_chunks[0] : (p.M + a.row_tile - 1) / a.row_tile, total = units * a.w_tiles;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
   struct Item {
-    int row0, rows, group, wt, nt;
+    int row0, rows, group, wt;
+    __device__ int nt() const { return __shfl_sync(0xffffffffu, (rows + 31) & ~31, 0); }
   };
-  // weight tiles first, so that pairs that run at once share the rows of x
+  // weight tiles first, so that pairs that run at once share the rows of x.  Everyone asks for the next item when it starts on one.
   const auto item = [&](int t) {
     Item i;
     const int u = t / a.w_tiles;
     i.wt = t - u * a.w_tiles;
     if (p.chunks) {
-      const ChunkDesc c = p.chunks[u];
-      i.row0 = c.slot_begin;
-      i.rows = c.n_tok;
-      i.group = c.expert;
+      const int4 c = t < total ? *reinterpret_cast<const int4*>(p.chunks + u) : make_int4(0, 0, 0, 0);
+      i.row0 = c.y;
+      i.rows = c.z;
+      i.group = c.x;
     } else {
       i.row0 = u * a.row_tile;
       i.rows = min(a.row_tile, p.M - i.row0);
       i.group = 0;
     }
-    i.nt = __shfl_sync(0xffffffffu, (i.rows + 31) & ~31, 0);
     return i;
   };
 
   if (warp >= 4) {
     more_registers<216>();
-    const int q = warp & 3, h = (warp - 4) >> 2, l = lane & 3, r = lane >> 2;
+    const int q = warp & 3, h = (warp - 4) >> 2;
     const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16);
     uint8_t* out_at = smem + kFOffOut + (warp - 4) * kFStageOut;
+    const int up = kGlu && lane >= 16 ? kFUp : 0;
     int b = 0;
     uint32_t aphase = 0, slot = 0, sphase = 0, tile = 0;
+    Item next = item(first);
     for (int t = first; t < total; t += step, ++tile) {
-      const Item i = item(t);
-      const int c0 = h * (i.nt / 2), cols = i.nt / 2, steps = (cols + 31) / 32;
-      uint64_t acc[4][2][4][2];                    // [32 columns][rows 16 apart][8 columns][rows 8 apart]
+      const Item i = next;
+      next = item(t + step);
+      const int nt = i.nt(), c0 = h * (nt / 2), cols = nt / 2, steps = (cols + 31) / 32;
+      uint64_t acc[4][16];                         // of this thread's weight row: 32 columns, two in each
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[s][j >> 3][j >> 1 & 3][j & 1] = 0;
+        for (int j = 0; j < 16; ++j) acc[s][j] = 0;
       for (int kb = 0; kb < nb; ++kb) {
-        const float* sc = reinterpret_cast<const float*>(smem + kFOffScale) + slot * 2 * kFMost + c0 + 4 * l;
+        const float* sc = reinterpret_cast<const float*>(smem + kFOffScale) + slot * kFSlot + up + c0;
         mbar_wait(&s_full[slot], sphase);
         mbar_wait(&acc_full[b], aphase);
         tc_fence_after_sync();
@@ -155,42 +156,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           if (s >= steps) break;
-          uint32_t v[2][16];
-          tmem_ld_rows16(from + s * 32, v[0]);
-          tmem_ld_rows16(from + s * 32 + (16u << 16), v[1]);
-          uint4 g[2], u[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            g[j] = *reinterpret_cast<const uint4*>(sc + s * 32 + j * 16);
-            if (kGlu) u[j] = *reinterpret_cast<const uint4*>(sc + kFMost + s * 32 + j * 16);
-          }
+          uint32_t v[32];
+          tmem_ld32(from + s * 32, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint64_t sg = j & 1 ? pack2(g[j / 2].z, g[j / 2].w) : pack2(g[j / 2].x, g[j / 2].y);
-            const uint64_t su = !kGlu ? sg : j & 1 ? pack2(u[j / 2].z, u[j / 2].w) : pack2(u[j / 2].x, u[j / 2].y);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              acc[s][e][j][0] = fma2(pack2(v[e][4 * j], v[e][4 * j + 1]), sg, acc[s][e][j][0]);
-              acc[s][e][j][1] = fma2(pack2(v[e][4 * j + 2], v[e][4 * j + 3]), su, acc[s][e][j][1]);
-            }
+          for (int j = 0; j < 8; ++j) {
+            const uint4 g = *reinterpret_cast<const uint4*>(sc + s * 32 + j * 4);
+            acc[s][2 * j] = fma2(pack2(v[4 * j], v[4 * j + 1]), pack2(g.x, g.y), acc[s][2 * j]);
+            acc[s][2 * j + 1] = fma2(pack2(v[4 * j + 2], v[4 * j + 3]), pack2(g.z, g.w), acc[s][2 * j + 1]);
           }
         }
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive_cluster(cluster_addr(&acc_empty[b], 0));
+          mbar_arrive_cluster_relaxed(cluster_addr(&acc_empty[b], 0));
           mbar_arrive(&s_empty[slot]);
         }
         if (++slot == kFScales) { slot = 0; sphase ^= 1; }
         b ^= 1;
         aphase ^= b == 0;
       }
-      // thread (r, l) has of columns c0 + 32 s + 8 j + 2 l and the one behind it the weight rows 32 q + 16 e + 8 k + r
       if constexpr (kGlu) {
-        // rows 16 e + r of the 32 are gate, 16 e + 8 + r up of the unit 64 rank + 16 q + 8 e + r of the tile
+        // a warp's rows are 16 of gate and the same 16 of up: lane f takes the even columns of unit f, lane 16 + f the odd ones
         uint32_t* most = reinterpret_cast<uint32_t*>(smem + kFOffMax) + (tile & 1) * kFMost;
         uint32_t* other = reinterpret_cast<uint32_t*>(smem + kFOffMax) + (~tile & 1) * kFMost;
+        float* inv = reinterpret_cast<float*>(smem + kFOffInv);
+        const bool odd = lane >= 16;
         named_bar_sync(1, 32 * kFWarps);           // everyone has read the last tile's maxima
         if (warp == 4)
           for (int c = lane; c < kFMost; c += 32) other[c] = 0;
@@ -198,35 +189,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           if (s >= steps) break;
+          uint32_t m[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t m0 = 0, m1 = 0;
+          for (int j = 0; j < 16; ++j) {
+            float even, odd_;
+            unpack2(acc[s][j], even, odd_);
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? even : odd_, 16);
+            const float v = kb2act::silu(odd ? got : even) * (odd ? odd_ : got);
+            acc[s][j] = __float_as_uint(v);
+            m[j] = __float_as_uint(v) & 0x7FFFFFFFu;
+          }
+          // over the 16 units: halves of the columns change sides until a lane has one of them
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float g0, g1, u0, u1;
-              unpack2(acc[s][e][j][0], g0, g1);
-              unpack2(acc[s][e][j][1], u0, u1);
-              const float v0 = kb2act::silu(g0) * u0, v1 = kb2act::silu(g1) * u1;
-              acc[s][e][j][0] = pack2(__float_as_uint(v0), __float_as_uint(v1));
-              m0 = max(m0, __float_as_uint(v0) & 0x7FFFFFFFu);
-              m1 = max(m1, __float_as_uint(v1) & 0x7FFFFFFFu);
-            }
+          for (int o = 8; o; o >>= 1)
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-              m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-              m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+            for (int j = 0; j < o; ++j) {
+              const bool high = lane & o;
+              m[j] = max(high ? m[j + o] : m[j], __shfl_xor_sync(0xffffffffu, high ? m[j] : m[j + o], o));
             }
-            const int c = s * 32 + j * 8 + 2 * l;
-            if (r < 2 && c < cols) {               // lanes of r 0 tell their own CTA, those of r 1 the other
-              const uint32_t to = (r ? peer : smem_u32(most)) + (c0 + c) * 4;
-              if (r) {
-                max_cluster(to, m0);
-                max_cluster(to + 4, m1);
-              } else {
-                atomicMax(&most[c0 + c], m0);
-                atomicMax(&most[c0 + c + 1], m1);
-              }
-            }
+          const int c = s * 32 + (lane & 15) * 2 + odd;
+          if (c < cols) {
+            atomicMax(&most[c0 + c], m[0]);
+            max_cluster(peer + (c0 + c) * 4, m[0]);
           }
         }
         __syncwarp();
@@ -235,111 +219,96 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
           mbar_arrive_cluster(cluster_addr(&max_full[tile & 1], rank ^ 1));
         }
         mbar_wait_cluster(&max_full[tile & 1], tile >> 1 & 1);
-        uint8_t* codes = reinterpret_cast<uint8_t*>(p.out);
-        const int f0 = i.wt * 128 + rank * 64 + q * 16;
+        {                                          // a column a thread; even columns of 32 lie ahead of odd ones, as the lanes want them
+          const int c = threadIdx.x - 128;
+          const Fp8Scale f = fp8_scale(most[c]);
+          const int half = c >= nt / 2 ? nt / 2 : 0, in = c - half;
+          if (c < nt) inv[(half ? kFMost / 2 : 0) + (in & ~31) + (in & 1) * 16 + (in >> 1 & 15)] = f.inv;
+          if (rank == 0 && c < i.rows) a.out_scales[i.wt * a.ld_out_scales + i.row0 + c] = f.scale;
+        }
+        named_bar_sync(1, 32 * kFWarps);
+        uint8_t* codes = reinterpret_cast<uint8_t*>(p.out) + (long long)i.row0 * F + i.wt * 128 + rank * 64 + q * 16 + (lane & 12);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           if (s >= steps) break;
-          uint32_t w[2][2];                        // [8 columns of gate and up][16 columns]: this thread's codes of them, a pair of columns in 16 bits
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int c = c0 + s * 32 + j * 8 + 2 * l;
-            const Fp8Scale s0 = fp8_scale(most[min(c, kFMost - 2)]), s1 = fp8_scale(most[min(c, kFMost - 2) + 1]);
-            if (q == 0 && rank == 0 && r == 0 && c - c0 < cols) {
-              if (c < i.rows) a.out_scales[i.wt * a.ld_out_scales + i.row0 + c] = s0.scale;
-              if (c + 1 < i.rows) a.out_scales[i.wt * a.ld_out_scales + i.row0 + c + 1] = s1.scale;
-            }
+          for (int k = 0; k < 4; ++k) {
+            const float4 n = *reinterpret_cast<const float4*>(inv + h * (kFMost / 2) + s * 32 + odd * 16 + k * 4);
+            const float f[4] = {n.x, n.y, n.z, n.w};
+            float v[4];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float v0, v1;
-              unpack2(acc[s][e][j][0], v0, v1);
-              v0 = s0.inv == 0.f ? 0.f : v0 * s0.inv;
-              v1 = s1.inv == 0.f ? 0.f : v1 * s1.inv;
-              const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v0, v1), __NV_SATFINITE, __NV_E4M3);
-              w[e][j >> 1] = j & 1 ? w[e][j >> 1] | two << 16 : two;
-            }
-          }
-          // matrix (e, j / 2): its column 2 l' + i is the pair l' of the eight columns 2 (j / 2) + i
-          __syncwarp();
-          stmatrix4_t(smem_u32(out_at) + (lane & 7) * 80 + (lane >> 3) * 16, w[0][0], w[0][1], w[1][0], w[1][1]);
-          __syncwarp();
-          // a thread takes row `lane & 7` of matrix lane >> 3: eight units of two columns
-          const uint4 x = *reinterpret_cast<const uint4*>(out_at + (lane & 7) * 80 + (lane >> 3) * 16);
-          const int c = s * 32 + (lane >> 3 & 1) * 16 + (lane & 1) * 8 + (lane >> 1 & 3) * 2;
-          const int m = c0 + c;
-          if (c < cols) {
-            uint8_t* to = codes + (long long)(i.row0 + m) * F + f0 + (lane >> 4) * 8;
-            if (m < i.rows) *reinterpret_cast<uint2*>(to) = make_uint2(__byte_perm(x.x, x.y, 0x6420), __byte_perm(x.z, x.w, 0x6420));
-            if (m + 1 < i.rows) *reinterpret_cast<uint2*>(to + F) = make_uint2(__byte_perm(x.x, x.y, 0x7531), __byte_perm(x.z, x.w, 0x7531));
+            for (int j = 0; j < 4; ++j) v[j] = f[j] == 0.f ? 0.f : __uint_as_float((uint32_t)acc[s][4 * k + j]) * f[j];
+            // codes of four columns of this lane's unit -> those of four units of one column
+            uint32_t w = fp8_codes4(v[0], v[1], v[2], v[3], 1.f);
+            const uint32_t x = __shfl_xor_sync(0xffffffffu, w, 2);
+            w = lane & 2 ? __byte_perm(x, w, 0x7632) : __byte_perm(w, x, 0x5410);
+            const uint32_t y = __shfl_xor_sync(0xffffffffu, w, 1);
+            w = lane & 1 ? __byte_perm(y, w, 0x7351) : __byte_perm(w, y, 0x6240);
+            const int m = c0 + s * 32 + (k * 4 + (lane & 2) + (lane & 1)) * 2 + odd;
+            if (m < min(i.rows, c0 + cols)) *reinterpret_cast<uint32_t*>(codes + (long long)m * F) = w;
           }
         }
       } else {
         const int n0 = i.wt * 256 + rank * 128 + q * 32;
-        float bias[2][2] = {};
-        if (p.bias != nullptr)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) bias[k >> 1][k & 1] = n0 + k * 8 + r < p.N ? p.bias[n0 + k * 8 + r] : 0.f;
+        const float bias = p.bias != nullptr && n0 + lane < p.N ? p.bias[n0 + lane] : 0.f;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           if (s >= steps) break;
           const int m0 = c0 + s * 32, have = min(i.rows, c0 + cols) - m0;
-          if constexpr (kOutF32) {
-            float* st = reinterpret_cast<float*>(out_at);                  // [16 columns][36]
+          uint32_t* st = reinterpret_cast<uint32_t*>(out_at);
+          if constexpr (kOutF32) {                 // [16 columns][36]
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if ((j & 1) == 0) __syncwarp();
+            for (int half = 0; half < 2; ++half) {
+              __syncwarp();
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
+              for (int j = 0; j < 8; ++j) {
                 float v0, v1;
-                unpack2(acc[s][e >> 1][j][e & 1], v0, v1);
-                float* to = st + ((j & 1) * 8 + 2 * l) * 36 + e * 8 + r;
-                to[0] = v0 + bias[e >> 1][e & 1];
-                to[36] = v1 + bias[e >> 1][e & 1];
+                unpack2(acc[s][half * 8 + j], v0, v1);
+                st[(2 * j) * 36 + lane] = __float_as_uint(v0 + bias);
+                st[(2 * j + 1) * 36 + lane] = __float_as_uint(v1 + bias);
               }
-              if (j & 1) {
-                __syncwarp();
+              __syncwarp();
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const int c = k * 4 + (lane >> 3), m = (j >> 1) * 16 + c, n = n0 + (lane & 7) * 4;
-                  if (m >= have || n >= p.N) continue;
-                  const float4 x = *reinterpret_cast<const float4*>(st + c * 36 + (lane & 7) * 4);
-                  float* to = reinterpret_cast<float*>(p.out) + (long long)(i.row0 + m0 + m) * p.N + n;
-                  if ((p.N & 3) == 0) *reinterpret_cast<float4*>(to) = x;
-                  else {
-                    to[0] = x.x;
-                    if (n + 1 < p.N) to[1] = x.y;
-                    if (n + 2 < p.N) to[2] = x.z;
-                    if (n + 3 < p.N) to[3] = x.w;
-                  }
+              for (int k = 0; k < 4; ++k) {
+                const int c = k * 4 + (lane >> 3), m = half * 16 + c, n = n0 + (lane & 7) * 4;
+                if (m >= have || n >= p.N) continue;
+                const float4 x = *reinterpret_cast<const float4*>(st + c * 36 + (lane & 7) * 4);
+                float* to = reinterpret_cast<float*>(p.out) + (long long)(i.row0 + m0 + m) * p.N + n;
+                if ((p.N & 3) == 0) *reinterpret_cast<float4*>(to) = x;
+                else {
+                  to[0] = x.x;
+                  if (n + 1 < p.N) to[1] = x.y;
+                  if (n + 2 < p.N) to[2] = x.z;
+                  if (n + 3 < p.N) to[3] = x.w;
                 }
               }
             }
-          } else {
+          } else {                                 // [16 pairs of columns][36]
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float v0, v1;
-                unpack2(acc[s][e >> 1][j][e & 1], v0, v1);
-                w[e] = bf16x2_bits_rn(v1 + bias[e >> 1][e & 1], v0 + bias[e >> 1][e & 1]);
-              }
-              stmatrix4_t(smem_u32(out_at) + (j * 8 + (lane & 7)) * 80 + (lane >> 3) * 16, w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < 16; ++j) {
+              float v0, v1;
+              unpack2(acc[s][j], v0, v1);
+              st[j * 36 + lane] = bf16x2_bits_rn(v1 + bias, v0 + bias);
             }
             __syncwarp();
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int m = k * 8 + (lane >> 2), n = n0 + l * 8;
-              if (m >= have || n >= p.N) continue;
-              const uint4 x = *reinterpret_cast<const uint4*>(out_at + m * 80 + l * 16);
-              __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(p.out) + (long long)(i.row0 + m0 + m) * p.N + n;
-              if ((p.N & 7) == 0) *reinterpret_cast<uint4*>(to) = x;
-              else {
-                const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+              const int c = k * 4 + (lane >> 3), n = n0 + (lane & 7) * 4;
+              const uint4 x = *reinterpret_cast<const uint4*>(st + c * 36 + (lane & 7) * 4);
+              if (n >= p.N) continue;
+              __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(p.out) + (long long)(i.row0 + m0 + 2 * c) * p.N + n;
 #pragma unroll
-                for (int y = 0; y < 8; ++y)
-                  if (n + y < p.N) to[y] = __ushort_as_bfloat16((unsigned short)(u[y >> 1] >> (y & 1) * 16));
+              for (int o = 0; o < 2; ++o, to += p.N) {
+                if (2 * c + o >= have) continue;
+                const uint32_t lo = __byte_perm(x.x, x.y, o ? 0x7632 : 0x5410), hi = __byte_perm(x.z, x.w, o ? 0x7632 : 0x5410);
+                if ((p.N & 3) == 0) *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+                else {
+                  to[0] = __ushort_as_bfloat16((unsigned short)lo);
+                  if (n + 1 < p.N) to[1] = __ushort_as_bfloat16((unsigned short)(lo >> 16));
+                  if (n + 2 < p.N) to[2] = __ushort_as_bfloat16((unsigned short)hi);
+                  if (n + 3 < p.N) to[3] = __ushort_as_bfloat16((unsigned short)(hi >> 16));
+                }
               }
             }
           }
@@ -349,19 +318,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
   } else if (fewer_registers<64>(), warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
+    Item next = item(first);
     for (int t = first; t < total; t += step) {
-      const Item i = item(t);
-      const uint32_t bytes = 2 * kFABytes + i.nt * 128;
-      const int x0 = i.row0 + rank * (i.nt / 2);
+      const Item i = next;
+      next = item(t + step);
+      const int nt = i.nt(), x0 = i.row0 + rank * (nt / 2);
+      const uint32_t bytes = 2 * kFABytes + nt * 128;
       for (int kb = 0; kb < nb; ++kb) {
         mbar_wait(&empty[stage], phase ^ 1);
         uint8_t* at = smem + stage * kFStage;
         if (elect_one()) {
           const uint32_t bar = cluster_addr(&full[stage], 0);
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
-          if constexpr (kGlu) tma_load_5d_pair(at, &tmap_w, kb * 128, 0, 0, (i.wt * 128 + (int)rank * 64) / 8, i.group, bar);
+          if constexpr (kGlu) tma_load_5d_pair(at, &tmap_w, kb * 128, 0, 0, (i.wt * 128 + (int)rank * 64) / 16, i.group, bar);
           else tma_load_2d_pair(at, &tmap_w, kb * 128, i.group * p.N + i.wt * 256 + rank * 128, bar);
-          for (int r = 0; r < i.nt / 2; r += kFBox) tma_load_2d_pair(at + kFABytes + r * 128, &tmap_x, kb * 128, x0 + r, bar);
+          for (int r = 0; r < nt / 2; r += kFBox) tma_load_2d_pair(at + kFABytes + r * 128, &tmap_x, kb * 128, x0 + r, bar);
         }
         __syncwarp();
         if (++stage == kFStages) { stage = 0; phase ^= 1; }
@@ -375,8 +346,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
     if (rank == 0) {
       int stage = 0, b = 0;
       uint32_t phase = 0, aphase = 0;
+      Item next = item(first);
       for (int t = first; t < total; t += step) {
-        const uint32_t idesc = umma_idesc_e4m3(256, item(t).nt);
+        const uint32_t idesc = umma_idesc_e4m3(256, next.nt());
+        next = item(t + step);
         for (int kb = 0; kb < nb; ++kb) {
           mbar_wait(&acc_empty[b], aphase ^ 1);
           mbar_wait(&full[stage], phase);
@@ -397,33 +370,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
       }
     }
   } else if (warp < 4) {
-    // the scales of a block: those of the rows of x times the weights', by two warps in turn
-    int turn = 0;
-    uint32_t slot = 0, phase = 0;
-    for (int t = first; t < total; t += step) {
-      const Item i = item(t);
+    // the scales of a block: those of the rows of x times the weights', by two warps in turn.  A block's are asked for while the one before it goes out: their way from L2
+    // takes longer than a block's products.
+    struct Scales {
+      float g, u, v[kFMost / 32];
+    };
+    const auto ask = [&](const Item& i, int kb) {
       const int blocks = fp8_blocks(p.N), n0 = kGlu ? i.wt : min(i.wt * 2 + (int)rank, blocks - 1);
-      const float* ws = p.ws + ((long long)i.group * blocks + n0) * nb;
-      for (int kb = 0; kb < nb; ++kb, turn ^= 1) {
-        if (turn == warp - 2) {
-          float v[kFMost / 32];
-          const float g = ws[kb], u = kGlu ? ws[(long long)(F / kFp8Block) * nb + kb] : 0.f;
-          const float* xs = p.xs + kb * p.ldxs + i.row0;
+      const float *ws = p.ws + ((long long)i.group * blocks + n0) * nb + kb, *xs = p.xs + kb * p.ldxs + i.row0;
+      Scales r;
+      r.g = ws[0];
+      r.u = kGlu ? ws[(long long)(F / kFp8Block) * nb] : 0.f;
 #pragma unroll
-          for (int j = 0; j < kFMost / 32; ++j) v[j] = j * 32 + lane < i.rows ? xs[j * 32 + lane] : 0.f;
-          mbar_wait(&s_empty[slot], phase ^ 1);
-          float* to = reinterpret_cast<float*>(smem + kFOffScale) + slot * 2 * kFMost;
+      for (int j = 0; j < kFMost / 32; ++j) r.v[j] = j * 32 + lane < i.rows ? xs[j * 32 + lane] : 0.f;
+      return r;
+    };
+    int t = first, kb = warp - 2;
+    while (kb >= nb) { kb -= nb; t += step; }
+    uint32_t slot = warp - 2, phase = 0;
+    Item i = item(t);
+    Scales now{};
+    if (t < total) now = ask(i, kb);
+    while (t < total) {
+      const int rows = i.rows, before = t;
+      for (kb += 2; kb >= nb; kb -= nb) t += step;
+      if (t != before) i = item(t);
+      Scales next{};
+      if (t < total) next = ask(i, kb);
+      mbar_wait(&s_empty[slot], phase ^ 1);
+      float* to = reinterpret_cast<float*>(smem + kFOffScale) + slot * kFSlot;
 #pragma unroll
-          for (int j = 0; j < kFMost / 32; ++j)
-            if (j * 32 < i.nt) {
-              to[scale_place(j * 32 + lane)] = v[j] * g;
-              if (kGlu) to[kFMost + scale_place(j * 32 + lane)] = v[j] * u;
-            }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_full[slot]);
+      for (int j = 0; j < kFMost / 32; ++j)
+        if (j * 32 < rows) {
+          to[j * 32 + lane] = now.v[j] * now.g;
+          if (kGlu) to[kFUp + j * 32 + lane] = now.v[j] * now.u;
         }
-        if (++slot == kFScales) { slot = 0; phase ^= 1; }
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_full[slot]);
+      slot += 2;
+      if (slot >= kFScales) { slot -= kFScales; phase ^= 1; }
+      now = next;
     }
   }
   __syncwarp();
