@@ -30,11 +30,12 @@ cudaError_t make_tmap_u8_gate_up(void* out_tmap, const void* base, long long gro
 // A CTA has 128 rows of x (the M side) and half the weight rows, 32 KB for 512 cycles of MMAs per block of K.  Sixteen warps hold the tile's sums, 64 a thread: a thread has one
 // row of x, so one scale of it per block, and 64 columns of one block of weights, so one of those.  With the weights on the M side a column's scale came from shared memory, 256
 // broadcast loads per block beside the MMAs' own reads, and a block took 1070 cycles of eight warps (M 8192, N 4096, K 4096: 150 us).
-constexpr int kFStages = 5, kFRows = 128, kFBox = 32, kFABytes = kFRows * 128, kFStage = 2 * kFABytes;
+constexpr int kFStages = 4, kFRows = 128, kFBox = 32, kFABytes = kFRows * 128, kFStage = 2 * kFABytes;
 constexpr int kFThreads = 640, kFWarps = 16;
-constexpr int kFScales = 8;                        // blocks whose scales are at hand: products for each row, for the first and the second 128 columns (gated: gate's, up's)
-constexpr int kFPitch = 80;                        // a row's 64 bytes on their way out
-constexpr int kFOffOut = kFStages * kFStage, kFOffScale = kFOffOut + kFWarps * 32 * kFPitch, kFOffMax = kFOffScale + kFScales * 2 * kFRows * 4,
+// The scales of kFGroup blocks are handed over at once, two groups are at hand: products for each row, for the first and the second 128 columns (gated: gate's, up's).
+constexpr int kFGroup = 4, kFScales = 2 * kFGroup;
+constexpr int kFOut = 32 * 128;                    // a warp's results on their way out
+constexpr int kFOffOut = kFStages * kFStage, kFOffScale = kFOffOut + kFWarps * kFOut, kFOffMax = kFOffScale + kFScales * 2 * kFRows * 4,
               kFOffBar = kFOffMax + 2 * 4 * kFRows * 4, kFUsed = kFOffBar + 512, kFSmem = kFUsed > 512 * 430 - 1024 ? kFUsed : 512 * 430 - 1024;
 static_assert(kFSmem <= 227 * 1024, "what a CTA of a cluster takes for 512 columns (tmem_smem)");
 static_assert(kFp8Run == 2 * kFRows, "a run is one tile's rows");
@@ -49,15 +50,15 @@ struct PairArgs {
 
 template <bool kGlu, bool kOutF32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
-    fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const PairArgs a) {
+    fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_out, const PairArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFOffBar);       // of the first CTA: both CTAs' loads
   uint64_t* empty = full + kFStages;
   uint64_t* acc_full = empty + kFStages;           // [2]
   uint64_t* acc_empty = acc_full + 2;              // [2], of the first CTA: both CTAs' read-outs
-  uint64_t* s_full = acc_empty + 2;                // [kFScales]
-  uint64_t* s_empty = s_full + kFScales;
-  uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(s_empty + kFScales);
+  uint64_t* s_full = acc_empty + 2;                // [2]
+  uint64_t* s_empty = s_full + 2;
+  uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(s_empty + 2);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const Fp8Product& p = a.p;
@@ -70,9 +71,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 2 * kFWarps);
-    }
-    for (int i = 0; i < kFScales; ++i) {
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[i], 2);
       mbar_init(&s_empty[i], kFWarps);
     }
     fence_mbar_init();
@@ -80,6 +79,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
   if (threadIdx.x == 64) {
     prefetch_tmap(&tmap_x);
     prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_out);
   }
   if (warp == 0) tmem_alloc_pair(tmem_ptr_smem, 512);
   tc_fence_before_sync();
@@ -126,12 +126,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
 #pragma unroll
       for (int j = 0; j < 32; ++j) acc[j] = 0;
       for (int kb = 0; kb < nb; ++kb) {
-        mbar_wait(&s_full[slot], sphase);
+        if ((slot & (kFGroup - 1)) == 0) mbar_wait(&s_full[slot / kFGroup], sphase);
         const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + kFOffScale) + slot * 2 * kFRows + q * 32 + lane;
         const uint32_t s0 = sc[kGlu ? 0 : (h >> 1) * kFRows], s1 = kGlu ? sc[kFRows] : s0;
         const uint64_t two0 = pack2(s0, s0), two1 = pack2(s1, s1);
         mbar_wait(&acc_full[b], aphase);
         tc_fence_after_sync();
+        const auto read = [&]() {                  // this block's sums are in registers
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(&acc_empty[b], 0));
+        };
         if (mine) {
           // 16 columns are on their way while those before them are added
           uint32_t v[2][16];
@@ -140,17 +145,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
           for (int c = 0; c < 4; ++c) {
             tmem_ld_wait();
             if (c < 3) tmem_ld16(from + b * 256 + (c + 1) * 16, v[(c + 1) & 1]);
+            else read();
 #pragma unroll
             for (int j = 0; j < 8; ++j) fma2_here(acc[c * 8 + j], pack2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), c >> 1 ? two1 : two0);
           }
+        } else {
+          read();
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive_cluster_relaxed(cluster_addr(&acc_empty[b], 0));
-          mbar_arrive(&s_empty[slot]);
+        ++slot;
+        if ((slot & (kFGroup - 1)) == 0) {
+          if (lane == 0) mbar_arrive(&s_empty[slot / kFGroup - 1]);
+          if (slot == kFScales) { slot = 0; sphase ^= 1; }
         }
-        if (++slot == kFScales) { slot = 0; sphase ^= 1; }
         b ^= 1;
         aphase ^= b == 0;
       }
@@ -188,15 +194,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
           to[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
       } else if (mine) {
-        // 64 bytes of a row at a time through shared memory: four lanes have a row's (16 bytes of a row by each lane, row by row, took 12000 cycles a tile)
-        constexpr int kCols = kOutF32 ? 16 : 32, kVec = kOutF32 ? 4 : 8;
-        uint8_t* st = smem + kFOffOut + (warp - 4) * 32 * kFPitch;
-        const int have = i.rows - (int)(rank * kFRows + q * 32);
-        const bool whole = p.N % kVec == 0;
+        // 32 rows x 128 bytes at a time go out from shared memory by one copy, while the next tile's blocks are added: all SMs end their tiles at the same time, and a tile's
+        // stores by the lanes took 3500 cycles (16 bytes of a row by each lane, row by row, 12000).  A run's last rows, and rows that are not on 16 bytes, are the lanes'.
+        constexpr int kCols = kOutF32 ? 32 : 64, kVec = kOutF32 ? 4 : 8;
+        uint8_t* st = smem + kFOffOut + (warp - 4) * kFOut;
+        const int row0 = i.row0 + rank * kFRows + q * 32, have = i.rows - (int)(rank * kFRows + q * 32);
+        const bool on16 = p.N % kVec == 0;
 #pragma unroll
         for (int c = 0; c < 64 / kCols; ++c) {
           const int n0 = i.wt * 256 + h * 64 + c * kCols;
           if (n0 >= p.N) break;
+          if (lane == 0) bulk_wait_group_read0();
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < kCols; j += kVec) {
@@ -209,17 +217,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
             uint4 x;
             if constexpr (kOutF32) x = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
             else x = make_uint4(bf16x2_bits_rn(v[1], v[0]), bf16x2_bits_rn(v[3], v[2]), bf16x2_bits_rn(v[5], v[4]), bf16x2_bits_rn(v[7], v[6]));
-            *reinterpret_cast<uint4*>(st + lane * kFPitch + j / kVec * 16) = x;
+            *reinterpret_cast<uint4*>(st + lane * 128 + (j / kVec ^ (lane & 7)) * 16) = x;       // the order that the copy reads them in
+          }
+          if (on16 && have >= 32) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmap_out, n0 * (kOutF32 ? 4 : 2), row0, st);
+              bulk_commit_group();
+            }
+            continue;
           }
           __syncwarp();
-          const int n = n0 + (lane & 3) * kVec;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = k * 8 + (lane >> 2);
-            if (r >= have || n >= p.N) continue;
-            const uint4 x = *reinterpret_cast<const uint4*>(st + r * kFPitch + (lane & 3) * 16);
-            const long long to = (long long)(i.row0 + rank * kFRows + q * 32 + r) * p.N + n;
-            if (whole) {
+          const int n = n0 + (lane & 7) * kVec;
+          for (int r = lane >> 3; r < min(have, 32); r += 4) {
+            if (n >= p.N) continue;
+            const uint4 x = *reinterpret_cast<const uint4*>(st + r * 128 + ((lane & 7) ^ (r & 7)) * 16);
+            const long long to = (long long)(row0 + r) * p.N + n;
+            if (on16) {
               *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + to * (16 / kVec)) = x;
             } else {
               const uint32_t u[4] = {x.x, x.y, x.z, x.w};
@@ -234,6 +249,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
         }
       }
     }
+    if (!kGlu && lane == 0) bulk_wait_group0();
   } else if (fewer_registers<56>(), warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
@@ -319,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
     };
     uint32_t slot = warp - 2, phase = 0;
     const auto put = [&](const Scales& s) {
-      mbar_wait(&s_empty[slot], phase ^ 1);
+      if ((slot & (kFGroup - 1)) < 2) mbar_wait(&s_empty[slot / kFGroup], phase ^ 1);
       float* to = reinterpret_cast<float*>(smem + kFOffScale) + slot * 2 * kFRows + lane;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -327,11 +343,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
         to[kFRows + j * 32] = s.x[j] * s.w[1];
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_full[slot]);
+      if ((slot & (kFGroup - 1)) >= kFGroup - 2 && lane == 0) mbar_arrive(&s_full[slot / kFGroup]);
       slot += 2;
       if (slot >= kFScales) { slot -= kFScales; phase ^= 1; }
     };
-    const int mine = total > first ? ((total - first + step - 1) / step * nb - (warp - 2) + 1) / 2 : 0;
+    const int all = total > first ? (total - first + step - 1) / step * nb : 0, mine = (all - (warp - 2) + 1) / 2;
     Scales s0{}, s1{};
     if (mine > 0) ask(s0);
     if (mine > 1) ask(s1);
@@ -340,6 +356,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
       if (n + 2 < mine) ask(s0);
       if (n + 1 < mine) put(s1);
       if (n + 3 < mine) ask(s1);
+    }
+    if (all % kFGroup > 0 && all % kFGroup < kFGroup - 3 + warp) {         // the last group is short: of either warp's two blocks, one or both are missing
+      if (all % kFGroup == 1 && warp == 3) mbar_wait(&s_empty[slot / kFGroup], phase ^ 1);
+      if (lane == 0) mbar_arrive(&s_full[slot / kFGroup]);
     }
   }
   __syncwarp();
@@ -353,14 +373,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
 template <bool kGlu, bool kOutF32>
 static cudaError_t launch_pair(const PairArgs& a, int num_sms, cudaStream_t s) {
   const Fp8Product& p = a.p;
-  alignas(64) CUtensorMap tx, tw;
+  alignas(64) CUtensorMap tx, tw, to;
   cudaError_t e = make_tmap_u8_rows(&tx, p.x, p.M, p.K, kFBox);
   if (e == cudaSuccess) e = kGlu ? make_tmap_u8_gate_up(&tw, p.w, p.groups, p.N / 2, p.K) : make_tmap_u8_rows(&tw, p.w, (long long)p.groups * p.N, p.K, kFRows);
+  to = tw;
+  const int wide = kOutF32 ? 4 : 2;
+  if (e == cudaSuccess && !kGlu && p.N * (long long)wide % 16 == 0) e = make_tmap_u8_rows(&to, p.out, p.M, (long long)p.N * wide, 32);      // as bytes
   if (e == cudaSuccess) e = allow_smem<fp8_pair_kernel<kGlu, kOutF32>>(kFSmem);
   if (e != cudaSuccess) return e;
   const long long total = (long long)a.w_tiles * (p.chunks ? p.max_chunks : (p.M + kFp8Run - 1) / kFp8Run);
   const int pairs = (int)(total < num_sms / 2 ? total : num_sms / 2);
-  return launch_pdl(fp8_pair_kernel<kGlu, kOutF32>, 2 * pairs, kFThreads, kFSmem, s, tx, tw, a);
+  return launch_pdl(fp8_pair_kernel<kGlu, kOutF32>, 2 * pairs, kFThreads, kFSmem, s, tx, tw, to, a);
 }
 
 cudaError_t launch_fp8_product(const Fp8Product& p, int num_sms, cudaStream_t s) {
