@@ -4,41 +4,54 @@
 
 namespace kb2 {
 
-// Eight numbers, `have` of them there.
-template <bool F32, bool VEC>
-__device__ __forceinline__ void load8(const void* p, long long at, int have, float (&v)[8]) {
+// Eight neighbouring numbers as they are in memory.
+template <bool F32>
+struct Eight {
+  uint32_t u[F32 ? 8 : 4];
+  // `have` of them are there
+  template <bool VEC>
+  __device__ __forceinline__ void load(const void* p, long long at, int have) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  if (have <= 0) return;
-  if constexpr (VEC) {                             // all eight: their number is a multiple of 16
-    if constexpr (F32) {
-      const float4 a = __ldcs(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + at)), b = __ldcs(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + at) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    for (int i = 0; i < (F32 ? 8 : 4); ++i) u[i] = 0;
+    if (have <= 0) return;
+    if constexpr (VEC) {                           // all eight: their number is a multiple of 16
+      const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + at * (F32 ? 4 : 2));
+#pragma unroll
+      for (int i = 0; i < (F32 ? 2 : 1); ++i) {
+        const uint4 a = __ldcs(q + i);
+        u[4 * i] = a.x; u[4 * i + 1] = a.y; u[4 * i + 2] = a.z; u[4 * i + 3] = a.w;
+      }
     } else {
-      const uint4 a = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p) + at));
-      const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+      for (int i = 0; i < 8; ++i) {
+        if (i >= have) continue;
+        if constexpr (F32) u[i] = reinterpret_cast<const uint32_t*>(p)[at + i];
+        else u[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[at + i] << (i & 1) * 16;
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < have) v[i] = F32 ? reinterpret_cast<const float*>(p)[at + i] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[at + i]);
   }
-}
-__device__ __forceinline__ uint32_t largest8(const float (&v)[8]) {
-  uint32_t a = 0;
+  __device__ __forceinline__ float number(int i) const {
+    if constexpr (F32) return __uint_as_float(u[i]);
+    else return __uint_as_float(i & 1 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16);
+  }
+  // the bits of the largest magnitude: as whole numbers infinities and NaN are the largest
+  __device__ __forceinline__ uint32_t largest() const {
+    if constexpr (F32) {
+      uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);      // as whole numbers infinities and NaN are the largest
-  return a;
-}
-// K is a multiple of 16 and the codes lie on 16 bytes: eight of them are there whole or not at all.
-__device__ __forceinline__ void store8(void* codes, long long at, const float (&v)[8], float inv) {
-  *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(codes) + at) = make_uint2(fp8_codes4(v[0], v[1], v[2], v[3], inv), fp8_codes4(v[4], v[5], v[6], v[7], inv));
-}
+      for (int i = 0; i < 8; ++i) a = max(a, u[i] & 0x7FFFFFFFu);
+      return a;
+    } else {
+      const uint32_t a = __vmaxu2(__vmaxu2(u[0] & 0x7FFF7FFFu, u[1] & 0x7FFF7FFFu), __vmaxu2(u[2] & 0x7FFF7FFFu, u[3] & 0x7FFF7FFFu));
+      return max(a << 16, a & 0xFFFF0000u);
+    }
+  }
+  // K is a multiple of 16 and the codes lie on 16 bytes: eight of them are there whole or not at all.
+  __device__ __forceinline__ void store(void* codes, long long at, float inv) const {
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(codes) + at) =
+        make_uint2(fp8_codes4(number(0), number(1), number(2), number(3), inv), fp8_codes4(number(4), number(5), number(6), number(7), inv));
+  }
+};
 
 // Sixteen lanes have a block of 128, eight numbers each; a thread block has 16 rows x kRowsAhead blocks, all of a thread's loads on their way at once.
 constexpr int kRowsAhead = 4;
@@ -46,41 +59,41 @@ template <bool F32, bool VEC>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(const void* x, long long ldx, int M, int K, void* codes, float* scales, long long lds) {
   pdl_wait();
   const int lane = threadIdx.x & 15, m = blockIdx.x * 16 + (threadIdx.x >> 4), b0 = blockIdx.y * kRowsAhead;
-  float v[kRowsAhead][8];
+  Eight<F32> v[kRowsAhead];
 #pragma unroll
   for (int i = 0; i < kRowsAhead; ++i) {
     const int k = (b0 + i) * kFp8Block + lane * 8;
-    load8<F32, VEC>(x, m * ldx + k, m < M ? K - k : 0, v[i]);
+    v[i].template load<VEC>(x, m * ldx + k, m < M ? K - k : 0);
   }
 #pragma unroll
   for (int i = 0; i < kRowsAhead; ++i) {
     const int k = (b0 + i) * kFp8Block + lane * 8;
-    uint32_t a = largest8(v[i]);
+    uint32_t a = v[i].largest();
 #pragma unroll
     for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
     const Fp8Scale s = fp8_scale(a);
     if (m >= M || (b0 + i) * kFp8Block >= K) continue;
-    if (k < K) store8(codes, (long long)m * K + k, v[i], s.inv);
+    if (k < K) v[i].store(codes, (long long)m * K + k, s.inv);
     if (lane == 0) scales[(b0 + i) * lds + m] = s.scale;
   }
 }
 
-// A thread block has one block of 128 x 128: sixteen lanes a row, eight rows a thread.
+// A thread block has one block of 128 x 128: sixteen lanes a row, eight rows a thread, all on their way at once and kept as they are.
 template <bool F32, bool VEC>
 __global__ void __launch_bounds__(256) fp8_blocks_kernel(const void* w, int N, int K, void* codes, float* scales) {
   pdl_wait();
   __shared__ uint32_t s_max[8];
   const int lane = threadIdx.x & 15, row0 = blockIdx.y * kFp8Block + (threadIdx.x >> 4), k = blockIdx.x * kFp8Block + lane * 8;
   const long long base = (long long)blockIdx.z * N * K + k;
-  float v[8][8];
+  Eight<F32> v[8];
   uint32_t a = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int n = row0 + i * 16;
-    load8<F32, VEC>(w, base + (long long)n * K, n < N ? K - k : 0, v[i]);
+    v[i].template load<VEC>(w, base + (long long)n * K, n < N ? K - k : 0);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max(a, largest8(v[i]));
+  for (int i = 0; i < 8; ++i) a = max(a, v[i].largest());
   a = __reduce_max_sync(0xffffffffu, a);
   if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = a;
   __syncthreads();
@@ -92,7 +105,7 @@ __global__ void __launch_bounds__(256) fp8_blocks_kernel(const void* w, int N, i
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int n = row0 + i * 16;
-    if (n < N) store8(codes, base + (long long)n * K, v[i], s.inv);
+    if (n < N) v[i].store(codes, base + (long long)n * K, s.inv);
   }
 }
 
