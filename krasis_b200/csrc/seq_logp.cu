@@ -1,23 +1,26 @@
 // Log probabilities of given tokens, entropy and the largest alternatives of rows of logits, in one pass over them.
 //
-// With a running maximum m: s = sum exp(z - m), u = sum exp(z - m) (z - m); where m rises by d, s <- s exp(-d) and u <- (u - d s) exp(-d).  At the end lse = m + log s, logprob =
-// z[token] - lse, entropy = log s - u / s.
+// In powers of two: with L = log2 e and a reference c near L max z, t = L z - c by one fused multiply-add, s = sum 2^t, u = sum 2^t t.  Where c rises by d, s <- s 2^-d and u <- (u -
+// d s) 2^-d.  At the end log2 sum exp z = c + log2 s, so logprob = (t(token) - log2 s) / L and entropy = (log2 s - u / s) / L; an L that is rounded is a temperature of 1 + 2^-26.
 // Bound: the rows' way from memory.  A block of sixteen warps has a row; where there are fewer rows than SMs, a cluster of up to eight blocks shares it and its first block
-// joins what they found, read through distributed shared memory.  Of the largest numbers every warp keeps a list of its own: what passes the least of the numbers that can still be among
-// the `top` goes to the list's end, and when it is full a sort of it leaves `top` of them.
+// joins what they found, read through distributed shared memory.
+// The largest numbers: the block's first numbers give a bound that `top` of the row pass (the top-th largest among the four largest lanes' maxima of each warp); what passes it
+// afterwards goes to the end of a list of the warp, of which a sort leaves `top` when it is full and at the end, and the warps' lists are merged two by two.  With a bound of each
+// warp's own, 20 alternatives of 2048 x 151936 logits took 815 us.
 #include "ptx.cuh"
 #include "seq_common.cuh"
 
 namespace kb2seq {
 
-constexpr int kLpWarps = 16, kLpThreads = 32 * kLpWarps, kLpTop = 64, kLpList = 128, kLpMostCtas = 8, kLpPieces = 4;
+constexpr int kLpWarps = 16, kLpThreads = 32 * kLpWarps, kLpTop = 64, kLpList = 128, kLpMostCtas = 8, kLpPieces = 4, kLpFirst = 4;
 
+typedef unsigned long long Key;
 // A number's place among a row's: larger numbers first, then lower indices; -0 and +0 are equal.  0: no number.
-__device__ __forceinline__ unsigned long long logp_key(float z, uint32_t i) {
+__device__ __forceinline__ Key logp_key(float z, uint32_t i) {
   const uint32_t b = __float_as_uint(z + 0.f), up = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (unsigned long long)up << 32 | (uint32_t)~i;
+  return (Key)up << 32 | (uint32_t)~i;
 }
-__device__ __forceinline__ float logp_number(unsigned long long key) {
+__device__ __forceinline__ float logp_number(Key key) {
   const uint32_t up = (uint32_t)(key >> 32);
   return __uint_as_float(up & 0x80000000u ? up & 0x7FFFFFFFu : ~up);
 }
@@ -26,12 +29,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// e^d for d <= 0: an approximate power of two, off by 2^-22 beside the rounding of d / ln 2
-__device__ __forceinline__ float exp_neg(float d) {
+__device__ __forceinline__ float exp2_fast(float t) {      // off by 2^-22
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogpArgs {
   const void* z;
@@ -42,70 +45,71 @@ struct LogpArgs {
   int* ids;
 };
 struct LogpSums {
-  float m, s, u;
-  // numbers with the maximum `most`
-  __device__ __forceinline__ void raise(float most) {
-    if (most > m) {
-      if (m > -INFINITY) {
-        const float d = m - most, f = exp_neg(d);
-        u = d > -200.f ? f * fmaf(d, s, u) : 0.f;
+  float c, s, u;
+  __device__ __forceinline__ void raise(float to) {
+    if (to > c) {
+      if (c > -INFINITY) {
+        const float d = c - to, f = exp2_fast(d);
+        u = f > 0.f ? f * fmaf(d, s, u) : 0.f;
         s *= f;
       }
-      m = most;
+      c = to;
     }
   }
   __device__ __forceinline__ void join(const LogpSums& o) {
     LogpSums b = o;
-    raise(b.m);
-    b.raise(m);
+    raise(b.c);
+    b.raise(c);
     s += b.s;
     u += b.u;
   }
 };
 
-// 128 keys of a warp, four a lane, sorted so that the largest come first (a bitonic network; place p is the lane p % 32's key p / 32).
-__device__ __forceinline__ void sort_list(unsigned long long* list, int n, int lane) {
-  unsigned long long k[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) k[i] = i * 32 + lane < n ? list[i * 32 + lane] : 0ull;
-#pragma unroll
-  for (int size = 2; size <= 128; size <<= 1)
-#pragma unroll
-    for (int half = size >> 1; half; half >>= 1) {
-      if (half >= 32) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = i ^ half / 32;
-          if (j > i) {
-            const bool down = ((i * 32 + lane) & size) == 0;      // the larger one ahead
-            const unsigned long long a = k[i], b = k[j];
-            k[i] = down == (a > b) ? a : b;
-            k[j] = down == (a > b) ? b : a;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned long long o = __shfl_xor_sync(0xffffffffu, k[i], half);
-          const bool ahead = (lane & half) == 0, down = ((i * 32 + lane) & size) == 0;
-          k[i] = (ahead == down) == (k[i] > o) ? k[i] : o;
-        }
-      }
-    }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) list[i * 32 + lane] = k[i];
-  __syncwarp();
+// Of keys a (lower place) and b those in their order, the larger one ahead if down.
+__device__ __forceinline__ void order(Key& a, Key& b, bool down) {
+  const Key x = a, y = b;
+  a = down == (x > y) ? x : y;
+  b = down == (x > y) ? y : x;
 }
-
-// The `top` largest of n keys (zeros are none) at `from`, to `to` in their order; `threads` threads.
-__device__ __forceinline__ void choose(const unsigned long long* from, int n, unsigned long long* to, int top) {
-  for (int i = threadIdx.x; i < n; i += kLpThreads) {
-    const unsigned long long k = from[i];
-    if (k == 0) continue;
-    int ahead = 0;
-    for (int j = 0; j < n; ++j) ahead += from[j] > k;
-    if (ahead < top) to[ahead] = k;
+// One step of a bitonic network over N * 32 keys of a warp, place i * 32 + lane in k[i]: partners `half` apart, blocks of `size` in turn down and up.
+template <int N>
+__device__ __forceinline__ void step(Key (&k)[N], int size, int half, int lane) {
+  if (half >= 32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & half / 32) == 0) order(k[i], k[i | half / 32], ((i * 32 + lane) & size) == 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const Key o = __shfl_xor_sync(0xffffffffu, k[i], half);
+      const bool ahead = (lane & half) == 0, down = ((i * 32 + lane) & size) == 0;
+      k[i] = (ahead == down) == (k[i] > o) ? k[i] : o;
+    }
   }
+}
+// The first n of a list's N * 32 places, the others taken as empty, in their order.
+template <int N>
+__device__ __forceinline__ void sort_list(Key* list, int n, int lane) {
+  Key k[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) k[i] = i * 32 + lane < n ? list[i * 32 + lane] : 0ull;
+#pragma unroll
+  for (int size = 2; size <= N * 32; size <<= 1)
+#pragma unroll
+    for (int half = size >> 1; half; half >>= 1) step<N>(k, size, half, lane);
+#pragma unroll
+  for (int i = 0; i < N; ++i) list[i * 32 + lane] = k[i];
+}
+// The N * 32 largest of two sorted lists, in their order, in the first one's place.
+template <int N>
+__device__ __forceinline__ void merge_lists(Key* a, const Key* b, int lane) {
+  Key k[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) k[i] = max(a[i * 32 + lane], b[N * 32 - 1 - (i * 32 + lane)]);
+#pragma unroll
+  for (int half = N * 16; half; half >>= 1) step<N>(k, N * 64, half, lane);
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i * 32 + lane] = k[i];
 }
 
 // What a thread knows of its numbers, and its warp of the largest ones.
@@ -114,81 +118,85 @@ struct LogpState {
   LogpSums sum;
   bool bad;
   int lane, top, listed;                           // keys in the warp's list
-  unsigned long long least;                        // only larger ones can still be among the `top`
-  unsigned long long* list;
+  Key least;                                       // only larger ones can still be among the `top`
+  float floor;                                     // its number
+  Key* list;
 
   __device__ __forceinline__ void prune() {
     __syncwarp();
-    sort_list(list, listed, lane);
+    if (listed <= 32 && top <= 32) sort_list<1>(list, listed, lane);      // what is merged is sorted whole: 32 places, or 64 for more alternatives
+    else if (listed <= 64) sort_list<2>(list, listed, lane);
+    else sort_list<4>(list, listed, lane);
+    __syncwarp();
     listed = min(listed, top);
-    if (listed == top) least = max(least, list[top - 1]);
+    if (listed == top && list[top - 1] > least) {
+      least = list[top - 1];
+      floor = logp_number(least);
+    }
     __syncwarp();
   }
   // where the j-th of a thread's numbers stands in the row
   static __device__ __forceinline__ uint32_t place(uint32_t first, int j) { return first + j / kVec * 32 * kVec + j % kVec; }
-  // The first `count` of the numbers, those that stand ahead of `end`, go to the list's end: of every lane the largest left over at a time.
-  __device__ __forceinline__ void offer(float (&v)[kHave], uint32_t first, int count, uint32_t end) {
-    for (;;) {
-      unsigned long long k = 0;
-      int which = -1;
+  // The first `count` of the numbers, those that stand ahead of `end`, go to the list's end.
+  __device__ __forceinline__ void offer(const float (&v)[kHave], uint32_t first, int count, uint32_t end) {
 #pragma unroll
-      for (int j = 0; j < kHave; ++j) {
-        const unsigned long long n = logp_key(v[j], place(first, j));
-        if (v[j] == v[j] && j < count && place(first, j) < end && n > k) {
-          k = n;
-          which = j;
-        }
-      }
-      const bool in = k > least;
-      const uint32_t who = __ballot_sync(0xffffffffu, in);
-      if (who == 0) return;
+    for (int j = 0; j < kHave; ++j) {
+      if (!__any_sync(0xffffffffu, v[j] >= floor && j < count && place(first, j) < end)) continue;
+      const Key k = v[j] >= floor && j < count && place(first, j) < end ? logp_key(v[j], place(first, j)) : 0ull;
+      uint32_t who = __ballot_sync(0xffffffffu, k > least);
       if (listed + __popc(who) > kLpList) {
         prune();
-        continue;
+        who = __ballot_sync(0xffffffffu, k > least);
       }
-      if (in) list[listed + __popc(who & ((1u << lane) - 1))] = k;
+      if (who >> lane & 1) list[listed + __popc(who & ((1u << lane) - 1))] = k;
       listed += __popc(who);
-#pragma unroll
-      for (int j = 0; j < kHave; ++j)
-        if (in && j == which) v[j] = NAN;          // taken
     }
   }
-  __device__ __forceinline__ void feed(float (&v)[kHave], uint32_t first, int count, uint32_t end) {
+  __device__ __forceinline__ void add(const float (&v)[kHave], float most) {
+    const float to = most * kLog2e;
+    bad |= !(to < INFINITY);                       // and numbers above 2.3e38
+    sum.raise(to);
+    if (sum.c > -INFINITY) {
+#pragma unroll
+      for (int j = 0; j < kHave; ++j) {
+        const float t = fmaxf(fmaf(v[j], kLog2e, -sum.c), -300.f), e = exp2_fast(t);
+        sum.s += e;
+        sum.u = fmaf(e, t, sum.u);
+      }
+    }
+  }
+  static __device__ __forceinline__ float largest(const float (&v)[kHave]) {
     float most = v[0];
 #pragma unroll
     for (int j = 1; j < kHave; ++j) most = max_nan(most, v[j]);
-    bad |= !(most < INFINITY);
-    sum.raise(most);
-    if (sum.m > -INFINITY) {
+    return most;
+  }
+  // The bound that the block's first numbers give; `firsts` is room for kLpWarps * kLpFirst numbers.  Lanes without numbers have -inf, which bounds nothing.
+  __device__ __forceinline__ void bound(float most, float* firsts, int warp) {
+    Key k[1] = {most == most ? logp_key(most, lane) : 0ull};
 #pragma unroll
-      for (int j = 0; j < kHave; ++j) {
-        const float d = fmaxf(v[j] - sum.m, -200.f), e = exp_neg(d);
-        sum.s += e;
-        sum.u = fmaf(e, d, sum.u);
-      }
-    }
-    if (top > 0 && __any_sync(0xffffffffu, logp_key(most, 0) > least)) {
-      if (least == 0 && listed == 0 && top <= 32) {
-        // the first numbers: of the lanes' largest ones the top-th bounds what can be among the largest
-        const unsigned long long k = most == most ? logp_key(most, 0xFFFFFFFFu) : 0ull;
-        int ahead = 0;
-        for (int j = 0; j < 32; ++j) {
-          const unsigned long long o = __shfl_sync(0xffffffffu, k, j);
-          ahead += o > k || (o == k && j < lane);
-        }
-        const uint32_t who = __ballot_sync(0xffffffffu, ahead == top - 1);
-        const unsigned long long bound = __shfl_sync(0xffffffffu, k, __ffs(who) - 1);
-        if (bound > 0) least = bound - 1;          // with an index behind all others: equal numbers pass
-      }
-      offer(v, first, count, end);
-    }
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+      for (int half = size >> 1; half; half >>= 1) step<1>(k, size, half, lane);
+    if (lane < kLpFirst) firsts[warp * kLpFirst + lane] = k[0] ? logp_number(k[0]) : -INFINITY;
+    __syncthreads();
+    Key all[2] = {logp_key(firsts[lane], 2 * lane), logp_key(firsts[32 + lane], 2 * lane + 1)};
+#pragma unroll
+    for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+      for (int half = size >> 1; half; half >>= 1) step<2>(all, size, half, lane);
+    const Key it = __shfl_sync(0xffffffffu, top > 32 ? all[1] : all[0], (top - 1) & 31);
+    floor = logp_number(it);
+    least = logp_key(floor, 0xFFFFFFFFu) - 1;      // equal numbers pass
   }
 };
+static_assert(kLpWarps * kLpFirst == 64 && kLpTop == 64, "the bound is found among 64 numbers");
 
 template <bool BF16>
 __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LogpArgs a) {
   constexpr int kVec = BF16 ? 8 : 4, kPieces = BF16 ? kLpPieces / 2 : kLpPieces, kHave = kVec * kPieces;      // sixteen numbers a thread at a time
-  __shared__ unsigned long long s_list[kLpWarps][kLpList], s_all[kLpMostCtas][kLpTop];
+  __shared__ Key s_list[kLpWarps][kLpList], s_all[kLpMostCtas][kLpTop];
+  __shared__ float s_first[kLpWarps * kLpFirst];
   __shared__ LogpSums s_sums[kLpWarps], s_cta[kLpMostCtas];
   __shared__ int s_bad[kLpMostCtas];
   kb2::pdl_wait();
@@ -212,6 +220,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
   st.top = top;
   st.listed = 0;
   st.least = 0;
+  st.floor = -INFINITY;
   st.list = s_list[warp];
   const auto whole = [&](const uint4 (&x)[kPieces], float (&v)[kHave]) {
 #pragma unroll
@@ -243,7 +252,12 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     float v[kHave];
     whole(x, v);
     if (p + kRound < p1) load(p + kRound, x);
-    st.feed(v, head + (p + warp * kPieces * 32 + lane) * kVec, kHave, head + p1 * kVec);
+    const float most = st.largest(v);
+    st.add(v, most);
+    if (top > 0) {
+      if (p == p0) st.bound(most, s_first, warp);
+      if (__any_sync(0xffffffffu, most >= st.floor)) st.offer(v, head + (p + warp * kPieces * 32 + lane) * kVec, kHave, head + p1 * kVec);
+    }
   }
   if (rank == 0 && warp == 0 && (head > 0 || tail0 < a.V)) {
     // up to 15 numbers: one a lane
@@ -253,37 +267,30 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     const int i = lane < 16 ? lane : tail0 + lane - 16;
     const bool there = lane < 16 ? lane < head : i < a.V;
     if (there) v[0] = number(i);
-    st.feed(v, there ? i : a.V, 1, a.V);
+    st.add(v, v[0]);
+    if (top > 0) st.offer(v, there ? i : a.V, 1, a.V);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     LogpSums b;
-    b.m = __shfl_xor_sync(0xffffffffu, st.sum.m, o);
+    b.c = __shfl_xor_sync(0xffffffffu, st.sum.c, o);
     b.s = __shfl_xor_sync(0xffffffffu, st.sum.s, o);
     b.u = __shfl_xor_sync(0xffffffffu, st.sum.u, o);
     st.sum.join(b);
   }
-  if (top > 0) {
-    st.prune();
-  }
+  if (top > 0) st.prune();
   if (lane == 0) s_sums[warp] = st.sum;
   bool bad = __syncthreads_or(st.bad);
-  // the block's lists one behind the other
+  const auto merge = [&](Key* to, const Key* from) {
+    if (top <= 32) merge_lists<1>(to, from, lane);
+    else merge_lists<2>(to, from, lane);
+  };
   if (top > 0) {
-    for (int i = tid; i < kLpTop; i += kLpThreads) s_all[0][i] = 0;
-    unsigned long long mine[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = r * kLpThreads + tid;
-      mine[r] = i < kLpWarps * top ? s_list[i / top][i % top] : 0ull;
+    for (int o = 1; o < kLpWarps; o *= 2) {        // two by two
+      if (warp % (2 * o) == 0) merge(s_list[warp], s_list[warp + o]);
+      __syncthreads();
     }
-    __syncthreads();
-    unsigned long long* all = &s_list[0][0];
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-      if (r * kLpThreads + tid < kLpWarps * top) all[r * kLpThreads + tid] = mine[r];
-    __syncthreads();
-    choose(all, kLpWarps * top, s_all[0], top);
+    if (tid < kLpTop) s_all[0][tid] = s_list[0][tid];
   }
   if (tid == 0) {
     LogpSums w = s_sums[0];
@@ -295,8 +302,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     kb2::cluster_sync_all();
     if (rank == 0) {
       for (int c = 1 + warp; c < (int)ctas; c += kLpWarps) {
-        for (int i = lane; i < top; i += 32) {
-          unsigned long long k;
+        for (int i = lane; i < kLpTop; i += 32) {
+          Key k;
           asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(kb2::cluster_addr(&s_all[0][i], c)) : "memory");
           s_all[c][i] = k;
         }
@@ -312,10 +319,10 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     kb2::cluster_sync_all();                       // nobody leaves while the first block reads
     if (rank != 0) return;
     if (top > 0) {
-      unsigned long long* all = &s_list[0][0];
-      for (int i = tid; i < (int)ctas * top; i += kLpThreads) all[i] = s_all[i / top][i % top];
-      __syncthreads();
-      choose(all, ctas * top, s_all[0], top);
+      for (int o = 1; o < (int)ctas; o *= 2) {
+        __syncthreads();
+        if (warp % (2 * o) == 0 && warp + o < (int)ctas) merge(s_all[warp], s_all[warp + o]);
+      }
     }
   }
   __syncthreads();
@@ -325,17 +332,18 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     w.join(s_cta[c]);
     bad |= s_bad[c] != 0;
   }
-  bad |= w.m == -INFINITY;
-  const float lse = logf(w.s);
+  bad |= w.c == -INFINITY;
+  const float lse = log2f(w.s);                    // of what is above c
+  const auto logprob = [&](float x) { return (fmaf(x, kLog2e, -w.c) - lse) * kLn2; };
   if (tid == 0) {
     const long long k = a.tokens[t];
-    a.logprob[t] = bad ? NAN : k < 0 || k >= a.V ? -INFINITY : number((int)k) - w.m - lse;
-    a.entropy[t] = bad ? NAN : lse - w.u / w.s;
+    a.logprob[t] = bad ? NAN : k < 0 || k >= a.V ? -INFINITY : logprob(number((int)k));
+    a.entropy[t] = bad ? NAN : (lse - w.u / w.s) * kLn2;
   }
   for (int i = tid; i < top; i += kLpThreads) {
-    const unsigned long long k = s_all[0][i];
+    const Key k = s_all[0][i];
     a.ids[(long long)t * top + i] = bad ? -1 : (int)~(uint32_t)k;
-    a.best[(long long)t * top + i] = bad ? NAN : logp_number(k) - w.m - lse;
+    a.best[(long long)t * top + i] = bad ? NAN : logprob(logp_number(k));
   }
 }
 
