@@ -2,17 +2,17 @@
 //
 // In powers of two: with L = log2 e and a reference c near L max z, t = L z - c by one fused multiply-add, s = sum 2^t, u = sum 2^t t.  Where c rises by d, s <- s 2^-d and u <- (u -
 // d s) 2^-d.  At the end log2 sum exp z = c + log2 s, so logprob = (t(token) - log2 s) / L and entropy = (log2 s - u / s) / L; an L that is rounded is a temperature of 1 + 2^-26.
-// Bound: the rows' way from memory.  A block of sixteen warps has a row; where there are fewer rows than SMs, a cluster of up to eight blocks shares it and its first block
-// joins what they found, read through distributed shared memory.
-// The largest numbers: the block's first numbers give a bound that `top` of the row pass (the top-th largest among the four largest lanes' maxima of each warp); what passes it
-// afterwards goes to the end of a list of the warp, of which a sort leaves `top` when it is full and at the end, and the warps' lists are merged two by two.  With a bound of each
-// warp's own, 20 alternatives of 2048 x 151936 logits took 815 us.
+// Bound: the rows' way from memory.  A block of eight warps has a row (of sixteen, 2048 rows of 32768 and five alternatives took 102 us instead of 81); where there are fewer rows
+// than SMs, a cluster of up to eight blocks shares it and its first block joins what they found, read through distributed shared memory.
+// The largest numbers: after one, four and sixteen rounds the block's numbers so far give a bound that `top` of the row pass (the top-th largest among the eight largest lanes'
+// maxima of each warp).  What passes it goes to the end of a list of the warp, of which a sort leaves `top` when it is full and at the end; the warps' lists are merged two by two.
+// With a bound of each warp's own, 20 alternatives of 2048 x 151936 logits took 815 us.
 #include "ptx.cuh"
 #include "seq_common.cuh"
 
 namespace kb2seq {
 
-constexpr int kLpWarps = 16, kLpThreads = 32 * kLpWarps, kLpTop = 64, kLpList = 128, kLpMostCtas = 8, kLpPieces = 4, kLpFirst = 4;
+constexpr int kLpWarps = 8, kLpThreads = 32 * kLpWarps, kLpTop = 64, kLpList = 128, kLpMostCtas = 8, kLpPieces = 4, kLpFirst = 8;
 
 typedef unsigned long long Key;
 // A number's place among a row's: larger numbers first, then lower indices; -0 and +0 are equal.  0: no number.
@@ -65,25 +65,22 @@ struct LogpSums {
   }
 };
 
-// Of keys a (lower place) and b those in their order, the larger one ahead if down.
-__device__ __forceinline__ void order(Key& a, Key& b, bool down) {
-  const Key x = a, y = b;
-  a = down == (x > y) ? x : y;
-  b = down == (x > y) ? y : x;
-}
-// One step of a bitonic network over N * 32 keys of a warp, place i * 32 + lane in k[i]: partners `half` apart, blocks of `size` in turn down and up.
-template <int N>
-__device__ __forceinline__ void step(Key (&k)[N], int size, int half, int lane) {
-  if (half >= 32) {
+// One step of a bitonic network over N * 32 keys or numbers of a warp, place i * 32 + lane in k[i]: partners `half` apart, blocks of `size` in turn down (the larger ones
+// ahead) and up.
+template <int N, typename T>
+__device__ __forceinline__ void step(T (&k)[N], int size, int half, int lane) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if ((i & half / 32) == 0) order(k[i], k[i | half / 32], ((i * 32 + lane) & size) == 0);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const Key o = __shfl_xor_sync(0xffffffffu, k[i], half);
-      const bool ahead = (lane & half) == 0, down = ((i * 32 + lane) & size) == 0;
-      k[i] = (ahead == down) == (k[i] > o) ? k[i] : o;
+  for (int i = 0; i < N; ++i) {
+    const bool down = ((i * 32 + lane) & size) == 0;
+    if (half >= 32) {
+      const int other = i | half / 32;
+      if (other == i) continue;
+      const T x = k[i], y = k[other < N ? other : i];
+      k[i] = down ? max(x, y) : min(x, y);
+      k[other < N ? other : i] = down ? min(x, y) : max(x, y);
+    } else {
+      const T o = __shfl_xor_sync(0xffffffffu, k[i], half);
+      k[i] = ((lane & half) == 0) == down ? max(k[i], o) : min(k[i], o);
     }
   }
 }
@@ -96,7 +93,7 @@ __device__ __forceinline__ void sort_list(Key* list, int n, int lane) {
 #pragma unroll
   for (int size = 2; size <= N * 32; size <<= 1)
 #pragma unroll
-    for (int half = size >> 1; half; half >>= 1) step<N>(k, size, half, lane);
+    for (int half = size >> 1; half; half >>= 1) step(k, size, half, lane);
 #pragma unroll
   for (int i = 0; i < N; ++i) list[i * 32 + lane] = k[i];
 }
@@ -107,7 +104,7 @@ __device__ __forceinline__ void merge_lists(Key* a, const Key* b, int lane) {
 #pragma unroll
   for (int i = 0; i < N; ++i) k[i] = max(a[i * 32 + lane], b[N * 32 - 1 - (i * 32 + lane)]);
 #pragma unroll
-  for (int half = N * 16; half; half >>= 1) step<N>(k, N * 64, half, lane);
+  for (int half = N * 16; half; half >>= 1) step(k, N * 64, half, lane);
 #pragma unroll
   for (int i = 0; i < N; ++i) a[i * 32 + lane] = k[i];
 }
@@ -137,19 +134,27 @@ struct LogpState {
   }
   // where the j-th of a thread's numbers stands in the row
   static __device__ __forceinline__ uint32_t place(uint32_t first, int j) { return first + j / kVec * 32 * kVec + j % kVec; }
-  // The first `count` of the numbers, those that stand ahead of `end`, go to the list's end.
-  __device__ __forceinline__ void offer(const float (&v)[kHave], uint32_t first, int count, uint32_t end) {
+  // Numbers that stand ahead of `end` go to the list's end.
+  __device__ __forceinline__ void offer(float (&v)[kHave], uint32_t first, uint32_t end) {
+    for (;;) {
+      bool full = false;
 #pragma unroll
-    for (int j = 0; j < kHave; ++j) {
-      if (!__any_sync(0xffffffffu, v[j] >= floor && j < count && place(first, j) < end)) continue;
-      const Key k = v[j] >= floor && j < count && place(first, j) < end ? logp_key(v[j], place(first, j)) : 0ull;
-      uint32_t who = __ballot_sync(0xffffffffu, k > least);
-      if (listed + __popc(who) > kLpList) {
-        prune();
-        who = __ballot_sync(0xffffffffu, k > least);
+      for (int j = 0; j < kHave; ++j) {
+        if (!__any_sync(0xffffffffu, v[j] >= floor && place(first, j) < end)) continue;
+        const Key k = v[j] >= floor && place(first, j) < end ? logp_key(v[j], place(first, j)) : 0ull;
+        const uint32_t who = __ballot_sync(0xffffffffu, k > least);
+        if (listed + __popc(who) > kLpList) {
+          full = true;
+          continue;
+        }
+        if (k > least) {
+          list[listed + __popc(who & ((1u << lane) - 1))] = k;
+          v[j] = NAN;                              // taken
+        }
+        listed += __popc(who);
       }
-      if (who >> lane & 1) list[listed + __popc(who & ((1u << lane) - 1))] = k;
-      listed += __popc(who);
+      if (!full) return;
+      prune();
     }
   }
   __device__ __forceinline__ void add(const float (&v)[kHave], float most) {
@@ -171,29 +176,32 @@ struct LogpState {
     for (int j = 1; j < kHave; ++j) most = max_nan(most, v[j]);
     return most;
   }
-  // The bound that the block's first numbers give; `firsts` is room for kLpWarps * kLpFirst numbers.  Lanes without numbers have -inf, which bounds nothing.
+  // The bound that the lanes' largest numbers so far give; `firsts` is room for kLpWarps * kLpFirst numbers.  Lanes without numbers have -inf, which bounds nothing.
   __device__ __forceinline__ void bound(float most, float* firsts, int warp) {
-    Key k[1] = {most == most ? logp_key(most, lane) : 0ull};
+    __syncthreads();                               // the last one's have been read
+    float k[1] = {most == most ? most : -INFINITY};
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
-      for (int half = size >> 1; half; half >>= 1) step<1>(k, size, half, lane);
-    if (lane < kLpFirst) firsts[warp * kLpFirst + lane] = k[0] ? logp_number(k[0]) : -INFINITY;
+      for (int half = size >> 1; half; half >>= 1) step(k, size, half, lane);
+    if (lane < kLpFirst) firsts[warp * kLpFirst + lane] = k[0];
     __syncthreads();
-    Key all[2] = {logp_key(firsts[lane], 2 * lane), logp_key(firsts[32 + lane], 2 * lane + 1)};
+    float all[2] = {firsts[lane], firsts[32 + lane]};
 #pragma unroll
     for (int size = 2; size <= 64; size <<= 1)
 #pragma unroll
-      for (int half = size >> 1; half; half >>= 1) step<2>(all, size, half, lane);
-    const Key it = __shfl_sync(0xffffffffu, top > 32 ? all[1] : all[0], (top - 1) & 31);
-    floor = logp_number(it);
-    least = logp_key(floor, 0xFFFFFFFFu) - 1;      // equal numbers pass
+      for (int half = size >> 1; half; half >>= 1) step(all, size, half, lane);
+    const float it = __shfl_sync(0xffffffffu, top > 32 ? all[1] : all[0], (top - 1) & 31);
+    if (it > floor) {
+      floor = it;
+      least = logp_key(it, 0xFFFFFFFFu) - 1;       // equal numbers pass
+    }
   }
 };
 static_assert(kLpWarps * kLpFirst == 64 && kLpTop == 64, "the bound is found among 64 numbers");
 
 template <bool BF16>
-__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LogpArgs a) {
+__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LogpArgs a) {
   constexpr int kVec = BF16 ? 8 : 4, kPieces = BF16 ? kLpPieces / 2 : kLpPieces, kHave = kVec * kPieces;      // sixteen numbers a thread at a time
   __shared__ Key s_list[kLpWarps][kLpList], s_all[kLpMostCtas][kLpTop];
   __shared__ float s_first[kLpWarps * kLpFirst];
@@ -248,6 +256,23 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
   };
   uint4 x[kPieces];
   load(p0, x);
+  if (rank == 0 && warp == 0 && (head > 0 || tail0 < a.V)) {
+    // up to 14 numbers: one a lane, and a place of the list for each
+    const int i = lane < 16 ? lane : tail0 + lane - 16;
+    const bool there = lane < 16 ? lane < head : i < a.V;
+    float v[kHave];
+#pragma unroll
+    for (int j = 0; j < kHave; ++j) v[j] = -INFINITY;
+    if (there) v[0] = number(i);
+    st.add(v, v[0]);
+    const uint32_t who = __ballot_sync(0xffffffffu, there);
+    if (top > 0) {
+      if (there) st.list[__popc(who & ((1u << lane) - 1))] = logp_key(v[0], i);
+      st.listed = __popc(who);
+    }
+  }
+  float best = -INFINITY;
+  int next_bound = p0;
   for (int p = p0; p < p1; p += kRound) {
     float v[kHave];
     whole(x, v);
@@ -255,20 +280,13 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     const float most = st.largest(v);
     st.add(v, most);
     if (top > 0) {
-      if (p == p0) st.bound(most, s_first, warp);
-      if (__any_sync(0xffffffffu, most >= st.floor)) st.offer(v, head + (p + warp * kPieces * 32 + lane) * kVec, kHave, head + p1 * kVec);
+      best = fmaxf(best, most);
+      if (p >= next_bound) {                       // after one, four and sixteen rounds
+        st.bound(best, s_first, warp);
+        next_bound = p0 + (4 * ((p - p0) / kRound + 1) - 1) * kRound;
+      }
+      if (__any_sync(0xffffffffu, most >= st.floor)) st.offer(v, head + (p + warp * kPieces * 32 + lane) * kVec, head + p1 * kVec);
     }
-  }
-  if (rank == 0 && warp == 0 && (head > 0 || tail0 < a.V)) {
-    // up to 15 numbers: one a lane
-    float v[kHave];
-#pragma unroll
-    for (int j = 0; j < kHave; ++j) v[j] = -INFINITY;
-    const int i = lane < 16 ? lane : tail0 + lane - 16;
-    const bool there = lane < 16 ? lane < head : i < a.V;
-    if (there) v[0] = number(i);
-    st.add(v, v[0]);
-    if (top > 0) st.offer(v, there ? i : a.V, 1, a.V);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {

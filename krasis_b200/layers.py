@@ -127,10 +127,13 @@ def _f32_code(t, name) -> int:
     return int(t.dtype is torch.float32)
 
 
-def _fp8_device(name, *tensors) -> int:
+def _fp8_device(name, first, *others) -> int:
     """The CUDA device that all tensors (None: not given) are on."""
-    dev = tensors[0].get_device()
-    if dev < 0 or any(t is not None and t.get_device() != dev for t in tensors):
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            dev = -1
+    if dev < 0:
         raise ValueError(f"{name}: the tensors belong on one CUDA device (krasis_b200 has no CPU path)")
     return dev
 
@@ -138,16 +141,18 @@ def _fp8_device(name, *tensors) -> int:
 def _fp8_input(name, x):
     if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] != 1):
         raise ValueError(f"{name}: rows [M, K] whose numbers lie side by side, got {tuple(x.shape)} with strides {x.stride()}")
-    if x.shape[1] == 0 or x.shape[1] % 16:
-        raise ValueError(f"{name}: rows of {x.shape[1]} numbers, a multiple of 16 is needed")
+    m, k = x.shape
+    if k == 0 or k % 16:
+        raise ValueError(f"{name}: rows of {k} numbers, a multiple of 16 is needed")
+    return m, k
 
 
-def _fp8_matrix(name, w, scales, shape):
+def _fp8_matrix(name, w, scales, *shape):
     """Codes of `shape` and a scale per block of 128 x 128 of its last two axes."""
-    want = tuple(shape[:-2]) + (_fp8_blocks(shape[-2]), _fp8_blocks(shape[-1]))
-    if w.dtype is not torch.float8_e4m3fn or tuple(w.shape) != tuple(shape) or not w.is_contiguous():
-        raise ValueError(f"{name}: contiguous float8_e4m3fn weights {tuple(shape)}, got {w.dtype} {tuple(w.shape)}")
-    if scales.dtype is not torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous():
+    want = (*shape[:-2], (shape[-2] + 127) // 128, (shape[-1] + 127) // 128)
+    if w.dtype is not torch.float8_e4m3fn or w.shape != shape or not w.is_contiguous():
+        raise ValueError(f"{name}: contiguous float8_e4m3fn weights {shape}, got {w.dtype} {tuple(w.shape)}")
+    if scales.dtype is not torch.float32 or scales.shape != want or not scales.is_contiguous():
         raise ValueError(f"{name}: contiguous float32 scales {want}, got {scales.dtype} {tuple(scales.shape)}")
 
 
@@ -155,13 +160,12 @@ def quantize_fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows [M, K] (bfloat16 or float32, any row stride, K a multiple of 16) in 8 bits: (codes [M, K] float8_e4m3fn, scales [M, ceil(K / 128)] float32, one for
     each 128 numbers of a row).  A block's scale is the least 2^k, k >= -126, that its largest magnitude is at most 448 times of; a block of zeros has scale 0, one
     with a number that is not finite scale NaN and codes 0.  The scales of one block of all rows lie side by side: strides (1, rows rounded up to 4)."""
-    _fp8_input("quantize_fp8_rows", x)
-    f32, dev, (m, k) = _f32_code(x, "quantize_fp8_rows"), _fp8_device("quantize_fp8_rows", x), x.shape
-    codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
-    ld = (m + 3) // 4 * 4
-    scales = torch.empty((_fp8_blocks(k), ld), dtype=torch.float32, device=x.device)
+    m, k = _fp8_input("quantize_fp8_rows", x)
+    f32, dev, device, ld = _f32_code(x, "quantize_fp8_rows"), _fp8_device("quantize_fp8_rows", x), x.device, (m + 3) // 4 * 4
+    codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty_strided((m, _fp8_blocks(k)), (1, ld), dtype=torch.float32, device=device)
     capi.check(capi.load().kb2_fp8_quantize_rows(x.data_ptr(), f32, x.stride(0), m, k, codes.data_ptr(), scales.data_ptr(), ld, dev, stream_on(dev)))
-    return codes, scales.t()[:m]
+    return codes, scales
 
 
 def quantize_fp8_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -186,9 +190,9 @@ def _fp8_out(name, x, n, bias, out_dtype):
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, bias: Optional[torch.Tensor] = None, out_dtype=None) -> torch.Tensor:
     """x [M, K] (bfloat16 or float32) times a matrix that is held in 8 bits, weight [N, K] float8_e4m3fn with any fp32 scales [ceil(N / 128), ceil(K / 128)], plus bias
     [N] float32: [M, N] in out_dtype (x's own).  The rows are quantised as by quantize_fp8_rows; sums are fp32."""
-    _fp8_input("fp8_linear", x)
-    (m, k), n = x.shape, weight.shape[0]
-    _fp8_matrix("fp8_linear", weight, weight_scales, (n, k))
+    m, k = _fp8_input("fp8_linear", x)
+    n = weight.shape[0]
+    _fp8_matrix("fp8_linear", weight, weight_scales, n, k)
     f32, dev = _f32_code(x, "fp8_linear"), _fp8_device("fp8_linear", x, weight, weight_scales, bias)
     out, o32 = _fp8_out("fp8_linear", x, n, bias, x.dtype if out_dtype is None else out_dtype)
     lib = capi.load()
@@ -203,11 +207,11 @@ def fp8_linear_rows(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Ten
                     out_dtype=torch.bfloat16) -> torch.Tensor:
     """fp8_linear on rows that are quantised already: codes [M, K] float8_e4m3fn and scales [M, ceil(K / 128)] float32 (in the order that quantize_fp8_rows leaves them;
     others are copied into it)."""
-    _fp8_input("fp8_linear_rows", codes)
-    (m, k), n = codes.shape, weight.shape[0]
+    m, k = _fp8_input("fp8_linear_rows", codes)
+    n = weight.shape[0]
     if codes.dtype is not torch.float8_e4m3fn or not codes.is_contiguous() or scales.dtype is not torch.float32 or tuple(scales.shape) != (m, _fp8_blocks(k)):
         raise ValueError(f"fp8_linear_rows: contiguous float8_e4m3fn codes [M, K] and float32 scales [M, {_fp8_blocks(k)}]")
-    _fp8_matrix("fp8_linear_rows", weight, weight_scales, (n, k))
+    _fp8_matrix("fp8_linear_rows", weight, weight_scales, n, k)
     dev = _fp8_device("fp8_linear_rows", codes, scales, weight, weight_scales, bias)
     out, o32 = _fp8_out("fp8_linear_rows", codes, n, bias, out_dtype)
     if scales.stride(0) != 1 or scales.stride(1) % 4 or scales.stride(1) < m or scales.data_ptr() % 16:
@@ -224,13 +228,12 @@ def fp8_experts(h: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gat
     quantisation of quantize_fp8_rows.  h [T, W] bfloat16 or float32; ids [T, top] int32, those outside [0, E) bring nothing; weights [T, top] float32; w_gate_up
     [E, 2 F, W] = [gate ; up] and w_down [E, W, F] float8_e4m3fn, with a scale for each block of 128 x 128; W a multiple of 16, F of 128, at most 1024 experts.
     [T, W] in out_dtype (h's own); for bfloat16 each expert's row is rounded to it ahead of the weighted sum."""
-    _fp8_input("fp8_experts", h)
-    T, W = h.shape
+    T, W = _fp8_input("fp8_experts", h)
     if w_gate_up.dim() != 3 or w_gate_up.shape[1] % 256 or w_gate_up.shape[1] == 0:
         raise ValueError(f"fp8_experts: gate and up projections [E, 2 F, W] with F a multiple of 128, got {tuple(w_gate_up.shape)}")
     E, F = w_gate_up.shape[0], w_gate_up.shape[1] // 2
-    _fp8_matrix("fp8_experts", w_gate_up, s_gate_up, (E, 2 * F, W))
-    _fp8_matrix("fp8_experts", w_down, s_down, (E, W, F))
+    _fp8_matrix("fp8_experts", w_gate_up, s_gate_up, E, 2 * F, W)
+    _fp8_matrix("fp8_experts", w_down, s_down, E, W, F)
     if ids.dtype is not torch.int32 or ids.dim() != 2 or ids.shape[0] != T or ids.shape[1] == 0 or not ids.is_contiguous():
         raise ValueError(f"fp8_experts: contiguous int32 ids [{T}, top]")
     if weights.dtype is not torch.float32 or weights.shape != ids.shape or not weights.is_contiguous():

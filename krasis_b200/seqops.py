@@ -650,20 +650,23 @@ MAX_TOP_LOGPROBS = 64
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """logits [T, V] (fp32 or bfloat16, any row stride) and tokens [T] (int64 or int32): log softmax at the tokens, the entropy of the softmax, and the `top` largest
     logits' ids (int32) and log probabilities, the lowest id first among equals.  All in fp32.  A token outside [0, V) has log probability -inf; logits of -inf weigh
-    nothing; a row with a NaN or +inf, or with nothing but -inf, gives NaN and ids of -1."""
-    _cuda(logits, "token_logprobs")
+    nothing; a row with a NaN or a logit above 2e38, or with nothing but -inf, gives NaN and ids of -1."""
+    dev = logits.get_device()
+    if dev < 0:
+        _cuda(logits, "token_logprobs")
     if logits.dim() != 2 or logits.shape[1] == 0 or (logits.stride(1) != 1 and logits.shape[1] != 1):
         raise ValueError(f"token_logprobs: logits [T, V] whose numbers lie side by side, got {tuple(logits.shape)} with strides {logits.stride()}")
     T, V = logits.shape
-    if tuple(tokens.shape) != (T,) or tokens.dtype not in (torch.int64, torch.int32) or tokens.get_device() != logits.get_device():
+    if tokens.shape != (T,) or tokens.dtype not in (torch.int64, torch.int32) or tokens.get_device() != dev:
         raise ValueError(f"token_logprobs: one int64 or int32 token per row, [{T}] on the logits' device")
-    top = int(top)
     if not 0 <= top <= min(V, MAX_TOP_LOGPROBS):
         raise ValueError(f"token_logprobs: {top} alternatives of {V}, at most {MAX_TOP_LOGPROBS}")
-    tokens = tokens.to(torch.int64).contiguous()
-    dev, dt = logits.device, dt_code(logits.dtype)
-    out = torch.empty(T * (2 + 2 * top), dtype=torch.float32, device=dev)          # one allocation
-    lp, en, best, ids = out[:T], out[T:2 * T], out[2 * T:(2 + top) * T].view(T, top), out[(2 + top) * T:].view(torch.int32).view(T, top)
+    if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
+    device, dt = logits.device, dt_code(logits.dtype)
+    lp, en = torch.empty((2, T), dtype=torch.float32, device=device).unbind()
+    best = torch.empty((T, top), dtype=torch.float32, device=device)
+    ids = torch.empty((T, top), dtype=torch.int32, device=device)
     check(load().kb2_seq_token_logprobs(logits.data_ptr(), dt, logits.stride(0), T, V, tokens.data_ptr(), top, lp.data_ptr(), en.data_ptr(), ids.data_ptr(),
-                                        best.data_ptr(), dev.index, _s(logits)))
+                                        best.data_ptr(), dev, stream_on(dev)))
     return TokenLogprobs(lp, en, ids, best)
