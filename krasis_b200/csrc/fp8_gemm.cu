@@ -30,14 +30,16 @@ cudaError_t make_tmap_u8_gate_up(void* out_tmap, const void* base, long long gro
 // A CTA has 128 rows of x (the M side) and half the weight rows, 32 KB for 512 cycles of MMAs per block of K.  Sixteen warps hold the tile's sums, 64 a thread: a thread has one
 // row of x, so one scale of it per block, and 64 columns of one block of weights, so one of those.  With the weights on the M side a column's scale came from shared memory, 256
 // broadcast loads per block beside the MMAs' own reads, and a block took 1070 cycles of eight warps (M 8192, N 4096, K 4096: 150 us).
-constexpr int kFStages = 4, kFRows = 128, kFBox = 32, kFABytes = kFRows * 128, kFStage = 2 * kFABytes;
+constexpr int kFRows = 128, kFBox = 32, kFABytes = kFRows * 128, kFStage = 2 * kFABytes;
 constexpr int kFThreads = 640, kFWarps = 16;
 // The scales of kFGroup blocks are handed over at once, two groups are at hand: products for each row, for the first and the second 128 columns (gated: gate's, up's).
 constexpr int kFGroup = 4, kFScales = 2 * kFGroup;
 constexpr int kFOut = 32 * 128;                    // a warp's results on their way out
-constexpr int kFOffOut = kFStages * kFStage, kFOffScale = kFOffOut + kFWarps * kFOut, kFOffMax = kFOffScale + kFScales * 2 * kFRows * 4,
-              kFOffBar = kFOffMax + 2 * 4 * kFRows * 4, kFUsed = kFOffBar + 512, kFSmem = kFUsed > 512 * 430 - 1024 ? kFUsed : 512 * 430 - 1024;
-static_assert(kFSmem <= 227 * 1024, "what a CTA of a cluster takes for 512 columns (tmem_smem)");
+constexpr int kFMostStages = 6;
+__host__ __device__ constexpr int pair_stages(bool glu) { return glu ? 6 : 4; }     // gated units have nothing on its way out in shared memory
+constexpr int kFOffOut = 4 * kFStage, kFOffScale = 6 * kFStage, kFOffMax = kFOffScale + kFScales * 2 * kFRows * 4, kFOffBar = kFOffMax + 2 * 4 * kFRows * 4, kFUsed = kFOffBar + 512,
+              kFSmem = kFUsed > 512 * 430 - 1024 ? kFUsed : 512 * 430 - 1024;
+static_assert(kFOffOut + kFWarps * kFOut <= kFOffScale && kFSmem <= 227 * 1024, "what a CTA of a cluster takes for 512 columns (tmem_smem)");
 static_assert(kFp8Run == 2 * kFRows, "a run is one tile's rows");
 
 struct PairArgs {
@@ -51,10 +53,11 @@ struct PairArgs {
 template <bool kGlu, bool kOutF32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_out, const PairArgs a) {
+  constexpr int kFStages = pair_stages(kGlu);
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFOffBar);       // of the first CTA: both CTAs' loads
-  uint64_t* empty = full + kFStages;
-  uint64_t* acc_full = empty + kFStages;           // [2]
+  uint64_t* empty = full + kFMostStages;
+  uint64_t* acc_full = empty + kFMostStages;       // [2]
   uint64_t* acc_empty = acc_full + 2;              // [2], of the first CTA: both CTAs' read-outs
   uint64_t* s_full = acc_empty + 2;                // [2]
   uint64_t* s_empty = s_full + 2;
@@ -112,7 +115,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
   };
 
   if (warp >= 4) {
-    more_registers<104>();
+    more_registers<112>();
     const int q = warp & 3, h = (warp - 4) >> 2, row = rank * kFRows + q * 32 + lane;     // of the tile
     const uint32_t from = tmem_base + ((uint32_t)(q * 32) << 16) + h * 64;
     int b = 0;
@@ -138,16 +141,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
           if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(&acc_empty[b], 0));
         };
         if (mine) {
-          // 16 columns are on their way while those before them are added
-          uint32_t v[2][16];
-          tmem_ld16(from + b * 256, v[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t v[32];
+            tmem_ld32(from + b * 256 + c * 32, v);
             tmem_ld_wait();
-            if (c < 3) tmem_ld16(from + b * 256 + (c + 1) * 16, v[(c + 1) & 1]);
-            else read();
+            if (c) read();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) fma2_here(acc[c * 8 + j], pack2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), c >> 1 ? two1 : two0);
+            for (int j = 0; j < 16; ++j) fma2_here(acc[c * 16 + j], pack2(v[2 * j], v[2 * j + 1]), c ? two1 : two0);
           }
         } else {
           read();
@@ -250,7 +251,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
       }
     }
     if (!kGlu && lane == 0) bulk_wait_group0();
-  } else if (fewer_registers<56>(), warp == 0) {
+  } else if (fewer_registers<32>(), warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
     Item next = item(first);
