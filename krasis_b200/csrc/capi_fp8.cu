@@ -10,8 +10,6 @@ namespace kb2 {
 cudaError_t launch_binning(const int* ids, const float* wts, int M, int top_k, int e_start, int e_end, int chunk_tokens, int* counts, int* offsets, int* cursor,
                            ChunkDesc* chunks, int* n_chunks, float* sorted_w, int* slot_of, int* sorted_ids, int* sorted_tok, const void* x, void* x_sorted, int H,
                            cudaStream_t s);
-cudaError_t launch_fp8_gather(const void* codes, const float* scales, long long lds, const int* token_of, const int* slots, int max_slots, int K, void* out,
-                              float* out_scales, long long ldo, cudaStream_t s);
 cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s);
 }  // namespace kb2
 
@@ -66,7 +64,7 @@ KB2_API int kb2_fp8_quantize_rows(const void* x_dev, int32_t x_f32, int64_t ldx,
   if (off16(codes_dev) || ldx < 0 || ld_scales < M) return failf(KB2_ERR_VALUE, "fp8_quantize_rows: codes on 16 bytes, ldx >= 0, ld_scales >= M");
   OnDevice on(device);
   CUDA_TRY(on.err);
-  CUDA_TRY(launch_fp8_rows(x_dev, x_f32 != 0, ldx, M, K, codes_dev, scales_dev, ld_scales, (cudaStream_t)stream));
+  CUDA_TRY(launch_fp8_rows(x_dev, x_f32 != 0, ldx, M, K, codes_dev, scales_dev, ld_scales, nullptr, 0, (cudaStream_t)stream));
   return KB2_OK;
 }
 
@@ -119,24 +117,21 @@ KB2_API int kb2_fp8_linear(const void* x_dev, int32_t x_f32, int64_t ldx, const 
 
 // ---- routed experts
 struct ExpertsWork {
-  uint8_t *hc, *xc, *ac;
-  float *hs, *xs, *as, *sorted_w;
+  uint8_t *xc, *ac;
+  float *xs, *as, *sorted_w;
   void* y;
   ChunkDesc* chunks;
   int *n_chunks, *counts, *offsets, *cursor, *slot_of, *token_of;
   int max_chunks;
-  long long ldh, ldx;
+  long long ldx;
   size_t bytes;
 };
 static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F, bool out_f32) {
   ExpertsWork k{};
   Carve c(work);
   const size_t slots = (size_t)T * top;
-  k.ldh = scale_ld(T);
   k.ldx = scale_ld((long long)slots);
   k.max_chunks = (int)std::min<size_t>(slots, slots / kFp8Run + E);
-  k.hc = c.take<uint8_t>((size_t)T * W);
-  k.hs = c.take<float>((size_t)k.ldh * fp8_blocks(W));
   k.xc = c.take<uint8_t>(slots * W);
   k.xs = c.take<float>((size_t)k.ldx * fp8_blocks(W));
   k.ac = c.take<uint8_t>(slots * F);
@@ -179,10 +174,9 @@ KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const
   CUDA_TRY(on.err);
   cudaStream_t s = (cudaStream_t)stream;
   const int slots = T * top;
-  CUDA_TRY(launch_binning(ids_dev, weights_dev, T, top, 0, E, kFp8Run, k.counts, k.offsets, k.cursor, k.chunks, k.n_chunks, k.sorted_w, k.slot_of, nullptr, k.token_of,
-                          nullptr, nullptr, 0, s));
-  CUDA_TRY(launch_fp8_rows(h_dev, h_f32 != 0, ldh, T, W, k.hc, k.hs, k.ldh, s));
-  CUDA_TRY(launch_fp8_gather(k.hc, k.hs, k.ldh, k.token_of, k.offsets + E, slots, W, k.xc, k.xs, k.ldx, s));
+  CUDA_TRY(launch_binning(ids_dev, weights_dev, T, top, 0, E, kFp8Run, k.counts, k.offsets, k.cursor, k.chunks, k.n_chunks, k.sorted_w, k.slot_of, nullptr, k.token_of, nullptr, nullptr,
+                          0, s));
+  CUDA_TRY(launch_fp8_rows(h_dev, h_f32 != 0, ldh, T, W, k.xc, k.xs, k.ldx, k.slot_of, top, s));      // in the experts' order
   Fp8Product p;
   p.x = k.xc; p.xs = k.xs; p.ldxs = k.ldx; p.w = w1_dev; p.ws = s1_dev; p.out = k.ac;
   p.M = slots; p.N = 2 * F; p.K = W; p.groups = E;
@@ -190,7 +184,7 @@ KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const
   CUDA_TRY(launch_fp8_gated(p, k.as, k.ldx, current_sms(), s));
   p.x = k.ac; p.xs = k.as; p.w = w2_dev; p.ws = s2_dev; p.out = k.y; p.out_f32 = out_f32 != 0;
   p.N = W; p.K = F;
-  CUDA_TRY(launch_fp8_product(p, current_sms(), s));
+  CUDA_TRY(launch_fp8_tiles(p, 1, current_sms(), s));
   CUDA_TRY(launch_fp8_combine(k.y, out_f32 != 0, k.slot_of, weights_dev, T, top, W, out_dev, s));
   return KB2_OK;
 }

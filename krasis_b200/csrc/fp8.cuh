@@ -11,11 +11,12 @@
 #include <cstdint>
 
 #include "moe_common.cuh"
+#include "ptx.cuh"
 
 namespace kb2 {
 
 constexpr int kFp8Block = 128;
-constexpr int kFp8Run = 256;      // the most rows of a run
+constexpr int kFp8Run = 128;      // the most rows of a run
 __host__ __device__ constexpr int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 
 // What the bits of a block's largest magnitude say: its scale, and the reciprocal that numbers are multiplied by (0 where the codes are zeros).
@@ -41,6 +42,18 @@ __device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float 
   return inv == 0.f ? 0u : lo | hi << 16;
 }
 
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+// c += a b for two numbers at once, where it stands among loads and waits
+__device__ __forceinline__ void fma2_here(uint64_t& c, uint64_t a, uint64_t b) { asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b)); }
 // out[m] = sum over the blocks of scales x codes of row m times those of w, per matrix of `groups` ones.  x [.][K] codes with scales xs[b * ldxs + row],
 // w [groups][N][K] with scales ws [groups][blocks of N][blocks of K].
 struct Fp8Product {
@@ -60,10 +73,16 @@ struct Fp8Product {
   int max_chunks = 0;
 };
 
-cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K, void* codes, float* scales, long long ld_scales, cudaStream_t s);
+// Rows of activations.  With slot_of [M][top] a row goes to each of its slots (negative: none) instead of its own place, codes and scales.
+cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K, void* codes, float* scales, long long ld_scales, const int* slot_of, int top, cudaStream_t s);
 cudaError_t launch_fp8_blocks(const void* w, bool f32, int groups, int N, int K, void* codes, float* scales, cudaStream_t s);
-cudaError_t launch_fp8_product(const Fp8Product& p, int num_sms, cudaStream_t s);
-// Runs of rows times matrices [gate: N / 2 | up: N / 2]: silu(gate) up in fp32, quantised by rows: codes [M][N / 2] in p.out, out_scales[b * ld + row].  N % 256 == 0.
+// One matrix, all M rows, on pairs of CTAs with tiles of 256 x 256.
+cudaError_t launch_fp8_pairs(const Fp8Product& p, int num_sms, cudaStream_t s);
+// Runs (one matrix: tiles of kFp8Run rows) on single CTAs; split: CTAs that share a tile of one matrix along K.
+cudaError_t launch_fp8_tiles(const Fp8Product& p, int split, int num_sms, cudaStream_t s);
+// Runs times matrices [gate: N / 2 | up: N / 2]: silu(gate) up in fp32, quantised by rows: codes [M][N / 2] in p.out, out_scales[b * ld + row].  N % 256 == 0.
 cudaError_t launch_fp8_gated(const Fp8Product& p, float* out_scales, long long ld_out_scales, int num_sms, cudaStream_t s);
+// One matrix, whichever of the two is estimated to be faster.
+cudaError_t launch_fp8_product(const Fp8Product& p, int num_sms, cudaStream_t s);
 
 }  // namespace kb2

@@ -3,28 +3,15 @@
 // The tensor cores' accumulators cannot be rescaled on the way, so each block of 128 products per result is a sum of its own in tensor memory (two of them in turn),
 // which the other warps multiply by its scales and add up in registers while the next one runs.
 #include <cuda.h>
+#include <cstdlib>
 
 #include "fp8.cuh"
 #include "prof.cuh"
 #include "ptx.cuh"
-#include "seq_act.cuh"
 
 namespace kb2 {
 
-template <int N>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-// c += a b for two numbers at once, where it stands among loads and waits
-__device__ __forceinline__ void fma2_here(uint64_t& c, uint64_t a, uint64_t b) { asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b)); }
 cudaError_t make_tmap_u8_rows(void* out_tmap, const void* base, long long rows, long long cols, int box_rows);
-cudaError_t make_tmap_u8_gate_up(void* out_tmap, const void* base, long long groups, long long F, long long cols);
 
 // ---- many rows: pairs of CTAs, 256 rows of x x 256 weight rows
 // A CTA has 128 rows of x (the M side) and half the weight rows, 32 KB for 512 cycles of MMAs per block of K.  Sixteen warps hold the tile's sums, 64 a thread: a thread has one
@@ -32,32 +19,26 @@ cudaError_t make_tmap_u8_gate_up(void* out_tmap, const void* base, long long gro
 // broadcast loads per block beside the MMAs' own reads, and a block took 1070 cycles of eight warps (M 8192, N 4096, K 4096: 150 us).
 constexpr int kFRows = 128, kFBox = 32, kFABytes = kFRows * 128, kFStage = 2 * kFABytes;
 constexpr int kFThreads = 640, kFWarps = 16;
-// The scales of kFGroup blocks are handed over at once, two groups are at hand: products for each row, for the first and the second 128 columns (gated: gate's, up's).
+// The scales of kFGroup blocks are handed over at once, two groups are at hand: products for each row, for the first and the second 128 columns.
 constexpr int kFGroup = 4, kFScales = 2 * kFGroup;
 constexpr int kFOut = 32 * 128;                    // a warp's results on their way out
-constexpr int kFMostStages = 6;
-__host__ __device__ constexpr int pair_stages(bool glu) { return glu ? 6 : 4; }     // gated units have nothing on its way out in shared memory
-constexpr int kFOffOut = 4 * kFStage, kFOffScale = 6 * kFStage, kFOffMax = kFOffScale + kFScales * 2 * kFRows * 4, kFOffBar = kFOffMax + 2 * 4 * kFRows * 4, kFUsed = kFOffBar + 512,
+constexpr int kFStages = 4, kFTile = 2 * kFRows;
+constexpr int kFOffOut = kFStages * kFStage, kFOffScale = kFOffOut + kFWarps * kFOut, kFOffBar = kFOffScale + kFScales * 2 * kFRows * 4, kFUsed = kFOffBar + 512,
               kFSmem = kFUsed > 512 * 430 - 1024 ? kFUsed : 512 * 430 - 1024;
-static_assert(kFOffOut + kFWarps * kFOut <= kFOffScale && kFSmem <= 227 * 1024, "what a CTA of a cluster takes for 512 columns (tmem_smem)");
-static_assert(kFp8Run == 2 * kFRows, "a run is one tile's rows");
+static_assert(kFSmem <= 227 * 1024, "what a CTA of a cluster takes for 512 columns (tmem_smem)");
 
 struct PairArgs {
   Fp8Product p;
-  int w_tiles;                                     // tiles of 256 weight rows (gated: 128 of either half)
-  // gated units: out is codes [M][N / 2] with scales
-  float* out_scales;
-  long long ld_out_scales;
+  int w_tiles;                                     // tiles of 256 weight rows
 };
 
-template <bool kGlu, bool kOutF32>
+template <bool kOutF32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_out, const PairArgs a) {
-  constexpr int kFStages = pair_stages(kGlu);
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFOffBar);       // of the first CTA: both CTAs' loads
-  uint64_t* empty = full + kFMostStages;
-  uint64_t* acc_full = empty + kFMostStages;       // [2]
+  uint64_t* empty = full + kFStages;
+  uint64_t* acc_full = empty + kFStages;       // [2]
   uint64_t* acc_empty = acc_full + 2;              // [2], of the first CTA: both CTAs' read-outs
   uint64_t* s_full = acc_empty + 2;                // [2]
   uint64_t* s_empty = s_full + 2;
@@ -91,26 +72,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_ptr_smem;
   pdl_wait();
-  const int nb = fp8_blocks(p.K), units = p.chunks ? p.n_chunks[0] : (p.M + kFp8Run - 1) / kFp8Run, total = units * a.w_tiles;
+  const int nb = fp8_blocks(p.K), total = (p.M + kFTile - 1) / kFTile * a.w_tiles;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
   struct Item {
-    int row0, rows, group, wt;
+    int row0, rows, wt;
   };
-  // weight tiles first, so that pairs that run at once share the rows of x.  Everyone asks for the next item when it starts on one.
+  // weight tiles first, so that pairs that run at once share the rows of x
   const auto item = [&](int t) {
     Item i;
     const int u = t / a.w_tiles;
     i.wt = t - u * a.w_tiles;
-    if (p.chunks) {
-      const int4 c = t < total ? *reinterpret_cast<const int4*>(p.chunks + u) : make_int4(0, 0, 0, 0);
-      i.row0 = c.y;
-      i.rows = c.z;
-      i.group = c.x;
-    } else {
-      i.row0 = u * kFp8Run;
-      i.rows = t < total ? min(kFp8Run, p.M - i.row0) : 0;
-      i.group = 0;
-    }
+    i.row0 = u * kFTile;
+    i.rows = min(kFTile, p.M - i.row0);
     return i;
   };
 
@@ -119,11 +92,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
     const int q = warp & 3, h = (warp - 4) >> 2, row = rank * kFRows + q * 32 + lane;     // of the tile
     const uint32_t from = tmem_base + ((uint32_t)(q * 32) << 16) + h * 64;
     int b = 0;
-    uint32_t aphase = 0, slot = 0, sphase = 0, tile = 0;
-    Item next = item(first);
-    for (int t = first; t < total; t += step, ++tile) {
-      const Item i = next;
-      next = item(t + step);
+    uint32_t aphase = 0, slot = 0, sphase = 0;
+    for (int t = first; t < total; t += step) {
+      const Item i = item(t);
       const bool mine = __any_sync(0xffffffffu, row < i.rows);
       uint64_t acc[32];                            // two columns in each
 #pragma unroll
@@ -131,8 +102,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
       for (int kb = 0; kb < nb; ++kb) {
         if ((slot & (kFGroup - 1)) == 0) mbar_wait(&s_full[slot / kFGroup], sphase);
         const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + kFOffScale) + slot * 2 * kFRows + q * 32 + lane;
-        const uint32_t s0 = sc[kGlu ? 0 : (h >> 1) * kFRows], s1 = kGlu ? sc[kFRows] : s0;
-        const uint64_t two0 = pack2(s0, s0), two1 = pack2(s1, s1);
+        const uint32_t s0 = sc[(h >> 1) * kFRows];
+        const uint64_t two = pack2(s0, s0);
         mbar_wait(&acc_full[b], aphase);
         tc_fence_after_sync();
         const auto read = [&]() {                  // this block's sums are in registers
@@ -148,7 +119,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
             tmem_ld_wait();
             if (c) read();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) fma2_here(acc[c * 16 + j], pack2(v[2 * j], v[2 * j + 1]), c ? two1 : two0);
+            for (int j = 0; j < 16; ++j) fma2_here(acc[c * 16 + j], pack2(v[2 * j], v[2 * j + 1]), two);
           }
         } else {
           read();
@@ -161,40 +132,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
         b ^= 1;
         aphase ^= b == 0;
       }
-      const long long at = i.row0 + row;
-      if constexpr (kGlu) {
-        // columns 0 to 31 are gate, the others up of units 32 h on of the tile's 128
-        uint32_t* most = reinterpret_cast<uint32_t*>(smem + kFOffMax) + (tile & 1) * 4 * kFRows + q * 32 + lane;
-        uint32_t m = 0;
-        if (mine) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float g0, g1, u0, u1;
-            unpack2(acc[j], g0, g1);
-            unpack2(acc[16 + j], u0, u1);
-            const uint32_t v0 = __float_as_uint(kb2act::silu(g0) * u0), v1 = __float_as_uint(kb2act::silu(g1) * u1);
-            acc[j] = pack2(v0, v1);
-            m = max(m, max(v0 & 0x7FFFFFFFu, v1 & 0x7FFFFFFFu));
-          }
-        }
-        most[h * kFRows] = m;
-        named_bar_sync(1, 32 * kFWarps);           // the tile after next writes here again, behind the next one's barrier
-        if (row < i.rows) {
-          const Fp8Scale f = fp8_scale(max(max(most[0], most[kFRows]), max(most[2 * kFRows], most[3 * kFRows])));
-          if (h == 0) a.out_scales[i.wt * a.ld_out_scales + at] = f.scale;
-          uint32_t w[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float v0, v1, v2, v3;
-            unpack2(acc[2 * j], v0, v1);
-            unpack2(acc[2 * j + 1], v2, v3);
-            w[j] = fp8_codes4(v0, v1, v2, v3, f.inv);
-          }
-          uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + at * (p.N / 2) + i.wt * 128 + h * 32);
-          to[0] = make_uint4(w[0], w[1], w[2], w[3]);
-          to[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        }
-      } else if (mine) {
+      if (mine) {
         // 32 rows x 128 bytes at a time go out from shared memory by one copy, while the next tile's blocks are added: all SMs end their tiles at the same time, and a tile's
         // stores by the lanes took 3500 cycles (16 bytes of a row by each lane, row by row, 12000).  A run's last rows, and rows that are not on 16 bytes, are the lanes'.
         constexpr int kCols = kOutF32 ? 32 : 64, kVec = kOutF32 ? 4 : 8;
@@ -250,14 +188,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
         }
       }
     }
-    if (!kGlu && lane == 0) bulk_wait_group0();
+    if (lane == 0) bulk_wait_group0();
   } else if (fewer_registers<32>(), warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
-    Item next = item(first);
     for (int t = first; t < total; t += step) {
-      const Item i = next;
-      next = item(t + step);
+      const Item i = item(t);
       // boxes of rows that are there; what lies behind them in a stage is multiplied, too, and looked at by nobody
       const int boxes0 = (min(i.rows, kFRows) + kFBox - 1) / kFBox, boxes1 = (max(i.rows - kFRows, 0) + kFBox - 1) / kFBox, boxes = rank ? boxes1 : boxes0;
       const uint32_t bytes = 2 * kFABytes + (boxes0 + boxes1) * kFBox * 128;
@@ -267,8 +203,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
         if (elect_one()) {
           const uint32_t bar = cluster_addr(&full[stage], 0);
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
-          if constexpr (kGlu) tma_load_5d_pair(at + kFABytes, &tmap_w, kb * 128, 0, 0, (i.wt * 128 + (int)rank * 64) / 32, i.group, bar);
-          else tma_load_2d_pair(at + kFABytes, &tmap_w, kb * 128, i.group * p.N + i.wt * 256 + rank * 128, bar);
+          tma_load_2d_pair(at + kFABytes, &tmap_w, kb * 128, i.wt * 256 + rank * 128, bar);
           for (int r = 0; r < boxes; ++r) tma_load_2d_pair(at + r * kFBox * 128, &tmap_x, kb * 128, i.row0 + rank * kFRows + r * kFBox, bar);
         }
         __syncwarp();
@@ -318,17 +253,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
     settle();
     Item i = item(t);
     const auto ask = [&](Scales& s) {
-      const int n = kGlu ? i.wt : i.wt * 2, n1 = kGlu ? i.wt + w_blocks / 2 : min(n + 1, w_blocks - 1);
-      const float *w = p.ws + (long long)i.group * w_blocks * nb + kb, *x = p.xs + kb * p.ldxs + i.row0;
+      const int n = i.wt * 2, n1 = min(n + 1, w_blocks - 1);
+      const float *w = p.ws + kb, *x = p.xs + kb * p.ldxs + i.row0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = rank * kFRows + j * 32 + lane;
         s.x[j] = row < i.rows ? x[row] : 0.f;
       }
-      if (i.rows > 0) {
-        s.w[0] = w[(long long)n * nb];
-        s.w[1] = w[(long long)n1 * nb];
-      }
+      s.w[0] = w[(long long)n * nb];
+      s.w[1] = w[(long long)n1 * nb];
       const int was = t;
       kb += 2;
       settle();
@@ -371,32 +304,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
   if (warp == 0) tmem_dealloc_pair(tmem_base, 512);
 }
 
-template <bool kGlu, bool kOutF32>
-static cudaError_t launch_pair(const PairArgs& a, int num_sms, cudaStream_t s) {
-  const Fp8Product& p = a.p;
+template <bool kOutF32>
+static cudaError_t launch_pair(const Fp8Product& p, int num_sms, cudaStream_t s) {
+  const PairArgs a{p, (p.N + 255) / 256};
+  const int wide = kOutF32 ? 4 : 2;
   alignas(64) CUtensorMap tx, tw, to;
   cudaError_t e = make_tmap_u8_rows(&tx, p.x, p.M, p.K, kFBox);
-  if (e == cudaSuccess) e = kGlu ? make_tmap_u8_gate_up(&tw, p.w, p.groups, p.N / 2, p.K) : make_tmap_u8_rows(&tw, p.w, (long long)p.groups * p.N, p.K, kFRows);
+  if (e == cudaSuccess) e = make_tmap_u8_rows(&tw, p.w, p.N, p.K, kFRows);
   to = tw;
-  const int wide = kOutF32 ? 4 : 2;
-  if (e == cudaSuccess && !kGlu && p.N * (long long)wide % 16 == 0) e = make_tmap_u8_rows(&to, p.out, p.M, (long long)p.N * wide, 32);      // as bytes
-  if (e == cudaSuccess) e = allow_smem<fp8_pair_kernel<kGlu, kOutF32>>(kFSmem);
+  if (e == cudaSuccess && p.N * (long long)wide % 16 == 0) e = make_tmap_u8_rows(&to, p.out, p.M, (long long)p.N * wide, 32);      // as bytes
+  if (e == cudaSuccess) e = allow_smem<fp8_pair_kernel<kOutF32>>(kFSmem);
   if (e != cudaSuccess) return e;
-  const long long total = (long long)a.w_tiles * (p.chunks ? p.max_chunks : (p.M + kFp8Run - 1) / kFp8Run);
+  const long long total = (long long)a.w_tiles * ((p.M + kFTile - 1) / kFTile);
   const int pairs = (int)(total < num_sms / 2 ? total : num_sms / 2);
-  return launch_pdl(fp8_pair_kernel<kGlu, kOutF32>, 2 * pairs, kFThreads, kFSmem, s, tx, tw, to, a);
+  return launch_pdl(fp8_pair_kernel<kOutF32>, 2 * pairs, kFThreads, kFSmem, s, tx, tw, to, a);
+}
+
+cudaError_t launch_fp8_pairs(const Fp8Product& p, int num_sms, cudaStream_t s) {
+  KernelSpan ks(K_FP8_PRODUCT, s);
+  return p.out_f32 ? launch_pair<true>(p, num_sms, s) : launch_pair<false>(p, num_sms, s);
 }
 
 cudaError_t launch_fp8_product(const Fp8Product& p, int num_sms, cudaStream_t s) {
-  KernelSpan ks(K_FP8_PRODUCT, s);
-  const PairArgs a{p, (p.N + 255) / 256, nullptr, 0};
-  return p.out_f32 ? launch_pair<false, true>(a, num_sms, s) : launch_pair<false, false>(a, num_sms, s);
-}
-
-cudaError_t launch_fp8_gated(const Fp8Product& p, float* out_scales, long long ld_out_scales, int num_sms, cudaStream_t s) {
-  KernelSpan ks(K_FP8_PRODUCT, s);
-  const PairArgs a{p, p.N / 256, out_scales, ld_out_scales};
-  return launch_pair<true, false>(a, num_sms, s);
+  if (const char* f = getenv("KB2_DSPLIT")) return atoi(f) ? launch_fp8_tiles(p, atoi(f), num_sms, s) : launch_fp8_pairs(p, num_sms, s);
+  return launch_fp8_pairs(p, num_sms, s);
 }
 
 }  // namespace kb2

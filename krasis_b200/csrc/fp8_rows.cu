@@ -46,17 +46,17 @@ struct Eight {
       return max(a << 16, a & 0xFFFF0000u);
     }
   }
-  // K is a multiple of 16 and the codes lie on 16 bytes: eight of them are there whole or not at all.
-  __device__ __forceinline__ void store(void* codes, long long at, float inv) const {
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(codes) + at) =
-        make_uint2(fp8_codes4(number(0), number(1), number(2), number(3), inv), fp8_codes4(number(4), number(5), number(6), number(7), inv));
+  __device__ __forceinline__ uint2 codes(float inv) const {
+    return make_uint2(fp8_codes4(number(0), number(1), number(2), number(3), inv), fp8_codes4(number(4), number(5), number(6), number(7), inv));
   }
+  // K is a multiple of 16 and the codes lie on 16 bytes: eight of them are there whole or not at all.
+  __device__ __forceinline__ void store(void* to, long long at, float inv) const { *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(to) + at) = codes(inv); }
 };
 
 // Sixteen lanes have a block of 128, eight numbers each; a thread block has 16 rows x kRowsAhead blocks, all of a thread's loads on their way at once.
 constexpr int kRowsAhead = 4;
 template <bool F32, bool VEC>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const void* x, long long ldx, int M, int K, void* codes, float* scales, long long lds) {
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const void* x, long long ldx, int M, int K, void* codes, float* scales, long long lds, const int* slot_of, int top) {
   pdl_wait();
   const int lane = threadIdx.x & 15, m = blockIdx.x * 16 + (threadIdx.x >> 4), b0 = blockIdx.y * kRowsAhead;
   Eight<F32> v[kRowsAhead];
@@ -73,8 +73,18 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(const void* x, long long 
     for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
     const Fp8Scale s = fp8_scale(a);
     if (m >= M || (b0 + i) * kFp8Block >= K) continue;
-    if (k < K) v[i].store(codes, (long long)m * K + k, s.inv);
-    if (lane == 0) scales[(b0 + i) * lds + m] = s.scale;
+    if (slot_of == nullptr) {
+      if (k < K) v[i].store(codes, (long long)m * K + k, s.inv);
+      if (lane == 0) scales[(b0 + i) * lds + m] = s.scale;
+    } else {
+      const uint2 c = v[i].codes(s.inv);
+      for (int j = 0; j < top; ++j) {
+        const int slot = slot_of[(long long)m * top + j];
+        if (slot < 0) continue;
+        if (k < K) *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(codes) + (long long)slot * K + k) = c;
+        if (lane == 0) scales[(b0 + i) * lds + slot] = s.scale;
+      }
+    }
   }
 }
 
@@ -111,11 +121,12 @@ __global__ void __launch_bounds__(256) fp8_blocks_kernel(const void* w, int N, i
 
 static bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K, void* codes, float* scales, long long ld_scales, cudaStream_t s) {
+cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K, void* codes, float* scales, long long ld_scales, const int* slot_of, int top,
+                            cudaStream_t s) {
   KernelSpan ks(K_FP8_QUANTIZE, s);
   const dim3 grid((M + 15) / 16, (fp8_blocks(K) + kRowsAhead - 1) / kRowsAhead);
   const bool vec = on16(x) && ldx % (f32 ? 4 : 8) == 0;
-  const auto go = [&](auto kernel) { return launch_pdl(kernel, grid, 256, 0, s, x, ldx, M, K, codes, scales, ld_scales); };
+  const auto go = [&](auto kernel) { return launch_pdl(kernel, grid, 256, 0, s, x, ldx, M, K, codes, scales, ld_scales, slot_of, top); };
   return f32 ? vec ? go(fp8_rows_kernel<true, true>) : go(fp8_rows_kernel<true, false>) : vec ? go(fp8_rows_kernel<false, true>) : go(fp8_rows_kernel<false, false>);
 }
 

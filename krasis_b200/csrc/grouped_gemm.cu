@@ -681,20 +681,6 @@ cudaError_t make_tmap_u8_rows(void* out_tmap, const void* base, long long rows, 
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// [groups][gate: F rows | up: F rows][K] 8-bit matrices, box = 64 rows of each, 32 of gate and 32 of up in turn, x 128 columns, 128 B swizzle.  Coordinates: column, 0, 0,
-// row of gate / 32, group.  F % 64 == 0.
-cudaError_t make_tmap_u8_gate_up(void* out_tmap, const void* base, long long groups, long long F, long long cols) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (!fn) return cudaErrorNotSupported;
-  cuuint64_t gdim[5] = {(cuuint64_t)cols, 32, 2, (cuuint64_t)F / 32, (cuuint64_t)groups};
-  cuuint64_t gstride[4] = {(cuuint64_t)cols, (cuuint64_t)(F * cols), (cuuint64_t)(32 * cols), (cuuint64_t)(2 * F * cols)};
-  cuuint32_t box[5] = {128u, 32, 2, 2, 1};
-  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  CUresult r = fn(reinterpret_cast<CUtensorMap*>(out_tmap), CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(base), gdim, gstride, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
 int gemm_b_box_rows() { return kBBoxRows; }
 
 // rows x cols BF16 row-major matrix for TMA gather4: box = 1 row x 64 columns, 128 B swizzle

@@ -299,13 +299,6 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst_smem, const void* tma
       "l"(tmap), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_5d_pair(void* dst_smem, const void* tmap, int c0, int c1, int c2, int c3, int c4, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(
-          smem_u32(dst_smem)),
-      "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
-      : "memory");
-}
 // M = 256: rows 0..127 of A and of the accumulator belong to the pair's first CTA, the others to its second; each CTA holds half the rows of B.
 // Issued by the first CTA; the descriptors name the same places in both.
 __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
