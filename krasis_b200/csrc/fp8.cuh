@@ -80,6 +80,8 @@ cudaError_t launch_fp8_blocks(const void* w, bool f32, int groups, int N, int K,
 cudaError_t launch_fp8_pairs(const Fp8Product& p, int num_sms, cudaStream_t s);
 // Runs (one matrix: tiles of kFp8Run rows) on single CTAs; split: CTAs that share a tile of one matrix along K.
 cudaError_t launch_fp8_tiles(const Fp8Product& p, int split, int num_sms, cudaStream_t s);
+// How many clusters of so many (1, 2, 4, 8) CTAs there can be at once.
+int fp8_clusters(int split);
 // Runs times matrices [gate: N / 2 | up: N / 2]: silu(gate) up in fp32, quantised by rows: codes [M][N / 2] in p.out, out_scales[b * ld + row].  N % 256 == 0.
 cudaError_t launch_fp8_gated(const Fp8Product& p, float* out_scales, long long ld_out_scales, int num_sms, cudaStream_t s);
 // One matrix, whichever of the two is estimated to be faster.

@@ -3,7 +3,6 @@
 // The tensor cores' accumulators cannot be rescaled on the way, so each block of 128 products per result is a sum of its own in tensor memory (two of them in turn),
 // which the other warps multiply by its scales and add up in registers while the next one runs.
 #include <cuda.h>
-#include <cstdlib>
 
 #include "fp8.cuh"
 #include "prof.cuh"
@@ -175,6 +174,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
             const long long to = (long long)(row0 + r) * p.N + n;
             if (on16) {
               *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + to * (16 / kVec)) = x;
+            } else if (p.N % (kVec / 2) == 0) {
+              uint2* at = reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.out) + to * (16 / kVec));
+              at[0] = make_uint2(x.x, x.y);
+              if (n + kVec / 2 < p.N) at[1] = make_uint2(x.z, x.w);
             } else {
               const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -325,9 +328,25 @@ cudaError_t launch_fp8_pairs(const Fp8Product& p, int num_sms, cudaStream_t s) {
   return p.out_f32 ? launch_pair<true>(p, num_sms, s) : launch_pair<false>(p, num_sms, s);
 }
 
+// Which kernel, by estimates fitted to times of 7 matrices (N 1024 to 16384, K 512 to 8192) with 4 to 4200 rows, us beside what all forms share: a round of tiles takes 0.39 a block of K on
+// pairs of CTAs and 0.43 on single ones (half as large), and 1.0 / 0.7 for its ends; a cluster's joining its sums 3 and 0.02 a row.  us in all on both sides of the lines: N 2048, K 8192,
+// M 4200 pairs 63.6 / tiles 69.7, N 16384, K 1024, M 520 24.6 / 22.6, N 7168, K 4096, M 520 36.9 / 26.7; N 2048, K 8192, M 333 tiles 36.9, two along K 28.7, four 22.7; N 1024, K 2048,
+// M 100 16.4 / 16.4 / 15.2.
 cudaError_t launch_fp8_product(const Fp8Product& p, int num_sms, cudaStream_t s) {
-  if (const char* f = getenv("KB2_DSPLIT")) return atoi(f) ? launch_fp8_tiles(p, atoi(f), num_sms, s) : launch_fp8_pairs(p, num_sms, s);
-  return launch_fp8_pairs(p, num_sms, s);
+  const int nb = fp8_blocks(p.K);
+  const long long w_tiles = (p.N + 255) / 256, tiles = w_tiles * ((p.M + kFp8Run - 1) / kFp8Run), pairs = w_tiles * ((p.M + kFTile - 1) / kFTile);
+  const auto rounds = [](long long n, int at_once) { return (float)((n + at_once - 1) / at_once); };
+  float least = rounds(pairs, num_sms / 2) * (nb * 0.39f + 1.f);
+  int split = 0;
+  for (int n = 1; n <= 8 && n <= nb; n *= 2) {
+    if (n > 1 && tiles > fp8_clusters(n)) break;             // a cluster's CTAs that have to wait for SMs are another round
+    const float time = rounds(tiles, n > 1 ? (int)tiles : num_sms) * ((float)((nb + n - 1) / n) * 0.43f + 0.7f) + (n > 1 ? 3.f + 0.02f * (p.M < kFp8Run ? p.M : kFp8Run) : 0.f);
+    if (time < least) {
+      least = time;
+      split = n;
+    }
+  }
+  return split ? launch_fp8_tiles(p, split, num_sms, s) : launch_fp8_pairs(p, num_sms, s);
 }
 
 }  // namespace kb2

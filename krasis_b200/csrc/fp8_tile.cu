@@ -8,6 +8,8 @@
 // Steps of few tokens, where tiles are fewer than SMs: a cluster shares a tile along K, and its CTAs' sums meet in shared memory, added in the order of the ranks.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "fp8.cuh"
 #include "prof.cuh"
 
@@ -240,6 +242,10 @@ __global__ void __launch_bounds__(kTThreads, 1)
             const long long to = (long long)(row0 + r) * p.N + n;
             if (on16) {
               *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + to * (16 / kVec)) = x;
+            } else if (p.N % (kVec / 2) == 0) {
+              uint2* at = reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.out) + to * (16 / kVec));
+              at[0] = make_uint2(x.x, x.y);
+              if (n + kVec / 2 < p.N) at[1] = make_uint2(x.z, x.w);
             } else {
               const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -434,6 +440,32 @@ static cudaError_t launch_tile(const TileArgs& a, int num_sms, cudaStream_t s) {
   const long long total = (long long)a.w_tiles * (p.chunks ? p.max_chunks : (p.M + kTRows - 1) / kTRows);
   const unsigned grid = kSplit ? (unsigned)(total * a.split) : (unsigned)(total < num_sms ? total : num_sms);
   return launch_pdl_clusters(fp8_tile_kernel<kGlu, kOutF32, kSplit>, grid, kTThreads, kTSmem, s, dim3(kSplit ? a.split : 1, 1, 1), tx, tw, to, a);
+}
+
+int fp8_clusters(int split) {
+  static std::atomic<int> known[64][4];            // by device, for clusters of 1, 2, 4 and 8
+  int dev = 0, n = 0, at = 0;
+  while ((2 << at) <= split) ++at;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if ((n = known[dev][at].load(std::memory_order_relaxed)) > 0) return n;
+  const auto kernel = fp8_tile_kernel<false, false, true>;
+  if (allow_smem<fp8_tile_kernel<false, false, true>>(kTSmem) != cudaSuccess) return 0;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = split;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(split);
+  cfg.blockDim = dim3(kTThreads);
+  cfg.dynamicSmemBytes = kTSmem;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 0;
+  }
+  known[dev][at].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 cudaError_t launch_fp8_tiles(const Fp8Product& p, int split, int num_sms, cudaStream_t s) {
