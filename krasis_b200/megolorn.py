@@ -120,13 +120,14 @@ class MegolornModel:
     architecture = "Megolorn"
     page_size = 64
 
-    def __init__(self, cfg: MegolornConfig, weights: dict, dtype=torch.bfloat16, device=0):
+    def __init__(self, cfg: MegolornConfig, weights: dict, dtype=torch.bfloat16, device=0, expert_format=None):
+        """expert_format "e4m3": routed experts held in 8 bits (see RoutedExperts)."""
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("dtype: bfloat16 or float32")
         if not torch.cuda.is_available():
             raise RuntimeError("MegolornModel needs a CUDA device (krasis_b200 has no CPU path)")
         ops.load()
-        self.cfg, self.dtype = cfg, dtype
+        self.cfg, self.dtype, self.expert_format = cfg, dtype, expert_format
         self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         dev, eps = self.device, cfg.eps
         d = lambda t: t.to(device=dev, dtype=dtype).contiguous()
@@ -154,15 +155,15 @@ class MegolornModel:
                 rt = mlp["router"]
                 grp = rt.get("groups") or {}
                 lay["mlp"] = RoutedExperts(_sub(weights, p + "mlp."), rt["experts"], rt.get("identity", 0), rt["top"], dtype, dev,
-                                           groups=grp.get("count", 1), keep=grp.get("keep", 1))
+                                           groups=grp.get("count", 1), keep=grp.get("keep", 1), expert_format=expert_format)
             self.layers.append(lay)
 
     # ------------------------------------------------------------------------------------------- construction
     @classmethod
-    def from_pretrained(cls, model_dir: str, dtype=torch.bfloat16, device=0, **_):
+    def from_pretrained(cls, model_dir: str, dtype=torch.bfloat16, device=0, expert_format=None, **_):
         from . import loader
         cfg = MegolornConfig.from_dict(json.load(open(os.path.join(model_dir, "config.json"))))
-        return cls(cfg, loader.read_named_tensors(model_dir), dtype=dtype, device=device)
+        return cls(cfg, loader.read_named_tensors(model_dir), dtype=dtype, device=device, expert_format=expert_format)
 
     @classmethod
     def random(cls, cfg: MegolornConfig, seed: int = 0, dtype=torch.bfloat16, device=0):

@@ -976,11 +976,16 @@ class RoutedExperts:
     (divided by their sum if `renorm`, times out_scale).  The last `identity` outputs are identity experts: they return their input.
 
     weight_input: the weight multiplies the expert's input, out = sum expert(w h).  Gate and up products are linear in it, so the weight
-    joins the activation pass (gated experts, no identity experts)."""
+    joins the activation pass (gated experts, no identity experts).
+
+    expert_format "e4m3": the experts' matrices are held in 8 bits with a scale for each block of 128 x 128 and multiplied so
+    (layers.fp8_experts: silu-gated experts of W a multiple of 16 and F of 128, no identity experts, weights on the outputs); router and
+    shared expert stay as they are."""
 
     def __init__(self, weights: dict, experts: int, identity: int, top: int, dtype, device, groups: int = 1, keep: int = 1,
                  score: str = "softmax", renorm: bool = False, out_scale: float = 1.0, gated: bool = True, act: str = "silu",
-                 group_score: str = "max", limit: float = 0.0, alpha: float = 1.0, shared_limit=None, weight_input: bool = False):
+                 group_score: str = "max", limit: float = 0.0, alpha: float = 1.0, shared_limit=None, weight_input: bool = False,
+                 expert_format: str = None):
         d = lambda t: t.to(device=device, dtype=dtype).contiguous()
         self.E, self.ident, self.top, self.groups, self.keep = int(experts), int(identity), int(top), int(groups), int(keep)
         self.score, self.renorm, self.out_scale, self.dtype, self.device = score, bool(renorm), float(out_scale), dtype, device
@@ -992,6 +997,11 @@ class RoutedExperts:
             raise ValueError("weights on the experts' inputs: no identity experts")
         if score not in ops.ROUTE_SCORES:
             raise ValueError(f"router score {score!r}")
+        self.expert_format = expert_format
+        if expert_format not in (None, "e4m3"):
+            raise ValueError(f"expert format {expert_format!r}: None (as the other weights) or \"e4m3\"")
+        if expert_format and (act != "silu" or self.ident or self.weight_input or not self.E):
+            raise ValueError("experts in e4m3: silu-gated, no identity experts, weights on the outputs")
         self.act_kind, self.limit, self.alpha = GatedMLP.KINDS[act], float(limit), float(alpha)
         if weights["router"].shape[0] != self.E + self.ident:
             raise ValueError("router rows must equal experts + identity experts")
@@ -1012,9 +1022,18 @@ class RoutedExperts:
             raise ValueError("one router bias per router row")
         if self.E:
             first = (lambda i: torch.cat([weights[f"e{i}_gate"], weights[f"e{i}_up"]], 0)) if gated else (lambda i: weights[f"e{i}_up"])
-            self.w_gu = d(torch.stack([first(i) for i in range(self.E)], 0))                         # [E, 2F | F, W]
-            self.w_down = d(torch.stack([weights[f"e{i}_down"] for i in range(self.E)], 0))          # [E, W, F]
-            self.F = self.w_down.shape[2]
+            self.F = weights["e0_down"].shape[1]
+            if expert_format:
+                from . import layers
+                if self.F % layers.FP8_BLOCK or weights["e0_down"].shape[0] % 16:
+                    raise ValueError(f"experts in e4m3: inner width {self.F} a multiple of {layers.FP8_BLOCK}, width {weights['e0_down'].shape[0]} of 16")
+                q = lambda w: layers.quantize_fp8_blocks(w.to(device=device, dtype=torch.float32).contiguous())      # one matrix at a time
+                stack = lambda parts: (torch.stack([c.view(torch.uint8) for c, _ in parts]).view(torch.float8_e4m3fn), torch.stack([s for _, s in parts]))
+                self.w_gu, self.s_gu = stack([q(first(i)) for i in range(self.E)])
+                self.w_down, self.s_down = stack([q(weights[f"e{i}_down"]) for i in range(self.E)])
+            else:
+                self.w_gu = d(torch.stack([first(i) for i in range(self.E)], 0))                     # [E, 2F | F, W]
+                self.w_down = d(torch.stack([weights[f"e{i}_down"] for i in range(self.E)], 0))      # [E, W, F]
         self.shared = GatedMLP({k[len("shared_"):]: v for k, v in weights.items() if k.startswith("shared_") and k != "shared_sg"}, dtype,
                                device, act=act, gated=gated, limit=limit if shared_limit is None else shared_limit,
                                alpha=alpha) if "shared_up" in weights else None
@@ -1101,7 +1120,13 @@ class RoutedExperts:
         slots = T * top
         in_w, out_w = (wts, None) if self.weight_input else (None, wts)       # where the weights go: into the activation pass or the sum
         y = pos = None
-        if E and T <= self.gemv_max_tokens:
+        if self.expert_format:
+            from . import layers
+            y = layers.fp8_experts(h, ids, wts, self.w_gu, self.s_gu, self.w_down, self.s_down, out_dtype=torch.float32)
+            if self.shared is None:
+                return y
+            ids, top, out_w = torch.zeros(T, dtype=torch.int32, device=dev), 1, None       # the sum is one row a token, and joins the shared expert's
+        elif E and T <= self.gemv_max_tokens:
             F2 = self.w_gu.shape[1]
             gu = torch.empty((slots, F2), dtype=dt, device=dev)
             ops.check(lib.kb2_seq_moe_gemv(h.data_ptr(), ops.dt_code(h.dtype), h.stride(0), top, ids.data_ptr(), E, self.w_gu.data_ptr(), dtc, W,

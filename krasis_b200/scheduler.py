@@ -6,6 +6,7 @@ A model takes part by offering
 `Scheduler.step` runs one explicit step (entries given by the caller: a trace replay, a server loop); `Scheduler.generate`
 is the generation entry point that plans the steps itself: requests are admitted while state slots and pages are free, prompts
 are cut into portions under a per-step token budget, and every running request adds one decoded token to each step.
+`Scheduler.score` gives the log probabilities of a text's tokens.
 Pages (`SequenceKVState` over the model's paged cache) and state slots (`RecurrentStatePool`) go back at `finish` and are reused.
 """
 from bisect import bisect_right
@@ -154,8 +155,12 @@ class Scheduler:
 
     # ------------------------------------------------------------------------------------------- generation
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, sampling: Optional[SamplingParams] = None,
-                 step_tokens: int = 512, eos: Optional[int] = None) -> List[List[int]]:
-        """Greedy (or sampled) continuation of every prompt; returns the generated ids per prompt, in order."""
+                 step_tokens: int = 512, eos: Optional[int] = None, logprobs: Optional[int] = None):
+        """Greedy (or sampled) continuation of every prompt; returns the generated ids per prompt, in order.
+
+        logprobs (0 to 64): returns (ids, details) instead, details with a dict for each generated token: "logprob" and "entropy" of the model's distribution (ahead of
+        temperature and filters) and "top", that many of its most likely tokens as (id, log probability)."""
+        details: List[List[dict]] = [[] for _ in prompts]
         sampler = Sampler(sampling, self.model.device)
         waiting = deque(enumerate(prompts))
         running: List[Request] = []
@@ -187,8 +192,12 @@ class Scheduler:
                         sampled_from.append(req)
             logits = self.step(entries)
             if sampled_from:
-                toks = sampler(logits).tolist()
-                for req, tok in zip(sampled_from, toks):
+                drawn = sampler(logits)
+                toks = drawn.tolist()
+                said = self._say(logits, drawn, logprobs) if logprobs is not None else [None] * len(toks)
+                for req, tok, what in zip(sampled_from, toks, said):
+                    if what is not None:
+                        details[req.index].append(what)
                     req.output.append(tok)
                     req.pending = tok
                     if len(req.output) >= max_new_tokens or (eos is not None and tok == eos):
@@ -197,4 +206,31 @@ class Scheduler:
                         self.finish(req.id)
         if torch.cuda.is_available() and prompts:
             ops.check_waits(torch.device(self.model.device).index or 0)
-        return results
+        return results if logprobs is None else (results, details)
+
+    @staticmethod
+    def _say(logits, tokens, top: int) -> List[dict]:
+        r = ops.token_logprobs(logits, tokens, top)
+        numbers, ids = torch.cat([r.logprob[:, None], r.entropy[:, None], r.top_logprobs], 1).tolist(), r.top_ids.tolist()
+        return [{"logprob": n[0], "entropy": n[1], "top": list(zip(i, n[2:]))} for n, i in zip(numbers, ids)]
+
+    def score(self, texts: Sequence[Sequence[int]], step_tokens: int = 512) -> List[List[float]]:
+        """Log probability of every token of every text but its first, given those before it (a text's perplexity is exp of minus their mean).  A text runs in portions of
+        step_tokens; the logits of a portion are gone when the next one runs."""
+        scores = []
+        for i, text in enumerate(texts):
+            text, parts = [int(t) for t in text], []
+            if text and not self.can_admit(len(text)):
+                raise RuntimeError("a text does not fit the cache pool")
+            for a in range(0, len(text), step_tokens):
+                part = text[a:a + step_tokens]
+                told = text[a + 1:a + 1 + len(part)]             # what follows each of them; behind the last one of all, nothing
+                logits = self.step([(("score", i), part, list(range(len(told))))])
+                if told:
+                    parts.append(ops.token_logprobs(logits, torch.tensor(told, device=logits.device)).logprob)
+            if text:
+                self.finish(("score", i))
+            scores.append(torch.cat(parts).tolist() if parts else [])
+        if torch.cuda.is_available() and texts:
+            ops.check_waits(torch.device(self.model.device).index or 0)
+        return scores
