@@ -38,7 +38,7 @@ static long long scale_ld(long long rows) { return (rows + 3) & ~3ll; }
 
 static int check_sizes(const char* what, long long M, long long N, long long K) {
   if (M < 0 || N <= 0 || K <= 0 || K % 16) return failf(KB2_ERR_VALUE, "%s: need M >= 0, N > 0, K %% 16 == 0 (M=%lld N=%lld K=%lld)", what, M, N, K);
-  if (M > INT32_MAX / 2 || N > 65535ll * kFp8Block || K > INT32_MAX / 2) return failf(KB2_ERR_VALUE, "%s: M=%lld N=%lld K=%lld is too large", what, M, N, K);
+  if (M > INT32_MAX / 2 || N > 65535ll * kFp8Block || K > 65535ll * kFp8Block) return failf(KB2_ERR_VALUE, "%s: M=%lld N=%lld K=%lld is too large", what, M, N, K);
   return KB2_OK;
 }
 

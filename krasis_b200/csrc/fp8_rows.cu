@@ -126,16 +126,16 @@ cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K
   KernelSpan ks(K_FP8_QUANTIZE, s);
   const dim3 grid((M + 15) / 16, (fp8_blocks(K) + kRowsAhead - 1) / kRowsAhead);
   const bool vec = on16(x) && ldx % (f32 ? 4 : 8) == 0;
-  const auto go = [&](auto kernel) { return launch_pdl(kernel, grid, 256, 0, s, x, ldx, M, K, codes, scales, ld_scales, slot_of, top); };
-  return f32 ? vec ? go(fp8_rows_kernel<true, true>) : go(fp8_rows_kernel<true, false>) : vec ? go(fp8_rows_kernel<false, true>) : go(fp8_rows_kernel<false, false>);
+  const auto kernel = f32 ? vec ? fp8_rows_kernel<true, true> : fp8_rows_kernel<true, false> : vec ? fp8_rows_kernel<false, true> : fp8_rows_kernel<false, false>;
+  return launch_pdl(kernel, grid, 256, 0, s, x, ldx, M, K, codes, scales, ld_scales, slot_of, top);
 }
 
 cudaError_t launch_fp8_blocks(const void* w, bool f32, int groups, int N, int K, void* codes, float* scales, cudaStream_t s) {
   KernelSpan ks(K_FP8_QUANTIZE, s);
   const dim3 grid(fp8_blocks(K), fp8_blocks(N), groups);
-  const auto go = [&](auto kernel) { return launch_pdl(kernel, grid, 256, 0, s, w, N, K, codes, scales); };
-  return f32 ? on16(w) ? go(fp8_blocks_kernel<true, true>) : go(fp8_blocks_kernel<true, false>)
-             : on16(w) ? go(fp8_blocks_kernel<false, true>) : go(fp8_blocks_kernel<false, false>);
+  const bool vec = on16(w);
+  const auto kernel = f32 ? vec ? fp8_blocks_kernel<true, true> : fp8_blocks_kernel<true, false> : vec ? fp8_blocks_kernel<false, true> : fp8_blocks_kernel<false, false>;
+  return launch_pdl(kernel, grid, 256, 0, s, w, N, K, codes, scales);
 }
 
 }  // namespace kb2

@@ -385,8 +385,8 @@ KB2SEQ_API int kb2_seq_token_logprobs(const void* z, int dt, long long ldz, int 
   while (ctas < kLpMostCtas && 2ll * ctas * T <= sms && V > ctas * round) ctas *= 2;
   if (T > INT32_MAX / kLpMostCtas) return failf(KB2SEQ_ERR_VALUE, "token_logprobs: %d rows are too many", T);
   const LogpArgs a{z, ldz, V, top, tokens, logprob, entropy, best, ids};
-  const auto go = [&](auto kernel) { return kb2::launch_pdl_clusters(kernel, dim3(T * ctas), dim3(kLpThreads), 0, (cudaStream_t)stream, dim3(ctas, 1, 1), a); };
-  SEQ_CUDA(dt ? go(token_logprobs_kernel<true>) : go(token_logprobs_kernel<false>));
+  const auto kernel = dt ? token_logprobs_kernel<true> : token_logprobs_kernel<false>;
+  SEQ_CUDA(kb2::launch_pdl_clusters(kernel, dim3(T * ctas), dim3(kLpThreads), 0, (cudaStream_t)stream, dim3(ctas, 1, 1), a));
   SEQ_LAUNCHED();
   return KB2SEQ_OK;
 }
