@@ -7,9 +7,9 @@
 #include "fp8.cuh"
 
 namespace kb2 {
-cudaError_t launch_binning(const int* ids, const float* wts, int M, int top_k, int e_start, int e_end, int chunk_tokens, int* counts, int* offsets, int* cursor,
-                           ChunkDesc* chunks, int* n_chunks, float* sorted_w, int* slot_of, int* sorted_ids, int* sorted_tok, const void* x, void* x_sorted, int H,
-                           cudaStream_t s);
+int fp8_bin_counts(int n, int E);
+cudaError_t launch_fp8_bin(const int* ids, const float* weights, int T, int top, int E, int* counts, int* offsets, float* sorted_w, ChunkDesc* runs, int* n_runs, int* slot_of,
+                           int* token_of, cudaStream_t s);
 cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s);
 }  // namespace kb2
 
@@ -121,7 +121,7 @@ struct ExpertsWork {
   float *xs, *as, *sorted_w;
   void* y;
   ChunkDesc* chunks;
-  int *n_chunks, *counts, *offsets, *cursor, *slot_of, *token_of;
+  int *n_chunks, *counts, *offsets, *slot_of, *token_of;
   int max_chunks;
   long long ldx;
   size_t bytes;
@@ -140,9 +140,8 @@ static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F,
   k.sorted_w = c.take<float>(slots);
   k.chunks = c.take<ChunkDesc>(k.max_chunks);
   k.n_chunks = c.take<int>(1);
-  k.counts = c.take<int>(E);
+  k.counts = c.take<int>(fp8_bin_counts((int)slots, E));
   k.offsets = c.take<int>(E + 1);
-  k.cursor = c.take<int>(E);
   k.slot_of = c.take<int>(slots);
   k.token_of = c.take<int>(slots);
   k.bytes = c.used;
@@ -174,8 +173,7 @@ KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const
   CUDA_TRY(on.err);
   cudaStream_t s = (cudaStream_t)stream;
   const int slots = T * top;
-  CUDA_TRY(launch_binning(ids_dev, weights_dev, T, top, 0, E, kFp8Run, k.counts, k.offsets, k.cursor, k.chunks, k.n_chunks, k.sorted_w, k.slot_of, nullptr, k.token_of, nullptr, nullptr,
-                          0, s));
+  CUDA_TRY(launch_fp8_bin(ids_dev, weights_dev, T, top, E, k.counts, k.offsets, k.sorted_w, k.chunks, k.n_chunks, k.slot_of, k.token_of, s));
   CUDA_TRY(launch_fp8_rows(h_dev, h_f32 != 0, ldh, T, W, k.xc, k.xs, k.ldx, k.slot_of, top, s));      // in the experts' order
   Fp8Product p;
   p.x = k.xc; p.xs = k.xs; p.ldxs = k.ldx; p.w = w1_dev; p.ws = s1_dev; p.out = k.ac;

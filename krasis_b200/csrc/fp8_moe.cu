@@ -1,9 +1,93 @@
-// Routed experts on 8-bit operands (fp8.cuh): what lies behind their two products.
+// Routed experts on 8-bit operands (fp8.cuh): what lies ahead of and behind their two products.
 #include "fp8.cuh"
 #include "prof.cuh"
 #include "ptx.cuh"
 
 namespace kb2 {
+
+cudaError_t launch_binning(const int* ids, const float* wts, int M, int top_k, int e_start, int e_end, int chunk_tokens, int* counts, int* offsets, int* cursor,
+                           ChunkDesc* chunks, int* n_chunks, float* sorted_w, int* slot_of, int* sorted_ids, int* sorted_tok, const void* x, void* x_sorted, int H,
+                           cudaStream_t s);
+constexpr int kBinRows = 4096;                     // choices up to which launch_binning takes one launch
+
+// Which rows of the experts' order the choices take: three launches, counters of each 4096 choices for themselves, so that no counter of the whole step is fought for (81920 choices of 512
+// experts: 15.5 us for the last of them with such, 5 here).  Within 4096 choices an expert's rows are in any order, which no result depends on.
+constexpr int kBinChoices = 4096;
+__global__ void __launch_bounds__(1024) fp8_count_kernel(const int* ids, int n, int E, int* counts) {
+  pdl_wait();
+  __shared__ int s_count[1024];
+  s_count[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kBinChoices / 1024; ++r) {
+    const int i = blockIdx.x * kBinChoices + r * 1024 + threadIdx.x, e = i < n ? ids[i] : -1;
+    if ((unsigned)e < (unsigned)E) atomicAdd(&s_count[e], 1);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < E) counts[(long long)blockIdx.x * E + threadIdx.x] = s_count[threadIdx.x];
+}
+// Every block's counters become its first row of each expert; the runs of at most kFp8Run rows.
+__global__ void __launch_bounds__(1024) fp8_runs_kernel(int* counts, int blocks, int E, ChunkDesc* runs, int* n_runs) {
+  pdl_wait();
+  __shared__ int s_warp[2][32];
+  const int e = threadIdx.x, lane = e & 31, warp = e >> 5;
+  int rows = 0;
+  if (e < E) {
+#pragma unroll 8
+    for (int b = 0; b < blocks; ++b) rows += counts[(long long)b * E + e];
+  }
+  const int n = (rows + kFp8Run - 1) / kFp8Run;
+  int row = rows, run = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, row, o), c = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) {
+      row += a;
+      run += c;
+    }
+  }
+  if (lane == 31) {
+    s_warp[0][warp] = row;
+    s_warp[1][warp] = run;
+  }
+  __syncthreads();
+  row -= rows;
+  run -= n;
+  for (int w = 0; w < warp; ++w) {
+    row += s_warp[0][w];
+    run += s_warp[1][w];
+  }
+  if (e == 1023) *n_runs = run + n;
+  const int per = n ? ((rows + n - 1) / n + 15) & ~15 : 0;
+  for (int i = 0; i < n; ++i) {
+    ChunkDesc d;
+    d.expert = e;
+    d.slot_begin = row + i * per;
+    d.n_tok = min(per, rows - i * per);
+    d.pad_ = 0;
+    runs[run + i] = d;
+  }
+  if (e < E)
+    for (int b = 0; b < blocks; ++b) {
+      int* at = counts + (long long)b * E + e;
+      const int c = *at;
+      *at = row;
+      row += c;
+    }
+}
+__global__ void __launch_bounds__(1024) fp8_place_kernel(const int* ids, int n, int E, const int* firsts, int* slot_of) {
+  pdl_wait();
+  __shared__ int s_next[1024];
+  if ((int)threadIdx.x < E) s_next[threadIdx.x] = firsts[(long long)blockIdx.x * E + threadIdx.x];
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kBinChoices / 1024; ++r) {
+    const int i = blockIdx.x * kBinChoices + r * 1024 + threadIdx.x;
+    if (i >= n) continue;
+    const int e = ids[i];
+    slot_of[i] = (unsigned)e < (unsigned)E ? atomicAdd(&s_next[e], 1) : -1;
+  }
+}
 
 // out[t] = sum_j weights[t][j] y[slot_of[t][j]] in the order of j; entries without a slot bring nothing.  A thread has 16 bytes of a row, four rows on their way at once.
 // W is a multiple of 16, so a row is whole pieces.
@@ -48,6 +132,18 @@ __global__ void __launch_bounds__(128) fp8_combine_kernel(const void* y, const i
   reinterpret_cast<uint4*>(out)[(long long)blockIdx.x * pieces + v] = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+int fp8_bin_counts(int n, int E) { return n <= kBinRows ? E : (n + kBinChoices - 1) / kBinChoices * E; }
+
+cudaError_t launch_fp8_bin(const int* ids, const float* weights, int T, int top, int E, int* counts, int* offsets, float* sorted_w, ChunkDesc* runs, int* n_runs, int* slot_of,
+                           int* token_of, cudaStream_t s) {
+  const int n = T * top, blocks = (n + kBinChoices - 1) / kBinChoices;
+  if (n <= kBinRows) return launch_binning(ids, weights, T, top, 0, E, kFp8Run, counts, offsets, nullptr, runs, n_runs, sorted_w, slot_of, nullptr, token_of, nullptr, nullptr, 0, s);
+  KernelSpan ks(K_BINNING, s, 3);
+  cudaError_t e = launch_pdl(fp8_count_kernel, blocks, 1024, 0, s, ids, n, E, counts);
+  if (e == cudaSuccess) e = launch_pdl(fp8_runs_kernel, 1, 1024, 0, s, counts, blocks, E, runs, n_runs);
+  if (e == cudaSuccess) e = launch_pdl(fp8_place_kernel, blocks, 1024, 0, s, ids, n, E, (const int*)counts, slot_of);
+  return e;
+}
 cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s) {
   KernelSpan ks(K_COMBINE, s);
   const dim3 grid(T, (W / (f32 ? 4 : 8) + 127) / 128);

@@ -115,6 +115,7 @@ def silu_and_mul(x: torch.Tensor) -> torch.Tensor:
 # ------------------------------------------------------------------------------------------------ 8-bit floating-point products, a scale per block of 128
 
 FP8_BLOCK = 128
+_fp8_sizes = {}        # workspace bytes of fp8_linear by (rows, numbers of a row)
 
 
 def _fp8_blocks(n: int) -> int:
@@ -195,8 +196,11 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     _fp8_matrix("fp8_linear", weight, weight_scales, n, k)
     f32, dev = _f32_code(x, "fp8_linear"), _fp8_device("fp8_linear", x, weight, weight_scales, bias)
     out, o32 = _fp8_out("fp8_linear", x, n, bias, x.dtype if out_dtype is None else out_dtype)
-    lib = capi.load()
-    size = lib.kb2_fp8_linear_workspace(m, k)
+    lib, size = capi.load(), _fp8_sizes.get((m, k))
+    if size is None:
+        if len(_fp8_sizes) >= 4096:
+            _fp8_sizes.clear()
+        size = _fp8_sizes[m, k] = lib.kb2_fp8_linear_workspace(m, k)
     work = torch.empty(size, dtype=torch.uint8, device=x.device)
     capi.check(lib.kb2_fp8_linear(x.data_ptr(), f32, x.stride(0), weight.data_ptr(), weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), o32,
                                   m, n, k, work.data_ptr(), size, dev, stream_on(dev)))
