@@ -9,7 +9,7 @@
 namespace kb2 {
 int fp8_bin_counts(int n, int E);
 cudaError_t launch_fp8_bin(const int* ids, const float* weights, int T, int top, int E, int* counts, int* offsets, float* sorted_w, ChunkDesc* runs, int* n_runs, int* slot_of,
-                           int* token_of, cudaStream_t s);
+                           cudaStream_t s);
 cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s);
 }  // namespace kb2
 
@@ -121,7 +121,7 @@ struct ExpertsWork {
   float *xs, *as, *sorted_w;
   void* y;
   ChunkDesc* chunks;
-  int *n_chunks, *counts, *offsets, *slot_of, *token_of;
+  int *n_chunks, *counts, *offsets, *slot_of;
   int max_chunks;
   long long ldx;
   size_t bytes;
@@ -143,7 +143,6 @@ static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F,
   k.counts = c.take<int>(fp8_bin_counts((int)slots, E));
   k.offsets = c.take<int>(E + 1);
   k.slot_of = c.take<int>(slots);
-  k.token_of = c.take<int>(slots);
   k.bytes = c.used;
   return k;
 }
@@ -173,7 +172,7 @@ KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const
   CUDA_TRY(on.err);
   cudaStream_t s = (cudaStream_t)stream;
   const int slots = T * top;
-  CUDA_TRY(launch_fp8_bin(ids_dev, weights_dev, T, top, E, k.counts, k.offsets, k.sorted_w, k.chunks, k.n_chunks, k.slot_of, k.token_of, s));
+  CUDA_TRY(launch_fp8_bin(ids_dev, weights_dev, T, top, E, k.counts, k.offsets, k.sorted_w, k.chunks, k.n_chunks, k.slot_of, s));
   CUDA_TRY(launch_fp8_rows(h_dev, h_f32 != 0, ldh, T, W, k.xc, k.xs, k.ldx, k.slot_of, top, s));      // in the experts' order
   Fp8Product p;
   p.x = k.xc; p.xs = k.xs; p.ldxs = k.ldx; p.w = w1_dev; p.ws = s1_dev; p.out = k.ac;

@@ -133,7 +133,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
       }
       if (mine) {
         // 32 rows x 128 bytes at a time go out from shared memory by one copy, while the next tile's blocks are added: all SMs end their tiles at the same time, and a tile's
-        // stores by the lanes took 3500 cycles (16 bytes of a row by each lane, row by row, 12000).  A run's last rows, and rows that are not on 16 bytes, are the lanes'.
+        // stores by the lanes took 3500 cycles (16 bytes of a row by each lane, row by row, 12000).  The last rows, and rows that are not on 16 bytes, are the lanes'.
         constexpr int kCols = kOutF32 ? 32 : 64, kVec = kOutF32 ? 4 : 8;
         uint8_t* st = smem + kFOffOut + (warp - 4) * kFOut;
         const int row0 = i.row0 + rank * kFRows + q * 32, have = i.rows - (int)(rank * kFRows + q * 32);

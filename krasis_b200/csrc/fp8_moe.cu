@@ -135,9 +135,9 @@ __global__ void __launch_bounds__(128) fp8_combine_kernel(const void* y, const i
 int fp8_bin_counts(int n, int E) { return n <= kBinRows ? E : (n + kBinChoices - 1) / kBinChoices * E; }
 
 cudaError_t launch_fp8_bin(const int* ids, const float* weights, int T, int top, int E, int* counts, int* offsets, float* sorted_w, ChunkDesc* runs, int* n_runs, int* slot_of,
-                           int* token_of, cudaStream_t s) {
+                           cudaStream_t s) {
   const int n = T * top, blocks = (n + kBinChoices - 1) / kBinChoices;
-  if (n <= kBinRows) return launch_binning(ids, weights, T, top, 0, E, kFp8Run, counts, offsets, nullptr, runs, n_runs, sorted_w, slot_of, nullptr, token_of, nullptr, nullptr, 0, s);
+  if (n <= kBinRows) return launch_binning(ids, weights, T, top, 0, E, kFp8Run, counts, offsets, nullptr, runs, n_runs, sorted_w, slot_of, nullptr, nullptr, nullptr, nullptr, 0, s);
   KernelSpan ks(K_BINNING, s, 3);
   cudaError_t e = launch_pdl(fp8_count_kernel, blocks, 1024, 0, s, ids, n, E, counts);
   if (e == cudaSuccess) e = launch_pdl(fp8_runs_kernel, 1, 1024, 0, s, counts, blocks, E, runs, n_runs);

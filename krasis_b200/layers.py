@@ -122,6 +122,11 @@ def _fp8_blocks(n: int) -> int:
     return (n + FP8_BLOCK - 1) // FP8_BLOCK
 
 
+def _rows_of(m, k, dtype, device):
+    """torch.empty((m, k)) in 1.6 us instead of 2.4."""
+    return torch.empty_strided((m, k), (k, 1), dtype=dtype, device=device)
+
+
 def _f32_code(t, name) -> int:
     if t.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"{name}: {t.dtype}, expected bfloat16 or float32")
@@ -163,7 +168,7 @@ def quantize_fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     with a number that is not finite scale NaN and codes 0.  The scales of one block of all rows lie side by side: strides (1, rows rounded up to 4)."""
     m, k = _fp8_input("quantize_fp8_rows", x)
     f32, dev, device, ld = _f32_code(x, "quantize_fp8_rows"), _fp8_device("quantize_fp8_rows", x), x.device, (m + 3) // 4 * 4
-    codes = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=device)
+    codes = _rows_of(m, k, torch.float8_e4m3fn, device)
     scales = torch.empty_strided((m, _fp8_blocks(k)), (1, ld), dtype=torch.float32, device=device)
     capi.check(capi.load().kb2_fp8_quantize_rows(x.data_ptr(), f32, x.stride(0), m, k, codes.data_ptr(), scales.data_ptr(), ld, dev, stream_on(dev)))
     return codes, scales
@@ -175,16 +180,20 @@ def quantize_fp8_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if w.dim() not in (2, 3) or not w.is_contiguous() or w.shape[-1] == 0 or w.shape[-2] == 0 or w.shape[-1] % 16:
         raise ValueError(f"quantize_fp8_blocks: contiguous [N, K] or [E, N, K] with K a multiple of 16, got {tuple(w.shape)}")
     f32, dev, (n, k) = _f32_code(w, "quantize_fp8_blocks"), _fp8_device("quantize_fp8_blocks", w), w.shape[-2:]
-    codes = torch.empty(w.shape, dtype=torch.float8_e4m3fn, device=w.device)
-    scales = torch.empty(tuple(w.shape[:-2]) + (_fp8_blocks(n), _fp8_blocks(k)), dtype=torch.float32, device=w.device)
-    capi.check(capi.load().kb2_fp8_quantize_blocks(w.data_ptr(), f32, w.shape[0] if w.dim() == 3 else 1, n, k, codes.data_ptr(), scales.data_ptr(), dev, stream_on(dev)))
+    e, nn, kk, device = w.shape[0] if w.dim() == 3 else 1, _fp8_blocks(n), _fp8_blocks(k), w.device
+    if w.dim() == 2:
+        codes, scales = _rows_of(n, k, torch.float8_e4m3fn, device), _rows_of(nn, kk, torch.float32, device)
+    else:
+        codes = torch.empty(w.shape, dtype=torch.float8_e4m3fn, device=device)
+        scales = torch.empty((e, nn, kk), dtype=torch.float32, device=device)
+    capi.check(capi.load().kb2_fp8_quantize_blocks(w.data_ptr(), f32, e, n, k, codes.data_ptr(), scales.data_ptr(), dev, stream_on(dev)))
     return codes, scales
 
 
 def _fp8_out(name, x, n, bias, out_dtype):
     if bias is not None and (bias.dtype is not torch.float32 or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
         raise ValueError(f"{name}: a float32 bias [{n}]")
-    out = torch.empty((x.shape[0], n), dtype=out_dtype, device=x.device)
+    out = _rows_of(x.shape[0], n, out_dtype, x.device)
     return out, _f32_code(out, name)
 
 
@@ -201,7 +210,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
         if len(_fp8_sizes) >= 4096:
             _fp8_sizes.clear()
         size = _fp8_sizes[m, k] = lib.kb2_fp8_linear_workspace(m, k)
-    work = torch.empty(size, dtype=torch.uint8, device=x.device)
+    work = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=x.device)
     capi.check(lib.kb2_fp8_linear(x.data_ptr(), f32, x.stride(0), weight.data_ptr(), weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), o32,
                                   m, n, k, work.data_ptr(), size, dev, stream_on(dev)))
     return out
@@ -243,10 +252,10 @@ def fp8_experts(h: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gat
     if weights.dtype is not torch.float32 or weights.shape != ids.shape or not weights.is_contiguous():
         raise ValueError(f"fp8_experts: contiguous float32 weights {tuple(ids.shape)}")
     dev = _fp8_device("fp8_experts", h, ids, weights, w_gate_up, s_gate_up, w_down, s_down)
-    out = torch.empty((T, W), dtype=h.dtype if out_dtype is None else out_dtype, device=h.device)
+    out = _rows_of(T, W, h.dtype if out_dtype is None else out_dtype, h.device)
     f32, o32, top, lib = _f32_code(h, "fp8_experts"), _f32_code(out, "fp8_experts"), ids.shape[1], capi.load()
     size = lib.kb2_fp8_experts_workspace(T, top, E, W, F, o32)
-    work = torch.empty(size, dtype=torch.uint8, device=h.device)
+    work = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=h.device)
     capi.check(lib.kb2_fp8_experts(h.data_ptr(), f32, h.stride(0), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(), s_gate_up.data_ptr(), w_down.data_ptr(),
                                    s_down.data_ptr(), out.data_ptr(), o32, T, top, E, W, F, work.data_ptr(), size, dev, stream_on(dev)))
     return out

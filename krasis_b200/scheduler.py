@@ -160,6 +160,8 @@ class Scheduler:
 
         logprobs (0 to 64): returns (ids, details) instead, details with a dict for each generated token: "logprob" and "entropy" of the model's distribution (ahead of
         temperature and filters) and "top", that many of its most likely tokens as (id, log probability)."""
+        if logprobs is not None and not 0 <= logprobs <= ops.MAX_TOP_LOGPROBS:
+            raise ValueError(f"{logprobs} alternatives, at most {ops.MAX_TOP_LOGPROBS}")
         details: List[List[dict]] = [[] for _ in prompts]
         sampler = Sampler(sampling, self.model.device)
         waiting = deque(enumerate(prompts))
@@ -217,19 +219,23 @@ class Scheduler:
     def score(self, texts: Sequence[Sequence[int]], step_tokens: int = 512) -> List[List[float]]:
         """Log probability of every token of every text but its first, given those before it (a text's perplexity is exp of minus their mean).  A text runs in portions of
         step_tokens; the logits of a portion are gone when the next one runs."""
+        if step_tokens < 1:
+            raise ValueError(f"portions of {step_tokens} tokens")
         scores = []
         for i, text in enumerate(texts):
             text, parts = [int(t) for t in text], []
             if text and not self.can_admit(len(text)):
                 raise RuntimeError("a text does not fit the cache pool")
-            for a in range(0, len(text), step_tokens):
-                part = text[a:a + step_tokens]
-                told = text[a + 1:a + 1 + len(part)]             # what follows each of them; behind the last one of all, nothing
-                logits = self.step([(("score", i), part, list(range(len(told))))])
-                if told:
-                    parts.append(ops.token_logprobs(logits, torch.tensor(told, device=logits.device)).logprob)
-            if text:
-                self.finish(("score", i))
+            try:
+                for a in range(0, len(text), step_tokens):
+                    part = text[a:a + step_tokens]
+                    told = text[a + 1:a + 1 + len(part)]         # what follows each of them; behind the last one of all, nothing
+                    logits = self.step([(("score", i), part, list(range(len(told))))])
+                    if told:
+                        parts.append(ops.token_logprobs(logits, torch.tensor(told, device=logits.device)).logprob)
+            finally:
+                if ("score", i) in self.live:
+                    self.finish(("score", i))
             scores.append(torch.cat(parts).tolist() if parts else [])
         if torch.cuda.is_available() and texts:
             ops.check_waits(torch.device(self.model.device).index or 0)

@@ -659,14 +659,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     T, V = logits.shape
     if tokens.shape != (T,) or tokens.dtype not in (torch.int64, torch.int32) or tokens.get_device() != dev:
         raise ValueError(f"token_logprobs: one int64 or int32 token per row, [{T}] on the logits' device")
+    top = int(top)
     if not 0 <= top <= min(V, MAX_TOP_LOGPROBS):
         raise ValueError(f"token_logprobs: {top} alternatives of {V}, at most {MAX_TOP_LOGPROBS}")
     if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
         tokens = tokens.to(torch.int64).contiguous()
     device, dt = logits.device, dt_code(logits.dtype)
-    lp, en = torch.empty((2, T), dtype=torch.float32, device=device).unbind()
-    best = torch.empty((T, top), dtype=torch.float32, device=device)
-    ids = torch.empty((T, top), dtype=torch.int32, device=device)
+    new = torch.empty_strided                       # 1.6 us, torch.empty 2.4
+    lp, en = new((T,), (1,), dtype=torch.float32, device=device), new((T,), (1,), dtype=torch.float32, device=device)
+    best, ids = new((T, top), (top, 1), dtype=torch.float32, device=device), new((T, top), (top, 1), dtype=torch.int32, device=device)
     check(load().kb2_seq_token_logprobs(logits.data_ptr(), dt, logits.stride(0), T, V, tokens.data_ptr(), top, lp.data_ptr(), en.data_ptr(), ids.data_ptr(),
                                         best.data_ptr(), dev, stream_on(dev)))
     return TokenLogprobs(lp, en, ids, best)

@@ -171,7 +171,7 @@ def _choices(T, top, E, seed, spare=0):
 
 
 EXPERTS = [(1, 1, 1, 128, 128), (1, 8, 64, 512, 256), (3, 2, 4, 272, 128), (4, 10, 512, 512, 128), (9, 6, 16, 1040, 384), (40, 4, 8, 640, 256), (100, 8, 300, 256, 128), (130, 3, 5, 2048, 512),
-           (333, 6, 64, 512, 256), (700, 2, 3, 400, 640), (1000, 10, 128, 256, 128), (2000, 1, 2, 256, 128)]
+           (333, 6, 64, 512, 256), (700, 2, 3, 400, 640), (1000, 10, 128, 256, 128), (2000, 1, 2, 256, 128), (50, 20, 40, 128, 128), (600, 17, 1024, 256, 128), (129, 2, 2, 384, 256), (5000, 2, 300, 128, 128)]
 
 
 @pytest.mark.parametrize("out", [BF, F32])

@@ -55,3 +55,9 @@ def test_generated_tokens_with_their_log_probabilities(sched):
 def test_a_text_that_does_not_fit(sched):
     with pytest.raises(RuntimeError, match="does not fit"):
         sched.score([list(range(65))])
+    with pytest.raises(ValueError):
+        sched.score([[1, 2]], step_tokens=0)
+    for bad in (-1, 65):
+        with pytest.raises(ValueError):
+            sched.generate([[1, 2]], 2, logprobs=bad)
+    assert not sched.live and sched.kv_cache.free_page_count == 16
