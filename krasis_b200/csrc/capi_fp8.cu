@@ -6,13 +6,6 @@
 #include "../../include/krasis_b200.h"
 #include "fp8.cuh"
 
-namespace kb2 {
-int fp8_bin_counts(int n, int E);
-cudaError_t launch_fp8_bin(const int* ids, const float* weights, int T, int top, int E, int* counts, int* offsets, float* sorted_w, ChunkDesc* runs, int* n_runs, int* slot_of,
-                           cudaStream_t s);
-cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s);
-}  // namespace kb2
-
 using namespace kb2;
 
 extern "C" int kb2_set_error_(int code, const char* msg);
@@ -118,10 +111,10 @@ KB2_API int kb2_fp8_linear(const void* x_dev, int32_t x_f32, int64_t ldx, const 
 // ---- routed experts
 struct ExpertsWork {
   uint8_t *xc, *ac;
-  float *xs, *as, *sorted_w;
+  float *xs, *as;
   void* y;
   ChunkDesc* chunks;
-  int *n_chunks, *counts, *offsets, *slot_of;
+  int *n_chunks, *counts, *slot_of;
   int max_chunks;
   long long ldx;
   size_t bytes;
@@ -137,11 +130,9 @@ static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F,
   k.ac = c.take<uint8_t>(slots * F);
   k.as = c.take<float>((size_t)k.ldx * fp8_blocks(F));
   k.y = c.take<uint8_t>(slots * W * (out_f32 ? 4 : 2));
-  k.sorted_w = c.take<float>(slots);
   k.chunks = c.take<ChunkDesc>(k.max_chunks);
   k.n_chunks = c.take<int>(1);
   k.counts = c.take<int>(fp8_bin_counts((int)slots, E));
-  k.offsets = c.take<int>(E + 1);
   k.slot_of = c.take<int>(slots);
   k.bytes = c.used;
   return k;
@@ -172,8 +163,7 @@ KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const
   CUDA_TRY(on.err);
   cudaStream_t s = (cudaStream_t)stream;
   const int slots = T * top;
-  CUDA_TRY(launch_fp8_bin(ids_dev, weights_dev, T, top, E, k.counts, k.offsets, k.sorted_w, k.chunks, k.n_chunks, k.slot_of, s));
-  CUDA_TRY(launch_fp8_rows(h_dev, h_f32 != 0, ldh, T, W, k.xc, k.xs, k.ldx, k.slot_of, top, s));      // in the experts' order
+  CUDA_TRY(launch_fp8_bin(ids_dev, T, top, E, k.counts, k.chunks, k.n_chunks, k.slot_of, h_dev, h_f32 != 0, ldh, W, k.xc, k.xs, k.ldx, s));
   Fp8Product p;
   p.x = k.xc; p.xs = k.xs; p.ldxs = k.ldx; p.w = w1_dev; p.ws = s1_dev; p.out = k.ac;
   p.M = slots; p.N = 2 * F; p.K = W; p.groups = E;

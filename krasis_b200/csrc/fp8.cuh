@@ -42,6 +42,55 @@ __device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float 
   return inv == 0.f ? 0u : lo | hi << 16;
 }
 
+// Eight neighbouring numbers as they are in memory.
+template <bool F32>
+struct Fp8Eight {
+  uint32_t u[F32 ? 8 : 4];
+  // `have` of them are there
+  template <bool VEC>
+  __device__ __forceinline__ void load(const void* p, long long at, int have) {
+#pragma unroll
+    for (int i = 0; i < (F32 ? 8 : 4); ++i) u[i] = 0;
+    if (have <= 0) return;
+    if constexpr (VEC) {                           // all eight: their number is a multiple of 16
+      const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + at * (F32 ? 4 : 2));
+#pragma unroll
+      for (int i = 0; i < (F32 ? 2 : 1); ++i) {
+        const uint4 a = __ldcs(q + i);
+        u[4 * i] = a.x; u[4 * i + 1] = a.y; u[4 * i + 2] = a.z; u[4 * i + 3] = a.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= have) continue;
+        if constexpr (F32) u[i] = reinterpret_cast<const uint32_t*>(p)[at + i];
+        else u[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[at + i] << (i & 1) * 16;
+      }
+    }
+  }
+  __device__ __forceinline__ float number(int i) const {
+    if constexpr (F32) return __uint_as_float(u[i]);
+    else return __uint_as_float(i & 1 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16);
+  }
+  // the bits of the largest magnitude: as whole numbers infinities and NaN are the largest
+  __device__ __forceinline__ uint32_t largest() const {
+    if constexpr (F32) {
+      uint32_t a = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a = max(a, u[i] & 0x7FFFFFFFu);
+      return a;
+    } else {
+      const uint32_t a = __vmaxu2(__vmaxu2(u[0] & 0x7FFF7FFFu, u[1] & 0x7FFF7FFFu), __vmaxu2(u[2] & 0x7FFF7FFFu, u[3] & 0x7FFF7FFFu));
+      return max(a << 16, a & 0xFFFF0000u);
+    }
+  }
+  __device__ __forceinline__ uint2 codes(float inv) const {
+    return make_uint2(fp8_codes4(number(0), number(1), number(2), number(3), inv), fp8_codes4(number(4), number(5), number(6), number(7), inv));
+  }
+  // K is a multiple of 16 and the codes lie on 16 bytes: eight of them are there whole or not at all.
+  __device__ __forceinline__ void store(void* to, long long at, float inv) const { *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(to) + at) = codes(inv); }
+};
+
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -75,6 +124,13 @@ struct Fp8Product {
 
 // Rows of activations.  With slot_of [M][top] a row goes to each of its slots (negative: none) instead of its own place, codes and scales.
 cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K, void* codes, float* scales, long long ld_scales, const int* slot_of, int top, cudaStream_t s);
+// Routed experts: the slots of the choices ids [T][top] (-1: outside the E experts), the runs of each expert's rows, and the tokens' quantised rows in their slots; counts:
+// fp8_bin_counts numbers.
+int fp8_bin_counts(int n, int E);
+cudaError_t launch_fp8_bin(const int* ids, int T, int top, int E, int* counts, ChunkDesc* runs, int* n_runs, int* slot_of, const void* x, bool f32, long long ldx, int K, void* codes,
+                           float* scales, long long lds, cudaStream_t s);
+// out[t] = sum_j weights[t][j] y[slot_of[t][j]]
+cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s);
 cudaError_t launch_fp8_blocks(const void* w, bool f32, int groups, int N, int K, void* codes, float* scales, cudaStream_t s);
 // One matrix, all M rows, on pairs of CTAs with tiles of 256 x 256.
 cudaError_t launch_fp8_pairs(const Fp8Product& p, int num_sms, cudaStream_t s);

@@ -4,55 +4,6 @@
 
 namespace kb2 {
 
-// Eight neighbouring numbers as they are in memory.
-template <bool F32>
-struct Eight {
-  uint32_t u[F32 ? 8 : 4];
-  // `have` of them are there
-  template <bool VEC>
-  __device__ __forceinline__ void load(const void* p, long long at, int have) {
-#pragma unroll
-    for (int i = 0; i < (F32 ? 8 : 4); ++i) u[i] = 0;
-    if (have <= 0) return;
-    if constexpr (VEC) {                           // all eight: their number is a multiple of 16
-      const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + at * (F32 ? 4 : 2));
-#pragma unroll
-      for (int i = 0; i < (F32 ? 2 : 1); ++i) {
-        const uint4 a = __ldcs(q + i);
-        u[4 * i] = a.x; u[4 * i + 1] = a.y; u[4 * i + 2] = a.z; u[4 * i + 3] = a.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i >= have) continue;
-        if constexpr (F32) u[i] = reinterpret_cast<const uint32_t*>(p)[at + i];
-        else u[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[at + i] << (i & 1) * 16;
-      }
-    }
-  }
-  __device__ __forceinline__ float number(int i) const {
-    if constexpr (F32) return __uint_as_float(u[i]);
-    else return __uint_as_float(i & 1 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16);
-  }
-  // the bits of the largest magnitude: as whole numbers infinities and NaN are the largest
-  __device__ __forceinline__ uint32_t largest() const {
-    if constexpr (F32) {
-      uint32_t a = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a = max(a, u[i] & 0x7FFFFFFFu);
-      return a;
-    } else {
-      const uint32_t a = __vmaxu2(__vmaxu2(u[0] & 0x7FFF7FFFu, u[1] & 0x7FFF7FFFu), __vmaxu2(u[2] & 0x7FFF7FFFu, u[3] & 0x7FFF7FFFu));
-      return max(a << 16, a & 0xFFFF0000u);
-    }
-  }
-  __device__ __forceinline__ uint2 codes(float inv) const {
-    return make_uint2(fp8_codes4(number(0), number(1), number(2), number(3), inv), fp8_codes4(number(4), number(5), number(6), number(7), inv));
-  }
-  // K is a multiple of 16 and the codes lie on 16 bytes: eight of them are there whole or not at all.
-  __device__ __forceinline__ void store(void* to, long long at, float inv) const { *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(to) + at) = codes(inv); }
-};
-
 // Sixteen lanes have a block of 128, eight numbers each; a thread block has 16 rows x kRowsAhead blocks, all of a thread's loads on their way at once, its row's slots among them.
 // 8191 x 4096 fp32 (169 MB): 24 us, 7.0 TB/s.  Into the slots of ten experts each, 8192 x 2048 bf16 (207 MB): 44 us with the slots read one after the other.
 constexpr int kRowsAhead = 4;
@@ -60,7 +11,7 @@ template <bool F32, bool VEC, bool SLOTS>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(const void* x, long long ldx, int M, int K, void* codes, float* scales, long long lds, const int* slot_of, int top) {
   pdl_wait();
   const int lane = threadIdx.x & 15, m = blockIdx.x * 16 + (threadIdx.x >> 4), b0 = blockIdx.y * kRowsAhead;
-  Eight<F32> v[kRowsAhead];
+  Fp8Eight<F32> v[kRowsAhead];
 #pragma unroll
   for (int i = 0; i < kRowsAhead; ++i) {
     const int k = (b0 + i) * kFp8Block + lane * 8;
@@ -110,7 +61,7 @@ __global__ void __launch_bounds__(256) fp8_blocks_kernel(const void* w, int N, i
   __shared__ uint32_t s_max[8];
   const int lane = threadIdx.x & 15, row0 = blockIdx.y * kFp8Block + (threadIdx.x >> 4), k = blockIdx.x * kFp8Block + lane * 8;
   const long long base = (long long)blockIdx.z * N * K + k;
-  Eight<F32> v[8];
+  Fp8Eight<F32> v[8];
   uint32_t a = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
