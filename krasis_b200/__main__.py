@@ -4,6 +4,7 @@
                                    [--temperature 0 --top-k 0 --top-p 1 --seed 0] [--max-tokens 8192] [--step-tokens 512]
                                    [--logprobs N] [--expert-format e4m3]
     python -m krasis_b200 score    --model DIR --prompt-ids 5,17,3 [--prompt-ids ...] [--dtype bfloat16] [--max-tokens 8192] [--step-tokens 512]
+                                   [--expert-format e4m3]
     python -m krasis_b200 trace    --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N        (same as bin/trace_run)
 
 `generate` loads the checkpoint through the model registry (config.json decides the class), runs continuous batching over the
@@ -12,7 +13,16 @@ and the N most likely tokens).  `score` prints the log probabilities of the give
 part of this package."""
 import argparse
 import json
+import math
 import sys
+
+
+def perplexity(logprobs):
+    """exp of minus the mean; None of nothing, inf of what passes a double."""
+    if not logprobs:
+        return None
+    mean = -sum(logprobs) / len(logprobs)
+    return math.inf if mean > 709 else math.exp(mean)
 
 
 def main(argv=None) -> int:
@@ -34,27 +44,26 @@ def main(argv=None) -> int:
     ap.add_argument("--max-tokens", type=int, default=8192, help="tokens the cache pool holds")
     ap.add_argument("--max-requests", type=int, default=4)
     ap.add_argument("--step-tokens", type=int, default=512, help="token budget of one step (prompt portions + decoded tokens)")
-    ap.add_argument("--expert-format", default=None, choices=["e4m3"], help="routed experts held in 8-bit floating point (models with silu-gated experts)")
+    ap.add_argument("--expert-format", default=None, choices=["e4m3"], help="routed experts held in 8-bit floating point (designs with silu-gated experts and weights on their outputs)")
     ap.add_argument("--logprobs", type=int, default=None, help="log probabilities of the generated tokens, with this many alternatives (0 to 64)")
     a = ap.parse_args(argv)
 
     import torch
-    from .registry import load_model
+    from .registry import E4M3_EXPERTS, architecture_of, load_model
     from .sampling import SamplingParams
     from .scheduler import Scheduler
-    model = load_model(a.model, dtype=torch.bfloat16 if a.dtype == "bfloat16" else torch.float32, **({"expert_format": a.expert_format} if a.expert_format else {}))
-    if a.expert_format and getattr(model, "expert_format", None) != a.expert_format:
-        print(f"{type(model).__name__} does not hold its experts in {a.expert_format}", file=sys.stderr)
+    if a.expert_format and architecture_of(a.model) not in E4M3_EXPERTS:
+        print(f"{architecture_of(a.model)} does not hold its experts in {a.expert_format}", file=sys.stderr)
         return 3
+    model = load_model(a.model, dtype=torch.bfloat16 if a.dtype == "bfloat16" else torch.float32, **({"expert_format": a.expert_format} if a.expert_format else {}))
     if not hasattr(model, "forward_step"):
         print(f"{type(model).__name__} has no step interface for generation", file=sys.stderr)
         return 3
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in a.prompt_ids]
     sched = Scheduler(model, max_tokens=a.max_tokens, max_requests=a.max_requests, cuda_graphs=True)
     if a.command == "score":
-        import math
         for p, s in zip(prompts, sched.score(prompts, step_tokens=a.step_tokens)):
-            print(json.dumps({"prompt_tokens": len(p), "logprobs": s, "perplexity": math.exp(-sum(s) / len(s)) if s else None}))
+            print(json.dumps({"prompt_tokens": len(p), "logprobs": s, "perplexity": perplexity(s)}))
         return 0
     outs = sched.generate(prompts, a.max_new_tokens, SamplingParams(a.temperature, a.top_k, a.top_p, a.seed), step_tokens=a.step_tokens,
                           eos=a.eos, logprobs=a.logprobs)

@@ -9,6 +9,7 @@ from typing import Callable, Dict
 import torch
 
 _REGISTRY: Dict[str, Callable] = {}
+E4M3_EXPERTS = ("Megolorn",)                       # designs whose routed experts can be held in 8-bit floating point (expert_format="e4m3")
 _HF_MOE = ("qwen3_next", "qwen3_5_moe", "qwen3_5_moe_text", "qwen3_moe", "deepseek_v2", "deepseek_v3")
 
 

@@ -159,7 +159,7 @@ class Scheduler:
         """Greedy (or sampled) continuation of every prompt; returns the generated ids per prompt, in order.
 
         logprobs (0 to 64): returns (ids, details) instead, details with a dict for each generated token: "logprob" and "entropy" of the model's distribution (ahead of
-        temperature and filters) and "top", that many of its most likely tokens as (id, log probability)."""
+        temperature and filters) and "top", that many of its most likely tokens (all of a smaller vocabulary) as (id, log probability)."""
         if logprobs is not None and not 0 <= logprobs <= ops.MAX_TOP_LOGPROBS:
             raise ValueError(f"{logprobs} alternatives, at most {ops.MAX_TOP_LOGPROBS}")
         details: List[List[dict]] = [[] for _ in prompts]
@@ -212,7 +212,7 @@ class Scheduler:
 
     @staticmethod
     def _say(logits, tokens, top: int) -> List[dict]:
-        r = ops.token_logprobs(logits, tokens, top)
+        r = ops.token_logprobs(logits, tokens, min(top, logits.shape[1]))
         numbers, ids = torch.cat([r.logprob[:, None], r.entropy[:, None], r.top_logprobs], 1).tolist(), r.top_ids.tolist()
         return [{"logprob": n[0], "entropy": n[1], "top": list(zip(i, n[2:]))} for n, i in zip(numbers, ids)]
 

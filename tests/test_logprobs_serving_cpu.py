@@ -1,4 +1,5 @@
 """Scoring and log probabilities of the scheduler with a stand-in model on the CPU, where the operator is replaced by its definition."""
+import json
 import math
 
 import pytest
@@ -61,3 +62,22 @@ def test_a_text_that_does_not_fit(sched):
         with pytest.raises(ValueError):
             sched.generate([[1, 2]], 2, logprobs=bad)
     assert not sched.live and sched.kv_cache.free_page_count == 16
+
+
+def test_more_alternatives_than_tokens(sched):
+    ids, details = sched.generate([[1, 2, 3]], max_new_tokens=2, logprobs=64)
+    assert len(ids[0]) == 2 and all(sorted(t for t, _ in d["top"]) == list(range(13)) for d in details[0]) and not sched.live
+
+
+def test_perplexity():
+    from krasis_b200.__main__ import perplexity
+    assert perplexity([]) is None and perplexity([0.0, 0.0]) == 1 and math.isclose(perplexity([-1.0, -3.0]), math.exp(2))
+    assert perplexity([-2e6, -1.0]) == perplexity([-math.inf]) == math.inf and math.isnan(perplexity([math.nan, -1.0]))
+
+
+def test_designs_that_do_not_hold_their_experts_in_8_bits(tmp_path, capsys):
+    from krasis_b200.__main__ import main
+    for cfg in ({"architecture": "Kivurax"}, {"model_type": "qwen3_moe"}):
+        (tmp_path / "config.json").write_text(json.dumps(cfg))
+        assert main(["score", "--model", str(tmp_path), "--prompt-ids", "1,2", "--expert-format", "e4m3"]) == 3
+        assert "does not hold its experts" in capsys.readouterr().err
