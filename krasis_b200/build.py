@@ -25,7 +25,7 @@ LIB = os.path.join(LIBDIR, "libkrasis_b200.so")
 SEQ_LIB = os.path.join(LIBDIR, "libkrasis_b200_seq.so")
 SEQ_SOURCES = ["seq_ops.cu", "seq_mix.cu", "seq_rec.cu", "seq_kv.cu", "seq_kv_attn.cu", "seq_kv_tile.cu", "seq_kv_pair.cu", "seq_logp.cu"]
 SOURCES = ["grouped_gemm.cu", "router_gemm.cu", "dense_gemm.cu", "split_gemm.cu", "gdn.cu", "gdn_tc.cu", "gqa.cu", "elementwise.cu", "moe_kernels.cu", "capi.cu", "capi_attn.cu", "capi_comm.cu",
-           "fp8_rows.cu", "fp8_gemm.cu", "fp8_tile.cu", "fp8_moe.cu", "capi_fp8.cu"]
+           "fp8_rows.cu", "fp8_gemm.cu", "fp8_moe.cu", "capi_fp8.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

@@ -6,7 +6,7 @@
 namespace kb2 {
 
 // Which rows of the experts' order the choices take, for many of them: three launches, counters of each 4096 choices for themselves, so that no counter of the whole step is fought for (81920 choices of 512
-// experts: 15.5 us for the last of them with such, 5 here).  Within 4096 choices an expert's rows are in any order, which no result depends on.
+// experts: 15.5 us for the last of them with such, 8 here; 4.5, 8 and 5 for the three).  Within 4096 choices an expert's rows are in any order, which no result depends on.
 constexpr int kBinChoices = 4096;
 // The rows of expert e from `row` on as n runs of about the same size, a multiple of 16.
 __device__ __forceinline__ void write_runs(ChunkDesc* runs, int e, int row, int rows, int n) {
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(1024) fp8_place_kernel(const int* ids, int n, 
 
 // Up to kBinRows choices: their places and their quantised rows in one launch.  Every block counts all choices in shared memory and adds the counters up by itself, so blocks need
 // nothing from one another; a warp finds its choice's place among its expert's by counting the equal ones before it, and quantises its token's row into it, sixteen lanes a
-// block of 128.  A token's row is read once a choice, from L2.  40 choices of rows of 2048: 10.6 us in two launches.
+// block of 128.  A token's row is read once a choice, from L2.  40 choices of rows of 2048: 7.5 us, 10.6 in two launches.
 constexpr int kBinRows = 4096, kBinAhead = 4;
 template <bool F32, bool VEC>
 __global__ void __launch_bounds__(256) fp8_bin_rows_kernel(const int* ids, int n, int top, int E, ChunkDesc* runs, int* n_runs, int* slot_of, const void* x, long long ldx, int K,

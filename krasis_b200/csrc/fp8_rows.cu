@@ -5,7 +5,7 @@
 namespace kb2 {
 
 // Sixteen lanes have a block of 128, eight numbers each; a thread block has 16 rows x kRowsAhead blocks, all of a thread's loads on their way at once, its row's slots among them.
-// 8191 x 4096 fp32 (169 MB): 24 us, 7.0 TB/s.  Into the slots of ten experts each, 8192 x 2048 bf16 (207 MB): 44 us with the slots read one after the other.
+// 8191 x 4096 fp32 (169 MB): 24 us, 7.0 TB/s.  Into the slots of ten experts each, 8192 x 2048 bf16 (207 MB): 40 us, 5.2 TB/s (44 with the slots read one after the other).
 constexpr int kRowsAhead = 4;
 template <bool F32, bool VEC, bool SLOTS>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(const void* x, long long ldx, int M, int K, void* codes, float* scales, long long lds, const int* slot_of, int top) {
