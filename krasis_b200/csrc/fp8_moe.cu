@@ -6,7 +6,7 @@
 namespace kb2 {
 
 // Which rows of the experts' order the choices take, for many of them: three launches, counters of each 4096 choices for themselves, so that no counter of the whole step is fought for (81920 choices of 512
-// experts: 15.5 us for the last of them with such, 8 here; 4.5, 8 and 5 for the three).  Within 4096 choices an expert's rows are in any order, which no result depends on.
+// experts: 15.5 us for the last launch with such; 4.5, 8 and 5 for the three).  Within 4096 choices an expert's rows are in any order, which no result depends on.
 constexpr int kBinChoices = 4096;
 // The rows of expert e from `row` on as n runs of about the same size, a multiple of 16.
 __device__ __forceinline__ void write_runs(ChunkDesc* runs, int e, int row, int rows, int n) {

@@ -1,12 +1,13 @@
 // Log probabilities of given tokens, entropy and the largest alternatives of rows of logits, in one pass over them.
 //
-// In powers of two: with L = log2 e and a reference c near L max z, t = L z - c by one fused multiply-add, s = sum 2^t, u = sum 2^t t.  Where c rises by d, s <- s 2^-d and u <- (u -
-// d s) 2^-d.  At the end log2 sum exp z = c + log2 s, so logprob = (t(token) - log2 s) / L and entropy = (log2 s - u / s) / L; an L that is rounded is a temperature of 1 + 2^-26.
-// Bound: the rows' way from memory.  A block of eight warps has a row (of sixteen, 2048 rows of 32768 and five alternatives took 102 us instead of 81); where there are fewer rows
+// With c the largest number so far and d = z - c: s = the sum of e^d without one of the largest's, which is 1, and u = the sum of d e^d.  Then log sum exp z = c + log(1 + s), logprob =
+// d(token) - log(1 + s) and entropy = log(1 + s) - u / (1 + s).  As the 1 stays out of the sums, the log probability of a token that has nearly all of the weight is as exact as the
+// others are beside it (with it inside, 0.05 was off by 2e-7).  Where c rises by x, u <- e^-x (u - x (1 + s)) and s <- e^-x (1 + s).
+// Bound: the rows' way from memory.  A block of eight warps has a row (of sixteen, 2048 rows of 32768 and five alternatives took 102 us instead of 80); where there are fewer rows
 // than SMs, a cluster of up to eight blocks shares it and its first block joins what they found, read through distributed shared memory.
 // The largest numbers: after one, four and sixteen rounds the block's numbers so far give a bound that `top` of the row pass (the top-th largest among the eight largest lanes'
 // maxima of each warp).  What passes it goes to the end of a list of the warp, of which a sort leaves `top` when it is full and at the end; the warps' lists are merged two by two.
-// With a bound of each warp's own, 20 alternatives of 2048 x 151936 logits took 815 us.
+// With a bound of each warp's own, 20 alternatives of 2048 x 151936 logits took 815 us.  Now, fp32: 194 us without alternatives (6.4 TB/s), 212 with one, 240 with 20, 351 with 64.
 #include "ptx.cuh"
 #include "seq_common.cuh"
 
@@ -34,7 +35,7 @@ __device__ __forceinline__ float exp2_fast(float t) {      // off by 2^-22
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct LogpArgs {
   const void* z;
@@ -44,27 +45,28 @@ struct LogpArgs {
   float *logprob, *entropy, *best;
   int* ids;
 };
+// What lies 210 below is e^-210 = 0, infinities too.
+__device__ __forceinline__ float below(float z, float c) { return fmaxf(z - c, -210.f); }
 struct LogpSums {
-  float c, s, u;
-  __device__ __forceinline__ void raise(float to) {
-    if (to > c) {
-      if (c > -INFINITY) {
-        const float d = c - to, f = exp2_fast(d);
-        u = f > 0.f ? f * fmaf(d, s, u) : 0.f;
-        s *= f;
-      }
-      c = to;
+  float c, s, u;                                   // c -inf: nothing yet
+  // `own`: the 1 that is not in s
+  __device__ __forceinline__ void raise(float to, float own) {
+    if (c > -INFINITY) {
+      const float d = below(c, to), f = exp2_fast(d * kLog2e);
+      u = f * fmaf(d, own + s, u);
+      s = f * (own + s);
     }
+    c = to;
   }
   __device__ __forceinline__ void join(const LogpSums& o) {
+    if (o.c == -INFINITY) return;
     LogpSums b = o;
-    raise(b.c);
-    b.raise(c);
+    if (b.c > c) raise(b.c, 1.f);                  // the 1 is the other's
+    else b.raise(c, 1.f);
     s += b.s;
     u += b.u;
   }
 };
-
 // One step of a bitonic network over N * 32 keys or numbers of a warp, place i * 32 + lane in k[i]: partners `half` apart, blocks of `size` in turn down (the larger ones
 // ahead) and up.
 template <int N, typename T>
@@ -113,6 +115,7 @@ __device__ __forceinline__ void merge_lists(Key* a, const Key* b, int lane) {
 template <int kVec, int kHave>
 struct LogpState {
   LogpSums sum;
+  float own;                                       // 1 where the warp's largest number is the lane's
   bool bad;
   int lane, top, listed;                           // keys in the warp's list
   Key least;                                       // only larger ones can still be among the `top`
@@ -157,16 +160,32 @@ struct LogpState {
       prune();
     }
   }
+  // A warp's c is one for all of its lanes, and rises a few times a row; one lane has the 1.  (A c of each lane's own rose in some lane in nearly every round: 254 us instead of 212 for
+  // 2048 x 151936 and one alternative.)
   __device__ __forceinline__ void add(const float (&v)[kHave], float most) {
-    const float to = most * kLog2e;
-    bad |= !(to < INFINITY);                       // and numbers above 2.3e38
-    sum.raise(to);
-    if (sum.c > -INFINITY) {
+    bad |= !(most * kLog2e < INFINITY);            // and numbers above 2.3e38
+    if (__any_sync(0xffffffffu, most > sum.c)) {
+      float to = most;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
+      sum.raise(to, own);
+      const uint32_t who = __ballot_sync(0xffffffffu, most == to);
+      own = lane == __ffs(who) - 1 ? 1.f : 0.f;
+      bool out = own == 0.f;                       // the first of the owner's largest stays out
 #pragma unroll
       for (int j = 0; j < kHave; ++j) {
-        const float t = fmaxf(fmaf(v[j], kLog2e, -sum.c), -300.f), e = exp2_fast(t);
+        const float d = below(v[j], to), e = exp2_fast(d * kLog2e);
+        const bool it = !out && v[j] == to;
+        out |= it;
+        sum.s += it ? 0.f : e;
+        sum.u = fmaf(e, d, sum.u);
+      }
+    } else if (sum.c > -INFINITY) {
+#pragma unroll
+      for (int j = 0; j < kHave; ++j) {
+        const float d = below(v[j], sum.c), e = exp2_fast(d * kLog2e);
         sum.s += e;
-        sum.u = fmaf(e, t, sum.u);
+        sum.u = fmaf(e, d, sum.u);
       }
     }
   }
@@ -223,6 +242,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
 
   LogpState<kVec, kHave> st;
   st.sum = {-INFINITY, 0.f, 0.f};
+  st.own = 0.f;
   st.bad = false;
   st.lane = lane;
   st.top = top;
@@ -290,11 +310,8 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    LogpSums b;
-    b.c = __shfl_xor_sync(0xffffffffu, st.sum.c, o);
-    b.s = __shfl_xor_sync(0xffffffffu, st.sum.s, o);
-    b.u = __shfl_xor_sync(0xffffffffu, st.sum.u, o);
-    st.sum.join(b);
+    st.sum.s += __shfl_xor_sync(0xffffffffu, st.sum.s, o);
+    st.sum.u += __shfl_xor_sync(0xffffffffu, st.sum.u, o);
   }
   if (top > 0) st.prune();
   if (lane == 0) s_sums[warp] = st.sum;
@@ -351,12 +368,12 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
     bad |= s_bad[c] != 0;
   }
   bad |= w.c == -INFINITY;
-  const float lse = log2f(w.s);                    // of what is above c
-  const auto logprob = [&](float x) { return (fmaf(x, kLog2e, -w.c) - lse) * kLn2; };
+  const float lse = log1pf(w.s);                   // of what is above c
+  const auto logprob = [&](float x) { return (x - w.c) - lse; };
   if (tid == 0) {
     const long long k = a.tokens[t];
     a.logprob[t] = bad ? NAN : k < 0 || k >= a.V ? -INFINITY : logprob(number((int)k));
-    a.entropy[t] = bad ? NAN : (lse - w.u / w.s) * kLn2;
+    a.entropy[t] = bad ? NAN : lse - w.u / (1.f + w.s);
   }
   for (int i = tid; i < top; i += kLpThreads) {
     const Key k = s_all[0][i];

@@ -130,3 +130,22 @@ def test_replayed_and_on_two_streams(T):
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(out, call()))
     _check(z, tokens, 12)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("T,V", [(1, 1500), (3, 1000), (2, 151936), (200, 4099), (400, 20000)])
+def test_a_token_that_has_nearly_all_of_the_weight(T, V, dtype):
+    """Its log probability is -log(1 + s) with s what the others weigh beside it: each weight is off by 2^-21 for the exponential and 2^-23 |d| for d = z - max and its product with
+    log2 e, with |d| < 64 here 2^-17 in all, and the sum of positive numbers by 2^-24 for each of at most 32 + V / 128 steps; the logarithm and the last rounding 2^-22."""
+    from krasis_b200 import seqops
+    g = torch.Generator(device="cuda").manual_seed(T + V)
+    z = torch.randn(T, V, device="cuda", generator=g) * 2
+    tokens = torch.randint(0, V, (T,), device="cuda", generator=g)
+    z[torch.arange(T), tokens] = 24.0 + 10 * torch.rand(T, device="cuda", generator=g)
+    z = z.to(dtype)
+    r = seqops.token_logprobs(z, tokens, 2)
+    d = z.double() - z.double().amax(1, keepdim=True)
+    d.scatter_(1, tokens[:, None], -float("inf"))
+    want = -torch.log1p(d.exp().sum(1))
+    off = 2.0 ** -17 + (32 + V / 128) * 2.0 ** -24 + 2.0 ** -22
+    assert bool(((r.logprob.double() - want).abs() <= off * want.abs()).all()) and torch.equal(r.top_logprobs[:, 0], r.logprob)
