@@ -3,8 +3,8 @@
 // With c the largest number so far and d = z - c: s = the sum of e^d without one of the largest's, which is 1, and u = the sum of d e^d.  Then log sum exp z = c + log(1 + s), logprob =
 // d(token) - log(1 + s) and entropy = log(1 + s) - u / (1 + s).  As the 1 stays out of the sums, the log probability of a token that has nearly all of the weight is as exact as the
 // others are beside it (with it inside, 0.05 was off by 2e-7).  Where c rises by x, u <- e^-x (u - x (1 + s)) and s <- e^-x (1 + s).
-// Bound: the rows' way from memory.  A block of eight warps has a row (of sixteen, 2048 rows of 32768 and five alternatives took 102 us instead of 80); where there are fewer rows
-// than SMs, a cluster of up to eight blocks shares it and its first block joins what they found, read through distributed shared memory.
+// Bound: the rows' way from memory.  A block of eight warps has a row (of sixteen, 2048 rows of 32768 and five alternatives took 102 us instead of 80); where more blocks
+// could run at once than there are rows, a cluster of up to eight shares it and its first block joins what they found, read through distributed shared memory.
 // The largest numbers: after one, four and sixteen rounds the block's numbers so far give a bound that `top` of the row pass (the top-th largest among the eight largest lanes'
 // maxima of each warp).  What passes it goes to the end of a list of the warp, of which a sort leaves `top` when it is full and at the end; the warps' lists are merged two by two.
 // With a bound of each warp's own, 20 alternatives of 2048 x 151936 logits took 815 us.  Now, fp32: 194 us without alternatives (6.4 TB/s), 212 with one, 240 with 20, 351 with 64.
@@ -396,10 +396,11 @@ KB2SEQ_API int kb2_seq_token_logprobs(const void* z, int dt, long long ldz, int 
   if (!z || !tokens || !logprob || !entropy || (top && (!ids || !best))) return failf(KB2SEQ_ERR_VALUE, "token_logprobs: null argument");
   kb2::OnDevice on(device);
   SEQ_CUDA(on.err);
-  // blocks of a row: as many as there are SMs for, each with a round's numbers at least
+  // Blocks of a row: as many as run at once, three an SM and some room for clusters, each with two rounds of numbers at least.  us with 1, 2, 4, 8 of them, V 151936 and one alternative:
+  // 16 rows 36.9, 26.6, 20.5, 18.5; 100 rows 38.9, 30.7, 26.7, 41.0; 200 rows 43.0, 36.9, 45.1, 65.5; 300 rows 49.2, 57.3, 61.5, 90.1.  V 8000, 100 rows 12.3, 14.4, 15.2, 26.6.
   const int round = kLpThreads * 16, sms = kb2::current_sms();
   int ctas = 1;
-  while (ctas < kLpMostCtas && 2ll * ctas * T <= sms && V > ctas * round) ctas *= 2;
+  while (ctas < kLpMostCtas && 4 * 2ll * ctas * T <= 11 * sms && V > 2 * ctas * round) ctas *= 2;
   if (T > INT32_MAX / kLpMostCtas) return failf(KB2SEQ_ERR_VALUE, "token_logprobs: %d rows are too many", T);
   const LogpArgs a{z, ldz, V, top, tokens, logprob, entropy, best, ids};
   const auto kernel = dt ? token_logprobs_kernel<true> : token_logprobs_kernel<false>;
