@@ -6,7 +6,7 @@
 // and 64 columns of one block of weights.  With the weights there a column's scale came from shared memory, 512 bytes of a warp's loads for every 16 numbers: 1024 cycles a block of 128
 // rows (8192 x 10 rows of 512 experts: 325 us a product, 225 so).  A tile is 256 weight rows, and
 //   one CTA has 128 rows of x: runs, and matrices whose tiles fill the SMs better so.  Few rows cost the same 512 cycles of MMAs a block, less than its 32 KB of weights take from
-//     memory (1380 cycles at the copy rate): 64 experts of 3 x 1408 x 2048 and 2334 rows run at 0.92 of it, 512 of 3 x 512 x 2048 and 81920 rows take 254 + 155 us for 202 + 146 of
+//     memory (1380 cycles at the copy rate): 64 experts of 3 x 1408 x 2048 and 2334 rows run at 0.88 of it, 512 of 3 x 512 x 2048 and 81920 rows take 254 + 155 us for 202 + 146 of
 //     weights, rows and results.  Pairs for such runs: 285 us a product against 211; at 8192 rows an expert 161 against 162;
 //   a pair of CTAs has 256, each half of the weights, so that a block's 32 KB of loads feed 512 cycles of its MMAs: many rows.  M 8192, N 12288, K 2048: 187 us, 2210 TFLOP/s; N 4096,
 //     K 4096: 117 us, 2345 of the 3341 that twice the bf16 rate is.  The tensor pipe is busy 61 % of the time, the issue slots 56 %;
