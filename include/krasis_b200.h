@@ -286,7 +286,7 @@ KB2_API int kb2_fp8_linear(const void* x_dev, int32_t x_f32, int64_t ldx, const 
                            int32_t out_f32, int32_t M, int32_t N, int32_t K, void* work_dev, size_t work_bytes, int32_t device, void* stream);
 /* Routed experts: out [T][W] = sum_j weights[t][j] down_e(q(silu(gate_e x) * up_e x)) with e = ids[t][j], x = q(h[t]), q the quantisation of rows and the products
  * in fp32.  w1 [E][2 F][W] = [gate ; up], w2 [E][W][F] with their scales; ids [T][top] int32, those outside [0, E) bring nothing.  F % 128 == 0, E <= 1024.
- * An expert's rows are rounded to bf16 ahead of the weighted sum (fp32) where out is bf16. */
+ * All sums are fp32; a bf16 result is rounded once.  The workspace is the same for either type of out. */
 KB2_API size_t kb2_fp8_experts_workspace(int32_t T, int32_t top, int32_t E, int32_t W, int32_t F, int32_t out_f32);
 KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const int32_t* ids_dev, const float* weights_dev, const void* w1_dev, const float* s1_dev,
                             const void* w2_dev, const float* s2_dev, void* out_dev, int32_t out_f32, int32_t T, int32_t top, int32_t E, int32_t W, int32_t F,

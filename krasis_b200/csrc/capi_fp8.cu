@@ -112,14 +112,14 @@ KB2_API int kb2_fp8_linear(const void* x_dev, int32_t x_f32, int64_t ldx, const 
 struct ExpertsWork {
   uint8_t *xc, *ac;
   float *xs, *as;
-  void* y;
+  float* y;                                        // the experts' rows
   ChunkDesc* chunks;
   int *n_chunks, *counts, *slot_of;
   int max_chunks;
   long long ldx;
   size_t bytes;
 };
-static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F, bool out_f32) {
+static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F) {
   ExpertsWork k{};
   Carve c(work);
   const size_t slots = (size_t)T * top;
@@ -129,7 +129,7 @@ static ExpertsWork experts_work(void* work, int T, int top, int E, int W, int F,
   k.xs = c.take<float>((size_t)k.ldx * fp8_blocks(W));
   k.ac = c.take<uint8_t>(slots * F);
   k.as = c.take<float>((size_t)k.ldx * fp8_blocks(F));
-  k.y = c.take<uint8_t>(slots * W * (out_f32 ? 4 : 2));
+  k.y = c.take<float>(slots * W);
   k.chunks = c.take<ChunkDesc>(k.max_chunks);
   k.n_chunks = c.take<int>(1);
   k.counts = c.take<int>(fp8_bin_counts((int)slots, E));
@@ -146,8 +146,8 @@ static int experts_sizes(long long T, int top, int E, int W, int F) {
   return KB2_OK;
 }
 
-KB2_API size_t kb2_fp8_experts_workspace(int32_t T, int32_t top, int32_t E, int32_t W, int32_t F, int32_t out_f32) {
-  return experts_sizes(T, top, E, W, F) || T == 0 ? 0 : experts_work(nullptr, T, top, E, W, F, out_f32 != 0).bytes;
+KB2_API size_t kb2_fp8_experts_workspace(int32_t T, int32_t top, int32_t E, int32_t W, int32_t F, int32_t) {
+  return experts_sizes(T, top, E, W, F) || T == 0 ? 0 : experts_work(nullptr, T, top, E, W, F).bytes;
 }
 
 KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const int32_t* ids_dev, const float* weights_dev, const void* w1_dev, const float* s1_dev,
@@ -157,7 +157,7 @@ KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const
   if (T == 0) return KB2_OK;
   if (!h_dev || !ids_dev || !weights_dev || !w1_dev || !s1_dev || !w2_dev || !s2_dev || !out_dev) return failf(KB2_ERR_VALUE, "null argument");
   if (off16(w1_dev) || off16(w2_dev) || off16(out_dev) || ldh < 0) return failf(KB2_ERR_VALUE, "fp8_experts: weights and out on 16 bytes, ldh >= 0");
-  const ExpertsWork k = experts_work(work_dev, T, top, E, W, F, out_f32 != 0);
+  const ExpertsWork k = experts_work(work_dev, T, top, E, W, F);
   if (!work_dev || off16(work_dev) || work_bytes < k.bytes) return failf(KB2_ERR_VALUE, "fp8_experts: a workspace of %zu bytes on 16, %zu needed", work_bytes, k.bytes);
   OnDevice on(device);
   CUDA_TRY(on.err);
@@ -169,10 +169,10 @@ KB2_API int kb2_fp8_experts(const void* h_dev, int32_t h_f32, int64_t ldh, const
   p.M = slots; p.N = 2 * F; p.K = W; p.groups = E;
   p.chunks = k.chunks; p.n_chunks = k.n_chunks; p.max_chunks = k.max_chunks;
   CUDA_TRY(launch_fp8_gated(p, k.as, k.ldx, current_sms(), s));
-  p.x = k.ac; p.xs = k.as; p.w = w2_dev; p.ws = s2_dev; p.out = k.y; p.out_f32 = out_f32 != 0;
+  p.x = k.ac; p.xs = k.as; p.w = w2_dev; p.ws = s2_dev; p.out = k.y; p.out_f32 = true;
   p.N = W; p.K = F;
   CUDA_TRY(launch_fp8_tiles(p, 1, current_sms(), s));
-  CUDA_TRY(launch_fp8_combine(k.y, out_f32 != 0, k.slot_of, weights_dev, T, top, W, out_dev, s));
+  CUDA_TRY(launch_fp8_combine(k.y, k.slot_of, weights_dev, T, top, W, out_dev, out_f32 != 0, s));
   return KB2_OK;
 }
 

@@ -129,8 +129,8 @@ cudaError_t launch_fp8_rows(const void* x, bool f32, long long ldx, int M, int K
 int fp8_bin_counts(int n, int E);
 cudaError_t launch_fp8_bin(const int* ids, int T, int top, int E, int* counts, ChunkDesc* runs, int* n_runs, int* slot_of, const void* x, bool f32, long long ldx, int K, void* codes,
                            float* scales, long long lds, cudaStream_t s);
-// out[t] = sum_j weights[t][j] y[slot_of[t][j]]
-cudaError_t launch_fp8_combine(const void* y, bool f32, const int* slot_of, const float* weights, int T, int top, int W, void* out, cudaStream_t s);
+// out[t] = sum_j weights[t][j] y[slot_of[t][j]], bf16 or fp32
+cudaError_t launch_fp8_combine(const float* y, const int* slot_of, const float* weights, int T, int top, int W, void* out, bool f32, cudaStream_t s);
 cudaError_t launch_fp8_blocks(const void* w, bool f32, int groups, int N, int K, void* codes, float* scales, cudaStream_t s);
 // One matrix, all M rows, on pairs of CTAs with tiles of 256 x 256.
 cudaError_t launch_fp8_pairs(const Fp8Product& p, int num_sms, cudaStream_t s);

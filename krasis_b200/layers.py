@@ -240,7 +240,7 @@ def fp8_experts(h: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gat
     """Routed experts whose matrices are held in 8 bits: out[t] = sum_j weights[t, j] down_e(q(silu(gate_e q(h[t])) * up_e q(h[t]))) with e = ids[t, j] and q the
     quantisation of quantize_fp8_rows.  h [T, W] bfloat16 or float32; ids [T, top] int32, those outside [0, E) bring nothing; weights [T, top] float32; w_gate_up
     [E, 2 F, W] = [gate ; up] and w_down [E, W, F] float8_e4m3fn, with a scale for each block of 128 x 128; W a multiple of 16, F of 128, at most 1024 experts.
-    [T, W] in out_dtype (h's own); for bfloat16 each expert's row is rounded to it ahead of the weighted sum."""
+    [T, W] in out_dtype (h's own); sums are fp32 and a bfloat16 result is rounded once."""
     T, W = _fp8_input("fp8_experts", h)
     if w_gate_up.dim() != 3 or w_gate_up.shape[1] % 256 or w_gate_up.shape[1] == 0:
         raise ValueError(f"fp8_experts: gate and up projections [E, 2 F, W] with F a multiple of 128, got {tuple(w_gate_up.shape)}")
