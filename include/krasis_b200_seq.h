@@ -361,7 +361,7 @@ KB2SEQ_API int kb2_seq_kv_keep(const kb2_seq_kv_cache* cache, const kb2_seq_kv_s
 
 /* ---- What a row of logits z [T][V] (dt, row stride ldz) says: logprob[t] = z[t][tokens[t]] - lse with lse = log sum exp z[t] (a token outside [0, V): -inf), entropy[t] = lse -
  * sum p z, and its `top` (at most min(V, 64)) largest logits as ids [T][top] with their log probabilities best [T][top], the largest first, the lowest index first among equals.
- * Sums in fp32.  Logits of -inf weigh nothing.  A row with a NaN or a logit above 2e38, or with nothing but -inf, gives NaN and ids
+ * Sums in fp32; a log probability below the least fp32 number is -inf.  Logits of -inf weigh nothing.  A row with a NaN or +inf, or with nothing but -inf, gives NaN and ids
  * of -1. */
 KB2SEQ_API int kb2_seq_token_logprobs(const void* z, int dt, long long ldz, int T, int V, const long long* tokens, int top, float* logprob, float* entropy, int* ids,
                                       float* best, int device, void* stream);

@@ -163,7 +163,7 @@ struct LogpState {
   // A warp's c is one for all of its lanes, and rises a few times a row; one lane has the 1.  (A c of each lane's own rose in some lane in nearly every round: 254 us instead of 212 for
   // 2048 x 151936 and one alternative.)
   __device__ __forceinline__ void add(const float (&v)[kHave], float most) {
-    bad |= !(most * kLog2e < INFINITY);            // and numbers above 2.3e38
+    bad |= !(most < INFINITY);                     // an infinity or a NaN; any other number is taken by its distance to the largest
     if (__any_sync(0xffffffffu, most > sum.c)) {
       float to = most;
 #pragma unroll

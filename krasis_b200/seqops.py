@@ -650,7 +650,7 @@ MAX_TOP_LOGPROBS = 64
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """logits [T, V] (fp32 or bfloat16, any row stride) and tokens [T] (int64 or int32): log softmax at the tokens, the entropy of the softmax, and the `top` largest
     logits' ids (int32) and log probabilities, the lowest id first among equals.  All in fp32.  A token outside [0, V) has log probability -inf; logits of -inf weigh
-    nothing; a row with a NaN or a logit above 2e38, or with nothing but -inf, gives NaN and ids of -1."""
+    nothing; a row with a NaN or +inf, or with nothing but -inf, gives NaN and ids of -1."""
     dev = logits.get_device()
     if dev < 0:
         _cuda(logits, "token_logprobs")
