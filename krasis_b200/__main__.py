@@ -44,17 +44,20 @@ def main(argv=None) -> int:
     ap.add_argument("--max-tokens", type=int, default=8192, help="tokens the cache pool holds")
     ap.add_argument("--max-requests", type=int, default=4)
     ap.add_argument("--step-tokens", type=int, default=512, help="token budget of one step (prompt portions + decoded tokens)")
-    ap.add_argument("--expert-format", default=None, choices=["e4m3"], help="routed experts held in 8-bit floating point (designs with silu-gated experts and weights on their outputs)")
+    ap.add_argument("--expert-format", default=None, choices=["e4m3"], help="routed experts held in 8-bit floating point (Megolorn, without identity experts)")
     ap.add_argument("--logprobs", type=int, default=None, help="log probabilities of the generated tokens, with this many alternatives (0 to 64)")
     a = ap.parse_args(argv)
 
     import torch
-    from .registry import E4M3_EXPERTS, architecture_of, load_model
+    from .registry import check_expert_format, load_model
     from .sampling import SamplingParams
     from .scheduler import Scheduler
-    if a.expert_format and architecture_of(a.model) not in E4M3_EXPERTS:
-        print(f"{architecture_of(a.model)} does not hold its experts in {a.expert_format}", file=sys.stderr)
-        return 3
+    if a.expert_format:
+        try:
+            check_expert_format(a.model, a.expert_format)
+        except ValueError as e:
+            print(e, file=sys.stderr)
+            return 3
     model = load_model(a.model, dtype=torch.bfloat16 if a.dtype == "bfloat16" else torch.float32, **({"expert_format": a.expert_format} if a.expert_format else {}))
     if not hasattr(model, "forward_step"):
         print(f"{type(model).__name__} has no step interface for generation", file=sys.stderr)

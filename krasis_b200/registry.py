@@ -93,5 +93,16 @@ def architecture_of(model_dir: str) -> str:
                      f"(architecture={raw.get('architecture')!r}, model_type={cfg.get('model_type')!r})")
 
 
+def check_expert_format(model_dir: str, expert_format) -> None:
+    """ValueError where the checkpoint's design does not hold its routed experts in that format.  A factory that was registered from outside takes the word itself."""
+    if not expert_format:
+        return
+    arch = architecture_of(model_dir)
+    ours = getattr(_REGISTRY.get(arch, _hf_moe), "__module__", None) == __name__
+    if ours and arch not in E4M3_EXPERTS:
+        raise ValueError(f"{arch} does not hold its experts in {expert_format}; {', '.join(E4M3_EXPERTS)} does")
+
+
 def load_model(model_dir: str, dtype=torch.bfloat16, device=0, **kw):
+    check_expert_format(model_dir, kw.get("expert_format"))
     return _REGISTRY[architecture_of(model_dir)](model_dir, dtype=dtype, device=device, **kw)

@@ -1,0 +1,36 @@
+"""Asking for experts in 8-bit floating point: which designs take it, and what is said ahead of reading a checkpoint."""
+import json
+
+import pytest
+
+
+def _dir(tmp_path, cfg):
+    (tmp_path / "config.json").write_text(json.dumps(cfg))
+    return str(tmp_path)
+
+
+@pytest.mark.parametrize("cfg", [{"architecture": a} for a in ("Vofelix", "Gurozen", "Zaronex", "Kugalorn", "Kivurax")]
+                         + [{"model_type": "qwen3_moe"}, {"text_config": {"model_type": "qwen3_5_moe_text"}}])
+def test_designs_that_do_not_take_the_format_refuse_it(tmp_path, monkeypatch, cfg):
+    """By load_model itself, ahead of building, importing or reading anything."""
+    from krasis_b200 import build, registry
+    for name in ("build", "build_seq"):
+        monkeypatch.setattr(build, name, lambda: pytest.fail("built"))
+    with pytest.raises(ValueError, match="does not hold its experts in e4m3"):
+        registry.load_model(_dir(tmp_path, cfg), expert_format="e4m3")
+
+
+def test_a_design_from_outside_takes_the_word_itself(tmp_path, monkeypatch):
+    from krasis_b200 import registry
+    monkeypatch.setattr(registry, "_REGISTRY", dict(registry._REGISTRY))
+    registry.register("Elsewhere", lambda d, dtype, device, **kw: kw)
+    assert registry.load_model(_dir(tmp_path, {"architecture": "Elsewhere"}), expert_format="e4m3") == {"expert_format": "e4m3"}
+
+
+@pytest.mark.parametrize("kw", [{}, {"expert_format": None}])
+def test_designs_load_without_the_word_as_before(tmp_path, monkeypatch, kw):
+    from krasis_b200 import registry
+    seen = []
+    monkeypatch.setitem(registry._REGISTRY, "Kivurax", lambda d, dtype, device, **k: seen.append(k))
+    registry.load_model(_dir(tmp_path, {"architecture": "Kivurax"}), **kw)
+    assert seen == [kw]
