@@ -26,8 +26,10 @@ def _vofelix(model_dir, dtype=torch.bfloat16, device=0, **kw):
 
 
 def _megolorn(model_dir, dtype=torch.bfloat16, device=0, **kw):
-    from .build import build_seq
+    from .build import build, build_seq
     build_seq()
+    if kw.get("expert_format"):
+        build()                                     # experts in 8 bits are quantised and multiplied by the core library
     from .megolorn import MegolornModel
     return MegolornModel.from_pretrained(model_dir, dtype=dtype, device=device, **kw)
 

@@ -34,3 +34,17 @@ def test_designs_load_without_the_word_as_before(tmp_path, monkeypatch, kw):
     monkeypatch.setitem(registry._REGISTRY, "Kivurax", lambda d, dtype, device, **k: seen.append(k))
     registry.load_model(_dir(tmp_path, {"architecture": "Kivurax"}), **kw)
     assert seen == [kw]
+
+
+@pytest.mark.parametrize("kw,want", [({}, ["seq"]), ({"expert_format": "e4m3"}, ["seq", "core"])])
+def test_the_libraries_that_a_load_needs_are_built_ahead_of_it(tmp_path, monkeypatch, kw, want):
+    """Experts in 8 bits run on the core library, which a design of the sequence library does not build otherwise."""
+    from krasis_b200 import build, megolorn, registry
+    done = []
+    monkeypatch.setattr(build, "build_seq", lambda: done.append("seq"))
+    monkeypatch.setattr(build, "build", lambda: done.append("core"))
+    monkeypatch.setattr(megolorn.MegolornModel, "from_pretrained", classmethod(lambda cls, *a, **k: done.append("read")))
+    layers = [{"type": "attention", "mixer": {"heads": 2, "kv_heads": 1, "dim": 16, "vdim": 16, "scale": 0.25},
+               "mlp": {"kind": "moe", "expert": {"ff": 128}, "router": {"experts": 4, "top": 2}}}]
+    registry.load_model(_dir(tmp_path, {"architecture": "Megolorn", "vocab": 50, "width": 32, "norm": {"eps": 1e-5}, "layers": layers}), **kw)
+    assert done == want + ["read"]
