@@ -26,7 +26,7 @@ import torch
 
 from . import seqops as ops
 from .attention import HeadKVCache, RecurrentStatePool
-from .mixers import GatedMLP, MultiMapAttention, RoutedExperts, lin
+from .mixers import GatedMLP, MultiMapAttention, RoutedExperts, check_expert_format, lin
 
 SWISH_ALPHA = 1.702      # slope inside the sigmoid of the dense feed-forward's activation
 MAPS = 2                 # attention maps per head
@@ -62,6 +62,13 @@ class MegolornConfig:
             if mlp and mlp.get("kind", "dense") not in ("dense", "moe"):
                 raise ValueError(f"unknown feed-forward kind {mlp.get('kind')!r}")
         return cfg
+
+    def check_expert_format(self, expert_format) -> None:
+        """ValueError where a layer's routed experts cannot be held in that format."""
+        moe = [L["mlp"] for L in self.layers if (L.get("mlp") or {}).get("kind", "dense") == "moe"]
+        for m in moe or [None]:
+            sizes = (m["router"]["experts"], m["router"].get("identity", 0), self.width, m["expert"]["ff"]) if m else (1, 0, 16, 128)
+            check_expert_format(expert_format, *sizes)
 
 
 def _sub(weights: dict, prefix: str) -> dict:
@@ -124,6 +131,7 @@ class MegolornModel:
         """expert_format "e4m3": routed experts held in 8 bits (see RoutedExperts)."""
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("dtype: bfloat16 or float32")
+        cfg.check_expert_format(expert_format)
         if not torch.cuda.is_available():
             raise RuntimeError("MegolornModel needs a CUDA device (krasis_b200 has no CPU path)")
         ops.load()
@@ -163,6 +171,7 @@ class MegolornModel:
     def from_pretrained(cls, model_dir: str, dtype=torch.bfloat16, device=0, expert_format=None, **_):
         from . import loader
         cfg = MegolornConfig.from_dict(json.load(open(os.path.join(model_dir, "config.json"))))
+        cfg.check_expert_format(expert_format)          # ahead of reading
         return cls(cfg, loader.read_named_tensors(model_dir), dtype=dtype, device=device, expert_format=expert_format)
 
     @classmethod

@@ -961,6 +961,17 @@ class MultiMapAttention:
                                           None, 0, int(self.gate_wide), positions, ops._ptr(self.vfreq), int(self.rot_half), s))
 
 
+def check_expert_format(expert_format, experts: int, identity: int, width: int, ff: int) -> None:
+    """ValueError unless routed experts of these sizes can be held so: None (as the other weights) or "e4m3" (layers.fp8_experts)."""
+    from .layers import FP8_BLOCK
+    if expert_format not in (None, "e4m3"):
+        raise ValueError(f"expert format {expert_format!r}: None (as the other weights) or \"e4m3\"")
+    if expert_format and (identity or not 1 <= experts <= 1024):
+        raise ValueError(f"experts in e4m3: 1 to 1024 of them and no identity experts, got {experts} and {identity}")
+    if expert_format and (ff % FP8_BLOCK or width % 16):
+        raise ValueError(f"experts in e4m3: inner width {ff} a multiple of {FP8_BLOCK}, width {width} of 16")
+
+
 class RoutedExperts:
     """weights: router [E + identity, W], correction [E + identity] (optional), e<i>_gate / e<i>_up [F, W], e<i>_down [W, F] for i < E,
     shared_gate / shared_up / shared_down (optional shared expert of the same form, run for every token and added), shared_sg [1, W]
@@ -979,7 +990,7 @@ class RoutedExperts:
     joins the activation pass (gated experts, no identity experts).
 
     expert_format "e4m3": the experts' matrices are held in 8 bits with a scale for each block of 128 x 128 and multiplied so
-    (layers.fp8_experts: silu-gated experts of W a multiple of 16 and F of 128, no identity experts, weights on the outputs); router and
+    (layers.fp8_experts: at most 1024 silu-gated experts of W a multiple of 16 and F of 128, no identity experts, weights on the outputs); router and
     shared expert stay as they are."""
 
     def __init__(self, weights: dict, experts: int, identity: int, top: int, dtype, device, groups: int = 1, keep: int = 1,
@@ -998,10 +1009,10 @@ class RoutedExperts:
         if score not in ops.ROUTE_SCORES:
             raise ValueError(f"router score {score!r}")
         self.expert_format = expert_format
-        if expert_format not in (None, "e4m3"):
-            raise ValueError(f"expert format {expert_format!r}: None (as the other weights) or \"e4m3\"")
-        if expert_format and (act != "silu" or self.ident or self.weight_input or not self.E):
-            raise ValueError("experts in e4m3: silu-gated, no identity experts, weights on the outputs")
+        W, F = weights["e0_down"].shape if self.E else (0, 0)
+        check_expert_format(expert_format, self.E, self.ident, W, F)
+        if expert_format and (act != "silu" or self.weight_input):
+            raise ValueError("experts in e4m3: silu-gated, weights on the outputs")
         self.act_kind, self.limit, self.alpha = GatedMLP.KINDS[act], float(limit), float(alpha)
         if weights["router"].shape[0] != self.E + self.ident:
             raise ValueError("router rows must equal experts + identity experts")
@@ -1022,11 +1033,9 @@ class RoutedExperts:
             raise ValueError("one router bias per router row")
         if self.E:
             first = (lambda i: torch.cat([weights[f"e{i}_gate"], weights[f"e{i}_up"]], 0)) if gated else (lambda i: weights[f"e{i}_up"])
-            self.F = weights["e0_down"].shape[1]
+            self.F = F
             if expert_format:
                 from . import layers
-                if self.F % layers.FP8_BLOCK or weights["e0_down"].shape[0] % 16:
-                    raise ValueError(f"experts in e4m3: inner width {self.F} a multiple of {layers.FP8_BLOCK}, width {weights['e0_down'].shape[0]} of 16")
                 q = lambda w: layers.quantize_fp8_blocks(w.to(device=device, dtype=torch.float32).contiguous())      # one matrix at a time
                 stack = lambda parts: (torch.stack([c.view(torch.uint8) for c, _ in parts]).view(torch.float8_e4m3fn), torch.stack([s for _, s in parts]))
                 self.w_gu, self.s_gu = stack([q(first(i)) for i in range(self.E)])

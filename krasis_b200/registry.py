@@ -96,13 +96,18 @@ def architecture_of(model_dir: str) -> str:
 
 
 def check_expert_format(model_dir: str, expert_format) -> None:
-    """ValueError where the checkpoint's design does not hold its routed experts in that format.  A factory that was registered from outside takes the word itself."""
+    """ValueError where the checkpoint's design, or this one of it, does not hold its routed experts in that format, by its config.json alone.
+    A factory that was registered from outside takes the word itself."""
     if not expert_format:
         return
     arch = architecture_of(model_dir)
     ours = getattr(_REGISTRY.get(arch, _hf_moe), "__module__", None) == __name__
     if ours and arch not in E4M3_EXPERTS:
         raise ValueError(f"{arch} does not hold its experts in {expert_format}; {', '.join(E4M3_EXPERTS)} does")
+    if ours and arch == "Megolorn":
+        from .megolorn import MegolornConfig
+        with open(os.path.join(model_dir, "config.json")) as f:
+            MegolornConfig.from_dict(json.load(f)).check_expert_format(expert_format)
 
 
 def load_model(model_dir: str, dtype=torch.bfloat16, device=0, **kw):

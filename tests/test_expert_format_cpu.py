@@ -48,3 +48,43 @@ def test_the_libraries_that_a_load_needs_are_built_ahead_of_it(tmp_path, monkeyp
                "mlp": {"kind": "moe", "expert": {"ff": 128}, "router": {"experts": 4, "top": 2}}}]
     registry.load_model(_dir(tmp_path, {"architecture": "Megolorn", "vocab": 50, "width": 32, "norm": {"eps": 1e-5}, "layers": layers}), **kw)
     assert done == want + ["read"]
+
+
+def _megolorn(experts=4, identity=0, ff=128, width=32):
+    router = {"experts": experts, "identity": identity, "top": 2}
+    layers = [{"type": "attention", "mixer": {"heads": 2, "kv_heads": 1, "dim": 16, "vdim": 16, "scale": 0.25}, "mlp": mlp}
+              for mlp in (None, {"ff": 56, "limit": 0.5}, {"kind": "moe", "expert": {"ff": ff}, "router": router})]
+    return {"architecture": "Megolorn", "vocab": 50, "width": width, "norm": {"eps": 1e-5}, "layers": layers}
+
+
+UNFIT = [({"identity": 1}, "identity"), ({"experts": 1025}, "1024"), ({"experts": 0, "identity": 0}, "1024"), ({"ff": 120}, "inner width 120"), ({"width": 24}, "width 24")]
+
+
+@pytest.mark.parametrize("sizes,said", UNFIT)
+def test_sizes_that_do_not_fit_are_named_ahead_of_reading(tmp_path, monkeypatch, capsys, sizes, said):
+    """By load_model, the class and the command line, from config.json alone."""
+    from krasis_b200 import build, loader, megolorn, registry
+    from krasis_b200.__main__ import main
+    for where, name in ((build, "build"), (build, "build_seq"), (loader, "read_named_tensors")):
+        monkeypatch.setattr(where, name, lambda *a: pytest.fail("built or read"))
+    d = _dir(tmp_path, _megolorn(**sizes))
+    for load in (registry.load_model, megolorn.MegolornModel.from_pretrained):
+        with pytest.raises(ValueError, match=said):
+            load(d, expert_format="e4m3")
+    assert main(["score", "--model", d, "--prompt-ids", "1,2", "--expert-format", "e4m3"]) == 3
+    assert said in capsys.readouterr().err
+
+
+def test_formats_that_there_are_not(tmp_path):
+    from krasis_b200 import registry
+    from krasis_b200.megolorn import MegolornConfig
+    with pytest.raises(ValueError, match="expert format 'e5m2'"):
+        registry.load_model(_dir(tmp_path, _megolorn()), expert_format="e5m2")
+    dense = _megolorn()
+    dense["layers"] = dense["layers"][:2]
+    for cfg in (_megolorn(), _megolorn(identity=2, ff=24), dense):
+        MegolornConfig.from_dict(cfg).check_expert_format(None)
+        with pytest.raises(ValueError):
+            MegolornConfig.from_dict(cfg).check_expert_format("int4")
+    for cfg in (_megolorn(), _megolorn(experts=1024, width=16, ff=256), dense):
+        MegolornConfig.from_dict(cfg).check_expert_format("e4m3")
