@@ -224,15 +224,14 @@ class Scheduler:
         scores = []
         for i, text in enumerate(texts):
             text, parts = [int(t) for t in text], []
-            if text and not self.can_admit(len(text)):
+            if len(text) > 1 and not self.can_admit(len(text)):
                 raise RuntimeError("a text does not fit the cache pool")
             try:
-                for a in range(0, len(text), step_tokens):
-                    part = text[a:a + step_tokens]
-                    told = text[a + 1:a + 1 + len(part)]         # what follows each of them; behind the last one of all, nothing
-                    logits = self.step([(("score", i), part, list(range(len(told))))])
-                    if told:
-                        parts.append(ops.token_logprobs(logits, torch.tensor(told, device=logits.device)).logprob)
+                for a in range(0, len(text) - 1, step_tokens):   # nothing follows the last token, so the model does not see it
+                    part = text[a:min(a + step_tokens, len(text) - 1)]
+                    told = text[a + 1:a + 1 + len(part)]         # what follows each of them
+                    logits = self.step([(("score", i), part, list(range(len(part))))])
+                    parts.append(ops.token_logprobs(logits, torch.tensor(told, device=logits.device)).logprob)
             finally:
                 if ("score", i) in self.live:
                     self.finish(("score", i))
