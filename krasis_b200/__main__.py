@@ -9,7 +9,8 @@
 
 `generate` loads the checkpoint through the model registry (config.json decides the class), runs continuous batching over the
 given prompts and prints one JSON line per prompt with the generated token ids (and, with --logprobs, the log probability and entropy of each
-and the N most likely tokens).  `score` prints the log probabilities of the given tokens, each after those before it, and the perplexity.  Token ids in, token ids out: tokenisers are not
+and the N most likely tokens).  `score` prints the log probabilities of the given tokens, each after those before it, and the perplexity;
+numbers that JSON does not have (the log probability of a token that cannot be, a perplexity beyond a double, NaN) are null.  Token ids in, token ids out: tokenisers are not
 part of this package."""
 import argparse
 import json
@@ -23,6 +24,17 @@ def perplexity(logprobs):
         return None
     mean = -sum(logprobs) / len(logprobs)
     return math.inf if mean > 709 else math.exp(mean)
+
+
+def json_line(record) -> str:
+    """One line of JSON; numbers that it cannot hold (infinities, NaN) are null."""
+    def held(x):
+        if isinstance(x, dict):
+            return {k: held(v) for k, v in x.items()}
+        if isinstance(x, (list, tuple)):
+            return [held(v) for v in x]
+        return None if isinstance(x, float) and not math.isfinite(x) else x
+    return json.dumps(held(record), allow_nan=False)
 
 
 def main(argv=None) -> int:
@@ -66,7 +78,7 @@ def main(argv=None) -> int:
     sched = Scheduler(model, max_tokens=a.max_tokens, max_requests=a.max_requests, cuda_graphs=True)
     if a.command == "score":
         for p, s in zip(prompts, sched.score(prompts, step_tokens=a.step_tokens)):
-            print(json.dumps({"prompt_tokens": len(p), "logprobs": s, "perplexity": perplexity(s)}))
+            print(json_line({"prompt_tokens": len(p), "logprobs": s, "perplexity": perplexity(s)}))
         return 0
     outs = sched.generate(prompts, a.max_new_tokens, SamplingParams(a.temperature, a.top_k, a.top_p, a.seed), step_tokens=a.step_tokens,
                           eos=a.eos, logprobs=a.logprobs)
@@ -75,7 +87,7 @@ def main(argv=None) -> int:
         outs, details = outs
         told = [{"logprobs": d} for d in details]
     for p, o, d in zip(prompts, outs, told):
-        print(json.dumps({"prompt_tokens": len(p), "generated": o, **d}))
+        print(json_line({"prompt_tokens": len(p), "generated": o, **d}))
     return 0
 
 
