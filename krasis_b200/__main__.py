@@ -64,6 +64,11 @@ def main(argv=None) -> int:
     from .registry import check_expert_format, load_model
     from .sampling import SamplingParams
     from .scheduler import Scheduler
+    from .seqops import MAX_TOP_LOGPROBS
+    if a.logprobs is not None and not 0 <= a.logprobs <= MAX_TOP_LOGPROBS:
+        ap.error(f"--logprobs {a.logprobs}: 0 to {MAX_TOP_LOGPROBS} alternatives")
+    if a.command == "score" and a.step_tokens < 1:
+        ap.error(f"--step-tokens {a.step_tokens}: portions of at least one token")
     if a.expert_format:
         try:
             check_expert_format(a.model, a.expert_format)

@@ -49,3 +49,13 @@ def test_generated_tokens_are_json_whatever_the_numbers_are(run):
     assert got["logprobs"][0]["logprob"] == 0 and got["logprobs"][0]["top"][0] == [5, 0.0] and got["logprobs"][0]["top"][1][1] is None
     (got,) = run("generate", "--prompt-ids", "5,5,6", "--max-new-tokens", "1", "--logprobs", "1")
     assert got["logprobs"][0]["logprob"] is None and got["logprobs"][0]["entropy"] is None
+
+
+@pytest.mark.parametrize("args,said", [(["generate", "--logprobs", "65"], "0 to 64"), (["generate", "--logprobs", "-1"], "0 to 64"), (["score", "--step-tokens", "0"], "at least one")])
+def test_numbers_out_of_range_are_refused_ahead_of_loading(monkeypatch, capsys, args, said):
+    from krasis_b200 import registry
+    from krasis_b200.__main__ import main
+    monkeypatch.setattr(registry, "load_model", lambda *a, **k: pytest.fail("loaded"))
+    with pytest.raises(SystemExit) as e:
+        main([*args, "--model", "-", "--prompt-ids", "1"])
+    assert e.value.code == 2 and said in capsys.readouterr().err
