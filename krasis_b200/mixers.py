@@ -1036,10 +1036,17 @@ class RoutedExperts:
             self.F = F
             if expert_format:
                 from . import layers
-                q = lambda w: layers.quantize_fp8_blocks(w.to(device=device, dtype=torch.float32).contiguous())      # one matrix at a time
-                stack = lambda parts: (torch.stack([c.view(torch.uint8) for c, _ in parts]).view(torch.float8_e4m3fn), torch.stack([s for _, s in parts]))
-                self.w_gu, self.s_gu = stack([q(first(i)) for i in range(self.E)])
-                self.w_down, self.s_down = stack([q(weights[f"e{i}_down"]) for i in range(self.E)])
+
+                def held(matrix):
+                    """Codes and scales of all experts; one matrix at a time is on the device in more bits."""
+                    for i in range(self.E):
+                        c, s = layers.quantize_fp8_blocks(matrix(i).to(device=device, dtype=torch.float32).contiguous())
+                        if i == 0:
+                            codes, scales = (torch.empty((self.E, *t.shape), dtype=t.dtype, device=t.device) for t in (c, s))
+                        codes[i], scales[i] = c, s
+                    return codes, scales
+                self.w_gu, self.s_gu = held(first)
+                self.w_down, self.s_down = held(lambda i: weights[f"e{i}_down"])
             else:
                 self.w_gu = d(torch.stack([first(i) for i in range(self.E)], 0))                     # [E, 2F | F, W]
                 self.w_down = d(torch.stack([weights[f"e{i}_down"] for i in range(self.E)], 0))      # [E, W, F]
