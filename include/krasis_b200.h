@@ -268,7 +268,8 @@ KB2_API int kb2_linear_f32(const float* x_dev, int64_t x_ld, int64_t x_group, co
 
 /* ---- Products of 8-bit floating-point numbers (e4m3) with a scale per block of 128 (activations: 128 numbers of a row; weights: 128 x 128; the last
  * blocks may be cut short).  With a = max |x| over a block: scale 2^k, k the least whole number >= -126 with a <= 448 2^k, codes e4m3(x / scale), ties to
- * even; a = 0: scale 0, codes 0; a number that is not finite: scale NaN, codes 0.  The products take any fp32 scales.
+ * even; a = 0: scale 0, codes 0; a number that is not finite: scale NaN, codes 0.  The products take any fp32 scales;
+ * a row's and a matrix's are multiplied with each other in fp32, so their product has to be a number of that type, too.
  * K (W) % 16 == 0.  x_f32 0: bf16, 1: fp32 rows of any stride; out_f32 likewise.  Codes, weights, outputs and workspaces on 16 bytes. */
 /* x [M][K] (row stride ldx) -> codes [M][K], scales[b * ld_scales + m] for the blocks b of a row (ld_scales >= M). */
 KB2_API int kb2_fp8_quantize_rows(const void* x_dev, int32_t x_f32, int64_t ldx, int32_t M, int32_t K, void* codes_dev, float* scales_dev, int64_t ld_scales,

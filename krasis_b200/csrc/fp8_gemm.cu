@@ -1,13 +1,14 @@
 // Products of 8-bit floating-point operands with a scale per block of 128 (fp8.cuh): out[m][n] = sum_b xs[m][b] ws[n / 128][b] sum_{k in block b} x[m][k] w[n][k], of one matrix or of
 // runs of rows that have a matrix each (routed experts).
 //
-// The tensor cores' accumulators cannot be rescaled on the way, so each block of 128 products per result is a sum of its own in tensor memory (two of them in turn), which sixteen
-// warps multiply by its scales and add up in registers, 64 sums a thread, while the next one runs.  The rows of x are the M side: a thread has one row, so one scale of it per block,
-// and 64 columns of one block of weights.  With the weights there a column's scale came from shared memory, 512 bytes of a warp's loads for every 16 numbers: 1024 cycles a block of 128
+// The scales are any fp32 numbers, by which the tensor cores' accumulators cannot be rescaled on the way (the products that scale their operands take powers of two alone), so each
+// block of 128 products per result is a sum of its own in tensor memory (two of them in turn), which sixteen warps multiply by its
+// scales and add up in registers, 64 sums a thread, while the next one runs.  The rows of x are the M side: a thread has one row, so one scale of it per block, and 64 columns of one
+// block of weights.  With the weights there a column's scale came from shared memory, 512 bytes of a warp's loads for every 16 numbers: 1024 cycles a block of 128
 // rows (8192 x 10 rows of 512 experts: 325 us a product, 225 so).  A tile is 256 weight rows, and
 //   one CTA has 128 rows of x: runs, and matrices whose tiles fill the SMs better so.  Few rows cost the same 512 cycles of MMAs a block, less than its 32 KB of weights take from
-//     memory (1380 cycles at the copy rate): 64 experts of 3 x 1408 x 2048 and 2334 rows run at 0.88 of it, 512 of 3 x 512 x 2048 and 81920 rows take 254 + 155 us for 202 + 146 of
-//     weights, rows and results.  Pairs for such runs: 285 us a product against 211; at 8192 rows an expert 161 against 162;
+//     memory (1380 cycles at the copy rate): 64 experts of 3 x 1408 x 2048 and 2334 rows take 66 + 40 us for 57 + 32 of weights, rows and results at that rate, 512 of 3 x 512 x 2048 and
+//     81920 rows 270 + 215 for 197 + 191 (results in fp32).  Pairs for such runs: 285 us a product against 211; at 8192 rows an expert 161 against 162;
 //   a pair of CTAs has 256, each half of the weights, so that a block's 32 KB of loads feed 512 cycles of its MMAs: many rows.  M 8192, N 12288, K 2048: 187 us, 2210 TFLOP/s; N 4096,
 //     K 4096: 117 us, 2345 of the 3341 that twice the bf16 rate is.  The tensor pipe is busy 61 % of the time, the issue slots 56 %;
 //   a cluster of 2 to 8 shares 128 rows along K, where tiles are fewer than SMs; the CTAs' sums meet in shared memory and are added in the order of the ranks.
@@ -37,6 +38,7 @@ constexpr int kTPart = 260;                        // numbers from row to row of
 static_assert(4 * tile_stage(kAlone) <= kTOffScale && 4 * tile_stage(kPair) <= kTOffOut && kTRows * kTPart * 4 <= kTOffOut && kTSmem <= 227 * 1024 && kTSmem >= 512 * 430 - 1024, "stages, results and scales; what a CTA of a cluster takes for 512 columns (tmem_smem)");
 
 // silu(g) u with one approximate power of two and one approximate reciprocal: off by 2^-21 of it, and for g below zero by |g| 2^-24 more, which is less than the rounding of g moves it.
+// Below g = -87.3 the reciprocal of 1 + e^-g, less than 2^-126, is flushed and the unit is 0 instead of 1e-36 u or less.
 __device__ __forceinline__ float gated(float g, float u) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
